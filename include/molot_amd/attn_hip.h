@@ -297,6 +297,122 @@ int molot_hip_attn_prefill_paged(const float* Qm, const void* K, const void* V, 
                                  int nkv, int M, int N, int d, float scale, int pos0, int window,
                                  int kv_dtype, void* stream);
 
+/* ---- Scored attention: capped scores, a bias by distance, keys by ranges ----
+ * (no reference counterpart: attn.h takes the scaled products as they are).
+ * The entries below are those above with the score of query position i and
+ * slot t formed as
+ *   s = scale * q.k
+ *   softcap > 0:   s = softcap * tanh(s / softcap)      (0: no cap; else
+ *                  within [1e-30, 1e30], MOLOT_EINVAL otherwise)
+ *   slopes:        s = s - slopes[h] * |i - t|          (device [nq], one a
+ *                  query head; NULL: none)
+ * and the softmax over the attended slots; an empty range yields o = 0.
+ * i is pos_cur, pos or pos0 + m as the entry's window takes it, t the slot.
+ * Same kernels, layouts, cache types, head dims, workspaces and accuracy as
+ * the plain entries.
+ *
+ * acc (NULL: none) is the weights a cache's eviction goes by: for every
+ * attended slot t and KV head g, the softmax weights of the query heads of
+ * g's group are added to acc of (g, t) in fp32, heads in order.  Token-major
+ * caches: acc[nkv][acc_cap], acc_cap >= the slots; paged ones: pages
+ * [num_blocks][nkv][page] through the same block table.  A step that appends
+ * a row sets that slot's acc instead, and its position in slot_pos (int32,
+ * same layout; NULL: none; only with acc).  The scores of a call with acc are
+ * kept for its second launch: 4 * B * nq * (attended rows + 1) bytes of the
+ * stream's prefill workspace, at most 1 GiB (MOLOT_ENOTSUP past it). */
+int molot_hip_attn_decode_scored(const float* Q, const void* K, const void* V, float* O, int nq,
+                                 int nkv, int n, int d, float scale, int pos_cur, int window,
+                                 float softcap, const float* slopes, float* acc, int acc_cap,
+                                 int kv_dtype, void* stream);
+
+/* molot_hip_decode_step_norm, scored (NULL norms and v_norm = 0: no norms). */
+int molot_hip_decode_step_scored(float* q, const float* k_new, const float* v_new, void* K,
+                                 void* V, float* O, int nq, int nkv, int d, int slot, int pos,
+                                 const float* q_norm, const float* k_norm, int v_norm, float eps,
+                                 const float* inv_freq, float scale, int window, float softcap,
+                                 const float* slopes, float* acc, int32_t* slot_pos, int acc_cap,
+                                 int kv_dtype, void* stream);
+
+/* molot_hip_attn_decode_paged and molot_hip_decode_step_paged_norm, scored. */
+int molot_hip_attn_decode_paged_scored(const float* Q, const void* K, const void* V, float* O,
+                                       const int32_t* block_table, const int32_t* seq_lens,
+                                       const int32_t* pos, int B, int max_blocks, int max_seq_len,
+                                       int nq, int nkv, int d, int page, float scale, int window,
+                                       float softcap, const float* slopes, float* acc,
+                                       int kv_dtype, void* stream);
+int molot_hip_decode_step_paged_scored(
+    float* q, const float* k_new, const float* v_new, void* K, void* V, float* O,
+    const int32_t* block_table, const int32_t* seq_lens, const int32_t* pos, int B, int max_blocks,
+    int max_seq_len, int nq, int nkv, int d, int page, const float* q_norm, const float* k_norm,
+    int v_norm, float eps, const float* inv_freq, float scale, int window, float softcap,
+    const float* slopes, float* acc, int32_t* slot_pos, int kv_dtype, void* stream);
+
+/* molot_hip_attn_prefill_gqa, _paged, molot_hip_prefill_step and _paged,
+ * scored, with the keys of every row as a range: row m attends [lo_m, hi_m),
+ *   lo_m = max(the window's start, key_lo[m])    (key_lo NULL: the window's)
+ *   hi_m = min(key_hi[m], N)                     (key_hi NULL: pos0 + m + 1)
+ * key_lo, key_hi: device int32 [M], any values (an empty range gives O = 0).
+ * So a packed prompt's documents keep to themselves (key_lo: the first slot
+ * of the row's document), a prefix sees itself both ways (key_hi: at least
+ * the prefix's end), and a padded row sees nothing. */
+int molot_hip_attn_prefill_scored(const float* Qm, const void* K, const void* V, float* Om, int nq,
+                                  int nkv, int M, int N, int d, float scale, int pos0, int window,
+                                  float softcap, const float* slopes, const int32_t* key_lo,
+                                  const int32_t* key_hi, int kv_dtype, void* stream);
+int molot_hip_attn_prefill_paged_scored(const float* Qm, const void* K, const void* V, float* Om,
+                                        const int32_t* block_row, int max_blocks, int page, int nq,
+                                        int nkv, int M, int N, int d, float scale, int pos0,
+                                        int window, float softcap, const float* slopes,
+                                        const int32_t* key_lo, const int32_t* key_hi,
+                                        int kv_dtype, void* stream);
+int molot_hip_prefill_step_scored(float* q, const float* k_new, const float* v_new, void* K,
+                                  void* V, float* O, int nq, int nkv, int d, int M, int slot0,
+                                  int pos0, const float* q_norm, const float* k_norm, int v_norm,
+                                  float eps, const float* inv_freq, float scale, int window,
+                                  float softcap, const float* slopes, const int32_t* key_lo,
+                                  const int32_t* key_hi, int kv_dtype, void* stream);
+int molot_hip_prefill_step_paged_scored(
+    float* q, const float* k_new, const float* v_new, void* K, void* V, float* O,
+    const int32_t* block_row, int max_blocks, int page, int nq, int nkv, int d, int M, int slot0,
+    int pos0, const float* q_norm, const float* k_norm, int v_norm, float eps,
+    const float* inv_freq, float scale, int window, float softcap, const float* slopes,
+    const int32_t* key_lo, const int32_t* key_hi, int kv_dtype, void* stream);
+
+/* ---- A cache held to a budget of rows ----
+ * (no reference counterpart: the reference's cache only grows, forward.h:570).
+ * acc and slot_pos (layouts as above) describe the slots in use: the weight a
+ * slot has got so far, and the position of the token it holds.  A scored step
+ * with both keeps them for the row it appends; molot_hip_kv_track does for
+ * rows appended otherwise (a prompt): the last M of n slots get acc 0 and the
+ * positions pos - M + 1 .. pos (slot_pos NULL: none).  The paged form takes
+ * the last min(M, seq_lens[b]) slots of every sequence, pos[b] its newest
+ * token's position (pos NULL: seq_lens[b] - 1). */
+int molot_hip_kv_track(float* acc, int32_t* slot_pos, int nkv, int n, int M, int pos, int acc_cap,
+                       void* stream);
+int molot_hip_kv_track_paged(float* acc, int32_t* slot_pos, const int32_t* block_table,
+                             const int32_t* seq_lens, const int32_t* pos, int B, int max_blocks,
+                             int max_seq_len, int M, int nkv, int page, void* stream);
+
+/* Cuts a cache of n slots to `keep`, per KV head by itself: the slots with
+ * slot_pos > pos - recent stay first, then those of the highest acc; of
+ * equals (the recent ones among themselves too), the lowest slots; a NaN acc
+ * is above every number.  The slots that stay and lie at or past keep move,
+ * in order, into the slots before keep that do not stay, in order: K and V
+ * rows, acc and slot_pos; everything else is left as it is, and slots keep
+ * .. n-1 are then free for the next rows (n = keep; n <= keep does nothing).
+ * Rows hold keys rotated at their own positions, so attention over the cut
+ * cache is over the tokens kept, with the next token's slot and position told
+ * apart (molot_hip_decode_step_scored's slot and pos, pos[] of the paged
+ * steps); windows and slopes go by slots, and no longer hold there.  The
+ * paged form cuts every sequence longer than keep (seq_lens is not written).
+ * K and V 16-byte aligned; every even head dim up to 512. */
+int molot_hip_kv_evict(void* K, void* V, float* acc, int32_t* slot_pos, int nkv, int n, int d,
+                       int keep, int recent, int pos, int acc_cap, int kv_dtype, void* stream);
+int molot_hip_kv_evict_paged(void* K, void* V, float* acc, int32_t* slot_pos,
+                             const int32_t* block_table, const int32_t* seq_lens,
+                             const int32_t* pos, int B, int max_blocks, int max_seq_len, int nkv,
+                             int d, int page, int keep, int recent, int kv_dtype, void* stream);
+
 /* The exponential of the split-K merges (the chunk weights e^(m_c - M),
  * the device expf), applied elementwise (x, y device [n]).  Counterpart of
  * exp_avx512_ps, include/molot/norm.h:35-47, exposed so its accuracy can be

@@ -57,8 +57,8 @@ def _run(cmd: list[str]) -> None:
 
 
 # the library's kernel sources, compiled side by side
-LIB_SOURCES = ("attn_flat.hip", "attn_paged.hip", "attn_decode.hip", "prefill_wide.hip",
-               "prefill_narrow.hip")
+LIB_SOURCES = ("attn_flat.hip", "attn_paged.hip", "attn_flat_scored.hip", "attn_paged_scored.hip",
+               "attn_decode.hip", "prefill_wide.hip", "prefill_narrow.hip", "kv_evict.hip")
 
 
 def _compile(name: str) -> str:

@@ -63,6 +63,28 @@ struct AttnArgs {
   int q8;                // host side: a matrix-core launch on Q8 rows
   int dyn_likely;        // host side: DynPlan::likely
   int dyn_pairs;         // host side: (sequence, chunk) pairs the grid holds
+  // Scored launches (the SC instances).  softcap > 0: a score s becomes softcap *
+  // tanh(s / softcap); slopes (device [nq], NULL: none): then s -= slope_h * |pos - t|
+  // at slot t; key_lo, key_hi (prefill rows; device [M], NULL: none): the first
+  // key of a row's range where that lies past its window's, and its end in
+  // place of pos + 1.
+  int scored;            // host side: the SC instances
+  float softcap;
+  const float* slopes;
+  const int32_t* key_lo;
+  const int32_t* key_hi;
+  // The weights (acc): the launch leaves its scores, in base-2 units, at
+  // scores[(sequence, KV head)][sc_rows rows from t0][nq / nkv heads] and each
+  // chunk's (max in base 2, sum) at stats[slot][nchunks][GH] for
+  // attn_weights_kernel, which adds the softmax weights to acc (layout of the
+  // C ABI) (NULL: no weights).  fresh: slot n - 1 was appended by this call: its
+  // acc is set, not added to, and with slot_pos so is its position.
+  float* scores;
+  float* stats;
+  float* acc;            // host side, as the rest
+  int32_t* slot_pos;
+  int64_t sc_rows;
+  int acc_cap, fresh;
 };
 using AttnFn = void (*)(AttnArgs);
 

@@ -1281,14 +1281,19 @@ static_assert(sizeof(CombArgs) <= 128, "two lines");
 // rows), as the attention kernel derives them.
 __device__ __forceinline__ int comb_chunks(const CombArgs& a, int b) {
   int n, pos;
+  int lo = 0;
   if (a.pf) {
     pos = a.pos0 + b;
     n = pos + 1 < a.n ? pos + 1 : a.n;
+    // prefill rows with key ranges: seq_lens is key_lo, pos_arr key_hi
+    if (a.pos_arr) n = max(0, min(a.pos_arr[b], a.n));
+    if (a.seq_lens) lo = a.seq_lens[b];
   } else {
     n = a.seq_lens[b];
     pos = a.pos_arr ? a.pos_arr[b] : n - 1;
   }
   int t0 = (a.window > 0 && pos - a.window + 1 > 0) ? pos - a.window + 1 : 0;
+  t0 = max(t0, lo);
   if (t0 > n) t0 = n;
   int span = (a.fold ? n - 1 : n) - t0;
   int chunk = a.chunk;
@@ -1527,6 +1532,86 @@ __global__ __launch_bounds__(kCombWaveThreads) void combine_rows_kernel(CombArgs
     for (int e = 0; e < V; ++e)
       if (pair + e < a.dh) a.o[slot * a.dh + pair + e] = o[e];
   }
+}
+
+// The softmax weights of a scored launch, summed over the query heads of each KV
+// head and added to acc: w = 2^(s - M) / L, M and L the merge of a head's chunk
+// statistics.  Thread: one row, its heads' scores side by side; grid (rows, KV
+// heads, sequences).  The sum runs over the heads in order, by one thread.
+struct WeightArgs {
+  CombArgs c;
+  const float* scores;
+  const float* stats;
+  float* acc;
+  int32_t* slot_pos;
+  const int32_t* block_table;
+  int64_t sc_rows;
+  int n, t0, pos, max_blocks, page_shift, acc_cap, fresh;
+};
+constexpr int kWeightThreads = 256;
+
+__global__ __launch_bounds__(kWeightThreads) void attn_weights_kernel(WeightArgs w) {
+  extern __shared__ float wsm[];
+  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int G = w.c.nq / w.c.nkv, gh = w.c.gh;
+  const bool paged = w.c.paged != 0;
+  int n = w.n, t0 = w.t0, pos = w.pos, nch = w.c.nchunks;
+  if (paged) {
+    n = w.c.seq_lens[b];
+    pos = w.c.pos_arr ? w.c.pos_arr[b] : n - 1;
+    t0 = (w.c.window > 0 && pos - w.c.window + 1 > 0) ? pos - w.c.window + 1 : 0;
+    if (t0 > n) t0 = n;
+    nch = comb_chunks(w.c, b);
+  }
+  const int span = (int)min((int64_t)(n - t0), w.sc_rows);
+  const int row0 = blockIdx.x * kWeightThreads;
+  auto index = [&](int t) -> int64_t {
+    if (!paged) return (int64_t)h * w.acc_cap + t;
+    const int64_t blk = w.block_table[(int64_t)b * w.max_blocks + (t >> w.page_shift)];
+    return ((blk * w.c.nkv + h) << w.page_shift) + (t & ((1 << w.page_shift) - 1));
+  };
+  // a fresh row outside the range (a position behind the cache's end)
+  if (w.fresh && n > 0 && n - 1 >= t0 + span && blockIdx.x == 0 && tid == 0) {
+    const int64_t i = index(n - 1);
+    w.acc[i] = 0.f;
+    if (w.slot_pos) w.slot_pos[i] = pos;
+  }
+  if (row0 >= span) return;
+  const int slot0 = b * w.c.nkv * w.c.nsub + h * w.c.nsub;
+  float *mx = wsm, *inv = wsm + G;
+  for (int g = tid >> 6; g < G; g += kWeightThreads / 64) {  // a wave a head
+    const float* st = w.stats + ((int64_t)(slot0 + g / gh) * w.c.nchunks * gh + g % gh) * 2;
+    float m = -INFINITY, l = 0.f;
+    for (int c = lane; c < nch; c += 64) m = fmaxf(m, st[(int64_t)c * gh * 2]);
+    m = group_max<64>(m);
+    for (int c = lane; c < nch; c += 64) {
+      const float mc = st[(int64_t)c * gh * 2];
+      l += mc == -INFINITY ? 0.f : st[(int64_t)c * gh * 2 + 1] * exp2_hw(mc - m);
+    }
+    l = group_sum<64>(l);
+    if (lane == 0) {
+      mx[g] = m;
+      inv[g] = 1.f / l;
+    }
+  }
+  __syncthreads();
+  if (row0 + tid >= span) return;
+  const int t = t0 + row0 + tid;
+  const float* s = w.scores + (((int64_t)b * w.c.nkv + h) * w.sc_rows + row0 + tid) * G;
+  float sum = 0.f;
+  if ((G & 3) == 0) {
+    for (int g = 0; g < G; g += 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(s + g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = fmaf(exp2_hw(x[e] - mx[g + e]), inv[g + e], sum);
+    }
+  } else {
+    for (int g = 0; g < G; ++g) sum = fmaf(exp2_hw(s[g] - mx[g]), inv[g], sum);
+  }
+  const int64_t i = index(t);
+  const bool set = w.fresh && t == n - 1;
+  w.acc[i] = set ? sum : w.acc[i] + sum;
+  if (set && w.slot_pos) w.slot_pos[i] = pos;
 }
 
 __global__ void vexp_kernel(const float* x, float* y, int64_t n) {
@@ -1886,15 +1971,27 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
   a.xmap = 0;
   a.slots = rows;
   a.mrg = 0;
-  if (a.nchunks == 1) return 0;  // single chunk: written directly, no combine
+  const size_t stats = a.acc ? (size_t)rows * a.nchunks * gh * 2 : 0;
+  if (a.nchunks == 1 && !stats) return 0;  // single chunk: written directly, no combine
   if ((long)rows > kMaxSlots) return MOLOT_ENOTSUP;
+  if (stats) {  // the scores of every attended row, for the weights
+    if (B > 65535) return MOLOT_ENOTSUP;  // attn_weights_kernel's grid
+    a.sc_rows = std::max(span, 0) + 1;
+    const size_t bytes = sizeof(float) * (size_t)B * a.nq * a.sc_rows;
+    if (bytes > kMaxPiecesBytes) return MOLOT_ENOTSUP;
+    void* sc = nullptr;
+    const int st = pieces_workspace(stream, bytes, &sc);
+    if (st) return st;
+    a.scores = reinterpret_cast<float*>(sc);
+  }
   const size_t P = (size_t)gh * d;
-  const size_t po = (size_t)rows * a.nchunks * P;
-  const size_t pml = (size_t)rows * a.nchunks * gh * 2;
-  const size_t qr = (size_t)rows * P;
+  const bool parts = a.nchunks > 1;
+  const size_t po = parts ? (size_t)rows * a.nchunks * P : 0;
+  const size_t pml = parts ? (size_t)rows * a.nchunks * gh * 2 : 0;
+  const size_t qr = parts ? (size_t)rows * P : 0;
   void* ws = nullptr;
   unsigned long long* ctr = nullptr;
-  const size_t need = sizeof(float) * (po + pml + qr);
+  const size_t need = sizeof(float) * (po + pml + qr + stats);
   if (a.ext_ws) {
     // a caller-provided workspace (molot_hip_decode_step_noalloc): no
     // allocation, and the combine kernel merges (no counters to keep)
@@ -1906,6 +2003,8 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
   }
   const int st = workspace(stream, need, &ctr, &ws);
   if (st) return st;
+  if (stats) a.stats = reinterpret_cast<float*>(ws) + po + pml + qr;
+  if (!parts) return 0;
   a.part_o = reinterpret_cast<float*>(ws);
   a.part_ml = a.part_o + po;
   a.qrot = a.part_ml + pml;
@@ -1935,6 +2034,62 @@ namespace {
 // geometry of this thread's last attention launch (molot_hip_last_plan)
 thread_local int t_last_nchunks = 0;
 thread_local int t_last_chunk = 0;
+
+CombArgs comb_args(const AttnArgs& a, int gh, int d, int nsubs, bool paged, bool rope) {
+  CombArgs cb{};
+  cb.part_o = a.part_o;
+  cb.part_ml = a.part_ml;
+  cb.qrot = a.qrot;
+  cb.o = a.o;
+  cb.q_out = a.q_out;
+  cb.seq_lens = a.seq_lens;
+  cb.pos_arr = a.pos_arr;
+  cb.nq = a.nq;
+  cb.nkv = a.nkv;
+  cb.gh = gh;
+  cb.nsub = nsubs;
+  cb.d = d;
+  cb.dh = a.dh;
+  cb.nchunks = a.nchunks;
+  cb.chunk = a.chunk;
+  cb.window = a.window;
+  cb.rope = rope ? 1 : 0;
+  cb.paged = !paged ? 0 : a.q8 ? 2 : 1;
+  cb.fold = rope && a.fold ? 1 : 0;
+  cb.pf = rope ? 0 : a.pf;
+  if (cb.pf) {  // the rows' key ranges (comb_chunks), in fields it has no other use for
+    cb.seq_lens = a.key_lo;
+    cb.pos_arr = a.key_hi;
+  }
+  cb.pos0 = a.dyn ? a.dyn_likely : a.pos;
+  cb.n = a.dyn ? a.dyn_span : a.n;
+  cb.dyn = a.dyn;
+  cb.nseq = a.nseq;
+  return cb;
+}
+
+// The weights of a launch that left its scores (AttnArgs::acc).
+int launch_weights(const CombArgs& cb, const AttnArgs& a, int B, void* stream) {
+  WeightArgs w{};
+  w.c = cb;
+  w.scores = a.scores;
+  w.stats = a.stats;
+  w.acc = a.acc;
+  w.slot_pos = a.slot_pos;
+  w.block_table = a.block_table;
+  w.sc_rows = a.sc_rows;
+  w.n = a.n;
+  w.t0 = a.t0;
+  w.pos = a.pos;
+  w.max_blocks = a.max_blocks;
+  w.page_shift = a.page_shift;
+  w.acc_cap = a.acc_cap;
+  w.fresh = a.fresh;
+  const dim3 grid((unsigned)((a.sc_rows + kWeightThreads - 1) / kWeightThreads), a.nkv, B);
+  hipLaunchKernelGGL(attn_weights_kernel, grid, dim3(kWeightThreads),
+                     2 * sizeof(float) * (a.nq / a.nkv), (hipStream_t)stream, w);
+  return (int)hipGetLastError();
+}
 
 // Launches an attention kernel of a planned problem and, for a split
 // context, combine_kernel after it on the same stream.
@@ -1986,33 +2141,9 @@ int molot_host::launch_pair(AttnFn kern, int threads, size_t lds, AttnArgs a, in
   int st = (int)hipGetLastError();
   if (st || !combine) {
     if (prof) g_prof.push_back(pr);
-    return st;
+    return st || !a.acc ? st : launch_weights(comb_args(a, gh, d, nsubs, paged, rope), a, B, stream);
   }
-  CombArgs cb{};
-  cb.part_o = a.part_o;
-  cb.part_ml = a.part_ml;
-  cb.qrot = a.qrot;
-  cb.o = a.o;
-  cb.q_out = a.q_out;
-  cb.seq_lens = a.seq_lens;
-  cb.pos_arr = a.pos_arr;
-  cb.nq = a.nq;
-  cb.nkv = a.nkv;
-  cb.gh = gh;
-  cb.nsub = nsubs;
-  cb.d = d;
-  cb.dh = a.dh;
-  cb.nchunks = a.nchunks;
-  cb.chunk = a.chunk;
-  cb.window = a.window;
-  cb.rope = rope ? 1 : 0;
-  cb.paged = !paged ? 0 : a.q8 ? 2 : 1;
-  cb.fold = rope && a.fold ? 1 : 0;
-  cb.pf = rope ? 0 : a.pf;
-  cb.pos0 = a.dyn ? a.dyn_likely : a.pos;
-  cb.n = a.dyn ? a.dyn_span : a.n;
-  cb.dyn = a.dyn;
-  cb.nseq = a.nseq;
+  CombArgs cb = comb_args(a, gh, d, nsubs, paged, rope);
   // At most 8 chunks (batches of sequences: many slots, few chunks): one
   // wave per 64 pairs (combine_wave_kernel<R>, R = 4 or 8 o loads per lane).
   // More chunks: combine_kernel, whose 4 phases per pair keep the loads per
@@ -2038,7 +2169,8 @@ int molot_host::launch_pair(AttnFn kern, int threads, size_t lds, AttnArgs a, in
   } else {
     hipLaunchKernelGGL(ck, cgrid, cblock, clds, (hipStream_t)stream, cb);
   }
-  return (int)hipGetLastError();
+  st = (int)hipGetLastError();
+  return st || !a.acc ? st : launch_weights(cb, a, B, stream);
 }
 namespace {
 
@@ -2107,6 +2239,9 @@ int zero_out(float* O, int64_t count, hipStream_t st) {
 
 template <bool PAGED, bool ROPE>
 int run_attn(AttnArgs& a, int d, int kv_dtype, int span, int B, void* stream) {
+  if (a.scored)
+    return PAGED ? run_paged_scored(a, ROPE, d, kv_dtype, span, B, stream)
+                 : run_flat_scored(a, ROPE, d, kv_dtype, span, B, stream);
   return PAGED ? run_paged(a, ROPE, d, kv_dtype, span, B, stream)
                : run_flat(a, ROPE, d, kv_dtype, span, B, stream);
 }
@@ -2120,6 +2255,36 @@ struct Norms {
 };
 
 bool norms_ok(const Norms& nm) { return nm.eps >= 0.f && nm.eps < INFINITY; }
+
+// How a scored entry forms its scores, and where its weights go.
+struct Scoring {
+  int on = 0;
+  float softcap = 0.f;
+  const float* slopes = nullptr;
+  float* acc = nullptr;
+  int32_t* slot_pos = nullptr;
+  int acc_cap = 0;
+  const int32_t* key_lo = nullptr;
+  const int32_t* key_hi = nullptr;
+};
+
+// softcap within the range whose reciprocal and products stay normal floats
+bool scoring_ok(const Scoring& sc) {
+  if (!(sc.softcap == 0.f || (sc.softcap >= 1e-30f && sc.softcap <= 1e30f))) return false;
+  return sc.acc || !sc.slot_pos;
+}
+
+void set_scoring(AttnArgs& a, const Scoring& sc, int fresh) {
+  a.scored = sc.on;
+  a.softcap = sc.softcap;
+  a.slopes = sc.slopes;
+  a.acc = sc.acc;
+  a.slot_pos = sc.slot_pos;
+  a.acc_cap = sc.acc_cap;
+  a.fresh = fresh;
+  a.key_lo = sc.key_lo;
+  a.key_hi = sc.key_hi;
+}
 
 std::atomic<int> g_presplit{1};  // molot_hip_set_prefill_presplit
 
@@ -2333,13 +2498,14 @@ int molot_hip_rope_append(float* q, const float* k_new, const float* v_new, void
                           Norms{}, stream);
 }
 
-int molot_hip_attn_decode_strided(const float* Q, const void* K, const void* V, float* O, int nq,
-                                  int nkv, int n, int d, int64_t tok_stride, int64_t head_stride,
-                                  float scale, int pos_cur, int window, int kv_dtype,
-                                  void* stream) {
+static int attn_decode_impl(const float* Q, const void* K, const void* V, float* O, int nq, int nkv,
+                            int n, int d, int64_t tok_stride, int64_t head_stride, float scale,
+                            int pos_cur, int window, int kv_dtype, const Scoring& sc,
+                            void* stream) {
   int st = check_common(nq, nkv, d, kv_dtype);
   if (st) return st;
   if (!Q || !O || n < 0) return MOLOT_EINVAL;
+  if (!scoring_ok(sc) || (sc.acc && sc.acc_cap < n)) return MOLOT_EINVAL;
   if (kv_dtype == MOLOT_KV_Q8 && (tok_stride != q8_row_bytes(nkv, d) || head_stride != d))
     return MOLOT_EINVAL;  // Q8: the token-major byte layout only
   int t0 = (window > 0 && pos_cur - window + 1 > 0) ? pos_cur - window + 1 : 0;
@@ -2374,7 +2540,31 @@ int molot_hip_attn_decode_strided(const float* Q, const void* K, const void* V, 
   a.pos = pos_cur;
   a.window = window;
   a.scale = scale;
+  set_scoring(a, sc, 0);
   return run_attn<false, false>(a, d, kv_dtype, n_att, 1, stream);
+}
+
+int molot_hip_attn_decode_strided(const float* Q, const void* K, const void* V, float* O, int nq,
+                                  int nkv, int n, int d, int64_t tok_stride, int64_t head_stride,
+                                  float scale, int pos_cur, int window, int kv_dtype,
+                                  void* stream) {
+  return attn_decode_impl(Q, K, V, O, nq, nkv, n, d, tok_stride, head_stride, scale, pos_cur,
+                          window, kv_dtype, Scoring{}, stream);
+}
+
+int molot_hip_attn_decode_scored(const float* Q, const void* K, const void* V, float* O, int nq,
+                                 int nkv, int n, int d, float scale, int pos_cur, int window,
+                                 float softcap, const float* slopes, float* acc, int acc_cap,
+                                 int kv_dtype, void* stream) {
+  Scoring sc;
+  sc.on = 1;
+  sc.softcap = softcap;
+  sc.slopes = slopes;
+  sc.acc = acc;
+  sc.acc_cap = acc_cap;
+  const int64_t row = kv_dtype == MOLOT_KV_Q8 ? q8_row_bytes(nkv, d) : (int64_t)nkv * d;
+  return attn_decode_impl(Q, K, V, O, nq, nkv, n, d, row, d, scale, pos_cur, window, kv_dtype, sc,
+                          stream);
 }
 
 int molot_hip_attn_decode_gqa_cache(const float* Q, const void* K, const void* V, float* O,
@@ -2408,12 +2598,13 @@ int molot_hip_attn_decode_head_win(const float* Q, const void* K, const void* V,
 static int decode_step_impl(float* q, const float* k_new, const float* v_new, void* K, void* V,
                             float* O, int nq, int nkv, int d, int slot, int pos,
                             const float* inv_freq, float scale, int window, int kv_dtype,
-                            const Norms& nm, void* stream, void* ext_ws = nullptr,
-                            int64_t ext_ws_bytes = 0) {
+                            const Norms& nm, const Scoring& sc, void* stream,
+                            void* ext_ws = nullptr, int64_t ext_ws_bytes = 0) {
   int st = check_common(nq, nkv, d, kv_dtype);
   if (st) return st;
   if (!norms_ok(nm)) return MOLOT_EINVAL;
   if (!q || !k_new || !v_new || !K || !V || !O || slot < 0) return MOLOT_EINVAL;
+  if (!scoring_ok(sc) || (sc.acc && sc.acc_cap <= slot)) return MOLOT_EINVAL;
   if (!aligned16(K) || !aligned16(V) || !aligned16(q) || !aligned16(O)) return MOLOT_EINVAL;
   const int n = slot + 1;
   int t0 = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
@@ -2423,6 +2614,10 @@ static int decode_step_impl(float* q, const float* k_new, const float* v_new, vo
     st = rope_append_impl(q, k_new, v_new, K, V, nq, nkv, d, slot, pos, inv_freq, kv_dtype, nm,
                           stream);
     if (st) return st;
+    if (sc.acc) {
+      st = kv_track(sc.acc, sc.slot_pos, nkv, n, 1, pos, sc.acc_cap, stream);
+      if (st) return st;
+    }
     return zero_out(O, (int64_t)nq * d, (hipStream_t)stream);
   }
   AttnArgs a{};
@@ -2449,6 +2644,7 @@ static int decode_step_impl(float* q, const float* k_new, const float* v_new, vo
   a.fold = 1;
   a.ext_ws = ext_ws;
   a.ext_ws_bytes = ext_ws_bytes;
+  set_scoring(a, sc, 1);
   return run_attn<false, true>(a, d, kv_dtype, n - 1 - t0, 1, stream);  // cache rows
 }
 
@@ -2457,7 +2653,7 @@ int molot_hip_decode_step(float* q, const float* k_new, const float* v_new, void
                           const float* inv_freq, float scale, int window, int kv_dtype,
                           void* stream) {
   return decode_step_impl(q, k_new, v_new, K, V, O, nq, nkv, d, slot, pos, inv_freq, scale,
-                          window, kv_dtype, Norms{}, stream);
+                          window, kv_dtype, Norms{}, Scoring{}, stream);
 }
 
 int molot_hip_decode_step_noalloc(float* q, const float* k_new, const float* v_new, void* K,
@@ -2468,7 +2664,7 @@ int molot_hip_decode_step_noalloc(float* q, const float* k_new, const float* v_n
   const int st = noalloc_scratch(&ws);
   if (st) return st;
   return decode_step_impl(q, k_new, v_new, K, V, O, nq, nkv, d, slot, pos, inv_freq, scale,
-                          window, kv_dtype, Norms{}, stream, ws, (int64_t)kScratchBytes);
+                          window, kv_dtype, Norms{}, Scoring{}, stream, ws, (int64_t)kScratchBytes);
 }
 
 int molot_hip_decode_step_norm(float* q, const float* k_new, const float* v_new, void* K,
@@ -2482,7 +2678,29 @@ int molot_hip_decode_step_norm(float* q, const float* k_new, const float* v_new,
   nm.v = v_norm ? 1 : 0;
   nm.eps = eps;
   return decode_step_impl(q, k_new, v_new, K, V, O, nq, nkv, d, slot, pos, inv_freq, scale,
-                          window, kv_dtype, nm, stream);
+                          window, kv_dtype, nm, Scoring{}, stream);
+}
+
+int molot_hip_decode_step_scored(float* q, const float* k_new, const float* v_new, void* K,
+                                 void* V, float* O, int nq, int nkv, int d, int slot, int pos,
+                                 const float* q_norm, const float* k_norm, int v_norm, float eps,
+                                 const float* inv_freq, float scale, int window, float softcap,
+                                 const float* slopes, float* acc, int32_t* slot_pos, int acc_cap,
+                                 int kv_dtype, void* stream) {
+  Norms nm;
+  nm.q = q_norm;
+  nm.k = k_norm;
+  nm.v = v_norm ? 1 : 0;
+  nm.eps = eps;
+  Scoring sc;
+  sc.on = 1;
+  sc.softcap = softcap;
+  sc.slopes = slopes;
+  sc.acc = acc;
+  sc.slot_pos = slot_pos;
+  sc.acc_cap = acc_cap;
+  return decode_step_impl(q, k_new, v_new, K, V, O, nq, nkv, d, slot, pos, inv_freq, scale,
+                          window, kv_dtype, nm, sc, stream);
 }
 
 static int paged_args(AttnArgs& a, const float* Q, void* K, void* V, float* O,
@@ -2536,6 +2754,29 @@ int molot_hip_attn_decode_paged(const float* Q, const void* K, const void* V, fl
   return run_attn<true, false>(a, d, kv_dtype, span, B, stream);
 }
 
+int molot_hip_attn_decode_paged_scored(const float* Q, const void* K, const void* V, float* O,
+                                       const int32_t* block_table, const int32_t* seq_lens,
+                                       const int32_t* pos, int B, int max_blocks, int max_seq_len,
+                                       int nq, int nkv, int d, int page, float scale, int window,
+                                       float softcap, const float* slopes, float* acc,
+                                       int kv_dtype, void* stream) {
+  Scoring sc;
+  sc.on = 1;
+  sc.softcap = softcap;
+  sc.slopes = slopes;
+  sc.acc = acc;
+  if (!scoring_ok(sc)) return MOLOT_EINVAL;
+  AttnArgs a{};
+  int span = 0;
+  int st = paged_args(a, Q, const_cast<void*>(K), const_cast<void*>(V), O, block_table, seq_lens,
+                      pos, B, max_blocks, max_seq_len, nq, nkv, d, page, scale, window, kv_dtype,
+                      &span);
+  if (st) return st;
+  if (B == 0) return 0;
+  set_scoring(a, sc, 0);
+  return run_attn<true, false>(a, d, kv_dtype, span, B, stream);
+}
+
 static int rope_append_paged_impl(float* q, const float* k_new, const float* v_new, void* K,
                                   void* V, const int32_t* block_table, const int32_t* seq_lens,
                                   const int32_t* pos, int B, int max_blocks, int nq, int nkv,
@@ -2547,8 +2788,8 @@ static int decode_step_paged_impl(float* q, const float* k_new, const float* v_n
                                   const int32_t* seq_lens, const int32_t* pos, int B,
                                   int max_blocks, int max_seq_len, int nq, int nkv, int d,
                                   int page, const float* inv_freq, float scale, int window,
-                                  int kv_dtype, const Norms& nm, void* stream) {
-  if (!norms_ok(nm)) return MOLOT_EINVAL;
+                                  int kv_dtype, const Norms& nm, const Scoring& sc, void* stream) {
+  if (!norms_ok(nm) || !scoring_ok(sc)) return MOLOT_EINVAL;
   AttnArgs a{};
   int span = 0;
   int st = paged_args(a, q, K, V, O, block_table, seq_lens, pos, B, max_blocks, max_seq_len, nq,
@@ -2556,10 +2797,12 @@ static int decode_step_paged_impl(float* q, const float* k_new, const float* v_n
   if (st) return st;
   if (!k_new || !v_new) return MOLOT_EINVAL;
   if (B == 0) return 0;
-  if (pos) {
+  set_scoring(a, sc, 1);
+  if (pos && (window > 0 || !sc.on)) {
     // a position behind the cache end can leave the new slot outside the
     // window; the split path only folds in rows it attends, so take the
-    // unfused kernels there (append, then attention over the cache)
+    // unfused kernels there (append, then attention over the cache; a scored
+    // step without a window attends every slot whatever the positions)
     st = rope_append_paged_impl(q, k_new, v_new, K, V, block_table, seq_lens, pos, B,
                                 max_blocks, nq, nkv, d, page, inv_freq, kv_dtype, nm, stream);
     if (st) return st;
@@ -2585,7 +2828,7 @@ int molot_hip_decode_step_paged(float* q, const float* k_new, const float* v_new
                                 void* stream) {
   return decode_step_paged_impl(q, k_new, v_new, K, V, O, block_table, seq_lens, pos, B,
                                 max_blocks, max_seq_len, nq, nkv, d, page, inv_freq, scale,
-                                window, kv_dtype, Norms{}, stream);
+                                window, kv_dtype, Norms{}, Scoring{}, stream);
 }
 
 int molot_hip_decode_step_paged_norm(float* q, const float* k_new, const float* v_new, void* K,
@@ -2602,7 +2845,29 @@ int molot_hip_decode_step_paged_norm(float* q, const float* k_new, const float* 
   nm.eps = eps;
   return decode_step_paged_impl(q, k_new, v_new, K, V, O, block_table, seq_lens, pos, B,
                                 max_blocks, max_seq_len, nq, nkv, d, page, inv_freq, scale,
-                                window, kv_dtype, nm, stream);
+                                window, kv_dtype, nm, Scoring{}, stream);
+}
+
+int molot_hip_decode_step_paged_scored(
+    float* q, const float* k_new, const float* v_new, void* K, void* V, float* O,
+    const int32_t* block_table, const int32_t* seq_lens, const int32_t* pos, int B, int max_blocks,
+    int max_seq_len, int nq, int nkv, int d, int page, const float* q_norm, const float* k_norm,
+    int v_norm, float eps, const float* inv_freq, float scale, int window, float softcap,
+    const float* slopes, float* acc, int32_t* slot_pos, int kv_dtype, void* stream) {
+  Norms nm;
+  nm.q = q_norm;
+  nm.k = k_norm;
+  nm.v = v_norm ? 1 : 0;
+  nm.eps = eps;
+  Scoring sc;
+  sc.on = 1;
+  sc.softcap = softcap;
+  sc.slopes = slopes;
+  sc.acc = acc;
+  sc.slot_pos = slot_pos;
+  return decode_step_paged_impl(q, k_new, v_new, K, V, O, block_table, seq_lens, pos, B,
+                                max_blocks, max_seq_len, nq, nkv, d, page, inv_freq, scale,
+                                window, kv_dtype, nm, sc, stream);
 }
 
 int molot_hip_rope_append_paged(float* q, const float* k_new, const float* v_new, void* K,
@@ -2699,7 +2964,8 @@ static int prefill_pieces(int nkv, int N, int d, int pos0, int window, int kv_dt
 // serve after the first.
 static int prefill_rows(const float* Qm, const void* K, const void* V, float* Om, int nq,
                         int nkv, int M, int N, int d, float scale, int pos0, int window,
-                        int kv_dtype, const int32_t* block_row, int page, void* stream) {
+                        int kv_dtype, const int32_t* block_row, int page, const Scoring& sc,
+                        void* stream) {
   if ((int64_t)M > 65535) return MOLOT_ENOTSUP;  // grid rows: one per query
   AttnArgs a{};
   a.q = Qm;
@@ -2722,6 +2988,7 @@ static int prefill_rows(const float* Qm, const void* K, const void* V, float* Om
   a.window = window;
   a.scale = scale;
   a.pf = 1;
+  set_scoring(a, sc, 0);
   // the widest attended range of any query row
   const int span = window > 0 && window < N ? window : N;
   return block_row ? run_attn<true, false>(a, d, kv_dtype, span, M, stream)
@@ -2913,6 +3180,13 @@ static bool prefill_takes_pieces(int d, int M, int N, int nq, int nkv, int kv_dt
   return true;
 }
 
+// The same of a scored prefill, whose other path is prefill_rows at every head dim:
+// TODO thresholds.
+static bool prefill_scored_pieces(int d, int M, int N, int nq, int nkv, int window, int presplit) {
+  const int64_t span = window > 0 && window < N ? window : N;
+  return presplit && M <= 65535 && (int64_t)M * nq * span >= 1;
+}
+
 // Their workspace for the attended keys [T0, N).
 static int pieces32_workspace(int nkv, int N, int d, int pos0, int window, int kv_dtype,
                               void* stream, void** ws, int* T0, int* R) {
@@ -2930,8 +3204,8 @@ static int pieces32_workspace(int nkv, int N, int d, int pos0, int window, int k
 // cap (the caller takes the other path).
 static int prefill_on_pieces(const float* Qm, const void* K, const void* V, float* Om, int nq,
                              int nkv, int M, int N, int d, float scale, int pos0, int window,
-                             int kv_dtype, const int32_t* block_row, int page, void* stream,
-                             int split_rows) {
+                             int kv_dtype, const int32_t* block_row, int page, const Scoring& sc,
+                             void* stream, int split_rows) {
   const int D = prefill_D(d), qb = wide_rows(D);
   PfArgs a{};
   a.q = Qm;
@@ -2946,7 +3220,11 @@ static int prefill_on_pieces(const float* Qm, const void* K, const void* V, floa
   a.pos0 = pos0;
   a.window = window;
   a.scale = scale;
-  a.own = prefill_by_rows(d, kv_dtype);
+  a.own = sc.on || prefill_by_rows(d, kv_dtype);
+  a.softcap = sc.softcap;
+  a.slopes = sc.slopes;
+  a.key_lo = sc.key_lo;
+  a.key_hi = sc.key_hi;
   a.kv_dtype = kv_dtype;
   if (block_row) {
     if (page <= 0 || (page & (page - 1)) || !q8_pages_ok(nkv, page, kv_dtype))
@@ -2986,7 +3264,8 @@ static int prefill_on_pieces(const float* Qm, const void* K, const void* V, floa
     st = (int)hipGetLastError();
     if (st) return st;
   }
-  return launch_prefill(D <= 128 ? prefill_narrow_fn(D, kv_dtype, a.own) : prefill_wide_fn(D, kv_dtype),
+  return launch_prefill(D <= 128 ? prefill_narrow_fn(D, kv_dtype, a.own, sc.on)
+                                 : prefill_wide_fn(D, kv_dtype, sc.on),
                         nqb * nkv * a.nsplit, 64 * kWideWaves, a, D, stream);
 }
 
@@ -2996,10 +3275,11 @@ static int prefill_on_pieces(const float* Qm, const void* K, const void* V, floa
 // appending step wrote the pieces of the others; -1: all of them)
 static int attn_prefill_impl(const float* Qm, const void* K, const void* V, float* Om, int nq,
                              int nkv, int M, int N, int d, float scale, int pos0, int window,
-                             int kv_dtype, const int32_t* block_row, int page, void* stream,
-                             int presplit, int split_rows = -1) {
+                             int kv_dtype, const int32_t* block_row, int page, const Scoring& sc,
+                             void* stream, int presplit, int split_rows = -1) {
   int st = check_common(nq, nkv, d, kv_dtype);
   if (st) return st;
+  if (!scoring_ok(sc)) return MOLOT_EINVAL;
   // The prefill kernels are built for D = 64, 128, 256.  Any other head dim
   // that is a multiple of 8 below 256 (fp32 or bf16) runs padded to the next
   // D: the split kernel and the per-tile loads read each row at its stored
@@ -3018,15 +3298,16 @@ static int attn_prefill_impl(const float* Qm, const void* K, const void* V, floa
   if (N == 0) return zero_out(Om, (int64_t)M * nq * d, (hipStream_t)stream);
   if (!K || !V || !aligned16(K) || !aligned16(V) || !aligned16(Qm) || !aligned16(Om))
     return MOLOT_EINVAL;
-  if (prefill_takes_pieces(d, M, N, nq, nkv, kv_dtype, window, presplit)) {
+  if (sc.on ? prefill_scored_pieces(d, M, N, nq, nkv, window, presplit)
+            : prefill_takes_pieces(d, M, N, nq, nkv, kv_dtype, window, presplit)) {
     st = prefill_on_pieces(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype, block_row,
-                           page, stream, split_rows);
+                           page, sc, stream, split_rows);
     if (st != MOLOT_ENOWS) return st;
     split_rows = -1;
   }
-  if (rows_path)
+  if (rows_path || sc.on)
     return prefill_rows(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype, block_row,
-                        page, stream);
+                        page, sc, stream);
   const int64_t rows = (int64_t)M * (nq / nkv);
   auto nqb_of = [&](int w) { return (rows + 16 * w - 1) / (16 * w); };
   int pw = kPfWaves;
@@ -3100,7 +3381,7 @@ static int attn_prefill_impl(const float* Qm, const void* K, const void* V, floa
       // a capture that would have to grow them, or past the cap: the vector-
       // ALU kernel reads the Q8 rows itself
       return prefill_rows(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype,
-                          block_row, page, stream);
+                          block_row, page, sc, stream);
     }
     if (ws) {
       a.pieces = reinterpret_cast<const uint16_t*>(ws);
@@ -3126,16 +3407,40 @@ int molot_hip_attn_prefill_gqa(const float* Qm, const void* K, const void* V, fl
                                int nkv, int M, int N, int d, float scale, int pos0, int window,
                                int kv_dtype, void* stream) {
   return attn_prefill_impl(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype,
-                           nullptr, 0, stream, g_presplit.load(std::memory_order_relaxed));
+                           nullptr, 0, Scoring{}, stream,
+                           g_presplit.load(std::memory_order_relaxed));
+}
+
+// A scored prefill's arguments.
+static Scoring prefill_scoring(float softcap, const float* slopes, const int32_t* key_lo,
+                               const int32_t* key_hi) {
+  Scoring sc;
+  sc.on = 1;
+  sc.softcap = softcap;
+  sc.slopes = slopes;
+  sc.key_lo = key_lo;
+  sc.key_hi = key_hi;
+  return sc;
+}
+
+int molot_hip_attn_prefill_scored(const float* Qm, const void* K, const void* V, float* Om, int nq,
+                                  int nkv, int M, int N, int d, float scale, int pos0, int window,
+                                  float softcap, const float* slopes, const int32_t* key_lo,
+                                  const int32_t* key_hi, int kv_dtype, void* stream) {
+  return attn_prefill_impl(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype,
+                           nullptr, 0, prefill_scoring(softcap, slopes, key_lo, key_hi), stream,
+                           g_presplit.load(std::memory_order_relaxed));
 }
 
 static int prefill_step_impl(float* q, const float* k_new, const float* v_new, void* K, void* V,
                              float* O, int nq, int nkv, int d, int M, int slot0, int pos0,
                              const float* q_norm, const float* k_norm, int v_norm, float eps,
                              const float* inv_freq, float scale, int window, int kv_dtype,
-                             const int32_t* block_row, int page, int max_blocks, void* stream) {
+                             const int32_t* block_row, int page, int max_blocks,
+                             const Scoring& sc, void* stream) {
   int st = check_common(nq, nkv, d, kv_dtype);
   if (st) return st;
+  if (!scoring_ok(sc)) return MOLOT_EINVAL;
   // the prefill kernels' head dims, a multiple of 8 below 256 run padded, or
   // prefill rows (d > 256, not a multiple of 8, or a padded Q8 cache; see
   // attn_prefill_impl)
@@ -3187,10 +3492,11 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   int T0 = 0;
   int split_rows = -1;
   const int presplit = g_presplit.load(std::memory_order_relaxed);
-  if (prefill_takes_pieces(d, M, slot0 + M, nq, nkv, kv_dtype, window, presplit)) {
+  if (sc.on ? prefill_scored_pieces(d, M, slot0 + M, nq, nkv, window, presplit)
+            : prefill_takes_pieces(d, M, slot0 + M, nq, nkv, kv_dtype, window, presplit)) {
     // at d = 512 the split of all rows is as fast (8q/2kv, 1999 tokens: 29 + 7
     // us against 49 for a RoPE/append that leaves the pieces)
-    if (d == 64 || d == 128) {
+    if (!sc.on && (d == 64 || d == 128)) {
       int R = 0;
       st = pieces32_workspace(nkv, slot0 + M, d, pos0, window, kv_dtype, stream, &pws, &T0, &R);
       if (st && st != MOLOT_ENOWS) return st;
@@ -3199,7 +3505,7 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
         r.pc_np = wide_pieces(kv_dtype == MOLOT_KV_F32);
       }
     }
-  } else if (supported_d(d)) {
+  } else if (supported_d(d) && !sc.on) {
     int64_t R = 0;
     st = prefill_pieces(nkv, slot0 + M, d, pos0, window, kv_dtype, stream, presplit, &pws, &T0, &R,
                         pieces_only);
@@ -3217,7 +3523,7 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   st = launch_rope_tok(r, M, stream);
   if (st) return st;
   return attn_prefill_impl(q, K, V, O, nq, nkv, M, slot0 + M, d, scale, pos0, window, kv_dtype,
-                           block_row, page, stream, presplit, split_rows);
+                           block_row, page, sc, stream, presplit, split_rows);
 }
 
 int molot_hip_prefill_step(float* q, const float* k_new, const float* v_new, void* K, void* V,
@@ -3226,7 +3532,19 @@ int molot_hip_prefill_step(float* q, const float* k_new, const float* v_new, voi
                            const float* inv_freq, float scale, int window, int kv_dtype,
                            void* stream) {
   return prefill_step_impl(q, k_new, v_new, K, V, O, nq, nkv, d, M, slot0, pos0, q_norm, k_norm,
-                           v_norm, eps, inv_freq, scale, window, kv_dtype, nullptr, 0, 0, stream);
+                           v_norm, eps, inv_freq, scale, window, kv_dtype, nullptr, 0, 0,
+                           Scoring{}, stream);
+}
+
+int molot_hip_prefill_step_scored(float* q, const float* k_new, const float* v_new, void* K,
+                                  void* V, float* O, int nq, int nkv, int d, int M, int slot0,
+                                  int pos0, const float* q_norm, const float* k_norm, int v_norm,
+                                  float eps, const float* inv_freq, float scale, int window,
+                                  float softcap, const float* slopes, const int32_t* key_lo,
+                                  const int32_t* key_hi, int kv_dtype, void* stream) {
+  return prefill_step_impl(q, k_new, v_new, K, V, O, nq, nkv, d, M, slot0, pos0, q_norm, k_norm,
+                           v_norm, eps, inv_freq, scale, window, kv_dtype, nullptr, 0, 0,
+                           prefill_scoring(softcap, slopes, key_lo, key_hi), stream);
 }
 
 int molot_hip_prefill_step_paged(float* q, const float* k_new, const float* v_new, void* K,
@@ -3238,7 +3556,19 @@ int molot_hip_prefill_step_paged(float* q, const float* k_new, const float* v_ne
   if (!block_row || max_blocks <= 0) return MOLOT_EINVAL;
   return prefill_step_impl(q, k_new, v_new, K, V, O, nq, nkv, d, M, slot0, pos0, q_norm, k_norm,
                            v_norm, eps, inv_freq, scale, window, kv_dtype, block_row, page,
-                           max_blocks, stream);
+                           max_blocks, Scoring{}, stream);
+}
+
+int molot_hip_prefill_step_paged_scored(
+    float* q, const float* k_new, const float* v_new, void* K, void* V, float* O,
+    const int32_t* block_row, int max_blocks, int page, int nq, int nkv, int d, int M, int slot0,
+    int pos0, const float* q_norm, const float* k_norm, int v_norm, float eps,
+    const float* inv_freq, float scale, int window, float softcap, const float* slopes,
+    const int32_t* key_lo, const int32_t* key_hi, int kv_dtype, void* stream) {
+  if (!block_row || max_blocks <= 0) return MOLOT_EINVAL;
+  return prefill_step_impl(q, k_new, v_new, K, V, O, nq, nkv, d, M, slot0, pos0, q_norm, k_norm,
+                           v_norm, eps, inv_freq, scale, window, kv_dtype, block_row, page,
+                           max_blocks, prefill_scoring(softcap, slopes, key_lo, key_hi), stream);
 }
 
 // Norm and RoPE of M rows of queries [M][nq][d] at positions pos0 + m, in
@@ -3334,7 +3664,21 @@ int molot_hip_attn_prefill_paged(const float* Qm, const void* K, const void* V, 
   if (!block_row || max_blocks <= 0 || N < 0 || (int64_t)N > (int64_t)max_blocks * page)
     return MOLOT_EINVAL;
   return attn_prefill_impl(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype,
-                           block_row, page, stream, g_presplit.load(std::memory_order_relaxed));
+                           block_row, page, Scoring{}, stream,
+                           g_presplit.load(std::memory_order_relaxed));
+}
+
+int molot_hip_attn_prefill_paged_scored(const float* Qm, const void* K, const void* V, float* Om,
+                                        const int32_t* block_row, int max_blocks, int page, int nq,
+                                        int nkv, int M, int N, int d, float scale, int pos0,
+                                        int window, float softcap, const float* slopes,
+                                        const int32_t* key_lo, const int32_t* key_hi,
+                                        int kv_dtype, void* stream) {
+  if (!block_row || max_blocks <= 0 || N < 0 || (int64_t)N > (int64_t)max_blocks * page)
+    return MOLOT_EINVAL;
+  return attn_prefill_impl(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype,
+                           block_row, page, prefill_scoring(softcap, slopes, key_lo, key_hi),
+                           stream, g_presplit.load(std::memory_order_relaxed));
 }
 
 int molot_hip_vexp(const float* x, float* y, int64_t n, void* stream) {

@@ -61,6 +61,11 @@ int run_paged(AttnArgs& a, bool rope, int d, int kv_dtype, int span, int B, void
 int run_flat_scored(AttnArgs& a, bool rope, int d, int kv_dtype, int span, int B, void* stream);
 int run_paged_scored(AttnArgs& a, bool rope, int d, int kv_dtype, int span, int B, void* stream);
 
+// The last M of a contiguous cache's n slots are new, the newest at pos
+// (molot_hip_kv_track; kv_evict.hip).
+int kv_track(float* acc, int32_t* slot_pos, int nkv, int n, int M, int pos, int acc_cap,
+             void* stream);
+
 }  // namespace molot_host
 
 #endif  // MOLOT_AMD_CSRC_ATTN_HOST_HPP_

@@ -12,6 +12,7 @@
 #include "attn_args.hpp"
 #include "device_util.hpp"
 #include "paged_plan.hpp"
+#include "score_mod.hpp"
 
 namespace {
 
@@ -537,7 +538,10 @@ __device__ __forceinline__ void arrive_and_merge(const AttnArgs& a, int64_t slot
   }
 }
 
-template <int D, int GH, int NW, int NT, bool ROPE, int RED, bool XSW = false, int QSTR = D>
+// SC: the waves' maxima at wm are in base-2 units, and (with scores) the chunk's
+// (max, sum) goes to stats in them too.
+template <int D, int GH, int NW, int NT, bool ROPE, int RED, bool XSW = false, int QSTR = D,
+          bool SC = false>
 __device__ __forceinline__ void finish_chunk(const AttnArgs& a, const float* wm, const float* wl,
                                              const float* red, int RS, const float* qs, int tid,
                                              int lane, bool split, int64_t slot, int c,
@@ -566,7 +570,9 @@ __device__ __forceinline__ void finish_chunk(const AttnArgs& a, const float* wm,
     const float mw_l = lane < NW ? wm[lane * GH + g] : -INFINITY;
     const float m = group_max<NW <= 16 ? 16 : 64>(mw_l);  // lanes >= NW hold -inf
     // waves without rows weigh 0 (also when no wave of the chunk has one)
-    const float e_l = lane < NW && mw_l != -INFINITY ? softmax_exp(mw_l - m) : 0.f;
+    const float d_l = mw_l - m;
+    const float e_l =
+        lane < NW && mw_l != -INFINITY ? (SC ? exp2_hw(d_l) : softmax_exp(d_l)) : 0.f;
     const float l = group_sum<NW <= 16 ? 16 : 64>(lane < NW ? e_l * wl[lane * GH + g] : 0.f);
     float o = 0.f;
     // XSW: head g's element j at g*D + (j ^ 4*(g % 8)) (the matrix-core
@@ -582,6 +588,17 @@ __device__ __forceinline__ void finish_chunk(const AttnArgs& a, const float* wm,
     pl[i] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(l)));
   }
   const bool lead = ph == 0;  // phase 0 threads own the chunk partial's outputs
+  if constexpr (SC) {
+#pragma unroll
+    for (int i = 0; i < PP; ++i) {
+      if (a.scores && lead && pv_[i] && pr_[i] - g_[i] * D == 0) {
+        float* st = a.stats + ((slot * a.nchunks + c) * GH + g_[i]) * 2;
+        st[0] = pm[i];
+        st[1] = pl[i];
+      }
+      pm[i] *= kLn2;
+    }
+  }
   if (!split) {
 #pragma unroll
     for (int i = 0; i < PP; ++i) {
@@ -668,7 +685,8 @@ __device__ void empty_range_q(const AttnArgs& a, int64_t qrow0, int gh, int dh, 
   }
 }
 
-template <int D, int GH, typename T, bool PAGED, bool ROPE, bool PAD, typename C>
+// SC: scored launches (AttnArgs::scored).
+template <int D, int GH, typename T, bool PAGED, bool ROPE, bool PAD, typename C, bool SC>
 __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
   using V16 = typename KVT<T>::vec;
   constexpr int VW = C::VW, LPR = C::LPR, NV = C::NV, EPL = C::EPL, RPS = C::RPS;
@@ -724,11 +742,17 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
     if (!ROPE && a.pf) {
       pos = a.pos + b;
       n = min(pos + 1, a.n);
+      if constexpr (SC) {
+        if (a.key_hi) n = max(0, min(a.key_hi[b], a.n));
+      }
     } else {
       n = a.seq_lens[b];
       pos = a.pos_arr ? a.pos_arr[b] : n - 1;
     }
     t0 = (a.window > 0 && pos - a.window + 1 > 0) ? pos - a.window + 1 : 0;
+    if constexpr (SC && !ROPE) {
+      if (a.pf && a.key_lo) t0 = max(t0, a.key_lo[b]);
+    }
     if (t0 > n) t0 = n;
   }
   // Chunks tile the cache rows [t0, cend); a fused step's new token (slot
@@ -1052,6 +1076,18 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
         qr[g][v * VW + e4 + 3] = x[3];
       }
 
+  // SC: the cap and the heads' slopes in base-2 units, and this (sequence, KV
+  // head)'s scores (row t at (t - t0) * G)
+  [[maybe_unused]] float slope[GH], cap2 = 0.f, rcap = 0.f;
+  [[maybe_unused]] float* swr = nullptr;
+  if constexpr (SC) {
+#pragma unroll
+    for (int g = 0; g < GH; ++g) slope[g] = a.slopes ? a.slopes[hq0 + g] * kLog2e : 0.f;
+    cap2 = a.softcap * kLog2e;
+    rcap = a.softcap > 0.f ? 1.f / cap2 : 0.f;
+    if (a.scores) swr = a.scores + ((int64_t)b * a.nkv + h) * a.sc_rows * G + sub * GH;
+  }
+
   // ---- 2. streaming blocks with a per-wave online softmax ----
   float* pw = smem + L.pw + w * RB * GH;
   float m_run[GH], l_run[GH], acc[GH][AW];
@@ -1098,8 +1134,43 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
 #pragma unroll
       for (int g = 0; g < GH; ++g) {
         const float t = group_sum<LPR>(d[g]) * (Q8 ? qsc * ksr[k] : qsc);
-        sc[k][g] = valid ? t : -INFINITY;
-        bmax[g] = fmaxf(bmax[g], sc[k][g]);
+        if constexpr (SC) {
+          sc[k][g] = t;
+        } else {
+          sc[k][g] = valid ? t : -INFINITY;
+          bmax[g] = fmaxf(bmax[g], sc[k][g]);
+        }
+      }
+    }
+    if constexpr (SC) {
+      if (a.softcap > 0.f) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) cap_scores<GH>(sc[k], cap2, rcap);
+      }
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int lr = rbase + k * RPS + rr;
+        const bool valid = lr < nrows;
+        const int t = rfirst + min(gmap(lr), rmax);
+        const float dist = fabsf((float)(pos - t));
+#pragma unroll
+        for (int g = 0; g < GH; ++g) {
+          const float x = fmaf(-slope[g], dist, sc[k][g]);
+          sc[k][g] = valid ? x : -INFINITY;
+          bmax[g] = fmaxf(bmax[g], sc[k][g]);
+        }
+        if (swr && s == 0 && valid && t - t0 < a.sc_rows) {
+          float* w0 = swr + (int64_t)(t - t0) * G;  // GH | G: aligned as a GH-vector
+          if constexpr (GH % 4 == 0) {
+#pragma unroll
+            for (int g = 0; g < GH; g += 4)
+              *reinterpret_cast<f32x4*>(w0 + g) =
+                  f32x4{sc[k][g], sc[k][g + 1], sc[k][g + 2], sc[k][g + 3]};
+          } else {
+#pragma unroll
+            for (int g = 0; g < GH; ++g) w0[g] = sc[k][g];
+          }
+        }
       }
     }
     // The running max moves only when a score passes it by more than
@@ -1253,9 +1324,20 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
 #pragma unroll
       for (int j = lane; j < D; j += 64) part[g] = fmaf(qs[g * D + j], knew[j], part[g]);
     }
+    if constexpr (SC) {  // (every lane: its part is then the whole score)
+#pragma unroll
+      for (int g = 0; g < GH; ++g) part[g] = wave_reduce<false>(part[g]) * qsc;
+      if (a.softcap > 0.f) cap_scores<GH>(part, cap2, rcap);
+      const float dist = fabsf((float)(pos - (n - 1)));
+#pragma unroll
+      for (int g = 0; g < GH; ++g) {
+        part[g] = fmaf(-slope[g], dist, part[g]);
+        if (swr && lane == 0 && n - 1 - t0 < a.sc_rows) swr[(int64_t)(n - 1 - t0) * G + g] = part[g];
+      }
+    }
 #pragma unroll
     for (int g = 0; g < GH; ++g) {
-      const float snew = wave_reduce<false>(part[g]) * qsc;
+      const float snew = SC ? part[g] : wave_reduce<false>(part[g]) * qsc;
       const float mn = fmaxf(m_run[g], snew);
       const float alpha = exp2_hw(m_run[g] - mn);
       const float p = exp2_hw(snew - mn);
@@ -1292,7 +1374,7 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
   if (lane == 0) {
 #pragma unroll
     for (int g = 0; g < GH; ++g) {
-      wm[w * GH + g] = m_run[g] * kLn2;  // natural units for the merges
+      wm[w * GH + g] = SC ? m_run[g] : m_run[g] * kLn2;  // natural units for the merges
       wl[w * GH + g] = l_run[g];
     }
   }
@@ -1306,7 +1388,7 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
           red[(w * GH + g) * D + (v2 * LPR2 + cs) * VW + e] = acc[g][v2 * VW + e];
   }
   lds_barrier();
-  finish_chunk<D, GH, NW, NT, ROPE, NW * P>(a, wm, wl, red, P, qs, tid, lane, split, slot, c,
+  finish_chunk<D, GH, NW, NT, ROPE, NW * P, false, D, SC>(a, wm, wl, red, P, qs, tid, lane, split, slot, c,
                                              qrow0, nch,
                                     smem + L.mrg, red, misc + 1, DH);
 
@@ -1543,7 +1625,8 @@ __device__ __forceinline__ void i8x16_to_bf16(const u32x4& x, u32x4& lo, u32x4& 
 // scales; they pass through a per-wave LDS slot to the accumulator lanes of
 // rows 16u + 4*(l/16) + r.  The new token's k (rotated) and v rows are
 // quantized in the workgroup like the cache rows and folded in as code * s.
-template <int D, int GH, bool PAGED, bool ROPE, bool Q8>
+// SC: scored launches (AttnArgs::scored).
+template <int D, int GH, bool PAGED, bool ROPE, bool Q8, bool SC>
 __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) {
   static_assert(D == 64 || D == 128, "MFMA tiles cover D = 64 or 128");
   static_assert(GH >= 1 && GH <= 16, "the group's q heads on the 16 MFMA columns");
@@ -1881,6 +1964,16 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
       }
     }
 
+  // SC, as attn_kernel; the lane's head is m16
+  [[maybe_unused]] float slope = 0.f, cap2 = 0.f, rcap = 0.f;
+  [[maybe_unused]] float* swr = nullptr;
+  if constexpr (SC) {
+    if (a.slopes && m16 < GH) slope = a.slopes[hq0 + m16] * kLog2e;
+    cap2 = a.softcap * kLog2e;
+    rcap = a.softcap > 0.f ? 1.f / cap2 : 0.f;
+    if (a.scores && m16 < GH) swr = a.scores + ((int64_t)b * a.nkv + h) * a.sc_rows * G + sub * GH + m16;
+  }
+
   // ---- stream ----
   char* vt = reinterpret_cast<char*>(smem + L.vt + w * RS);
   f32x4 o[DT];
@@ -1964,6 +2057,21 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
     // 16u + 4*(l/16) + r
     float sv[2][4];
     float tmax = -INFINITY;
+    if constexpr (SC) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = Q8 ? sacc[i / 4][i % 4] * sk4[i / 4][i % 4] : sacc[i / 4][i % 4];
+      if (a.softcap > 0.f) cap_scores<8>(x, cap2, rcap);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = tile_row(tile) + 16 * (i / 4) + 4 * g4 + i % 4;
+        const int t = rfirst + row;
+        const float y = fmaf(-slope, fabsf((float)(pos - t)), x[i]);
+        sv[i / 4][i % 4] = row < rlim ? y : -INFINITY;
+        tmax = fmaxf(tmax, sv[i / 4][i % 4]);
+        if (swr && row < rlim && t - t0 < a.sc_rows) swr[(int64_t)(t - t0) * G] = y;
+      }
+    } else
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -2056,7 +2164,13 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
         part = fmaf(qs[m16 * QSTR + d], knew[d], part);
     }
     part = sum_xor32(sum_xor16(part));
-    const float snew = part * qsc;  // base 2, as the streamed scores
+    float snew = part * qsc;  // base 2, as the streamed scores
+    if constexpr (SC) {
+      float x[1] = {snew};
+      if (a.softcap > 0.f) cap_scores<1>(x, cap2, rcap);
+      snew = fmaf(-slope, fabsf((float)(pos - (n - 1))), x[0]);
+      if (swr && g4 == 0 && n - 1 - t0 < a.sc_rows) swr[(int64_t)(n - 1 - t0) * G] = snew;
+    }
     const float mn = fmaxf(m_run, snew);
     const float alpha = exp2_hw(m_run - mn);
     const float p = exp2_hw(snew - mn);
@@ -2075,7 +2189,7 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
   float* red = smem + L.vt;
   if (m16 < GH) {
     if (g4 == 0) {
-      wm[w * GH + m16] = m_run * kLn2;  // natural units for the merge
+      wm[w * GH + m16] = SC ? m_run : m_run * kLn2;  // natural units for the merge
       wl[w * GH + m16] = l_run;
     }
     // head m16's row with its float index XOR 4*(m16 % 8): the 8 lanes of a
@@ -2086,7 +2200,7 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
           o[dt];
   }
   lds_barrier();
-  finish_chunk<D, GH, NW, NT, ROPE, NW * RS, true, QSTR>(a, wm, wl, red, RS, qs, tid, lane, split, slot, c,
+  finish_chunk<D, GH, NW, NT, ROPE, NW * RS, true, QSTR, SC>(a, wm, wl, red, RS, qs, tid, lane, split, slot, c,
                                               qrow0, nch,
                                     smem + L.mrg, red, misc + 1, DH);
 

@@ -14,17 +14,17 @@ namespace {
 using namespace molot_host;
 
 // A planned launch of attn_kernel with configuration C.
-template <int D, int GH, typename T, bool PAGED, bool ROPE, bool PAD, typename C>
+template <int D, int GH, typename T, bool PAGED, bool ROPE, bool PAD, typename C, bool SC>
 int launch_planned(AttnArgs a, int nsubs, int B, void* stream) {
   if (a.mrg && sizeof(float) * (size_t)Lds(D, GH, C::NW, C::RB, a.chunk, a.page_shift, PAGED,
                                            a.mrg).total > kMaxLds)
     no_merge(a);  // the merge's statistics do not fit beside the kernel's LDS
   const Lds L(D, GH, C::NW, C::RB, a.chunk, a.page_shift, PAGED, a.mrg);
-  return launch_pair(attn_kernel<D, GH, T, PAGED, ROPE, PAD, C>, C::NT, sizeof(float) * (size_t)L.total,
-                     a, GH, D, nsubs, B, PAGED, ROPE, stream);
+  return launch_pair(attn_kernel<D, GH, T, PAGED, ROPE, PAD, C, SC>, C::NT,
+                     sizeof(float) * (size_t)L.total, a, GH, D, nsubs, B, PAGED, ROPE, stream);
 }
 
-template <int D, int GH, typename T, bool PAGED, bool ROPE, bool PAD, typename C>
+template <int D, int GH, typename T, bool PAGED, bool ROPE, bool PAD, typename C, bool SC>
 int launch_cfg(AttnArgs a, int span, int nsubs, int B, void* stream) {
   // Q8 (d = 256): the heads of a token share 128-byte lines (see launch_pair)
   a.chunk_fast = sizeof(T) == 1;
@@ -42,9 +42,9 @@ int launch_cfg(AttnArgs a, int span, int nsubs, int B, void* stream) {
     // chunks (32k tokens, no window) stay on 16 waves (26.0 against 27.8 us)
     if (a.chunk <= 8 * 4 * C::RB)
       return launch_planned<D, GH, T, PAGED, ROPE, PAD,
-                            Cfg<D, GH, T, C::LPR, C::RB, 8, C::NBUF>>(a, nsubs, B, stream);
+                            Cfg<D, GH, T, C::LPR, C::RB, 8, C::NBUF>, SC>(a, nsubs, B, stream);
   }
-  return launch_planned<D, GH, T, PAGED, ROPE, PAD, C>(a, nsubs, B, stream);
+  return launch_planned<D, GH, T, PAGED, ROPE, PAD, C, SC>(a, nsubs, B, stream);
 }
 
 // bf16 or Q8 KV, D = 64 or 128: the matrix-core kernel.  Workgroups per CU
@@ -53,7 +53,7 @@ int launch_cfg(AttnArgs a, int span, int nsubs, int B, void* stream) {
 // half the rate of the first, and the chunks left to it form the tail);
 // paged batches are cut finer, their sequences differing in length: bf16
 // 16 (c4 240.2 -> 235.6 us against 8), Q8 8 (c4q8: 141.5 us, 150.1 at 16).
-template <int D, int GH, bool PAGED, bool ROPE, bool Q8>
+template <int D, int GH, bool PAGED, bool ROPE, bool Q8, bool SC>
 int launch_mfma(AttnArgs a, int span, int nsubs, int B, void* stream) {
   constexpr int kWpc = PAGED ? (Q8 ? 8 : 16) : 1;
   a.chunk_fast = Q8;
@@ -79,13 +79,13 @@ int launch_mfma(AttnArgs a, int span, int nsubs, int B, void* stream) {
                    kMaxLds)
     no_merge(a);
   const LdsM L(D, GH, a.chunk, a.page_shift, PAGED, Q8, a.mrg);
-  return launch_pair(attn_mfma_kernel<D, GH, PAGED, ROPE, Q8>, kMfmaThreads,
+  return launch_pair(attn_mfma_kernel<D, GH, PAGED, ROPE, Q8, SC>, kMfmaThreads,
                      sizeof(float) * (size_t)L.total, a, GH, D, nsubs, B, PAGED, ROPE, stream);
 }
 
-template <int D, int GH, typename T, bool PAGED, bool ROPE, bool PAD>
+template <int D, int GH, typename T, bool PAGED, bool ROPE, bool PAD, bool SC>
 int launch_attn(const AttnArgs& a, int span, int nsubs, int B, void* stream) {
-  return launch_cfg<D, GH, T, PAGED, ROPE, PAD, typename Tune<D, GH, T>::C>(a, span, nsubs, B,
+  return launch_cfg<D, GH, T, PAGED, ROPE, PAD, typename Tune<D, GH, T>::C, SC>(a, span, nsubs, B,
                                                                            stream);
 }
 
@@ -93,15 +93,15 @@ int launch_attn(const AttnArgs& a, int span, int nsubs, int B, void* stream) {
 // 8-head workgroup would need 99 KB of LDS for its waves' partial o; 8 q
 // heads of a KV head then run as two subgroups reading the rows twice).
 constexpr int kMaxGhWide = 4;
-template <int D, typename T, bool PAGED, bool ROPE, bool PAD>
+template <int D, typename T, bool PAGED, bool ROPE, bool PAD, bool SC>
 int dispatch_gh(int gh, const AttnArgs& a, int span, int nsubs, int B, void* st) {
   switch (gh) {
-    case 1: return launch_attn<D, 1, T, PAGED, ROPE, PAD>(a, span, nsubs, B, st);
-    case 2: return launch_attn<D, 2, T, PAGED, ROPE, PAD>(a, span, nsubs, B, st);
-    case 4: return launch_attn<D, 4, T, PAGED, ROPE, PAD>(a, span, nsubs, B, st);
+    case 1: return launch_attn<D, 1, T, PAGED, ROPE, PAD, SC>(a, span, nsubs, B, st);
+    case 2: return launch_attn<D, 2, T, PAGED, ROPE, PAD, SC>(a, span, nsubs, B, st);
+    case 4: return launch_attn<D, 4, T, PAGED, ROPE, PAD, SC>(a, span, nsubs, B, st);
     case 8:
       if constexpr (D <= 256 && !(sizeof(T) == 1 && D <= 128))
-        return launch_attn<D, 8, T, PAGED, ROPE, PAD>(a, span, nsubs, B, st);
+        return launch_attn<D, 8, T, PAGED, ROPE, PAD, SC>(a, span, nsubs, B, st);
       break;
   }
   return MOLOT_EINVAL;
@@ -110,47 +110,47 @@ int dispatch_gh(int gh, const AttnArgs& a, int span, int nsubs, int B, void* st)
 // The vector-ALU kernels are built for D = 64, 128, 256 and 512; any other
 // even head dim d <= 512 runs padded in the next of them (q zero-padded to
 // D, K/V rows read at their stored length d).
-template <int D, typename T, bool PAGED, bool ROPE>
+template <int D, typename T, bool PAGED, bool ROPE, bool SC>
 int dispatch_pad(int d, int gh, const AttnArgs& a, int span, int nsubs, int B, void* st) {
-  return d == D ? dispatch_gh<D, T, PAGED, ROPE, false>(gh, a, span, nsubs, B, st)
-                : dispatch_gh<D, T, PAGED, ROPE, true>(gh, a, span, nsubs, B, st);
+  return d == D ? dispatch_gh<D, T, PAGED, ROPE, false, SC>(gh, a, span, nsubs, B, st)
+                : dispatch_gh<D, T, PAGED, ROPE, true, SC>(gh, a, span, nsubs, B, st);
 }
 
-template <typename T, bool PAGED, bool ROPE>
+template <typename T, bool PAGED, bool ROPE, bool SC>
 int dispatch_d(int d, int gh, const AttnArgs& a, int span, int nsubs, int B, void* st) {
   if constexpr (sizeof(T) == 1) {  // Q8: 64 and 128 whole take the matrix cores (run_attn)
-    if (d < 64) return dispatch_gh<64, T, PAGED, ROPE, true>(gh, a, span, nsubs, B, st);
-    if (d < 128) return dispatch_gh<128, T, PAGED, ROPE, true>(gh, a, span, nsubs, B, st);
+    if (d < 64) return dispatch_gh<64, T, PAGED, ROPE, true, SC>(gh, a, span, nsubs, B, st);
+    if (d < 128) return dispatch_gh<128, T, PAGED, ROPE, true, SC>(gh, a, span, nsubs, B, st);
   } else {
-    if (d <= 64) return dispatch_pad<64, T, PAGED, ROPE>(d, gh, a, span, nsubs, B, st);
-    if (d <= 128) return dispatch_pad<128, T, PAGED, ROPE>(d, gh, a, span, nsubs, B, st);
+    if (d <= 64) return dispatch_pad<64, T, PAGED, ROPE, SC>(d, gh, a, span, nsubs, B, st);
+    if (d <= 128) return dispatch_pad<128, T, PAGED, ROPE, SC>(d, gh, a, span, nsubs, B, st);
   }
-  if (d <= 256) return dispatch_pad<256, T, PAGED, ROPE>(d, gh, a, span, nsubs, B, st);
-  return dispatch_pad<512, T, PAGED, ROPE>(d, gh, a, span, nsubs, B, st);
+  if (d <= 256) return dispatch_pad<256, T, PAGED, ROPE, SC>(d, gh, a, span, nsubs, B, st);
+  return dispatch_pad<512, T, PAGED, ROPE, SC>(d, gh, a, span, nsubs, B, st);
 }
 
-template <bool PAGED, bool ROPE>
+template <bool PAGED, bool ROPE, bool SC>
 int dispatch_attn(int d, int kv_dtype, int gh, const AttnArgs& a, int span, int nsubs, int B,
                   void* st) {
-  if (kv_dtype == MOLOT_KV_F32) return dispatch_d<float, PAGED, ROPE>(d, gh, a, span, nsubs, B, st);
+  if (kv_dtype == MOLOT_KV_F32) return dispatch_d<float, PAGED, ROPE, SC>(d, gh, a, span, nsubs, B, st);
   if (kv_dtype == MOLOT_KV_Q8)  // 64 and 128 take the matrix cores (run_attn)
-    return dispatch_d<q8_t, PAGED, ROPE>(d, gh, a, span, nsubs, B, st);
-  return dispatch_d<bf16_t, PAGED, ROPE>(d, gh, a, span, nsubs, B, st);
+    return dispatch_d<q8_t, PAGED, ROPE, SC>(d, gh, a, span, nsubs, B, st);
+  return dispatch_d<bf16_t, PAGED, ROPE, SC>(d, gh, a, span, nsubs, B, st);
 }
 
-template <int D, bool PAGED, bool ROPE, bool Q8>
+template <int D, bool PAGED, bool ROPE, bool Q8, bool SC>
 int dispatch_mfma(int gh, const AttnArgs& a, int span, int nsubs, int B, void* st) {
   switch (gh) {
-    case 1: return launch_mfma<D, 1, PAGED, ROPE, Q8>(a, span, nsubs, B, st);
-    case 2: return launch_mfma<D, 2, PAGED, ROPE, Q8>(a, span, nsubs, B, st);
-    case 4: return launch_mfma<D, 4, PAGED, ROPE, Q8>(a, span, nsubs, B, st);
-    case 8: return launch_mfma<D, 8, PAGED, ROPE, Q8>(a, span, nsubs, B, st);
-    case 16: return launch_mfma<D, 16, PAGED, ROPE, Q8>(a, span, nsubs, B, st);
+    case 1: return launch_mfma<D, 1, PAGED, ROPE, Q8, SC>(a, span, nsubs, B, st);
+    case 2: return launch_mfma<D, 2, PAGED, ROPE, Q8, SC>(a, span, nsubs, B, st);
+    case 4: return launch_mfma<D, 4, PAGED, ROPE, Q8, SC>(a, span, nsubs, B, st);
+    case 8: return launch_mfma<D, 8, PAGED, ROPE, Q8, SC>(a, span, nsubs, B, st);
+    case 16: return launch_mfma<D, 16, PAGED, ROPE, Q8, SC>(a, span, nsubs, B, st);
   }
   return MOLOT_EINVAL;
 }
 
-template <bool PAGED, bool ROPE>
+template <bool PAGED, bool ROPE, bool SC>
 int run_attn(AttnArgs& a, int d, int kv_dtype, int span, int B, void* stream) {
   a.dh = d;
   const int G = a.nq / a.nkv;
@@ -162,16 +162,16 @@ int run_attn(AttnArgs& a, int d, int kv_dtype, int span, int B, void* stream) {
     const int gh = G % 16 == 0 ? 16 : pick_gh(G);
     const int nsubs = G / gh;
     if (q8)
-      return d == 64 ? dispatch_mfma<64, PAGED, ROPE, true>(gh, a, span, nsubs, B, stream)
-                     : dispatch_mfma<128, PAGED, ROPE, true>(gh, a, span, nsubs, B, stream);
-    return d == 64 ? dispatch_mfma<64, PAGED, ROPE, false>(gh, a, span, nsubs, B, stream)
-                   : dispatch_mfma<128, PAGED, ROPE, false>(gh, a, span, nsubs, B, stream);
+      return d == 64 ? dispatch_mfma<64, PAGED, ROPE, true, SC>(gh, a, span, nsubs, B, stream)
+                     : dispatch_mfma<128, PAGED, ROPE, true, SC>(gh, a, span, nsubs, B, stream);
+    return d == 64 ? dispatch_mfma<64, PAGED, ROPE, false, SC>(gh, a, span, nsubs, B, stream)
+                   : dispatch_mfma<128, PAGED, ROPE, false, SC>(gh, a, span, nsubs, B, stream);
   }
   // Q8 rows padded to D <= 128 hold 16 q elements a lane per head: at most
   // 4 heads a workgroup there too
   const int gh = d > 256 || (q8 && d < 128) ? std::min(pick_gh(G), kMaxGhWide) : pick_gh(G);
   const int nsubs = G / gh;
-  return dispatch_attn<PAGED, ROPE>(d, kv_dtype, gh, a, span, nsubs, B, stream);
+  return dispatch_attn<PAGED, ROPE, SC>(d, kv_dtype, gh, a, span, nsubs, B, stream);
 }
 
 }  // namespace

@@ -30,6 +30,12 @@ struct PfArgs {
   int nsplit;
   float* part_o;
   float* part_ml;
+  // Scored launches of the 32-row kernels (their SC instances): the scores and the
+  // rows' key ranges as AttnArgs has them
+  float softcap;
+  const float* slopes;
+  const int32_t* key_lo;
+  const int32_t* key_hi;
 };
 
 using PfFn = void (*)(PfArgs);

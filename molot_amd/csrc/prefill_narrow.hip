@@ -45,8 +45,8 @@
 
 namespace {
 
-// OWN: PfArgs::own (prefill_tile.hpp).
-template <int D, int NP, bool OWN>
+// OWN: PfArgs::own (prefill_tile.hpp).  SC: a scored launch (PfArgs::softcap).
+template <int D, int NP, bool OWN, bool SC>
 __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
   static_assert(D == 64 || D == 128, "head dims up to 128");
   constexpr int KT = kWideTile;
@@ -80,14 +80,10 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
   const int rows = a.M * G;
   const int r0 = qb * QB;
   const int rl = min(r0 + QB, rows) - 1;
-  auto t0_of = [&](int m) {
-    const int pos = a.pos0 + m;
-    int t0 = (a.window > 0 && pos - a.window + 1 > 0) ? pos - a.window + 1 : 0;
-    return t0 > a.N ? a.N : t0;
-  };
-  auto nn_of = [&](int m) { return a.pos0 + m + 1 < a.N ? a.pos0 + m + 1 : a.N; };
-  const int kt_lo = t0_of(r0 / G);
-  const int kt_hi = nn_of(rl / G);
+  auto t0_of = [&](int m) { return key_lo_of<SC>(a, m); };
+  auto nn_of = [&](int m) { return key_hi_of<SC>(a, m); };
+  int kt_lo, kt_hi;
+  block_keys<SC>(a, r0 / G, rl / G, kt_lo, kt_hi);
   const int ntile_all = kt_hi > kt_lo ? (kt_hi - kt_lo + KT - 1) / KT : 0;
   const int tb0 = (int)((int64_t)sp * ntile_all / a.nsplit);
   const int ntile = (int)((int64_t)(sp + 1) * ntile_all / a.nsplit) - tb0;
@@ -197,6 +193,9 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
     }
   }
 
+  [[maybe_unused]] RowScore rsc;
+  if constexpr (SC) rsc = row_score(a, m, h * G + g);
+
   f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -268,13 +267,17 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
                       reinterpret_cast<const float*>(unit_buf(1, it & 1, kg))[c32],
                   0.f, mark);
     const bool full = __builtin_amdgcn_ballot_w64(tk < rt0 || tk + KT > rnn) == 0;
-    fac = softmax_tile<16>(
-        x, ku, vu, qunit, rs, full, [](float v) { return max_xor32(v); },
-        [&](int e) {
-          const int t = tk + 8 * (e >> 2) + 4 * hh + (e & 3);
-          return t < rt0 || t >= rnn;
-        },
-        yh, yl);
+    auto slot = [&](int e) { return tk + 8 * (e >> 2) + 4 * hh + (e & 3); };
+    auto gmax = [](float v) { return max_xor32(v); };
+    auto dead = [&](int e) {
+      const int t = slot(e);
+      return t < rt0 || t >= rnn;
+    };
+    if constexpr (SC)
+      fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl,
+                             [&](float (&s)[16]) { rsc.apply<16>(s, slot); });
+    else
+      fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
   };
   // O^T += V^T . P^T of the tile of interval it.  A transposed read's 16-lane
   // group (2*h + x) takes keys 16j + 8u + 4h .. +3 (lane/4 of it) of the
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
   const f32x4 st = ml[c32];
   if constexpr (OWN) {
     if (redo + st[3] != 0.f) {  // wave-uniform
-      own_rows<D>(own_args(), h, r0 + 32 * rg, 32, kt_s, kt_s + ntile * KT, sp);
+      own_rows<D, SC>(own_args(), h, r0 + 32 * rg, 32, kt_s, kt_s + ntile * KT, sp);
       return;
     }
   }
@@ -412,12 +415,20 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
 
 }  // namespace
 
-PfFn prefill_narrow_fn(int D, int kv_dtype, bool own) {
+namespace {
+
+template <int D, bool OWN, bool SC>
+PfFn narrow_fn(bool f32) {
+  return f32 ? prefill_narrow_kernel<D, 2, OWN, SC> : prefill_narrow_kernel<D, 1, OWN, SC>;
+}
+
+}  // namespace
+
+PfFn prefill_narrow_fn(int D, int kv_dtype, bool own, bool scored) {
   const bool f32 = kv_dtype == MOLOT_KV_F32;
-  if (D == 64) {
-    if (own) return f32 ? prefill_narrow_kernel<64, 2, true> : prefill_narrow_kernel<64, 1, true>;
-    return f32 ? prefill_narrow_kernel<64, 2, false> : prefill_narrow_kernel<64, 1, false>;
-  }
-  if (own) return f32 ? prefill_narrow_kernel<128, 2, true> : prefill_narrow_kernel<128, 1, true>;
-  return f32 ? prefill_narrow_kernel<128, 2, false> : prefill_narrow_kernel<128, 1, false>;
+  if (D == 64)
+    return scored ? narrow_fn<64, true, true>(f32)
+                  : own ? narrow_fn<64, true, false>(f32) : narrow_fn<64, false, false>(f32);
+  return scored ? narrow_fn<128, true, true>(f32)
+                : own ? narrow_fn<128, true, false>(f32) : narrow_fn<128, false, false>(f32);
 }

@@ -10,6 +10,7 @@
 #include "molot_amd/attn_hip.h"
 #include "prefill.hpp"
 #include "prefill_wide.hpp"
+#include "score_mod.hpp"
 
 namespace {
 
@@ -148,6 +149,75 @@ __device__ __forceinline__ int64_t own_row_off(const PfArgs& a, int h, int t, in
   return q8 ? wide_row_off<q8_t, false>(a, h, t, soff) : wide_row_off<float, false>(a, h, t, soff);
 }
 
+// The keys [lo, hi) of the query row of token m (SC: a scored launch).
+template <bool SC, typename A>
+__device__ __forceinline__ int key_lo_of(const A& a, int m) {
+  const int pos = a.pos0 + m;
+  int t0 = (a.window > 0 && pos - a.window + 1 > 0) ? pos - a.window + 1 : 0;
+  if constexpr (SC) {
+    if (a.key_lo) t0 = max(t0, a.key_lo[m]);
+  }
+  return t0 > a.N ? a.N : t0;
+}
+template <bool SC, typename A>
+__device__ __forceinline__ int key_hi_of(const A& a, int m) {
+  if constexpr (SC) {
+    if (a.key_hi) return max(0, min(a.key_hi[m], a.N));
+  }
+  return a.pos0 + m + 1 < a.N ? a.pos0 + m + 1 : a.N;
+}
+
+// The keys [lo, hi) that the tokens m0 .. m1 of a block see between them.  With
+// ranges of their own: every lane of the wave takes some, an empty one counts for
+// nothing.
+template <bool SC>
+__device__ __forceinline__ void block_keys(const PfArgs& a, int m0, int m1, int& lo, int& hi) {
+  if (!SC || (!a.key_lo && !a.key_hi)) {
+    lo = key_lo_of<false>(a, m0);
+    hi = key_hi_of<false>(a, m1);
+    return;
+  }
+  int l = a.N, h = 0;
+  for (int m = m0 + (int)(threadIdx.x & 63); m <= m1; m += 64) {
+    const int x = key_lo_of<SC>(a, m), y = key_hi_of<SC>(a, m);
+    if (x < y) {
+      l = min(l, x);
+      h = max(h, y);
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    l = min(l, __shfl_xor(l, off));
+    h = max(h, __shfl_xor(h, off));
+  }
+  lo = __builtin_amdgcn_readfirstlane(l);
+  hi = __builtin_amdgcn_readfirstlane(h);
+}
+
+// A scored launch's scores of one query row: N of them in base-2 units at slots
+// t(e), to the capped and biased ones.
+struct RowScore {
+  float cap2 = 0.f, rcap = 0.f, slope = 0.f;
+  int pos = 0;
+  template <int N, typename SLOT>
+  __device__ __forceinline__ void apply(float (&s)[N], SLOT&& slot) const {
+    if (cap2 > 0.f) cap_scores<N>(s, cap2, rcap);  // wave-uniform
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] = fmaf(-slope, fabsf((float)(pos - slot(e))), s[e]);
+  }
+};
+template <typename A>
+__device__ __forceinline__ RowScore row_score(const A& a, int m, int head) {
+  RowScore r;
+  r.pos = a.pos0 + m;
+  if (a.softcap > 0.f) {
+    r.cap2 = a.softcap * kLog2e;
+    r.rcap = 1.f / r.cap2;
+  }
+  if (a.slopes) r.slope = a.slopes[head] * kLog2e;
+  return r;
+}
+
 // The address of the kernel's arguments (a PfArgs, its only parameter), to be
 // taken in the kernel itself: a called function has no such pointer (the
 // builtin gives null there), so it and own_rows are inlined.
@@ -163,7 +233,7 @@ __device__ __forceinline__ uint64_t own_args() {
 // arguments are read again from args (own_args), where the compiler cannot move
 // the loads ahead: kept in registers through the kernel's loop they would
 // spill.
-template <int D>
+template <int D, bool SC = false>
 __device__ __forceinline__ void own_rows(uint64_t args, int h, int row0, int n, int k_lo, int k_hi,
                                          int sp) {
   const auto* ka = (const __attribute__((address_space(4))) PfArgs*)args;
@@ -172,6 +242,8 @@ __device__ __forceinline__ void own_rows(uint64_t args, int h, int row0, int n, 
   a.nq = ka->nq, a.nkv = ka->nkv, a.M = ka->M, a.N = ka->N, a.pos0 = ka->pos0;
   a.window = ka->window, a.dh = ka->dh, a.page_shift = ka->page_shift, a.scale = ka->scale;
   a.kv_dtype = ka->kv_dtype, a.nsplit = ka->nsplit, a.part_o = ka->part_o, a.part_ml = ka->part_ml;
+  if constexpr (SC)
+    a.softcap = ka->softcap, a.slopes = ka->slopes, a.key_lo = ka->key_lo, a.key_hi = ka->key_hi;
   constexpr int EPL = D / 64;  // elements lane + 64*i of a lane
   const int lane = threadIdx.x & 63;
   const int G = a.nq / a.nkv;
@@ -179,11 +251,12 @@ __device__ __forceinline__ void own_rows(uint64_t args, int h, int row0, int n, 
   const char* kb = reinterpret_cast<const char*>(a.k);
   const char* vb = reinterpret_cast<const char*>(a.v);
   for (int row = row0; row < min(row0 + n, a.M * G); ++row) {
-    const int m = row / G, pos = a.pos0 + m;
+    const int m = row / G;
     const int64_t slot = (int64_t)m * a.nq + h * G + (row - m * G);
-    int lo = (a.window > 0 && pos - a.window + 1 > 0) ? pos - a.window + 1 : 0;
-    lo = max(lo, k_lo);
-    const int hi = min(min(pos + 1, a.N), k_hi);
+    const int lo = max(key_lo_of<SC>(a, m), k_lo);
+    const int hi = min(key_hi_of<SC>(a, m), k_hi);
+    RowScore rsc;
+    if constexpr (SC) rsc = row_score(a, m, h * G + (row - m * G));
     float q[EPL], o[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
@@ -209,7 +282,12 @@ __device__ __forceinline__ void own_rows(uint64_t args, int h, int row0, int n, 
           if (in) acc = fmaf(q[i], own_elem(a, kb, off, e), acc);
           v[u][i] = in ? own_elem(a, vb, off, e) * vs : 0.f;
         }
-        s[u] = t0 + u < hi ? wave_reduce<false>(acc) * (ks * qsc) : -INFINITY;
+        const float x = wave_reduce<false>(acc) * (ks * qsc);
+        s[u] = SC || t0 + u < hi ? x : -INFINITY;
+      }
+      if constexpr (SC) {
+        rsc.apply<2>(s, [&](int u) { return t0 + u; });
+        if (t0 + 1 >= hi) s[1] = -INFINITY;
       }
       const float mn = fmaxf(mx, fmaxf(s[0], s[1]));
       if (mn > mx) {
@@ -288,16 +366,27 @@ __device__ __forceinline__ float div_by(float o, float l, float inv) {
 // follows o down with it, and is lowered where y would pass 2^14, by kRoom
 // bits more than needed, so that the next records of 32 rows do not each
 // rescale o.
-template <int NK, typename GMAX, typename DEAD>
+//
+// mod(s): the scores in base-2 units past the product (NoMod: as they are).
+struct NoMod {};
+template <int NK, typename GMAX, typename DEAD, typename MOD = NoMod>
 __device__ __forceinline__ float softmax_tile(float (&s)[NK], const float (&ku)[NK],
-                                              const float (&vu)[NK], float qunit, RowState& st,
+                                              const float (&vu)[NK], float unit, RowState& st,
                                               bool full, GMAX&& gmax, DEAD&& dead,
-                                              uint32_t (&yh)[NK / 2], uint32_t (&yl)[NK / 2]) {
+                                              uint32_t (&yh)[NK / 2], uint32_t (&yl)[NK / 2],
+                                              MOD&& mod = MOD{}) {
+  constexpr bool SC = !std::is_same<typename std::decay<MOD>::type, NoMod>::value;
+  const float qunit = SC ? 1.f : unit;
   constexpr int kRoom = 3;
   constexpr int kNoShift = 1 << 20;
   float ps, zt, z[NK];
 #pragma unroll
   for (int e = 0; e < NK; ++e) s[e] *= ku[e];
+  if constexpr (SC) {
+#pragma unroll
+    for (int e = 0; e < NK; ++e) s[e] *= unit;
+    mod(s);
+  }
   if (!full) {
 #pragma unroll
     for (int e = 0; e < NK; ++e) s[e] = dead(e) ? -INFINITY : s[e];

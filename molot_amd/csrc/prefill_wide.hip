@@ -96,7 +96,8 @@ __global__ __launch_bounds__(256) void wide_split_kernel(PfArgs a, uint16_t* out
         (kv ? f16_vrow_unit(xm, shift) : f16_row_unit(shift)) * s + mark;
 }
 
-template <int D, int NP>
+// SC: a scored launch (PfArgs::softcap).
+template <int D, int NP, bool SC>
 __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   constexpr int KT = kWideTile;
   constexpr int NSL = D / 128;       // slices of the head dim
@@ -104,14 +105,14 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   constexpr int QB = 32 * RG;        // query rows a workgroup
   constexpr int RPO = 32 / NSL;      // rows of its group a wave owns in the softmax
   constexpr int LPR = 64 / RPO;      // lanes of an owned row
-  constexpr int KPL = KT / LPR;      // keys a lane of it holds
+  constexpr int KPL = KT / LPR;      // keys a lane of it holds (4 or 8)
   constexpr int RB = 2 * D;          // bytes of a staged row of one piece
   constexpr int TB = NP * KT * RB;   // bytes of a staged tile (K or V)
   constexpr int SXB = 8 * 4096;      // score shares, then P (8 owner regions)
   constexpr bool DB = 4 * TB + SXB <= 160 * 1024;  // two buffers of K and of V
   constexpr int NB = DB ? 2 : 1;
   constexpr int NL = TB / 1024 / 8;  // 1 KB copies a wave issues per K or V tile
-  static_assert(NSL == 4 && KPL == 4, "the layout of the shares and of P");
+  static_assert((NSL == 4 && KPL == 4) || (NSL == 2 && KPL == 8), "the layout of the shares and of P");
   static_assert(2 * NB * TB + SXB <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(16))) char kbuf[NB][TB];
   __shared__ __attribute__((aligned(16))) char vbuf[NB][TB];
@@ -129,14 +130,10 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   const int rows = a.M * G;
   const int r0 = qb * QB;
   const int rl = min(r0 + QB, rows) - 1;
-  auto t0_of = [&](int m) {
-    const int pos = a.pos0 + m;
-    int t0 = (a.window > 0 && pos - a.window + 1 > 0) ? pos - a.window + 1 : 0;
-    return t0 > a.N ? a.N : t0;
-  };
-  auto nn_of = [&](int m) { return a.pos0 + m + 1 < a.N ? a.pos0 + m + 1 : a.N; };
-  const int kt_lo = t0_of(r0 / G);
-  const int kt_hi = nn_of(rl / G);
+  auto t0_of = [&](int m) { return key_lo_of<SC>(a, m); };
+  auto nn_of = [&](int m) { return key_hi_of<SC>(a, m); };
+  int kt_lo, kt_hi;
+  block_keys<SC>(a, r0 / G, rl / G, kt_lo, kt_hi);
   const int ntile_all = kt_hi > kt_lo ? (kt_hi - kt_lo + KT - 1) / KT : 0;
   const int tb0 = (int)((int64_t)sp * ntile_all / a.nsplit);
   const int ntile = (int)((int64_t)(sp + 1) * ntile_all / a.nsplit) - tb0;
@@ -227,12 +224,14 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   const int orr = lane / LPR, oc = lane % LPR;
   int rt0, rnn;
   float qunit;
+  [[maybe_unused]] RowScore rsc;
   {
     const int row = r0 + 32 * rg + RPO * sl + orr;
     const bool orv = row < rows;
     const int m = orv ? row / G : 0;
     rt0 = orv ? t0_of(m) : 0;  // a row past the last: any keys (not stored)
     rnn = orv ? nn_of(m) : 0x7FFFFFFF;
+    if constexpr (SC) rsc = row_score(a, m, h * G + (orv ? row - m * G : 0));
     const float* qmx = reinterpret_cast<const float*>(sx);
     float qm = 0.f;
 #pragma unroll
@@ -253,28 +252,33 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   // hit distinct units; then, read by its owner alone, overwritten with P:
   // [piece][key octet][row] 16 bytes, and the rows' (alpha, dsh).
   auto region = [&](int ow) { return sx + (rg * NSL + ow) * 4096; };
-  auto swz = [](int rr) { return rr & 7; };
+  auto swz = [](int rr) {
+    return NSL == 4 ? rr & 7 : ((rr >> 1) & 1) | ((rr & 1) << 1) | (rr & 4);
+  };
   const int my_ow = c32 / RPO, my_rr = c32 % RPO;  // this lane's MFMA column
   char* s_st = region(my_ow) + sl * (RPO * 128) + my_rr * 128;
   const int s_sw = 16 * (hh ^ swz(my_rr));
   const char* s_ld = region(sl) + orr * 128;
   const int o_sw = 16 * swz(orr);
-  const char* p_ld = region(my_ow) + (my_ow & 1) * 128 + my_rr * 16;
-  char* p_st = region(sl) + (sl & 1) * 128 + orr * 16;
+  const char* p_ld = region(my_ow) + (NSL == 4 ? (my_ow & 1) * 128 : 0) + my_rr * 16;
+  char* p_st = region(sl) + (NSL == 4 ? (sl & 1) * 128 : 0) + orr * 16;
 
   const float* kun = reinterpret_cast<const float*>(khead + NP * Rp * D) - a.T0 + KPL * oc;
   const float* vun = reinterpret_cast<const float*>(vhead + NP * Rp * D) - a.T0 + KPL * oc;
   float ku[KPL], vu[KPL];
   auto load_units = [&](int tk) {
-    const f32x4_u x = *reinterpret_cast<const f32x4_u*>(kun + tk);
-    const f32x4_u y = *reinterpret_cast<const f32x4_u*>(vun + tk);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      ku[e] = x[e];
-      vu[e] = y[e];
+    for (int q = 0; q < KPL; q += 4) {
+      const f32x4_u x = *reinterpret_cast<const f32x4_u*>(kun + tk + q);
+      const f32x4_u y = *reinterpret_cast<const f32x4_u*>(vun + tk + q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ku[q + e] = x[e];
+        vu[q + e] = y[e];
+      }
     }
   };
-  float mark = 0.f;  // NaN once a tile's units held one (a row's 8 lanes hold all its keys)
+  float mark = 0.f;  // NaN once a tile's units held one (a row's lanes hold all its keys)
   if (ntile > 0) load_units(kt_s);
   wait_vmcnt<0>();
   __syncthreads();
@@ -342,16 +346,18 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
     };
     {  // 2. softmax of the owned rows
       float sv[KPL];
-      {
+#pragma unroll
+      for (int q = 0; q < KPL; q += 4) {
+        const int un = 16 * ((KPL / 4) * oc + q / 4);
         f32x4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < NSL; ++s) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(s_ld + s * (RPO * 128) + (16 * oc ^ o_sw));
+          const f32x4 y = *reinterpret_cast<const f32x4*>(s_ld + s * (RPO * 128) + (un ^ o_sw));
           t = s ? t + y : y;
         }
-        next_k(0);
+        if (q == 0) next_k(0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sv[e] = t[e];
+        for (int e = 0; e < 4; ++e) sv[q + e] = t[e];
       }
       const int k0 = tk + KPL * oc;
       const bool full = __builtin_amdgcn_ballot_w64(tk < rt0 || tk + KT > rnn) == 0;
@@ -359,14 +365,26 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
 #pragma unroll
       for (int e = 0; e < KPL; ++e) mark = fmaf(ku[e] + vu[e], 0.f, mark);
       uint32_t yh[KPL / 2], yl[KPL / 2];
-      const float fac = softmax_tile<KPL>(
-          sv, ku, vu, qunit, rs, full, [](float x) { return group_max<LPR>(x); },
-          [&](int e) { return k0 + e < rt0 || k0 + e >= rnn; }, yh, yl);
+      float fac;
+      auto gmax = [](float x) { return group_max<LPR>(x); };
+      auto dead = [&](int e) { return k0 + e < rt0 || k0 + e >= rnn; };
+      if constexpr (SC)
+        fac = softmax_tile<KPL>(sv, ku, vu, qunit, rs, full, gmax, dead, yh, yl, [&](float (&s)[KPL]) {
+          rsc.template apply<KPL>(s, [&](int e) { return k0 + e; });
+        });
+      else
+        fac = softmax_tile<KPL>(sv, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
       next_k(2);
       next_k(3);
-      char* d = p_st + (oc >> 1) * 256 + (oc & 1) * 8;
-      *reinterpret_cast<u32x2*>(d) = u32x2{yh[0], yh[1]};
-      *reinterpret_cast<u32x2*>(d + 1024) = u32x2{yl[0], yl[1]};
+      if constexpr (KPL == 4) {
+        char* d = p_st + (oc >> 1) * 256 + (oc & 1) * 8;
+        *reinterpret_cast<u32x2*>(d) = u32x2{yh[0], yh[1]};
+        *reinterpret_cast<u32x2*>(d + 1024) = u32x2{yl[0], yl[1]};
+      } else {
+        char* d = p_st + oc * 256;
+        *reinterpret_cast<u32x4*>(d) = u32x4{yh[0], yh[1], yh[KPL / 2 - 2], yh[KPL / 2 - 1]};
+        *reinterpret_cast<u32x4*>(d + 1024) = u32x4{yl[0], yl[1], yl[KPL / 2 - 2], yl[KPL / 2 - 1]};
+      }
       if (oc == 0)
         *reinterpret_cast<f32x4*>(region(sl) + 2048 + 16 * orr) = f32x4{fac, 0.f, 0.f, 0.f};
     }
@@ -444,7 +462,7 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
 
   // (every wave met the same units: the workgroup decides alike)
   if (__builtin_amdgcn_ballot_w64(mark != 0.f) != 0) {
-    own_rows<D>(own_args(), h, r0 + (QB / 8) * w, QB / 8, kt_s, kt_s + ntile * KT, sp);
+    own_rows<D, SC>(own_args(), h, r0 + (QB / 8) * w, QB / 8, kt_s, kt_s + ntile * KT, sp);
     return;
   }
   // the rows' (l, m, wsh) from their owners to the waves that hold their o
@@ -512,10 +530,15 @@ SplitFn prefill_wide_split(int D, int kv_dtype, bool paged) {
   };
   if (D == 64) return of(std::integral_constant<int, 64>{});
   if (D == 128) return of(std::integral_constant<int, 128>{});
+  if (D == 256) return of(std::integral_constant<int, 256>{});
   return of(std::integral_constant<int, 512>{});
 }
 
-PfFn prefill_wide_fn(int D, int kv_dtype) {
+PfFn prefill_wide_fn(int D, int kv_dtype, bool scored) {
+  const bool f32 = kv_dtype == MOLOT_KV_F32;
+  if (D == 256 && scored)
+    return f32 ? prefill_wide_kernel<256, 2, true> : prefill_wide_kernel<256, 1, true>;
   if (D != 512) return nullptr;
-  return kv_dtype == MOLOT_KV_F32 ? prefill_wide_kernel<512, 2> : prefill_wide_kernel<512, 1>;
+  if (scored) return f32 ? prefill_wide_kernel<512, 2, true> : prefill_wide_kernel<512, 1, true>;
+  return f32 ? prefill_wide_kernel<512, 2, false> : prefill_wide_kernel<512, 1, false>;
 }

@@ -19,7 +19,7 @@ constexpr int wide_pieces_v = sizeof(T) == 4 ? 2 : 1;
 inline int wide_pieces(bool f32) { return f32 ? 2 : 1; }
 
 // Query rows of a workgroup.
-constexpr int wide_rows(int D) { return D <= 128 ? 128 : 64; }
+constexpr int wide_rows(int D) { return D <= 256 ? 128 : 64; }
 
 // Workspace of R attended rows, per K and V and KV head: [pieces][Rp][D] fp16,
 // then the rows' units [Rp] floats (Rp rows: the tail, and heads stay 16-byte
@@ -35,9 +35,10 @@ inline size_t wide_bytes(int nkv, int D, int np, int64_t R) {
 }
 
 // The split of the cached rows, and the attention kernels over the pieces:
-// prefill_narrow.hip (D = 64 and 128), prefill_wide.hip (D = 512).
-PfFn prefill_narrow_fn(int D, int kv_dtype, bool own) __attribute__((visibility("hidden")));
+// prefill_narrow.hip (D = 64 and 128), prefill_wide.hip (D = 512; scored, 256 too).
+PfFn prefill_narrow_fn(int D, int kv_dtype, bool own, bool scored)
+    __attribute__((visibility("hidden")));
 SplitFn prefill_wide_split(int D, int kv_dtype, bool paged) __attribute__((visibility("hidden")));
-PfFn prefill_wide_fn(int D, int kv_dtype) __attribute__((visibility("hidden")));
+PfFn prefill_wide_fn(int D, int kv_dtype, bool scored) __attribute__((visibility("hidden")));
 
 #endif  // MOLOT_AMD_CSRC_PREFILL_WIDE_HPP_

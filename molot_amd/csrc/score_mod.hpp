@@ -1,0 +1,55 @@
+// Attention scores past the dot product: a cap by tanh and a bias by distance.
+#ifndef MOLOT_AMD_CSRC_SCORE_MOD_HPP_
+#define MOLOT_AMD_CSRC_SCORE_MOD_HPP_
+
+#include <hip/hip_runtime.h>
+
+#include "device_util.hpp"
+
+namespace {
+
+// Scores s in base-2 units (times log2 e) to c * tanh(s / c), c = cap * log2 e.
+//
+// With x = s / c, c * tanh(x) = s + s * x^2 * P(x^2): near 0 the result keeps s's
+// own bits, where cap * tanh(s / cap) would lose some to a division and two more
+// roundings.  P is of degree 4, fitted for this bound (least squares, reweighted
+// until the relative errors were even) on |x| < 0.625: 4.4e-9 of tanh, below
+// fp32's half step.  Past it c * (1 - 2 / (1 + e^(2|x|))), whose subtraction
+// loses at most a bit there.  It is formed only where a lane of the wave has such
+// a score: the scores of capped layers are mostly some tenths of the cap.  An
+// infinity ends at +-c, a NaN stays one.
+template <int N>
+__device__ __forceinline__ void cap_scores(float (&s)[N], float cap2, float rcap) {
+  constexpr float kSmall = 0.625f;
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) big = fmaxf(big, fabsf(s[i]));
+  if (__builtin_amdgcn_ballot_w64(big * rcap >= kSmall) == 0) {  // wave-uniform
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float x = s[i] * rcap, y = x * x;
+      float p = fmaf(-0.00570497056f, y, 0.0206390712f);
+      p = fmaf(p, y, -0.0537397079f);
+      p = fmaf(p, y, 0.133314416f);
+      p = fmaf(p, y, -0.333332807f);
+      s[i] = fmaf(s[i] * y, p, s[i]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float x = fabsf(s[i] * rcap), y = x * x;
+    float p = fmaf(-0.00570497056f, y, 0.0206390712f);
+    p = fmaf(p, y, -0.0537397079f);
+    p = fmaf(p, y, 0.133314416f);
+    p = fmaf(p, y, -0.333332807f);
+    const float near = fmaf(s[i] * y, p, s[i]);
+    const float e = exp2_hw(x * (2.f * kLog2e));  // an infinity's reciprocal is 0
+    const float far = copysignf(fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + e), cap2), s[i]);
+    s[i] = x >= kSmall ? far : near;  // (a NaN takes the series, and stays one)
+  }
+}
+
+}  // namespace
+
+#endif  // MOLOT_AMD_CSRC_SCORE_MOD_HPP_

@@ -38,6 +38,27 @@ _I64 = ctypes.c_int64
 
 # name -> argtypes (all return int status unless listed in _VOID / _STR)
 _SIGS = {
+    "molot_hip_attn_decode_scored": [_P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _F, _P, _P, _I, _I,
+                                     _P],
+    "molot_hip_decode_step_scored": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P,
+                                     _F, _I, _F, _P, _P, _P, _I, _I, _P],
+    "molot_hip_attn_decode_paged_scored": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
+                                           _F, _I, _F, _P, _P, _I, _P],
+    "molot_hip_decode_step_paged_scored": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
+                                           _I, _I, _P, _P, _I, _F, _P, _F, _I, _F, _P, _P, _P, _I,
+                                           _P],
+    "molot_hip_attn_prefill_scored": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _F, _P, _P, _P,
+                                      _I, _P],
+    "molot_hip_attn_prefill_paged_scored": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I,
+                                            _I, _F, _P, _P, _P, _I, _P],
+    "molot_hip_prefill_step_scored": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _F,
+                                      _P, _F, _I, _F, _P, _P, _P, _I, _P],
+    "molot_hip_prefill_step_paged_scored": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
+                                            _I, _P, _P, _I, _F, _P, _F, _I, _F, _P, _P, _P, _I, _P],
+    "molot_hip_kv_track": [_P, _P, _I, _I, _I, _I, _I, _P],
+    "molot_hip_kv_track_paged": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+    "molot_hip_kv_evict": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
+    "molot_hip_kv_evict_paged": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "molot_hip_rope_apply": [_P, _I, _I, _I, _P, _P],
     "molot_hip_rope_append": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P],
     "molot_hip_attn_decode_gqa_cache": [_P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P],

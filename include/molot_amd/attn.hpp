@@ -201,6 +201,15 @@ struct LayerNorms {
   float eps = 1e-6f;
 };
 
+// A layer's scores past the product (attn_hip.h: scored attention; no reference
+// counterpart): slopes, key_lo and key_hi are device tables.
+struct Scores {
+  float softcap = 0.f;
+  const float* slopes = nullptr;    // [nq]
+  const int32_t* key_lo = nullptr;  // prefill: [M]
+  const int32_t* key_hi = nullptr;
+};
+
 // Device KV cache of one layer (Runner::KVC, forward.h:48-51) with the
 // decode-attention block of forward.h:554-591 in one fused launch, the
 // layer prefill (forward.h:367-399), and the same blocks for layers that
@@ -225,6 +234,8 @@ class DeviceKV {
   ~DeviceKV() {
     if (k) (void)hipFree(k);
     if (v) (void)hipFree(v);
+    if (acc) (void)hipFree(acc);
+    if (slot_pos) (void)hipFree(slot_pos);
   }
   DeviceKV(const DeviceKV&) = delete;
   DeviceKV& operator=(const DeviceKV&) = delete;
@@ -259,6 +270,7 @@ class DeviceKV {
                                   inv_freq, scale, window, kv_dtype, s),
             "decode_step");
     ++n;
+    track(1, pos, s);
     view.finish();
   }
 
@@ -291,6 +303,7 @@ class DeviceKV {
                                  kv_dtype, s),
           "prefill_step");
     n += M;
+    track(M, pos0 + M - 1, s);
   }
 
   // forward.h:367-399 for a layer without its own KV reading this cache
@@ -317,6 +330,65 @@ class DeviceKV {
     view.finish();
   }
 
+  // ---- scored layers and a cache held to a budget (no reference counterpart) ----
+
+  // decode() with the layer's Scores.  With track_weights() on, the step's weights
+  // are added to acc and the new row's position kept.
+  void decode_scored(float* q, const float* knew, const float* vnew, float* ao, int nq, int pos,
+                     const float* inv_freq, float scale, int window, const LayerNorms& nm,
+                     const Scores& sc, hipStream_t s = nullptr) {
+    if (n >= cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:570
+    const size_t qf = (size_t)nq * hd, kf = (size_t)nkv * hd;
+    CallStage view(q, true, ao, qf, qf, s, knew, vnew, kf);
+    check(molot_hip_decode_step_scored(view.q, view.k, view.v, k, v, view.o, nq, nkv, hd, n, pos,
+                                       nm.q_norm, nm.k_norm, nm.v_norm ? 1 : 0, nm.eps, inv_freq,
+                                       scale, window, sc.softcap, sc.slopes, acc, slot_pos, cap,
+                                       kv_dtype, s),
+          "decode_step_scored");
+    ++n;
+    view.finish();
+  }
+
+  // prefill() with the layer's Scores and key ranges; device pointers, asynchronous.
+  void prefill_scored(float* Q, const float* K_new, const float* V_new, float* AO, int nq, int M,
+                      int pos0, const float* inv_freq, float scale, int window,
+                      const LayerNorms& nm, const Scores& sc, hipStream_t s = nullptr) {
+    if (n + M > cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:385
+    check(molot_hip_prefill_step_scored(Q, K_new, V_new, k, v, AO, nq, nkv, hd, M, n, pos0,
+                                        nm.q_norm, nm.k_norm, nm.v_norm ? 1 : 0, nm.eps, inv_freq,
+                                        scale, window, sc.softcap, sc.slopes, sc.key_lo, sc.key_hi,
+                                        kv_dtype, s),
+          "prefill_step_scored");
+    n += M;
+    track(M, pos0 + M - 1, s);
+  }
+
+  // Keep every slot's weight and position from here on (an empty cache).
+  void track_weights() {
+    if (acc) return;
+    if (n) throw std::runtime_error("DeviceKV: track_weights on a cache in use");
+    const size_t slots = (size_t)nkv * cap;
+    check_hip(hipMalloc((void**)&acc, slots * sizeof(float)), "hipMalloc acc");
+    check_hip(hipMalloc((void**)&slot_pos, slots * sizeof(int32_t)), "hipMalloc slot_pos");
+  }
+
+  // The cache cut to `keep` slots: the `recent` newest positions (pos: the newest
+  // token's), then the highest weights.
+  void evict(int keep, int recent, int pos, hipStream_t s = nullptr) {
+    if (!acc) throw std::runtime_error("DeviceKV: evict without track_weights");
+    check(molot_hip_kv_evict(k, v, acc, slot_pos, nkv, n, hd, keep, recent, pos, cap, kv_dtype, s),
+          "kv_evict");
+    if (keep < n) n = keep;
+  }
+
+  float* acc = nullptr;         // [nkv][cap] (track_weights)
+  int32_t* slot_pos = nullptr;  // [nkv][cap]
+
+ private:
+  // The last M rows are new, the newest at pos.
+  void track(int M, int pos, hipStream_t s) {
+    if (acc) check(molot_hip_kv_track(acc, slot_pos, nkv, n, M, pos, cap, s), "kv_track");
+  }
 };
 
 }  // namespace molot::amd

@@ -351,6 +351,8 @@ int molot_hip_decode_step_paged_scored(
  * scored, with the keys of every row as a range: row m attends [lo_m, hi_m),
  *   lo_m = max(the window's start, key_lo[m])    (key_lo NULL: the window's)
  *   hi_m = min(key_hi[m], N)                     (key_hi NULL: pos0 + m + 1)
+ * (the steps: min(pos0, slot0) in place of pos0, there and as i, so that no row
+ * sees the rows appended after it in a cache that was cut by molot_hip_kv_evict).
  * key_lo, key_hi: device int32 [M], any values (an empty range gives O = 0).
  * So a packed prompt's documents keep to themselves (key_lo: the first slot
  * of the row's document), a prefix sees itself both ways (key_hi: at least

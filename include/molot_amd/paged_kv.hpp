@@ -50,6 +50,8 @@ class PagedKVCache {
                       : (size_t)num_blocks * nkv * page * hd * esz;
     k_.assign(layers, nullptr);
     v_.assign(layers, nullptr);
+    acc_.assign(layers, nullptr);
+    slot_pos_.assign(layers, nullptr);
     for (int l = 0; l < layers; ++l) {
       check_hip(hipMalloc(&k_[l], pool_bytes_), "hipMalloc K pages");
       check_hip(hipMalloc(&v_[l], pool_bytes_), "hipMalloc V pages");
@@ -60,6 +62,10 @@ class PagedKVCache {
     for (void* p : k_)
       if (p) (void)hipFree(p);
     for (void* p : v_)
+      if (p) (void)hipFree(p);
+    for (float* p : acc_)
+      if (p) (void)hipFree(p);
+    for (int32_t* p : slot_pos_)
       if (p) (void)hipFree(p);
     if (d_table_) (void)hipFree(d_table_);
     if (h_table_) (void)hipHostFree(h_table_);
@@ -86,6 +92,8 @@ class PagedKVCache {
     s = Seq{};
   }
   int length(int id) const { return seq(id).len; }
+  // The position of the sequence's next token: its length, and the rows evicted.
+  int position(int id) const { return seq(id).len + seq(id).gone; }
   int free_blocks() const { return (int)free_.size(); }
   const std::vector<int>& blocks(int id) const { return seq(id).blocks; }
 
@@ -115,10 +123,11 @@ class PagedKVCache {
               hipStream_t s = nullptr) {
     if (mode_ != Mode::Decode) throw std::runtime_error("PagedKVCache: decode outside a step");
     check(molot_hip_decode_step_paged_norm(
-              q, k, v, k_.at(layer), v_.at(layer), o, d_table_, d_lens_, nullptr,
+              q, k, v, k_.at(layer), v_.at(layer), o, d_table_, d_lens_, pos_array(),
               (int)batch_.size(), maxb_, max_len_, nq, nkv_, hd_, page_, nm.q_norm, nm.k_norm,
               nm.v_norm ? 1 : 0, nm.eps, inv_freq, scale, window, kv_dtype_, s),
           "decode_step_paged");
+    track(layer, 1, s);
   }
   // forward.h:554-558, 578-591 for a layer without its own KV (L.has_kv
   // false) reading layer `src`'s pages: q normed and rotated in place
@@ -129,10 +138,23 @@ class PagedKVCache {
                      hipStream_t s = nullptr) const {
     if (mode_ != Mode::Decode) throw std::runtime_error("PagedKVCache: decode outside a step");
     check(molot_hip_decode_step_paged_shared(
-              q, k_.at(src), v_.at(src), o, d_table_, d_lens_, nullptr, (int)batch_.size(), maxb_,
-              max_len_, nq, nkv_, hd_, page_, nm.q_norm, nm.eps, inv_freq, scale, window,
+              q, k_.at(src), v_.at(src), o, d_table_, d_lens_, pos_array(), (int)batch_.size(),
+              maxb_, max_len_, nq, nkv_, hd_, page_, nm.q_norm, nm.eps, inv_freq, scale, window,
               kv_dtype_, s),
           "decode_step_paged_shared");
+  }
+  // decode() with the layer's Scores; with track_weights() on, the step's weights are
+  // added to the layer's acc and the new rows' positions kept.
+  void decode_scored(int layer, float* q, const float* k, const float* v, float* o, int nq,
+                     const float* inv_freq, float scale, int window, const LayerNorms& nm,
+                     const Scores& sc, hipStream_t s = nullptr) {
+    if (mode_ != Mode::Decode) throw std::runtime_error("PagedKVCache: decode outside a step");
+    check(molot_hip_decode_step_paged_scored(
+              q, k, v, k_.at(layer), v_.at(layer), o, d_table_, d_lens_, pos_array(),
+              (int)batch_.size(), maxb_, max_len_, nq, nkv_, hd_, page_, nm.q_norm, nm.k_norm,
+              nm.v_norm ? 1 : 0, nm.eps, inv_freq, scale, window, sc.softcap, sc.slopes,
+              acc_.at(layer), slot_pos_.at(layer), kv_dtype_, s),
+          "decode_step_paged_scored");
   }
   // The batch's token is in every layer's pages: lengths advance by one.
   void end_decode() {
@@ -164,6 +186,7 @@ class PagedKVCache {
                                        pos0, nm.q_norm, nm.k_norm, nm.v_norm ? 1 : 0, nm.eps,
                                        inv_freq, scale, window, kv_dtype_, s),
           "prefill_step_paged");
+    track(layer, prefill_m_, s);
   }
   // forward.h:367-399 for a layer without its own KV reading layer `src`'s
   // pages: the prompt's q [M][nq][hd] normed and rotated in place, causal
@@ -180,6 +203,18 @@ class PagedKVCache {
                                        scale, pos0, window, kv_dtype_, s),
           "attn_prefill_paged");
   }
+  // prefill() with the layer's Scores and key ranges (device [M]).
+  void prefill_scored(int layer, float* q, const float* k, const float* v, float* o, int nq,
+                      int pos0, const float* inv_freq, float scale, int window,
+                      const LayerNorms& nm, const Scores& sc, hipStream_t s = nullptr) {
+    if (mode_ != Mode::Prefill) throw std::runtime_error("PagedKVCache: prefill outside a step");
+    check(molot_hip_prefill_step_paged_scored(
+              q, k, v, k_.at(layer), v_.at(layer), o, d_table_, maxb_, page_, nq, nkv_, hd_,
+              prefill_m_, seq(batch_[0]).len, pos0, nm.q_norm, nm.k_norm, nm.v_norm ? 1 : 0, nm.eps,
+              inv_freq, scale, window, sc.softcap, sc.slopes, sc.key_lo, sc.key_hi, kv_dtype_, s),
+          "prefill_step_paged_scored");
+    track(layer, prefill_m_, s);
+  }
   void end_prefill() {
     if (mode_ != Mode::Prefill) throw std::runtime_error("PagedKVCache: no prefill step to end");
     seq(batch_[0]).len += prefill_m_;
@@ -187,7 +222,57 @@ class PagedKVCache {
     mode_ = Mode::None;
   }
 
+  // ---- a budget of rows a sequence ----
+  // Keep every slot's weight and position from here on, in every layer (call it
+  // before the first sequence's rows).
+  void track_weights() {
+    if (acc_[0]) return;
+    for (const Seq& s : seqs_)
+      if (s.live && s.len) throw std::runtime_error("PagedKVCache: track_weights on a cache in use");
+    const size_t slots = (size_t)nblocks_ * nkv_ * page_;
+    for (int l = 0; l < layers_; ++l) {
+      check_hip(hipMalloc((void**)&acc_[l], slots * sizeof(float)), "hipMalloc acc");
+      check_hip(hipMalloc((void**)&slot_pos_[l], slots * sizeof(int32_t)), "hipMalloc slot_pos");
+    }
+  }
+  // Every sequence of ids that is longer than keep is cut to it, in every layer and
+  // KV head by itself: its `recent` newest positions, then the highest weights.  The
+  // blocks past the budget return to the pool.
+  void evict(const std::vector<int>& ids, int keep, int recent, hipStream_t s = nullptr) {
+    if (mode_ != Mode::None) throw std::runtime_error("PagedKVCache: a step is in progress");
+    if (!acc_[0]) throw std::runtime_error("PagedKVCache: evict without track_weights");
+    if (keep < 0 || recent < 0) throw std::runtime_error("PagedKVCache: bad budget");
+    if (ids.empty()) return;
+    std::vector<int32_t> lens(ids.size());
+    int maxb = 1;
+    for (size_t i = 0; i < ids.size(); ++i) {
+      for (size_t j = 0; j < i; ++j)
+        if (ids[j] == ids[i]) throw std::runtime_error("PagedKVCache: a sequence twice");
+      lens[i] = seq(ids[i]).len;
+      maxb = std::max(maxb, (int)seq(ids[i]).blocks.size());
+    }
+    upload(ids, maxb, lens, s);
+    for (int l = 0; l < layers_; ++l)
+      check(molot_hip_kv_evict_paged(k_[l], v_[l], acc_[l], slot_pos_[l], d_table_, d_lens_, d_pos_,
+                                     (int)ids.size(), maxb_, max_len_, nkv_, hd_, page_, keep,
+                                     recent, kv_dtype_, s),
+            "kv_evict_paged");
+    for (int id : ids) {
+      Seq& q = seq(id);
+      if (q.len <= keep) continue;
+      q.gone += q.len - keep;
+      q.len = keep;
+      const size_t need = (size_t)(keep + page_ - 1) / page_;
+      while (q.blocks.size() > need) {
+        free_.push_back(q.blocks.back());
+        q.blocks.pop_back();
+      }
+    }
+  }
+
   // ---- device views (tests, other kernels) ----
+  float* acc_pages(int layer) const { return acc_.at(layer); }
+  int32_t* slot_pos_pages(int layer) const { return slot_pos_.at(layer); }
   void* k_pages(int layer) const { return k_.at(layer); }
   void* v_pages(int layer) const { return v_.at(layer); }
   int layers() const { return layers_; }
@@ -199,6 +284,7 @@ class PagedKVCache {
   struct Seq {
     bool live = false;
     int len = 0;
+    int gone = 0;  // rows evicted: the next token's position is len + gone
     std::vector<int> blocks;
   };
   enum class Mode { None, Decode, Prefill };
@@ -213,6 +299,15 @@ class PagedKVCache {
       throw std::runtime_error("PagedKVCache: no such sequence");
     return seqs_[id];
   }
+  // The batch's last M rows of a layer are new.
+  void track(int layer, int M, hipStream_t s) {
+    if (acc_.at(layer))
+      check(molot_hip_kv_track_paged(acc_[layer], slot_pos_[layer], d_table_, d_lens_, d_pos_,
+                                     (int)batch_.size(), maxb_, max_len_, M, nkv_, page_, s),
+            "kv_track_paged");
+  }
+  // The batch's positions where a sequence's differ from its slots.
+  const int32_t* pos_array() const { return cut_ ? d_pos_ : nullptr; }
   // Blocks for `tokens` more tokens of sequence id, from the shared pool.
   void reserve(int id, int tokens) {
     Seq& s = seq(id);
@@ -229,7 +324,7 @@ class PagedKVCache {
   void upload(const std::vector<int>& ids, int maxb, const std::vector<int32_t>& lens,
               hipStream_t s) {
     const size_t B = ids.size();
-    const size_t n = B * maxb + B, bytes = n * sizeof(int32_t);
+    const size_t n = B * maxb + 2 * B, bytes = n * sizeof(int32_t);
     if (uploaded_) check_hip(hipEventSynchronize(uploaded_), "hipEventSynchronize");
     if (bytes > table_cap_) {
       // the previous step's kernels may still read the old table
@@ -244,8 +339,11 @@ class PagedKVCache {
     }
     std::fill(h_table_, h_table_ + n, 0);
     max_len_ = 0;
+    cut_ = false;
     for (size_t i = 0; i < B; ++i) {
       const Seq& q = seq(ids[i]);
+      h_table_[B * maxb + B + i] = lens[i] - 1 + q.gone;  // the newest token's position
+      cut_ = cut_ || q.gone > 0;
       for (size_t j = 0; j < q.blocks.size(); ++j) h_table_[i * maxb + j] = q.blocks[j];
       h_table_[B * maxb + i] = lens[i];
       max_len_ = std::max(max_len_, (int)lens[i]);
@@ -255,12 +353,15 @@ class PagedKVCache {
     if (!uploaded_) check_hip(hipEventCreate(&uploaded_), "hipEventCreate");
     check_hip(hipEventRecord(uploaded_, s), "hipEventRecord");
     d_lens_ = d_table_ + B * maxb;
+    d_pos_ = d_lens_ + B;
     maxb_ = maxb;
   }
 
   int layers_, nblocks_, nkv_, hd_, page_, kv_dtype_;
   size_t pool_bytes_ = 0;
   std::vector<void*> k_, v_;
+  std::vector<float*> acc_;          // [num_blocks][nkv][page] a layer (track_weights)
+  std::vector<int32_t*> slot_pos_;
   std::vector<int> free_;
   std::vector<Seq> seqs_;
   std::vector<int> batch_;
@@ -270,6 +371,8 @@ class PagedKVCache {
   int32_t* h_table_ = nullptr;
   hipEvent_t uploaded_ = nullptr;
   int32_t* d_lens_ = nullptr;
+  int32_t* d_pos_ = nullptr;
+  bool cut_ = false;
   size_t table_cap_ = 0;
   int maxb_ = 1, max_len_ = 0;
 };

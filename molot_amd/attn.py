@@ -25,6 +25,10 @@ __all__ = [
     "attn_decode_strided", "decode_step", "attn_decode_paged", "decode_step_paged",
     "rope_append_paged", "vexp", "decode_step_shared", "decode_step_paged_shared", "prefill_q",
     "attn_prefill_paged", "set_merge", "set_prefill_presplit",
+    "attn_decode_scored", "decode_step_scored", "attn_decode_paged_scored",
+    "decode_step_paged_scored", "attn_prefill_scored", "attn_prefill_paged_scored",
+    "prefill_step_scored", "prefill_step_paged_scored", "kv_track", "kv_track_paged", "kv_evict",
+    "kv_evict_paged", "alibi_slopes", "document_starts",
     "last_plan", "set_split_chunk", "attn_prefill_gqa", "prefill_step", "KVCache", "kv_dtype_of",
 ]
 
@@ -443,6 +447,309 @@ def rope_append_paged(q, k_new, v_new, K, V, block_table, seq_lens, pos, B, max_
         _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(K), _ptr(V), _ptr(block_table), _ptr(seq_lens),
         _ptr(pos), B, max_blocks, nq, nkv, d, page, _ptr(inv_freq), kvd, _stream()),
         "rope_append_paged")
+
+
+# --- scored attention, and a cache held to a budget of rows ------------------
+
+
+def alibi_slopes(nq: int) -> torch.Tensor:
+    """Host fp32 table of geometric slopes 2^(-8 (h + 1) / nq), a query head each."""
+    return torch.exp2(-8.0 * torch.arange(1, nq + 1, dtype=torch.float64) / nq).float()
+
+
+def document_starts(lengths, slot0: int = 0) -> torch.Tensor:
+    """Host int32 key_lo of a packed prompt of documents of these lengths, whose
+    first row is at slot0: the first slot of each row's document."""
+    n = torch.as_tensor(list(lengths), dtype=torch.int64)
+    if n.numel() and int(n.min()) < 0:
+        raise ValueError("document_starts: a negative length")
+    return torch.repeat_interleave(slot0 + n.cumsum(0) - n, n).to(torch.int32)
+
+
+def _need_scoring(slopes, nq, key_lo=None, key_hi=None, M=0):
+    if slopes is not None:
+        _need(slopes, "slopes", torch.float32, nq)
+    if key_lo is not None:
+        _need(key_lo, "key_lo", torch.int32, M)
+    if key_hi is not None:
+        _need(key_hi, "key_hi", torch.int32, M)
+
+
+def _acc_cap(acc, slot_pos, nkv, rows):
+    """Slots a KV head of acc [nkv][cap] (and slot_pos alike) has room for."""
+    if acc is None:
+        if slot_pos is not None:
+            raise ValueError("slot_pos needs acc")
+        return 0
+    _need(acc, "acc", torch.float32, nkv * rows)
+    if acc.numel() % nkv:
+        raise ValueError(f"acc: {acc.numel()} elements are not {nkv} KV heads of slots")
+    if slot_pos is not None:
+        _need(slot_pos, "slot_pos", torch.int32, acc.numel())
+    return acc.numel() // nkv
+
+
+def _need_acc_pages(acc, slot_pos, nblocks, nkv, page):
+    if acc is not None:
+        _need(acc, "acc", torch.float32, nblocks * nkv * page)
+    if slot_pos is not None:
+        if acc is None:
+            raise ValueError("slot_pos needs acc")
+        _need(slot_pos, "slot_pos", torch.int32, nblocks * nkv * page)
+
+
+def attn_decode_scored(Q, K, V, O, nq, nkv, n, d, scale, pos_cur, window=0, softcap=0.0,
+                       slopes=None, acc=None):
+    """attn_decode_gqa_cache with capped scores (softcap > 0), a bias by distance
+    (slopes [nq]), and the weights of every row added to acc [nkv][cap]; see
+    molot_hip_attn_decode_scored."""
+    kvd = kv_dtype_of(K)
+    row = _row_units(kvd, nkv, d)
+    _need(Q, "Q", torch.float32, nq * d)
+    _need(O, "O", torch.float32, nq * d)
+    _need(K, "K", _KV_DTYPES, n * row)
+    _need(V, "V", K.dtype, n * row)
+    _need_scoring(slopes, nq)
+    cap = _acc_cap(acc, None, nkv, n)
+    check(_lib.load().molot_hip_attn_decode_scored(
+        _ptr(Q), _ptr(K), _ptr(V), _ptr(O), nq, nkv, int(n), d, float(scale), int(pos_cur),
+        int(window), float(softcap), _ptr(slopes), _ptr(acc), cap, kvd, _stream()),
+        "attn_decode_scored")
+    return O
+
+
+def decode_step_scored(q, k_new, v_new, K, V, O, nq, nkv, d, slot, pos, inv_freq, scale, window=0,
+                       softcap=0.0, slopes=None, acc=None, slot_pos=None, q_norm=None,
+                       k_norm=None, v_norm=False, eps=1e-6):
+    """decode_step with attn_decode_scored's scores; the new row's acc is set, and
+    its position in slot_pos [nkv][cap]."""
+    kvd = kv_dtype_of(K)
+    row = _row_units(kvd, nkv, d)
+    if slot < 0 or slot >= K.numel() // row:
+        raise RuntimeError("fwd: KV cache full")  # forward.h:570
+    _need(q, "q", torch.float32, nq * d)
+    _need(k_new, "k_new", torch.float32, nkv * d)
+    _need(v_new, "v_new", torch.float32, nkv * d)
+    _need(K, "K", _KV_DTYPES, (slot + 1) * row)
+    _need(V, "V", K.dtype, (slot + 1) * row)
+    _need(O, "O", torch.float32, nq * d)
+    _need_table(inv_freq, d)
+    _need_norms(q_norm, k_norm, d)
+    _need_scoring(slopes, nq)
+    cap = _acc_cap(acc, slot_pos, nkv, slot + 1)
+    check(_lib.load().molot_hip_decode_step_scored(
+        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(K), _ptr(V), _ptr(O), nq, nkv, d, int(slot),
+        int(pos), _ptr(q_norm), _ptr(k_norm), int(bool(v_norm)), float(eps), _ptr(inv_freq),
+        float(scale), int(window), float(softcap), _ptr(slopes), _ptr(acc), _ptr(slot_pos), cap,
+        kvd, _stream()), "decode_step_scored")
+    return O
+
+
+def attn_decode_paged_scored(Q, K, V, O, block_table, seq_lens, pos, B, max_blocks, nq, nkv, d,
+                             page, scale, window=0, softcap=0.0, slopes=None, acc=None):
+    """attn_decode_paged with attn_decode_scored's scores; acc [blocks][nkv][page]."""
+    kvd = kv_dtype_of(K)
+    _need(Q, "Q", torch.float32, B * nq * d)
+    _need(O, "O", torch.float32, B * nq * d)
+    max_len = _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V)
+    _need_scoring(slopes, nq)
+    _need_acc_pages(acc, None, K.numel() // _block_units(kvd, nkv, d, page), nkv, page)
+    check(_lib.load().molot_hip_attn_decode_paged_scored(
+        _ptr(Q), _ptr(K), _ptr(V), _ptr(O), _ptr(block_table), _ptr(seq_lens), _ptr(pos), B,
+        max_blocks, max_len, nq, nkv, d, page, float(scale), int(window), float(softcap),
+        _ptr(slopes), _ptr(acc), kvd, _stream()), "attn_decode_paged_scored")
+    return O
+
+
+def decode_step_paged_scored(q, k_new, v_new, K, V, O, block_table, seq_lens, pos, B, max_blocks,
+                             nq, nkv, d, page, inv_freq, scale, window=0, softcap=0.0, slopes=None,
+                             acc=None, slot_pos=None, q_norm=None, k_norm=None, v_norm=False,
+                             eps=1e-6):
+    """decode_step_paged with attn_decode_scored's scores; acc and slot_pos
+    [blocks][nkv][page], the new rows' entries set."""
+    kvd = kv_dtype_of(K)
+    _need(q, "q", torch.float32, B * nq * d)
+    _need(O, "O", torch.float32, B * nq * d)
+    _need(k_new, "k_new", torch.float32, B * nkv * d)
+    _need(v_new, "v_new", torch.float32, B * nkv * d)
+    _need_table(inv_freq, d)
+    _need_norms(q_norm, k_norm, d)
+    max_len = _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V)
+    if B and int(seq_lens.min()) < 1:
+        raise ValueError("decode_step_paged_scored: every sequence needs seq_lens >= 1")
+    _need_scoring(slopes, nq)
+    _need_acc_pages(acc, slot_pos, K.numel() // _block_units(kvd, nkv, d, page), nkv, page)
+    check(_lib.load().molot_hip_decode_step_paged_scored(
+        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(K), _ptr(V), _ptr(O), _ptr(block_table),
+        _ptr(seq_lens), _ptr(pos), B, max_blocks, max_len, nq, nkv, d, page, _ptr(q_norm),
+        _ptr(k_norm), int(bool(v_norm)), float(eps), _ptr(inv_freq), float(scale), int(window),
+        float(softcap), _ptr(slopes), _ptr(acc), _ptr(slot_pos), kvd, _stream()),
+        "decode_step_paged_scored")
+    return O
+
+
+def attn_prefill_scored(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window=0, softcap=0.0,
+                        slopes=None, key_lo=None, key_hi=None):
+    """attn_prefill_gqa with attn_decode_scored's scores and the keys of row m in
+    [max(window's start, key_lo[m]), key_hi[m]) (device int32; None: causal)."""
+    kvd = kv_dtype_of(K)
+    row = _row_units(kvd, nkv, d)
+    _need(Qm, "Qm", torch.float32, M * nq * d)
+    _need(Om, "Om", torch.float32, M * nq * d)
+    _need(K, "K", _KV_DTYPES, N * row)
+    _need(V, "V", K.dtype, N * row)
+    _need_scoring(slopes, nq, key_lo, key_hi, M)
+    check(_lib.load().molot_hip_attn_prefill_scored(
+        _ptr(Qm), _ptr(K), _ptr(V), _ptr(Om), nq, nkv, int(M), int(N), d, float(scale), int(pos0),
+        int(window), float(softcap), _ptr(slopes), _ptr(key_lo), _ptr(key_hi), kvd, _stream()),
+        "attn_prefill_scored")
+    return Om
+
+
+def _need_block_row(block_row, max_blocks, page, used_rows, K, V, nkv, d):
+    kvd = kv_dtype_of(K)
+    _need(block_row, "block_row", torch.int32, max_blocks)
+    bu = _block_units(kvd, nkv, d, page)
+    nblocks = K.numel() // bu
+    _need(K, "K", _KV_DTYPES, nblocks * bu)
+    _need(V, "V", K.dtype, nblocks * bu)
+    used = (used_rows + page - 1) // page
+    row = block_row.cpu()
+    if used and (int(row[:used].min()) < 0 or int(row[:used].max()) >= nblocks):
+        raise ValueError("block_row names a block outside the pool")
+    return kvd
+
+
+def attn_prefill_paged_scored(Qm, K, V, Om, block_row, max_blocks, page, nq, nkv, M, N, d, scale,
+                              pos0, window=0, softcap=0.0, slopes=None, key_lo=None, key_hi=None):
+    """attn_prefill_scored over one sequence's pages."""
+    _need(Qm, "Qm", torch.float32, M * nq * d)
+    _need(Om, "Om", torch.float32, M * nq * d)
+    if N < 0 or N > max_blocks * page:
+        raise ValueError("N outside [0, max_blocks*page]")
+    kvd = _need_block_row(block_row, max_blocks, page, N, K, V, nkv, d)
+    _need_scoring(slopes, nq, key_lo, key_hi, M)
+    check(_lib.load().molot_hip_attn_prefill_paged_scored(
+        _ptr(Qm), _ptr(K), _ptr(V), _ptr(Om), _ptr(block_row), int(max_blocks), int(page), nq, nkv,
+        int(M), int(N), d, float(scale), int(pos0), int(window), float(softcap), _ptr(slopes),
+        _ptr(key_lo), _ptr(key_hi), kvd, _stream()), "attn_prefill_paged_scored")
+    return Om
+
+
+def prefill_step_scored(q, k_new, v_new, K, V, O, nq, nkv, d, M, slot0, pos0, inv_freq, scale,
+                        window=0, softcap=0.0, slopes=None, key_lo=None, key_hi=None, q_norm=None,
+                        k_norm=None, v_norm=False, eps=1e-6):
+    """prefill_step with attn_prefill_scored's scores and key ranges."""
+    kvd = kv_dtype_of(K)
+    row = _row_units(kvd, nkv, d)
+    cap = K.numel() // row
+    if slot0 < 0 or slot0 + M > cap:
+        raise RuntimeError("fwd: KV cache full")  # forward.h:380
+    _need(q, "q", torch.float32, M * nq * d)
+    _need(k_new, "k_new", torch.float32, M * nkv * d)
+    _need(v_new, "v_new", torch.float32, M * nkv * d)
+    _need(O, "O", torch.float32, M * nq * d)
+    _need(K, "K", _KV_DTYPES, cap * row)
+    _need(V, "V", K.dtype, cap * row)
+    _need_table(inv_freq, d)
+    _need_norms(q_norm, k_norm, d)
+    _need_scoring(slopes, nq, key_lo, key_hi, M)
+    check(_lib.load().molot_hip_prefill_step_scored(
+        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(K), _ptr(V), _ptr(O), nq, nkv, d, int(M),
+        int(slot0), int(pos0), _ptr(q_norm), _ptr(k_norm), int(bool(v_norm)), float(eps),
+        _ptr(inv_freq), float(scale), int(window), float(softcap), _ptr(slopes), _ptr(key_lo),
+        _ptr(key_hi), kvd, _stream()), "prefill_step_scored")
+    return O
+
+
+def prefill_step_paged_scored(q, k_new, v_new, K, V, O, block_row, max_blocks, page, nq, nkv, d, M,
+                              slot0, pos0, inv_freq, scale, window=0, softcap=0.0, slopes=None,
+                              key_lo=None, key_hi=None, q_norm=None, k_norm=None, v_norm=False,
+                              eps=1e-6):
+    """prefill_step_paged with attn_prefill_scored's scores and key ranges."""
+    if slot0 < 0 or slot0 + M > max_blocks * page:
+        raise RuntimeError("fwd: KV cache full")
+    _need(q, "q", torch.float32, M * nq * d)
+    _need(k_new, "k_new", torch.float32, M * nkv * d)
+    _need(v_new, "v_new", torch.float32, M * nkv * d)
+    _need(O, "O", torch.float32, M * nq * d)
+    _need_table(inv_freq, d)
+    kvd = _need_block_row(block_row, max_blocks, page, slot0 + M, K, V, nkv, d)
+    _need_norms(q_norm, k_norm, d)
+    _need_scoring(slopes, nq, key_lo, key_hi, M)
+    check(_lib.load().molot_hip_prefill_step_paged_scored(
+        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(K), _ptr(V), _ptr(O), _ptr(block_row),
+        int(max_blocks), int(page), nq, nkv, d, int(M), int(slot0), int(pos0), _ptr(q_norm),
+        _ptr(k_norm), int(bool(v_norm)), float(eps), _ptr(inv_freq), float(scale), int(window),
+        float(softcap), _ptr(slopes), _ptr(key_lo), _ptr(key_hi), kvd, _stream()),
+        "prefill_step_paged_scored")
+    return O
+
+
+def kv_track(acc, slot_pos, nkv, n, M, pos):
+    """The last M of n slots are new: acc [nkv][cap] 0, slot_pos pos-M+1 .. pos."""
+    cap = _acc_cap(acc, slot_pos, nkv, n)
+    check(_lib.load().molot_hip_kv_track(_ptr(acc), _ptr(slot_pos), nkv, int(n), int(M), int(pos),
+                                         cap, _stream()), "kv_track")
+
+
+def _check_slot_pages(block_table, seq_lens, pos, B, max_blocks, nblocks, page):
+    _need(block_table, "block_table", torch.int32, B * max_blocks)
+    _need(seq_lens, "seq_lens", torch.int32, B)
+    if pos is not None:
+        _need(pos, "pos", torch.int32, B)
+    lens = seq_lens[:B].cpu()
+    if B and (int(lens.min()) < 0 or int(lens.max()) > max_blocks * page):
+        raise ValueError("seq_lens outside [0, max_blocks*page]")
+    bt = block_table.view(-1)[:B * max_blocks].view(B, max_blocks).cpu()
+    for b in range(B):
+        used = (int(lens[b]) + page - 1) // page
+        if used and (int(bt[b, :used].min()) < 0 or int(bt[b, :used].max()) >= nblocks):
+            raise ValueError(f"block_table row {b} names a block outside the pool")
+    return int(lens.max()) if B else 0
+
+
+def kv_track_paged(acc, slot_pos, block_table, seq_lens, pos, B, max_blocks, M, nkv, page):
+    """kv_track of the last min(M, seq_lens[b]) slots of every sequence, the newest
+    at pos[b] (None: seq_lens[b] - 1); acc and slot_pos [blocks][nkv][page]."""
+    nblocks = acc.numel() // (nkv * page)
+    _need_acc_pages(acc, slot_pos, nblocks, nkv, page)
+    max_len = _check_slot_pages(block_table, seq_lens, pos, B, max_blocks, nblocks, page)
+    check(_lib.load().molot_hip_kv_track_paged(
+        _ptr(acc), _ptr(slot_pos), _ptr(block_table), _ptr(seq_lens), _ptr(pos), B, max_blocks,
+        max_len, int(M), nkv, page, _stream()), "kv_track_paged")
+
+
+def kv_evict(K, V, acc, slot_pos, nkv, n, d, keep, recent, pos):
+    """Cut a token-major cache of n slots to `keep` a KV head, in place: the slots at
+    the `recent` newest positions (slot_pos > pos - recent), then the highest acc,
+    ties to the lowest slot; see molot_hip_kv_evict.  Returns the slots left."""
+    kvd = kv_dtype_of(K)
+    row = _row_units(kvd, nkv, d)
+    _need(K, "K", _KV_DTYPES, n * row)
+    _need(V, "V", K.dtype, n * row)
+    if acc is None or slot_pos is None:
+        raise ValueError("kv_evict needs acc and slot_pos")
+    cap = _acc_cap(acc, slot_pos, nkv, n)
+    check(_lib.load().molot_hip_kv_evict(
+        _ptr(K), _ptr(V), _ptr(acc), _ptr(slot_pos), nkv, int(n), d, int(keep), int(recent),
+        int(pos), cap, kvd, _stream()), "kv_evict")
+    return min(int(n), int(keep))
+
+
+def kv_evict_paged(K, V, acc, slot_pos, block_table, seq_lens, pos, B, max_blocks, nkv, d, page,
+                   keep, recent):
+    """kv_evict of every sequence of a paged batch that is longer than keep
+    (seq_lens is not written)."""
+    kvd = kv_dtype_of(K)
+    if acc is None or slot_pos is None:
+        raise ValueError("kv_evict_paged needs acc and slot_pos")
+    max_len = _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V)
+    _need_acc_pages(acc, slot_pos, K.numel() // _block_units(kvd, nkv, d, page), nkv, page)
+    check(_lib.load().molot_hip_kv_evict_paged(
+        _ptr(K), _ptr(V), _ptr(acc), _ptr(slot_pos), _ptr(block_table), _ptr(seq_lens), _ptr(pos),
+        B, max_blocks, max_len, nkv, d, page, int(keep), int(recent), kvd, _stream()),
+        "kv_evict_paged")
 
 
 def vexp(x: torch.Tensor, y: torch.Tensor | None = None) -> torch.Tensor:

@@ -2990,7 +2990,7 @@ static int prefill_rows(const float* Qm, const void* K, const void* V, float* Om
   a.pf = 1;
   set_scoring(a, sc, 0);
   // the widest attended range of any query row
-  const int span = window > 0 && window < N ? window : N;
+  const int span = window > 0 && window < N && !sc.key_hi ? window : N;
   return block_row ? run_attn<true, false>(a, d, kv_dtype, span, M, stream)
                    : run_attn<false, false>(a, d, kv_dtype, span, M, stream);
 }
@@ -3522,8 +3522,11 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   }
   st = launch_rope_tok(r, M, stream);
   if (st) return st;
-  return attn_prefill_impl(q, K, V, O, nq, nkv, M, slot0 + M, d, scale, pos0, window, kv_dtype,
-                           block_row, page, sc, stream, presplit, split_rows);
+  // (scored: a row never sees the rows appended after it, whatever positions a cache
+  // that rows were evicted from has)
+  return attn_prefill_impl(q, K, V, O, nq, nkv, M, slot0 + M, d, scale,
+                           sc.on ? std::min(pos0, slot0) : pos0, window, kv_dtype, block_row, page,
+                           sc, stream, presplit, split_rows);
 }
 
 int molot_hip_prefill_step(float* q, const float* k_new, const float* v_new, void* K, void* V,

@@ -155,7 +155,9 @@ int run_attn(AttnArgs& a, int d, int kv_dtype, int span, int B, void* stream) {
   a.dh = d;
   const int G = a.nq / a.nkv;
   const bool q8 = kv_dtype == MOLOT_KV_Q8;
-  if ((q8 || (kv_dtype == MOLOT_KV_BF16 && g_bf16_mfma)) && (d == 64 || d == 128)) {
+  // (prefill rows have ranges of their own in a contiguous cache, which the
+  // matrix-core kernel does not take: the vector-ALU kernel)
+  if (!a.pf && (q8 || (kv_dtype == MOLOT_KV_BF16 && g_bf16_mfma)) && (d == 64 || d == 128)) {
     // up to 16 q heads of a group share each K/V tile on the MFMA columns;
     // Q8 caches of D = 64, 128 run here, D = 256 and 512 on the vector-ALU
     // kernel

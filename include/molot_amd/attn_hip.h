@@ -406,7 +406,8 @@ int molot_hip_kv_track_paged(float* acc, int32_t* slot_pos, const int32_t* block
  * cache is over the tokens kept, with the next token's slot and position told
  * apart (molot_hip_decode_step_scored's slot and pos, pos[] of the paged
  * steps); windows and slopes go by slots, and no longer hold there.  The
- * paged form cuts every sequence longer than keep (seq_lens is not written).
+ * paged form cuts every sequence longer than keep (seq_lens is not written; the
+ * sequences of a call share no block).
  * K and V 16-byte aligned; every even head dim up to 512. */
 int molot_hip_kv_evict(void* K, void* V, float* acc, int32_t* slot_pos, int nkv, int n, int d,
                        int keep, int recent, int pos, int acc_cap, int kv_dtype, void* stream);

@@ -1489,17 +1489,6 @@ __device__ __forceinline__ int seq_span(SeqLen s, int window, bool fold, int lim
   if (t0 > s.n) t0 = s.n;
   return min(max((fold ? s.n - 1 : s.n) - t0, 0), limit);
 }
-// Inclusive sum over the lanes up to this one (row shifts, then row
-// broadcasts of the rows before).
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
-  return x;
-}
 // The launch's chunk (wave-uniform; every lane of the wave takes part).
 // first: sequence (lane)'s, loaded by the caller.
 __device__ __forceinline__ int paged_chunk(const int32_t* seq_lens, const int32_t* pos_arr,

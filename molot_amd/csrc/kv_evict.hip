@@ -77,73 +77,168 @@ __device__ __forceinline__ uint32_t slot_key(float acc, bool recent) {
 
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 
-// Sum over the workgroup's waves of 1 to 3 wave-uniform counts (c[i] of every
-// wave), in every lane.  buf: kSelWaves ints a count; the caller alternates two of
-// them from call to call, so that one barrier is enough.
-template <int N>
-__device__ __forceinline__ void count_all(int (&c)[N], int* buf) {
-  static_assert(N >= 1 && N <= 3, "16 lanes a count");
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) buf[i * kSelWaves + w] = c[i];
+// A workgroup's keys in LDS, in slot order: thread t has the `each` slots from t * each
+// on (odd: the threads' reads then fall in different banks).  Absent slots' keys are 0,
+// below every slot's (at least 1).  So a thread counts its own slots in vector
+// registers and one scan gives every thread its place; with a wave on 64 neighbouring
+// slots the ballots and their counts were bound by the scalar unit, which 16 waves
+// share (4352 slots: 7000 cycles for the lists, 22500 for a selection by ballots).
+struct Keys {
+  uint32_t* k;
+  int each;
+  template <typename F>
+  __device__ __forceinline__ void own(F&& fn) const {  // fn(slot, key) of this thread's slots
+    const int t0 = (int)threadIdx.x * each;
+#pragma unroll 4
+    for (int i = 0; i < each; ++i) fn(t0 + i, k[t0 + i]);
   }
-  lds_barrier();
-  int x = lane < N * kSelWaves ? buf[lane] : 0;
-#pragma unroll
-  for (int off = 1; off < 16; off *= 2) x += __shfl_xor(x, off);
-#pragma unroll
-  for (int i = 0; i < N; ++i) c[i] = __builtin_amdgcn_readlane(x, 16 * i);
+};
+__host__ __device__ constexpr int key_each(int n) { return (n + kSelThreads - 1) / kSelThreads | 1; }
+
+// x summed over aligned groups of 16 lanes (DPP within a row; no LDS round trip).
+__device__ __forceinline__ int row_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false);   // quad_perm [1,0,3,2]
+  x += __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false);   // quad_perm [2,3,0,1]
+  x += __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false);  // row_half_mirror
+  x += __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false);  // row_mirror
+  return x;
 }
-// The sum of one count over the waves before this one, and over all.
+// Lanes below this one in a ballot.
+__device__ __forceinline__ int lanes_below(uint64_t m) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+
+// The sums over the waves before this one, and over all, of a wave-uniform count.
+// buf: kSelWaves ints, free again after the next barrier.
 __device__ __forceinline__ void count_before(int c, int* buf, int& before, int& all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   if (lane == 0) buf[w] = c;
   lds_barrier();
   const int x = lane < kSelWaves ? buf[lane] : 0;
-  int y = lane < w ? x : 0, z = x;
-#pragma unroll
-  for (int off = 1; off < 16; off *= 2) {
-    y += __shfl_xor(y, off);
-    z += __shfl_xor(z, off);
-  }
-  before = __builtin_amdgcn_readlane(y, 0);
-  all = __builtin_amdgcn_readlane(z, 0);
+  before = __builtin_amdgcn_readlane(row_sum(lane < w ? x : 0), 0);
+  all = __builtin_amdgcn_readlane(row_sum(x), 0);
+}
+// The sums over the threads before this one, and over all, of a count each.
+__device__ __forceinline__ int place_of(int c, int* buf, int& all) {
+  const int upto = wave_scan(c);
+  int before;
+  count_before(__builtin_amdgcn_readlane(upto, 63), buf, before, all);
+  return before + upto - c;
 }
 
-// Keys of a thread: K of them, wave w's i-th of slot first + (w * K + i) * 64 + lane,
-// so that the waves, their steps and the lanes run in slot order; absent ones are 0,
-// below every key of a slot (those are of numbers >= -NaN's image, at least 1).
-template <int K>
-struct Keys {
-  uint32_t k[K];
-  __device__ __forceinline__ static int slot(int i) {
-    return ((int)(threadIdx.x >> 6) * K + i) * 64 + (int)(threadIdx.x & 63);
-  }
-  // How many are at least t, in this wave.
-  __device__ __forceinline__ int at_least(uint32_t t) const {
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < K; ++i) c += __popcll(__builtin_amdgcn_ballot_w64(k[i] >= t));
-    return c;
-  }
+// The keep-th largest key T, the keys past it and those equal to it.
+struct Cut {
+  uint32_t T;
+  int above, equal;
+};
+constexpr int kFew = 256;
+struct alignas(16) SelectLds {
+  int hist[4096];
+  uint32_t few[kFew];
+  int buf[4 * kSelWaves];
+  uint32_t ends[2];
+  int nfew;
+  int pick[2];
+  Cut cut;
 };
 
-// The `want`-th largest of the workgroup's keys, two bits a step from bit 31 (top:
-// the bits above `from` are known): the largest T that at least want keys reach.
-// Each step counts three candidates, whatever the keys are; a radix pass's counters
-// would meet most lanes of a wave in a few bins (weights of a few exponents).
-template <int K>
-__device__ __forceinline__ uint32_t kth_largest(const Keys<K>& keys, uint32_t top, int from,
-                                                int want, int* buf) {
-  uint32_t T = top;
-  for (int s = from; s >= 0; s -= 2) {
-    const uint32_t one = 1u << s;
-    int c[3] = {keys.at_least(T + one), keys.at_least(T + 2 * one), keys.at_least(T + 3 * one)};
-    count_all<3>(c, buf + ((s >> 1) & 1) * 3 * kSelWaves);
-    T += c[2] >= want ? 3 * one : c[1] >= want ? 2 * one : c[0] >= want ? one : 0u;
+// The `want`-th largest of the workgroup's keys, which share the bits above shift + 12
+// (top): 12 bits by counters in LDS, then, of the keys in that bin, the one that
+// enough others are above where they are few, at once where they are all one value,
+// else a bit a step.
+__device__ __forceinline__ Cut kth_largest(const Keys& keys, uint32_t top, int shift, int want,
+                                           SelectLds& L) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  reinterpret_cast<u32x4*>(L.hist)[tid] = u32x4{0u, 0u, 0u, 0u};
+  if (tid < 2) L.ends[tid] = tid ? 0u : 0xFFFFFFFFu;
+  if (tid == 2) L.nfew = 0;
+  lds_barrier();
+  const int total_keys = keys.each * kSelThreads;
+#pragma unroll 4
+  for (int t = tid; t < total_keys; t += kSelThreads) {  // (neighbours' keys differ more than a
+    const uint32_t k = keys.k[t];                        // thread's order would: fewer clashes)
+    if (k) atomicAdd(&L.hist[(k >> shift) & 4095u], 1);
   }
-  return T;
+  lds_barrier();
+  {
+    const u32x4 c = reinterpret_cast<const u32x4*>(L.hist)[tid];  // bins 4 tid ..
+    const int mine = (int)(c[0] + c[1] + c[2] + c[3]);
+    int all;
+    const int place = place_of(mine, L.buf, all);
+    int above = all - place - mine;  // keys of the bins above this thread's
+    if (above < want && above + mine >= want) {  // one thread
+      int i = 3;
+      for (; i > 0; --i) {
+        if (above + (int)c[i] >= want) break;
+        above += (int)c[i];
+      }
+      L.pick[0] = 4 * tid + i;
+      L.pick[1] = above;
+    }
+  }
+  lds_barrier();
+  const uint32_t bin = (uint32_t)L.pick[0];
+  const int above = L.pick[1], left = want - above, total = L.hist[bin];
+  auto in_bin = [&](uint32_t k) { return k != 0u && ((k >> shift) & 4095u) == bin; };
+  if (total <= kFew) {  // (uniform)
+#pragma unroll 4
+    for (int t = tid; t < total_keys; t += kSelThreads) {
+      const uint32_t k = keys.k[t];
+      if (in_bin(k)) L.few[atomicAdd(&L.nfew, 1)] = k;  // (in any order)
+    }
+    if (tid < kFew && tid >= total) L.few[tid] = 0u;
+    lds_barrier();
+    // four threads a key, a quarter of the others each
+    const uint32_t mine = L.few[tid >> 2];
+    int gt = 0, eq = 0;
+#pragma unroll 4
+    for (int i = tid & 3; i < total; i += 4) {
+      const uint32_t k = L.few[i];
+      gt += k > mine;
+      eq += k == mine;
+    }
+    int both = gt | eq << 16;
+    both += __builtin_amdgcn_update_dpp(0, both, 0xB1, 0xF, 0xF, false);  // quad_perm [1,0,3,2]
+    both += __builtin_amdgcn_update_dpp(0, both, 0x4E, 0xF, 0xF, false);  // quad_perm [2,3,0,1]
+    gt = both & 0xFFFF;
+    eq = both >> 16;
+    if ((tid >> 2) < total && gt < left && gt + eq >= left)  // one value: equal keys write the same
+      L.cut = Cut{mine, above + gt, eq};
+    lds_barrier();
+    return L.cut;
+  }
+  uint32_t mn = 0xFFFFFFFFu, mx = 0u;
+  keys.own([&](int, uint32_t k) {
+    mn = min(mn, in_bin(k) ? k : 0xFFFFFFFFu);
+    mx = max(mx, in_bin(k) ? k : 0u);
+  });
+#pragma unroll 1
+  for (int off = 1; off < 64; off *= 2) {
+    mn = min(mn, (uint32_t)__shfl_xor((int)mn, off));
+    mx = max(mx, (uint32_t)__shfl_xor((int)mx, off));
+  }
+  if (lane == 0) {
+    atomicMin(&L.ends[0], mn);
+    atomicMax(&L.ends[1], mx);
+  }
+  lds_barrier();
+  if (L.ends[0] == L.ends[1]) return Cut{L.ends[0], above, total};
+  auto reach = [&](uint32_t t, int* buf) {
+    int c = 0, all;
+    keys.own([&](int, uint32_t k) { c += in_bin(k) && k >= t; });
+    (void)place_of(c, buf, all);
+    return all;
+  };
+  uint32_t T = top | bin << shift;
+  int turn = 0;
+#pragma unroll 1
+  for (uint32_t one = 1u << (shift - 1); one; one >>= 1) {
+    if (reach(T + one, L.buf + turn) >= left) T += one;
+    turn ^= kSelWaves;  // (two buffers by turns: one barrier a step)
+  }
+  const int more = T == 0xFFFFFFFFu ? 0 : reach(T + 1u, L.buf + turn);
+  const int from = reach(T, L.buf + 2 * kSelWaves);
+  return Cut{T, above + more, from - more};
 }
 
 // A row move: the units of a row of K and V that this thread takes.  U: bytes of a
@@ -170,37 +265,58 @@ __device__ __forceinline__ int64_t row_offset(const SlotArgs& a, int b, int h, i
   return blk * a.block + h * a.head + sl * a.tok;
 }
 
-// Moves [first, count) of the lists, step `threads` (this thread's number tid of
-// them): K and V rows, their scales, acc and slot_pos.  Flat over (move, unit), R
-// units a thread in flight.
+// The listed moves 0 .. count - 1, by `threads` threads of which this is number tid:
+// K and V rows flat over (move, unit), R units a thread in flight; acc, slot_pos and a
+// Q8 row's scales a thread a move, loaded before the rows' first units.
 template <int U, int R>
 __device__ __forceinline__ void move_rows(const SlotArgs& a, int b, int h, const int32_t* dst,
                                           const int32_t* src, int count, int tid, int threads) {
   using T = typename Unit<U>::type;
+  struct Slot {
+    float acc, ks, vs;
+    int32_t pos;
+  };
+  auto load = [&](int i) {
+    Slot x{};
+    const int64_t at = slot_index(a, b, h, src[i]);
+    x.acc = a.acc[at];
+    x.pos = a.slot_pos[at];
+    if (a.q8) {
+      int64_t sc;
+      (void)row_offset(a, b, h, src[i], sc);
+      x.ks = *reinterpret_cast<const float*>(a.k + sc);
+      x.vs = *reinterpret_cast<const float*>(a.v + sc);
+    }
+    return x;
+  };
+  auto store = [&](int i, const Slot& x) {
+    const int64_t to = slot_index(a, b, h, dst[i]);
+    a.acc[to] = x.acc;
+    a.slot_pos[to] = x.pos;
+    if (a.q8) {
+      int64_t sc;
+      (void)row_offset(a, b, h, dst[i], sc);
+      *reinterpret_cast<float*>(a.k + sc) = x.ks;
+      *reinterpret_cast<float*>(a.v + sc) = x.vs;
+    }
+  };
+  Slot first{};
+  if (tid < count) first = load(tid);
   const int upr = (int)(a.row / U);
-  const int total = count * upr;  // (a launch's lists are bounded: launch_evict)
+  const int total = count * upr;  // (bounded by launch_evict)
+#pragma unroll 1
   for (int u0 = tid; u0 < total; u0 += R * threads) {
     T kx[R], vx[R];
     int64_t to[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int u = u0 + r * threads;
-      if (u >= total) break;
+      const int u = min(u0 + r * threads, total - 1);  // (past the end: loaded, not stored)
       const int i = u / upr, j = u - i * upr;
-      int64_t sto, sat;
-      const int64_t at = row_offset(a, b, h, src[i], sat) + (int64_t)j * U;
-      to[r] = row_offset(a, b, h, dst[i], sto) + (int64_t)j * U;
+      int64_t sc;
+      const int64_t at = row_offset(a, b, h, src[i], sc) + (int64_t)j * U;
+      to[r] = row_offset(a, b, h, dst[i], sc) + (int64_t)j * U;
       kx[r] = *reinterpret_cast<const T*>(a.k + at);
       vx[r] = *reinterpret_cast<const T*>(a.v + at);
-      if (j == 0) {
-        if (a.q8) {
-          *reinterpret_cast<float*>(a.k + sto) = *reinterpret_cast<const float*>(a.k + sat);
-          *reinterpret_cast<float*>(a.v + sto) = *reinterpret_cast<const float*>(a.v + sat);
-        }
-        const int64_t ito = slot_index(a, b, h, dst[i]), iat = slot_index(a, b, h, src[i]);
-        a.acc[ito] = a.acc[iat];
-        a.slot_pos[ito] = a.slot_pos[iat];
-      }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -209,69 +325,79 @@ __device__ __forceinline__ void move_rows(const SlotArgs& a, int b, int h, const
       *reinterpret_cast<T*>(a.v + to[r]) = vx[r];
     }
   }
+  if (tid < count) store(tid, first);
+#pragma unroll 1
+  for (int i = tid + threads; i < count; i += threads) store(i, load(i));
 }
 
-// The moves among a workgroup's slots, whose first is `first`: of the slots with key
-// > T or, the first `ties` of them in slot order from number eq0 on, == T, those at
-// or past keep (lo false), or of the others those before it (lo), to list[at ..].
-// Returns how many.  buf: 2 * kSelWaves ints.
-template <int K>
-__device__ __forceinline__ int list_slots(const Keys<K>& keys, int first, int n, int keep, uint32_t T,
-                                          int ties, int eq0, bool want_holes, bool want_moves,
-                                          int32_t* holes, int32_t* moves, int hole0, int move0,
-                                          int most, int* buf, int& nmoves) {
-  const int lane = threadIdx.x & 63;
-  const uint64_t below = ((uint64_t)1 << lane) - 1;
-  int eqs = 0;
-#pragma unroll
-  for (int i = 0; i < K; ++i) {
-    const bool in = first + Keys<K>::slot(i) < n;
-    eqs += __popcll(__builtin_amdgcn_ballot_w64(in && keys.k[i] == T));
+// The holes and moves among a workgroup's slots first .. end - 1: a slot stays whose
+// key is past T, or is T and among the first `ties` such from number eq0 on (`equal`
+// of them in all); holes are the others before keep, moves the stayers at or past it.
+// They go, in order, to holes[hole0 ..] and moves[move0 ..] (NULL: not wanted); their
+// numbers come back in nholes, nmoves.
+__device__ __forceinline__ void list_slots(const Keys& keys, int first, int end, int keep, uint32_t T,
+                                           int ties, int equal, int eq0, int32_t* holes,
+                                           int32_t* moves, int hole0, int move0, int most,
+                                           SelectLds& L, int& nholes, int& nmoves) {
+  const bool split = ties < equal;  // (uniform) some equals stay, some go
+  int eq_at = 0;                    // this thread's first equal is number eq_at
+  if (split) {
+    int c = 0, all;
+    keys.own([&](int, uint32_t k) { c += k == T; });
+    eq_at = eq0 + place_of(c, L.buf, all);
   }
-  int eq_at, all;
-  count_before(eqs, buf, eq_at, all);
-  eq_at += eq0;
-  uint64_t hm[K], mm[K];  // a step's holes and moves, a bit a lane
-  int ch = 0, cm = 0;
-#pragma unroll
-  for (int i = 0; i < K; ++i) {
-    const int t = first + Keys<K>::slot(i);
-    const bool in = t < n;
-    const bool eq = in && keys.k[i] == T;
-    const uint64_t be = __builtin_amdgcn_ballot_w64(eq);
-    const bool stays = in && (keys.k[i] > T || (eq && eq_at + __popcll(be & below) < ties));
-    eq_at += __popcll(be);
-    hm[i] = __builtin_amdgcn_ballot_w64(in && t < keep && !stays);
-    mm[i] = __builtin_amdgcn_ballot_w64(t >= keep && stays);
-    ch += __popcll(hm[i]);
-    cm += __popcll(mm[i]);
+  // this thread's slots before keep, and then those past it: keys from k0 on, first
+  // slot t0
+  const uint32_t* k0 = keys.k + (int)threadIdx.x * keys.each;
+  const int t0 = first + (int)threadIdx.x * keys.each;
+  const int low = min(keys.each, max(0, min(keep, end) - t0));
+  const int upto = min(keys.each, max(0, end - t0));
+  int c = 0, all;  // holes, moves << 16 (at most 17408 slots)
+  if (!split) {
+#pragma unroll 4
+    for (int i = 0; i < low; ++i) c += k0[i] < T;
+    if (low < upto) {
+      int m = 0;
+#pragma unroll 4
+      for (int i = low; i < upto; ++i) m += k0[i] >= T;
+      c += m << 16;
+    }
+  } else {
+    int eq = eq_at;
+    for (int i = 0; i < upto; ++i) {
+      const uint32_t k = k0[i];
+      const bool st = k > T || (k == T && eq++ < ties);
+      if (st == (i >= low)) c += i < low ? 1 : 1 << 16;
+    }
   }
-  int h_at, m_at, nh;
-  count_before(ch, buf + kSelWaves, h_at, nh);
-  lds_barrier();
-  count_before(cm, buf, m_at, nmoves);
-  h_at += hole0;
-  m_at += move0;
-#pragma unroll
-  for (int i = 0; i < K; ++i) {
-    const int t = first + Keys<K>::slot(i);
+  const int place = place_of(c, L.buf + kSelWaves, all);
+  nholes = all & 0xFFFF;
+  nmoves = all >> 16;
+  if (c == 0) return;
+  int h_at = hole0 + (place & 0xFFFF), m_at = move0 + (place >> 16), eq = eq_at;
+  for (int i = 0; i < upto; ++i) {
+    const uint32_t k = k0[i];
+    const bool st = split ? k > T || (k == T && eq++ < ties) : k >= T;
+    if (st != (i >= low)) continue;
     // (as many moves as holes; the bound holds whatever another stream does to acc)
-    const int hi = h_at + __popcll(hm[i] & below), mi = m_at + __popcll(mm[i] & below);
-    if (want_holes && (hm[i] >> lane & 1) && hi < most) holes[hi] = t;
-    if (want_moves && (mm[i] >> lane & 1) && mi < most) moves[mi] = t;
-    h_at += __popcll(hm[i]);
-    m_at += __popcll(mm[i]);
+    if (i < low) {
+      if (holes && h_at < most) holes[h_at] = t0 + i;
+      ++h_at;
+    } else {
+      if (moves && m_at < most) moves[m_at] = t0 + i;
+      ++m_at;
+    }
   }
-  return nh;
 }
 
-// Sequences of at most 1024 K rows: a workgroup a (KV head, sequence) holds the
-// keys in registers.  FUSE: it makes the moves too (lists in LDS, most <=
-// kFuseMoves); else the lists go to evict_move_kernel.
+// Sequences of at most kSelMax rows: a workgroup a (KV head, sequence), its keys in
+// LDS.  FUSE: it makes the moves too (lists in LDS, most <= kFuseMoves); else the
+// lists go to evict_move_kernel.
+constexpr int kSelMax = 16384;
 constexpr int kFuseMoves = 2048;
-constexpr int64_t kFuseBytes = 32 * 1024;  // of K (and of V) a head
+constexpr int64_t kFuseBytes = 64 * 1024;  // of K (and of V) a head
 
-template <int K, bool FUSE>
+template <bool FUSE>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(SlotArgs a, int keep, int recent,
                                                                    int most, int32_t* counts,
                                                                    int32_t* lists, int unit16) {
@@ -282,38 +408,39 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(SlotArgs a, i
     if (!FUSE && threadIdx.x == 0) counts[pair] = 0;
     return;
   }
-  const int oldest = newest_of(a, b, n) - recent;  // recent: past it
-  Keys<K> keys;
-  float x[K];
-  int32_t p[K];
-#pragma unroll
-  for (int i = 0; i < K; ++i) {
-    const int64_t j = slot_index(a, b, h, min(Keys<K>::slot(i), n - 1));
-    x[i] = a.acc[j];
-    p[i] = a.slot_pos[j];
-  }
-#pragma unroll
-  for (int i = 0; i < K; ++i) keys.k[i] = Keys<K>::slot(i) < n ? slot_key(x[i], p[i] > oldest) : 0u;
-  __shared__ int buf[6 * kSelWaves];
+  extern __shared__ uint32_t key_lds[];  // [key_each(longest) * kSelThreads]
+  __shared__ SelectLds L;
   __shared__ int32_t own[FUSE ? 2 * kFuseMoves : 1];
-  const uint32_t T = kth_largest<K>(keys, 0u, 30, keep, buf);
-  int more[1] = {keys.at_least(T + 1u)};  // (T + 1 of the largest key, all recent: 0, none past it)
-  if (T == 0xFFFFFFFFu) more[0] = 0;
-  lds_barrier();
-  count_all<1>(more, buf);
+  const int oldest = newest_of(a, b, n) - recent;  // recent: past it
+  const Keys keys{key_lds, key_each(n)};
+  for (int t0 = threadIdx.x; t0 < keys.each * kSelThreads; t0 += 8 * kSelThreads) {
+    float x[8];
+    int32_t p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t j = slot_index(a, b, h, min(t0 + i * kSelThreads, n - 1));
+      x[i] = a.acc[j];
+      p[i] = a.slot_pos[j];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = t0 + i * kSelThreads;
+      if (t < keys.each * kSelThreads) key_lds[t] = t < n ? slot_key(x[i], p[i] > oldest) : 0u;
+    }
+  }
+  const Cut cut = kth_largest(keys, 0u, 20, keep, L);
   lds_barrier();
   int32_t* dst = FUSE ? own : lists + pair * 2 * most;
   int32_t* src = dst + (FUSE ? kFuseMoves : most);
-  int nm;
-  const int nh = list_slots<K>(keys, 0, n, keep, T, keep - more[0], 0, true, true, dst, src, 0, 0, most,
-                               buf, nm);
+  int nh, nm;
+  list_slots(keys, 0, n, keep, cut.T, keep - cut.above, cut.equal, 0, dst, src, 0, 0, most, L, nh, nm);
   const int moves = min(min(nm, nh), most);
   if constexpr (FUSE) {
     __syncthreads();
     if (unit16)
-      move_rows<16, 2>(a, b, h, dst, src, moves, threadIdx.x, kSelThreads);
+      move_rows<16, 4>(a, b, h, dst, src, moves, threadIdx.x, kSelThreads);
     else
-      move_rows<4, 2>(a, b, h, dst, src, moves, threadIdx.x, kSelThreads);
+      move_rows<4, 4>(a, b, h, dst, src, moves, threadIdx.x, kSelThreads);
   } else if (threadIdx.x == 0) {
     counts[pair] = moves;
   }
@@ -343,17 +470,18 @@ __global__ __launch_bounds__(256) void evict_move_kernel(SlotArgs a, int most, c
 //   evict_list_kernel   the chunks' holes and moves.
 constexpr int kChunkK = 8, kChunk = kSelThreads * kChunkK;
 constexpr int kTopBits = 12, kBins = 1 << kTopBits, kLowBits = 32 - kTopBits;
-static_assert(kLowBits % 2 == 0 && kBins == 4 * kSelThreads, "two bits a step; four bins a thread");
-constexpr int kRankK = 16;  // listed keys a thread keeps in registers
+static_assert(kBins == 4 * kSelThreads, "four bins a thread");
 
+constexpr int kAt = 6;
 struct LongArgs {
   SlotArgs s;
   int keep, recent, most, nlo, nhi;
   uint32_t* keys;      // [pair][chunks][kChunk]
   uint32_t* listed;    // [pair][chunks][kChunk]: the keys of the bin
   uint16_t* bins;      // [pair][chunks][kBins]
-  int32_t* chunk_at;   // [pair][chunks][4]: keys above the bin, listed; then equals and entries before
-  int32_t* rank;       // [pair][4]: bin, still wanted in it, T, equals that stay
+  int32_t* chunk_at;   // [pair][chunks][kAt]: keys above the bin, listed; then equals and entries
+                       // before; the smallest and largest listed
+  int32_t* rank;       // [pair][4]: bin, still wanted in it (then the equals of T), T, equals that stay
   int32_t* counts;     // [pair]
   int32_t* lists;      // [pair][2][most]
 };
@@ -367,20 +495,20 @@ __device__ __forceinline__ void chunk_range(const LongArgs& g, int n, int c, int
 
 __global__ __launch_bounds__(kSelThreads) void evict_keys_kernel(LongArgs g) {
   const SlotArgs& a = g.s;
-  const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nc = g.nlo + g.nhi;
+  const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nc = g.nlo + g.nhi, tid = threadIdx.x;
   const int n = rows_of(a, b);
   if (n <= g.keep) return;
   int first, end;
   chunk_range(g, n, c, first, end);
   const int64_t pair = (int64_t)b * a.nkv + h;
-  __shared__ int hist[kBins];
-  for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
+  __shared__ __attribute__((aligned(16))) int hist[kBins];
+  reinterpret_cast<u32x4*>(hist)[tid] = u32x4{0u, 0u, 0u, 0u};
   const int oldest = newest_of(a, b, n) - g.recent;
   float x[kChunkK];
   int32_t p[kChunkK];
 #pragma unroll
   for (int i = 0; i < kChunkK; ++i) {
-    const int64_t j = slot_index(a, b, h, min(first + Keys<kChunkK>::slot(i), n - 1));
+    const int64_t j = slot_index(a, b, h, min(first + kSelThreads * i + tid, n - 1));
     x[i] = a.acc[j];
     p[i] = a.slot_pos[j];
   }
@@ -388,15 +516,16 @@ __global__ __launch_bounds__(kSelThreads) void evict_keys_kernel(LongArgs g) {
   uint32_t* keys = g.keys + (pair * nc + c) * kChunk;
 #pragma unroll
   for (int i = 0; i < kChunkK; ++i) {
-    const int t = Keys<kChunkK>::slot(i);
+    const int t = kSelThreads * i + tid;
     if (first + t >= end) continue;
     const uint32_t k = slot_key(x[i], p[i] > oldest);
     keys[t] = k;
     atomicAdd(&hist[k >> kLowBits], 1);
   }
   __syncthreads();
-  uint16_t* bins = g.bins + (pair * nc + c) * kBins;
-  for (int i = threadIdx.x; i < kBins; i += kSelThreads) bins[i] = (uint16_t)hist[i];
+  const u32x4 v = reinterpret_cast<const u32x4*>(hist)[tid];  // (a chunk's counts fit 16 bits)
+  reinterpret_cast<u32x2*>(g.bins + (pair * nc + c) * kBins)[tid] =
+      u32x2{v[0] | v[1] << 16, v[2] | v[3] << 16};
 }
 
 __global__ __launch_bounds__(kSelThreads) void evict_pick_kernel(LongArgs g) {
@@ -405,31 +534,45 @@ __global__ __launch_bounds__(kSelThreads) void evict_pick_kernel(LongArgs g) {
   const int n = rows_of(a, b);
   const int64_t pair = (int64_t)b * a.nkv + h;
   if (n <= g.keep) return;
+  int first, end;
+  chunk_range(g, n, c, first, end);
+  const uint32_t* keys = g.keys + (pair * nc + c) * kChunk;
+  uint32_t k[kChunkK];
+#pragma unroll
+  for (int i = 0; i < kChunkK; ++i) {
+    const int t = kSelThreads * i + tid;
+    k[i] = keys[first + t < end ? t : 0];
+  }
   // bins 4 tid .. 4 tid + 3 over the chunks; then the sums of the bins above
-  __shared__ int buf[6 * kSelWaves];
+  __shared__ int buf[kSelWaves];
   __shared__ int pick[2];
-  const uint32_t* bins = reinterpret_cast<const uint32_t*>(g.bins + pair * nc * kBins) + 2 * tid;
+  __shared__ int found[2];      // the chunk's keys above the bin, and in it
+  __shared__ uint32_t ends[2];  // the smallest and largest in it
+  if (tid < 2) {
+    found[tid] = 0;
+    ends[tid] = tid ? 0u : 0xFFFFFFFFu;
+  }
+  const u32x2* bins = reinterpret_cast<const u32x2*>(g.bins + pair * nc * kBins) + tid;
   int cnt[4] = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int i = 0; i < nc; ++i) {  // (a chunk of no slots has counts of 0)
-    const uint32_t x = bins[(int64_t)i * (kBins / 2)], y = bins[(int64_t)i * (kBins / 2) + 1];
-    cnt[0] += (int)(x & 0xFFFFu);
-    cnt[1] += (int)(x >> 16);
-    cnt[2] += (int)(y & 0xFFFFu);
-    cnt[3] += (int)(y >> 16);
+#pragma unroll 1
+  for (int i0 = 0; i0 < nc; i0 += 8) {  // (a chunk of no slots has counts of 0)
+    u32x2 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = bins[(int64_t)min(i0 + i, nc - 1) * (kBins / 4)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i >= nc) continue;
+      cnt[0] += (int)(x[i][0] & 0xFFFFu);
+      cnt[1] += (int)(x[i][0] >> 16);
+      cnt[2] += (int)(x[i][1] & 0xFFFFu);
+      cnt[3] += (int)(x[i][1] >> 16);
+    }
   }
   const int lane = tid & 63;
-  const int mine = cnt[0] + cnt[1] + cnt[2] + cnt[3];
-  int up = mine;  // this lane's and the lanes' after it
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const int y = __shfl_down(up, off);
-    if (lane + off < 64) up += y;
-  }
-  const int wave = __builtin_amdgcn_readlane(up, 0);
+  const int upto = wave_scan(cnt[0] + cnt[1] + cnt[2] + cnt[3]);  // the lanes' up to this one
   int before, all;
-  count_before(wave, buf, before, all);
-  int above = all - before - wave + up - mine;  // keys of the bins above this thread's
+  count_before(__builtin_amdgcn_readlane(upto, 63), buf, before, all);
+  int above = all - before - upto;  // keys of the bins above this thread's
 #pragma unroll
   for (int i = 3; i >= 0; --i) {
     if (above < g.keep && above + cnt[i] >= g.keep) {  // one bin of all
@@ -440,44 +583,52 @@ __global__ __launch_bounds__(kSelThreads) void evict_pick_kernel(LongArgs g) {
   }
   __syncthreads();
   const uint32_t bin = (uint32_t)pick[0];
-  int first, end;
-  chunk_range(g, n, c, first, end);
-  const uint32_t* keys = g.keys + (pair * nc + c) * kChunk;
   uint32_t* listed = g.listed + (pair * nc + c) * kChunk;
-  uint32_t k[kChunkK];
+  uint32_t mn = 0xFFFFFFFFu, mx = 0u;
 #pragma unroll
   for (int i = 0; i < kChunkK; ++i) {
-    const int t = Keys<kChunkK>::slot(i);
-    k[i] = first + t < end ? keys[t] : 0u;
+    const bool live = first + kSelThreads * i + tid < end;
+    const uint64_t more = __builtin_amdgcn_ballot_w64(live && (k[i] >> kLowBits) > bin);
+    const bool in = live && (k[i] >> kLowBits) == bin;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+    int at = 0;
+    if (lane == 0) {
+      if (more) atomicAdd(&found[0], __popcll(more));
+      if (m) at = atomicAdd(&found[1], __popcll(m));
+    }
+    at = __builtin_amdgcn_readfirstlane(at);
+    if (in) {
+      listed[at + lanes_below(m)] = k[i];  // (in any order within the chunk)
+      mn = min(mn, k[i]);
+      mx = max(mx, k[i]);
+    }
   }
-  int more = 0, in = 0;
-  uint64_t m[kChunkK];
-#pragma unroll
-  for (int i = 0; i < kChunkK; ++i) {
-    const bool live = first + Keys<kChunkK>::slot(i) < end;
-    more += __popcll(__builtin_amdgcn_ballot_w64(live && (k[i] >> kLowBits) > bin));
-    m[i] = __builtin_amdgcn_ballot_w64(live && (k[i] >> kLowBits) == bin);
-    in += __popcll(m[i]);
+  // a wave whose keys are one value adds them at once
+  const uint64_t some = __builtin_amdgcn_ballot_w64(mx != 0u);
+  if (some) {
+    const uint32_t v = __builtin_amdgcn_readlane(mx, __builtin_ctzll(some));
+    const bool same = __builtin_amdgcn_ballot_w64(mx != 0u && (mn != v || mx != v)) == 0;
+    if (same ? lane == 0 : mx != 0u) {
+      atomicMin(&ends[0], same ? v : mn);
+      atomicMax(&ends[1], same ? v : mx);
+    }
   }
-  int at, total, m_before, m_all;
-  count_before(in, buf + kSelWaves, at, total);
-  count_before(more, buf + 2 * kSelWaves, m_before, m_all);
-  const uint64_t below = ((uint64_t)1 << lane) - 1;
-#pragma unroll
-  for (int i = 0; i < kChunkK; ++i) {
-    if (m[i] >> lane & 1) listed[at + __popcll(m[i] & below)] = k[i];
-    at += __popcll(m[i]);
-  }
+  __syncthreads();
   if (tid == 0) {
-    int32_t* ca = g.chunk_at + (pair * nc + c) * 4;
-    ca[0] = m_all;
-    ca[1] = total;
+    int32_t* ca = g.chunk_at + (pair * nc + c) * kAt;
+    ca[0] = found[0];
+    ca[1] = found[1];
+    ca[4] = (int32_t)ends[0];
+    ca[5] = (int32_t)ends[1];
     if (c == 0) {
       g.rank[pair * 4] = (int32_t)bin;
       g.rank[pair * 4 + 1] = pick[1];
     }
   }
 }
+
+// Listed keys that the rank kernel holds in LDS at once.
+constexpr int kRankMax = 17 * kSelThreads;  // (key_each: odd)
 
 __global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(LongArgs g) {
   const SlotArgs& a = g.s;
@@ -489,144 +640,159 @@ __global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(LongArgs g) {
     if (tid == 0) g.counts[pair] = 0;
     return;
   }
-  __shared__ int buf[6 * kSelWaves];
-  __shared__ uint32_t ends[2];
-  extern __shared__ int32_t cn[];  // [nc][3]: listed before the chunk, its keys past T, equals
-  int32_t* ca = g.chunk_at + pair * nc * 4;
+  __shared__ SelectLds L;
+  extern __shared__ uint32_t rank_lds[];  // [kRankMax] keys, then cn
+  int32_t* cn = reinterpret_cast<int32_t*>(rank_lds + kRankMax);  // [nc][3]: listed before the
+                                                                  // chunk, its keys past T, equals
+  int32_t* ca = g.chunk_at + pair * nc * kAt;
   const uint32_t* listed = g.listed + pair * nc * kChunk;
   const uint32_t top = (uint32_t)g.rank[pair * 4] << kLowBits;
   const int want = g.rank[pair * 4 + 1];
-  if (tid < 2) ends[tid] = tid ? 0u : 0xFFFFFFFFu;
-  int total = 0;
+  // (a chunk past the sequence's end has written no counts)
+  auto live = [&](int c) {
+    int first, end;
+    chunk_range(g, n, c, first, end);
+    return first < end;
+  };
+  if (tid < 2) L.ends[tid] = tid ? 0u : 0xFFFFFFFFu;
+  __syncthreads();
   if (w == 0) {  // the chunks' starts in the concatenated list
+    int total = 0;
+#pragma unroll 1
     for (int c0 = 0; c0 < nc; c0 += 64) {
-      int first, end;
       const int c = c0 + lane;
-      if (c < nc) chunk_range(g, n, c, first, end);
-      const int x = c < nc && first < end ? ca[4 * c + 1] : 0;
-      int y = x;
-#pragma unroll
-      for (int off = 1; off < 64; off *= 2) {
-        const int z = __shfl_up(y, off);
-        if (lane >= off) y += z;
+      const int x = c < nc && live(c) ? ca[kAt * c + 1] : 0;
+      if (x) {
+        atomicMin(&L.ends[0], (uint32_t)ca[kAt * c + 4]);
+        atomicMax(&L.ends[1], (uint32_t)ca[kAt * c + 5]);
       }
+      const int y = wave_scan(x);
       if (c < nc) {
         cn[3 * c] = total + y - x;
         cn[3 * c + 1] = cn[3 * c + 2] = 0;
       }
       total += __builtin_amdgcn_readlane(y, 63);
     }
-    if (lane == 0) buf[0] = total;
+    if (lane == 0) L.nfew = total;
   }
   __syncthreads();
-  total = buf[0];
-  __syncthreads();
-  // key j of the concatenated list: chunk by bisection
-  auto key_at = [&](int j) -> uint32_t {
-    int lo = 0, hi = nc - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (cn[3 * mid] <= j) lo = mid;
-      else hi = mid - 1;
-    }
-    return listed[(int64_t)lo * kChunk + j - cn[3 * lo]];
-  };
-  uint32_t T;
-  Keys<kRankK> keys;
-  const bool fits = total <= kSelThreads * kRankK;
-  if (fits) {
+  const int total = L.nfew;
+  auto count_of = [&](int c) { return (c + 1 < nc ? cn[3 * c + 3] : total) - cn[3 * c]; };
+  // a wave a chunk, its listed keys 256 at a time: fn(first place in the list, chunk, keys)
+  auto each_chunk = [&](auto&& fn) {
+#pragma unroll 1
+    for (int c = w; c < nc; c += kSelWaves) {
+      const int cnt = count_of(c);
+      const uint32_t* from = listed + (int64_t)c * kChunk;
+#pragma unroll 1
+      for (int j0 = 0; j0 < cnt; j0 += 256) {
+        uint32_t k[4];
 #pragma unroll
-    for (int i = 0; i < kRankK; ++i) {
-      const int j = Keys<kRankK>::slot(i);
-      keys.k[i] = j < total ? key_at(j) : 0u;
-    }
-    T = kth_largest<kRankK>(keys, top, kLowBits - 2, want, buf);
-  } else {
-    // too many of one bin for the registers: the smallest and the largest first (weights
-    // that are all one value end here), then a bit a step over the list
-    uint32_t mn = 0xFFFFFFFFu, mx = 0u;
-    for (int j = tid; j < total; j += kSelThreads) {
-      const uint32_t k = key_at(j);
-      mn = min(mn, k);
-      mx = max(mx, k);
-    }
-    atomicMin(&ends[0], mn);
-    atomicMax(&ends[1], mx);
-    __syncthreads();
-    T = top;
-    if (ends[0] == ends[1]) {
-      T = ends[0];
-    } else {
-      for (int s = kLowBits - 1; s >= 0; --s) {
-        int c[1] = {0};
-        for (int j0 = 0; j0 < total; j0 += kSelThreads)
-          c[0] += __popcll(__builtin_amdgcn_ballot_w64(j0 + tid < total &&
-                                                       key_at(min(j0 + tid, total - 1)) >= T + (1u << s)));
-        count_all<1>(c, buf + (s & 1) * kSelWaves);
-        if (c[0] >= want) T += 1u << s;
+        for (int i = 0; i < 4; ++i) k[i] = from[min(j0 + 64 * i + lane, cnt - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j0 + 64 * i < cnt) fn(c, j0 + 64 * i + lane, j0 + 64 * i + lane < cnt, k[i]);
       }
     }
-  }
-  // every chunk's listed keys past T and equal to it
+  };
+  Cut cut;
+  const uint32_t smallest = L.ends[0];
+  const bool one_value = smallest == L.ends[1];
   __syncthreads();
-  for (int c = w; c < nc; c += kSelWaves) {
-    int first, end;
-    chunk_range(g, n, c, first, end);
-    const int cnt = first < end ? ca[4 * c + 1] : 0;
-    int gt = 0, eq = 0;
-    for (int j0 = 0; j0 < cnt; j0 += 64) {
-      const uint32_t k = j0 + lane < cnt ? listed[(int64_t)c * kChunk + j0 + lane] : 0u;
-      gt += __popcll(__builtin_amdgcn_ballot_w64(j0 + lane < cnt && k > T));
-      eq += __popcll(__builtin_amdgcn_ballot_w64(j0 + lane < cnt && k == T));
+  if (one_value) {  // (weights that are all 0, say)
+    cut.T = smallest;
+    for (int c = tid; c < nc; c += kSelThreads) cn[3 * c + 2] = count_of(c);
+  } else if (total <= kRankMax) {
+    const Keys keys{rank_lds, key_each(total)};
+    for (int j = total + tid; j < keys.each * kSelThreads; j += kSelThreads) rank_lds[j] = 0u;
+    for (int j0 = tid; j0 < total; j0 += 8 * kSelThreads) {
+      uint32_t k[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = min(j0 + i * kSelThreads, total - 1);
+        int lo = 0, hi = nc - 1;  // its chunk
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) / 2;
+          if (cn[3 * mid] <= j) lo = mid;
+          else hi = mid - 1;
+        }
+        k[i] = listed[(int64_t)lo * kChunk + j - cn[3 * lo]];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (j0 + i * kSelThreads < total) rank_lds[j0 + i * kSelThreads] = k[i];
     }
-    if (lane == 0) {
-      cn[3 * c + 1] = gt;
-      cn[3 * c + 2] = eq;
+    __syncthreads();
+    cut = kth_largest(keys, top, kLowBits - 12, want, L);
+    // every chunk's listed keys past T and equal to it: a wave a chunk
+    for (int c = w; c < nc; c += kSelWaves) {
+      const int cnt = count_of(c), at = cn[3 * c];
+      int both = 0;
+      for (int j = lane; j < cnt; j += 64) {
+        const uint32_t k = rank_lds[at + j];
+        both += k > cut.T ? 1 : k == cut.T ? 1 << 16 : 0;
+      }
+      both = __builtin_amdgcn_readlane(wave_scan(both), 63);  // (a chunk's counts fit 16 bits)
+      if (lane == 0) {
+        cn[3 * c + 1] = both & 0xFFFF;
+        cn[3 * c + 2] = both >> 16;
+      }
     }
+  } else {
+    // too many of one bin for LDS: a bit a step over the lists
+    cut.T = top;
+    int turn = 0;
+#pragma unroll 1
+    for (uint32_t one = 1u << (kLowBits - 1); one; one >>= 1) {
+      int c = 0;
+      each_chunk([&](int, int, bool in, uint32_t k) {
+        c += __popcll(__builtin_amdgcn_ballot_w64(in && k >= cut.T + one));
+      });
+      int before, all;
+      count_before(c, L.buf + turn, before, all);
+      if (all >= want) cut.T += one;
+      turn ^= kSelWaves;
+    }
+    each_chunk([&](int c, int, bool in, uint32_t k) {
+      const int gt = __popcll(__builtin_amdgcn_ballot_w64(in && k > cut.T));
+      const int eq = __popcll(__builtin_amdgcn_ballot_w64(in && k == cut.T));
+      if (lane == 0) {
+        cn[3 * c + 1] += gt;
+        cn[3 * c + 2] += eq;
+      }
+    });
   }
   __syncthreads();
   if (w != 0) return;
   // equals that stay, and the starts of the chunks' equals and list entries
   int gt = 0;
   for (int c = lane; c < nc; c += 64) gt += cn[3 * c + 1];
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) gt += __shfl_xor(gt, off);
+  gt = __builtin_amdgcn_readlane(wave_scan(gt), 63);
   const int ties = want - gt;
   int eq0 = 0, hole0 = 0, move0 = 0;
+#pragma unroll 1
   for (int c0 = 0; c0 < nc; c0 += 64) {
     const int c = c0 + lane;
     int first = 0, end = 0;
     if (c < nc) chunk_range(g, n, c, first, end);
-    const bool live = c < nc && first < end;
-    const int eq = live ? cn[3 * c + 2] : 0;
-    int e = eq;
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-      const int z = __shfl_up(e, off);
-      if (lane >= off) e += z;
-    }
+    const bool some = c < nc && first < end;
+    const int eq = some ? cn[3 * c + 2] : 0;
+    const int e = wave_scan(eq);
     const int eq_at = eq0 + e - eq;
-    const int stay = live ? ca[4 * c] + cn[3 * c + 1] + min(max(ties - eq_at, 0), eq) : 0;
-    const int hole = live && c < g.nlo ? end - first - stay : 0, move = live && c >= g.nlo ? stay : 0;
-    int x = hole, y = move;
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-      const int z = __shfl_up(x, off), q = __shfl_up(y, off);
-      if (lane >= off) {
-        x += z;
-        y += q;
-      }
-    }
+    const int stay = some ? ca[kAt * c] + cn[3 * c + 1] + min(max(ties - eq_at, 0), eq) : 0;
+    const int hole = some && c < g.nlo ? end - first - stay : 0, move = some && c >= g.nlo ? stay : 0;
+    const int x = wave_scan(hole), y = wave_scan(move);
     if (c < nc) {
-      ca[4 * c + 2] = eq_at;
-      ca[4 * c + 3] = c < g.nlo ? hole0 + x - hole : move0 + y - move;
+      ca[kAt * c + 2] = eq_at;
+      ca[kAt * c + 3] = c < g.nlo ? hole0 + x - hole : move0 + y - move;
     }
     eq0 += __builtin_amdgcn_readlane(e, 63);
     hole0 += __builtin_amdgcn_readlane(x, 63);
     move0 += __builtin_amdgcn_readlane(y, 63);
   }
   if (lane == 0) {
-    g.rank[pair * 4 + 2] = (int32_t)T;
+    g.rank[pair * 4 + 1] = eq0;  // (the equals in all)
+    g.rank[pair * 4 + 2] = (int32_t)cut.T;
     g.rank[pair * 4 + 3] = ties;
     g.counts[pair] = min(min(hole0, move0), g.most);
   }
@@ -634,27 +800,38 @@ __global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(LongArgs g) {
 
 __global__ __launch_bounds__(kSelThreads) void evict_list_kernel(LongArgs g) {
   const SlotArgs& a = g.s;
-  const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nc = g.nlo + g.nhi;
+  const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nc = g.nlo + g.nhi, tid = threadIdx.x;
   const int n = rows_of(a, b);
   if (n <= g.keep) return;
   int first, end;
   chunk_range(g, n, c, first, end);
   if (first >= end) return;
   const int64_t pair = (int64_t)b * a.nkv + h;
-  const uint32_t* keys = g.keys + (pair * nc + c) * kChunk;
-  Keys<kChunkK> k;
+  const uint32_t* from = g.keys + (pair * nc + c) * kChunk;
+  __shared__ uint32_t k[key_each(kChunk) * kSelThreads];
+  __shared__ SelectLds L;
+  uint32_t x[kChunkK];
 #pragma unroll
   for (int i = 0; i < kChunkK; ++i) {
-    const int t = Keys<kChunkK>::slot(i);
-    k.k[i] = first + t < end ? keys[t] : 0u;
+    const int t = kSelThreads * i + tid;
+    x[i] = from[first + t < end ? t : 0];
   }
-  __shared__ int buf[6 * kSelWaves];
-  const int32_t* ca = g.chunk_at + (pair * nc + c) * 4;
+#pragma unroll
+  for (int i = 0; i < kChunkK; ++i) {
+    const int t = kSelThreads * i + tid;
+    k[t] = first + t < end ? x[i] : 0u;
+  }
+  k[kChunk + tid] = 0u;
+  const int32_t* ca = g.chunk_at + (pair * nc + c) * kAt;
+  const int32_t* rk = g.rank + pair * 4;
+  const int eq0 = ca[2], at = ca[3], equal = rk[1], ties = rk[3];
+  const uint32_t T = (uint32_t)rk[2];
   int32_t* dst = g.lists + pair * 2 * g.most;
-  int nm;
-  (void)list_slots<kChunkK>(k, first, end, g.keep, (uint32_t)g.rank[pair * 4 + 2], g.rank[pair * 4 + 3],
-                            ca[2], c < g.nlo, c >= g.nlo, dst, dst + g.most, ca[3], ca[3], g.most, buf,
-                            nm);
+  const bool lo = c < g.nlo;
+  __syncthreads();
+  int nh, nm;
+  list_slots(Keys{k, key_each(kChunk)}, first, end, g.keep, T, ties, equal, eq0, lo ? dst : nullptr,
+             lo ? nullptr : dst + g.most, at, at, g.most, L, nh, nm);
 }
 
 int launch_track(const SlotArgs& a, int M, int B, void* stream) {
@@ -664,37 +841,19 @@ int launch_track(const SlotArgs& a, int M, int B, void* stream) {
   return (int)hipGetLastError();
 }
 
-// Longest sequence the one-workgroup selection takes.
-constexpr int kSelMax = kSelThreads * 16;
-
-template <bool FUSE>
-void launch_select(const SlotArgs& a, int n, int keep, int recent, int most, int32_t* counts,
-                   int32_t* lists, int unit16, int B, hipStream_t st) {
-  auto go = [&](auto k) {
-    hipLaunchKernelGGL((evict_select_kernel<decltype(k)::value, FUSE>), dim3(a.nkv, B),
-                       dim3(kSelThreads), 0, st, a, keep, recent, most, counts, lists, unit16);
-  };
-  const int K = (n + kSelThreads - 1) / kSelThreads;
-  if (K <= 1) go(std::integral_constant<int, 1>{});
-  else if (K <= 2) go(std::integral_constant<int, 2>{});
-  else if (K <= 4) go(std::integral_constant<int, 4>{});
-  else if (K <= 6) go(std::integral_constant<int, 6>{});
-  else if (K <= 8) go(std::integral_constant<int, 8>{});
-  else if (K <= 12) go(std::integral_constant<int, 12>{});
-  else go(std::integral_constant<int, 16>{});
-}
-
 // n: rows of the longest sequence.
 int launch_evict(const SlotArgs& a, int n, int keep, int recent, int B, void* stream) {
   if (n <= keep || keep == 0 || B == 0) return 0;  // nothing moves
   const hipStream_t hs = (hipStream_t)stream;
   const int most = std::min(n - keep, keep);
   // units of 16 bytes where every row, head and token starts on one
+  const size_t key_bytes = sizeof(uint32_t) * kSelThreads * (size_t)key_each(std::min(n, kSelMax));
   const int unit16 = a.row % 16 == 0 && a.tok % 16 == 0 && a.head % 16 == 0 && a.block % 16 == 0;
   const int upr = (int)(a.row / (unit16 ? 16 : 4));
   if ((int64_t)most * upr > 0x70000000) return MOLOT_ENOTSUP;  // units of a head's moves
   if (n <= kSelMax && most <= kFuseMoves && (int64_t)most * a.row <= kFuseBytes) {
-    launch_select<true>(a, n, keep, recent, most, nullptr, nullptr, unit16, B, hs);
+    hipLaunchKernelGGL(evict_select_kernel<true>, dim3(a.nkv, B), dim3(kSelThreads), key_bytes, hs, a,
+                       keep, recent, most, nullptr, nullptr, unit16);
     return (int)hipGetLastError();
   }
   const size_t pairs = (size_t)B * a.nkv;
@@ -706,24 +865,25 @@ int launch_evict(const SlotArgs& a, int n, int keep, int recent, int B, void* st
   g.nlo = (keep + kChunk - 1) / kChunk;
   g.nhi = (n - keep + kChunk - 1) / kChunk;
   const size_t nc = n <= kSelMax ? 0 : (size_t)g.nlo + g.nhi;
-  const size_t lds = sizeof(int32_t) * 3 * nc;
-  if (lds > 128 * 1024) return MOLOT_ENOTSUP;  // 89 million rows
-  // [lists | counts | rank, chunk_at | keys | listed | bins]
-  const size_t words = pairs * (2 * (size_t)most + 1 + (nc ? 4 + 4 * nc + 2 * nc * kChunk + nc * (kBins / 2) : 0));
+  const size_t lds = sizeof(int32_t) * (kRankMax + 3 * nc);
+  if (lds + sizeof(SelectLds) > kMaxLds) return MOLOT_ENOTSUP;  // past 40 million rows
+  // [bins | lists | counts | rank, chunk_at | keys | listed]
+  const size_t words = pairs * (2 * (size_t)most + 1 + (nc ? 4 + kAt * nc + 2 * nc * kChunk + nc * (kBins / 2) : 0));
   unsigned long long* ctr = nullptr;
   void* ws = nullptr;
   int st = workspace(stream, sizeof(int32_t) * words, &ctr, &ws);
   if (st) return st;
-  g.lists = reinterpret_cast<int32_t*>(ws);
+  g.bins = reinterpret_cast<uint16_t*>(ws);
+  g.lists = reinterpret_cast<int32_t*>(ws) + pairs * nc * (kBins / 2);
   g.counts = g.lists + pairs * 2 * most;
   if (!nc) {
-    launch_select<false>(a, n, keep, recent, most, g.counts, g.lists, unit16, B, hs);
+    hipLaunchKernelGGL(evict_select_kernel<false>, dim3(a.nkv, B), dim3(kSelThreads), key_bytes, hs, a,
+                       keep, recent, most, g.counts, g.lists, unit16);
   } else {
     g.rank = g.counts + pairs;
     g.chunk_at = g.rank + 4 * pairs;
-    g.keys = reinterpret_cast<uint32_t*>(g.chunk_at + 4 * pairs * nc);
+    g.keys = reinterpret_cast<uint32_t*>(g.chunk_at + kAt * pairs * nc);
     g.listed = g.keys + pairs * nc * kChunk;
-    g.bins = reinterpret_cast<uint16_t*>(g.listed + pairs * nc * kChunk);
     const dim3 chunks((unsigned)nc, a.nkv, B), block(kSelThreads);
     hipLaunchKernelGGL(evict_keys_kernel, chunks, block, 0, hs, g);
     hipLaunchKernelGGL(evict_pick_kernel, chunks, block, 0, hs, g);

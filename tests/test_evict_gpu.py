@@ -83,6 +83,61 @@ def test_rule(gpu, n, keep, recent, kind):
         assert torch.equal(raw(got), raw(exp))
 
 
+@pytest.mark.parametrize("kind", ["smooth", "ties", "equal", "odd", "zeros"])
+@pytest.mark.parametrize("n,keep,recent", [(16384, 16000, 500), (16385, 16000, 500), (20001, 8192, 3),
+                                           (40000, 39999, 0), (40000, 1, 0), (60000, 24576, 40000),
+                                           (33333, 30000, 2500)])
+def test_rule_long(gpu, n, keep, recent, kind):
+    """Caches past one workgroup's: chunks on both sides of keep, up to one bin of them."""
+    nkv, d, pos = 2, 2, n - 1
+    g = gen(n + keep)
+    acc = weights(g, "smooth" if kind == "zeros" else kind, nkv, n)
+    if kind == "zeros":  # most rows never seen
+        acc = torch.where(torch.rand(nkv, n, device="cuda", generator=g) < 0.9, torch.zeros_like(acc), acc)
+    sp = torch.stack([torch.randperm(n, device="cuda", generator=g) for _ in range(nkv)]).int()
+    K = torch.randn(n, nkv * d, device="cuda", generator=g)
+    V = torch.randn(n, nkv * d, device="cuda", generator=g)
+    want = [x.clone() for x in (K, V, acc, sp)]
+    for h, moves in enumerate(ref.evict(acc.cpu(), sp.cpu(), n, keep, recent, pos)):
+        if not moves:
+            continue
+        to, at = (torch.tensor([m[i] for m in moves], device="cuda") for i in (0, 1))
+        for x in want[:2]:
+            rows = x.view(-1, nkv, d)
+            rows[to, h] = rows[at, h]
+        for x in want[2:]:
+            x[h, to] = x[h, at]
+    attn.kv_evict(K, V, acc, sp, nkv, n, d, keep, recent, pos)
+    for got, exp in zip((K, V, acc, sp), want):
+        assert torch.equal(raw(got), raw(exp))
+
+
+def test_paged_long(gpu):
+    """Sequences on either side of the one-workgroup limit in a batch."""
+    kv, nkv, d, page, lens, keep, recent = "f32", 2, 4, 32, (17000, 20, 9000, 30001), 8000, 100
+    g = gen(8)
+    table, blocks, pools = paged(g, kv, nkv, d, lens, page)
+    acc = weights(g, "smooth", blocks, nkv * page).view(blocks, nkv, page)
+    sp = torch.randint(0, 30000, (blocks, nkv, page), device="cuda", generator=g).int()
+    want_acc, want_sp, want = acc.clone(), sp.clone(), [p.clone() for p in pools]
+    for b, n in enumerate(lens):
+        if n <= keep:
+            continue
+        t = torch.arange(n)
+        blk, sl = table[b].long()[t // page].cuda(), (t % page).cuda()
+        a, p = acc[blk, :, sl].T.cpu(), sp[blk, :, sl].T.cpu()
+        for h, moves in enumerate(ref.evict(a, p, n, keep, recent, n - 1)):
+            to, at = (torch.tensor([m[i] for m in moves], device="cuda") for i in (0, 1))
+            for x in [want_acc, want_sp] + [w.view(blocks, nkv, page, d) for w in want]:
+                x[blk[to], h, sl[to]] = x[blk[at], h, sl[at]]
+    L = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    attn.kv_evict_paged(*pools, acc, sp, table.cuda(), L, None, len(lens), table.shape[1], nkv, d, page,
+                        keep, recent)
+    assert torch.equal(raw(acc), raw(want_acc)) and torch.equal(sp, want_sp)
+    for x, y in zip(pools, want):
+        assert torch.equal(raw(x), raw(y))
+
+
 @pytest.mark.parametrize("kv,nkv,d", [("f32", 8, 128), ("bf16", 8, 128), ("q8", 8, 128), ("bf16", 5, 6),
                                       ("q8", 3, 4), ("q8", 2, 512), ("f32", 1, 2), ("f32", 2, 510)])
 def test_rows(gpu, kv, nkv, d):

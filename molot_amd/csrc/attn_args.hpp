@@ -74,7 +74,8 @@ struct AttnArgs {
   const int32_t* key_lo;
   const int32_t* key_hi;
   // The weights (acc): the launch leaves its scores, in base-2 units, at
-  // scores[(sequence, KV head)][sc_rows rows from t0][nq / nkv heads] and each
+  // scores[(sequence, KV head)][sc_rows rows from t0][nq / nkv heads] (the
+  // matrix-core kernel: [sc_rows / 4][heads][4 rows]) and each
   // chunk's (max in base 2, sum) at stats[slot][nchunks][GH] for
   // attn_weights_kernel, which adds the softmax weights to acc (layout of the
   // C ABI) (NULL: no weights).  fresh: slot n - 1 was appended by this call: its

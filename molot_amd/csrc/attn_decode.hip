@@ -1555,6 +1555,7 @@ struct WeightArgs {
   const int32_t* block_table;
   int64_t sc_rows;
   int n, t0, pos, max_blocks, page_shift, acc_cap, fresh;
+  int blocked;  // the scores in the matrix-core kernel's order
 };
 constexpr int kWeightThreads = 256;
 
@@ -1605,16 +1606,21 @@ __device__ __forceinline__ void weigh_rows(const WeightArgs& w, int rb, int h, i
   __syncthreads();
   if (row0 + tid >= span) return;
   const int t = t0 + row0 + tid;
-  const float* s = w.scores + (((int64_t)b * w.c.nkv + h) * w.sc_rows + row0 + tid) * G;
+  const float* s = w.scores + ((int64_t)b * w.c.nkv + h) * w.sc_rows * G;
+  const int row = row0 + tid;
   float sum = 0.f;
-  if ((G & 3) == 0) {
+  if (w.blocked) {
+    const float* x = s + (int64_t)(row & ~3) * G + (row & 3);
+#pragma unroll 8
+    for (int g = 0; g < G; ++g) sum = fmaf(exp2_hw(x[4 * g] - mx[g]), inv[g], sum);
+  } else if ((G & 3) == 0) {
     for (int g = 0; g < G; g += 4) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(s + g);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(s + (int64_t)row * G + g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum = fmaf(exp2_hw(x[e] - mx[g + e]), inv[g + e], sum);
     }
   } else {
-    for (int g = 0; g < G; ++g) sum = fmaf(exp2_hw(s[g] - mx[g]), inv[g], sum);
+    for (int g = 0; g < G; ++g) sum = fmaf(exp2_hw(s[(int64_t)row * G + g] - mx[g]), inv[g], sum);
   }
   const int64_t i = index(t);
   const bool set = w.fresh && t == n - 1;
@@ -2014,7 +2020,7 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
   if ((long)rows > kMaxSlots) return MOLOT_ENOTSUP;
   if (stats) {  // the scores of every attended row, for the weights
     if (B > 65535) return MOLOT_ENOTSUP;  // attn_weights_kernel's grid
-    a.sc_rows = std::max(span, 0) + 1;
+    a.sc_rows = (std::max(span, 0) + 4) & ~3;  // (and the appended row)
     const size_t bytes = sizeof(float) * (size_t)B * a.nq * a.sc_rows;
     if (bytes > kMaxPiecesBytes) return MOLOT_ENOTSUP;
     void* sc = nullptr;
@@ -2123,6 +2129,7 @@ WeightArgs weight_args(const CombArgs& cb, const AttnArgs& a) {
   w.page_shift = a.page_shift;
   w.acc_cap = a.acc_cap;
   w.fresh = a.fresh;
+  w.blocked = a.matrix;
   return w;
 }
 

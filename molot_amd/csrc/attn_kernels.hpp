@@ -1078,11 +1078,12 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
 
   // SC: the cap and the heads' slopes in base-2 units, and this (sequence, KV
   // head)'s scores (row t at (t - t0) * G)
-  [[maybe_unused]] float slope[GH], cap2 = 0.f, rcap = 0.f;
+  static_assert(!SC || (LPR >= GH && LPR % GH == 0), "a lane of a row for every head");
+  [[maybe_unused]] float slope = 0.f, cap2 = 0.f, rcap = 0.f;  // of head s % GH
+  [[maybe_unused]] float m_own = -INFINITY;                    // and its running max
   [[maybe_unused]] float* swr = nullptr;
   if constexpr (SC) {
-#pragma unroll
-    for (int g = 0; g < GH; ++g) slope[g] = a.slopes ? a.slopes[hq0 + g] * kLog2e : 0.f;
+    if (a.slopes) slope = a.slopes[hq0 + s % GH] * kLog2e;
     cap2 = a.softcap * kLog2e;
     rcap = a.softcap > 0.f ? 1.f / cap2 : 0.f;
     if (a.scores) swr = a.scores + ((int64_t)b * a.nkv + h) * a.sc_rows * G + sub * GH;
@@ -1143,36 +1144,61 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
       }
     }
     if constexpr (SC) {
-      if (a.softcap > 0.f) {
-#pragma unroll
-        for (int k = 0; k < KS; ++k) cap_scores<GH>(sc[k], cap2, rcap);
-      }
+      // Every lane of a row holds the row's GH sums; from here on lane s takes head
+      // s % GH alone: one cap, bias, comparison and exponential a row instead of GH
+      // (32q/8kv/d128 fp32, 16385 rows, cap and slopes: SCORED_FIGURES).
+      const int g0 = s % GH;
+      float x[KS];
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        const int lr = rbase + k * RPS + rr;
-        const bool valid = lr < nrows;
-        const int t = rfirst + min(gmap(lr), rmax);
-        const float dist = fabsf((float)(pos - t));
+        x[k] = sc[k][0];
 #pragma unroll
-        for (int g = 0; g < GH; ++g) {
-          const float x = fmaf(-slope[g], dist, sc[k][g]);
-          sc[k][g] = valid ? x : -INFINITY;
-          bmax[g] = fmaxf(bmax[g], sc[k][g]);
-        }
-        if (swr && s == 0 && valid && t - t0 < a.sc_rows) {
-          float* w0 = swr + (int64_t)(t - t0) * G;  // GH | G: aligned as a GH-vector
-          if constexpr (GH % 4 == 0) {
+        for (int g = 1; g < GH; ++g) x[k] = g0 == g ? sc[k][g] : x[k];
+      }
+      if (a.softcap > 0.f) cap_scores<KS>(x, cap2, rcap);
+      // rows of a block follow each other in the cache (blocks lie within 32-row groups)
+      const int t_lane = rfirst + gmap(rbase) + rr;
+      float top = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < GH; g += 4)
-              *reinterpret_cast<f32x4*>(w0 + g) =
-                  f32x4{sc[k][g], sc[k][g + 1], sc[k][g + 2], sc[k][g + 3]};
-          } else {
+      for (int k = 0; k < KS; ++k) {
+        const float y = fmaf(-slope, fabsf((float)(pos - t_lane - k * RPS)), x[k]);
+        x[k] = rbase + k * RPS + rr < nrows ? y : -INFINITY;
+        top = fmaxf(top, x[k]);
+      }
+      if (swr && s < GH) {
 #pragma unroll
-            for (int g = 0; g < GH; ++g) w0[g] = sc[k][g];
-          }
+        for (int k = 0; k < KS; ++k) {
+          const int at = t_lane + k * RPS - t0;
+          if (rbase + k * RPS + rr < nrows && at < a.sc_rows) swr[(int64_t)at * G + s] = x[k];
         }
       }
-    }
+      if (__builtin_amdgcn_ballot_w64(top > m_own + kLazyMax) != 0) {  // wave-uniform
+        auto top_off = [&](auto OFFC) {
+          constexpr int off = decltype(OFFC)::value;
+          if constexpr (off >= LPR) top = max_xor<off>(top);
+        };
+        top_off(std::integral_constant<int, 1>{});
+        top_off(std::integral_constant<int, 2>{});
+        top_off(std::integral_constant<int, 4>{});
+        top_off(std::integral_constant<int, 8>{});
+        top_off(std::integral_constant<int, 16>{});
+        top_off(std::integral_constant<int, 32>{});
+        const float mn = fmaxf(m_own, top);
+        const float alpha = exp2_hw(m_own - mn);  // m_own = -inf -> 0
+        m_own = mn;
+#pragma unroll
+        for (int g = 0; g < GH; ++g) {
+          const float al = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(alpha), g));
+          l_run[g] *= al;
+#pragma unroll
+          for (int e = 0; e < AW; ++e) acc[g][e] *= al;
+        }
+      }
+      if (s < GH) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) pw[(k * RPS + rr) * GH + s] = exp2_hw(x[k] - m_own);
+      }
+    } else {
     // The running max moves only when a score passes it by more than
     // kLazyMax (p <= 2^8 otherwise; o and l always share the max they were
     // formed with): most blocks skip the block max across the wave's row
@@ -1207,6 +1233,7 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
 #pragma unroll
         for (int g = 0; g < GH; ++g) pw[(k * RPS + rr) * GH + g] = exp2_hw(sc[k][g] - m_run[g]);
       }
+    }
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -1272,6 +1299,12 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
     }
   }
 
+  if constexpr (SC) {
+#pragma unroll
+    for (int g = 0; g < GH; ++g)
+      m_run[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_own), g));
+  }
+
   // ---- 3. the new token, folded in by wave 0 from LDS (its append to the
   // cache comes last, below) ----
   // Q8: wave 0 quantizes the k and v rows as the cache will hold them (the
@@ -1331,7 +1364,8 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
       const float dist = fabsf((float)(pos - (n - 1)));
 #pragma unroll
       for (int g = 0; g < GH; ++g) {
-        part[g] = fmaf(-slope[g], dist, part[g]);
+        const float sl = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(slope), g));
+        part[g] = fmaf(-sl, dist, part[g]);
         if (swr && lane == 0 && n - 1 - t0 < a.sc_rows) swr[(int64_t)(n - 1 - t0) * G + g] = part[g];
       }
     }
@@ -1960,7 +1994,8 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
     if (a.slopes && m16 < GH) slope = a.slopes[hq0 + m16] * kLog2e;
     cap2 = a.softcap * kLog2e;
     rcap = a.softcap > 0.f ? 1.f / cap2 : 0.f;
-    if (a.scores && m16 < GH) swr = a.scores + ((int64_t)b * a.nkv + h) * a.sc_rows * G + sub * GH + m16;
+    if (a.scores && m16 < GH)
+      swr = a.scores + ((int64_t)b * a.nkv + h) * a.sc_rows * G + 4 * (sub * GH + m16);
   }
 
   // ---- stream ----
@@ -2058,7 +2093,20 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
         const float y = fmaf(-slope, fabsf((float)(pos - t)), x[i]);
         sv[i / 4][i % 4] = row < rlim ? y : -INFINITY;
         tmax = fmaxf(tmax, sv[i / 4][i % 4]);
-        if (swr && row < rlim && t - t0 < a.sc_rows) swr[(int64_t)(t - t0) * G] = y;
+      }
+      if (swr) {  // rows 16u + 4*g4 .. +3 of a head side by side (chunks start at multiples of 4)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = tile_row(tile) + 16 * u + 4 * g4, at = rfirst - t0 + row;
+          float* to = swr + (int64_t)at * G;
+          if (at + 4 > a.sc_rows) continue;
+          if (row + 4 <= rlim)
+            *reinterpret_cast<f32x4*>(to) = f32x4{sv[u][0], sv[u][1], sv[u][2], sv[u][3]};
+          else
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (row + r < rlim) to[r] = sv[u][r];
+        }
       }
     } else
 #pragma unroll
@@ -2158,7 +2206,8 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
       float x[1] = {snew};
       if (a.softcap > 0.f) cap_scores<1>(x, cap2, rcap);
       snew = fmaf(-slope, fabsf((float)(pos - (n - 1))), x[0]);
-      if (swr && g4 == 0 && n - 1 - t0 < a.sc_rows) swr[(int64_t)(n - 1 - t0) * G] = snew;
+      const int at = n - 1 - t0;
+      if (swr && g4 == 0 && at < a.sc_rows) swr[(int64_t)(at & ~3) * G + (at & 3)] = snew;
     }
     const float mn = fmaxf(m_run, snew);
     const float alpha = exp2_hw(m_run - mn);

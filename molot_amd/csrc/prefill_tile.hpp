@@ -199,11 +199,14 @@ __device__ __forceinline__ void block_keys(const PfArgs& a, int m0, int m1, int&
 struct RowScore {
   float cap2 = 0.f, rcap = 0.f, slope = 0.f;
   int pos = 0;
+  bool sloped = false;
   template <int N, typename SLOT>
   __device__ __forceinline__ void apply(float (&s)[N], SLOT&& slot) const {
-    if (cap2 > 0.f) cap_scores<N>(s, cap2, rcap);  // wave-uniform
+    if (cap2 > 0.f) cap_scores<N>(s, cap2, rcap);  // wave-uniform, as the next
+    if (sloped) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) s[e] = fmaf(-slope, fabsf((float)(pos - slot(e))), s[e]);
+      for (int e = 0; e < N; ++e) s[e] = fmaf(-slope, fabsf((float)(pos - slot(e))), s[e]);
+    }
   }
 };
 template <typename A>
@@ -214,7 +217,8 @@ __device__ __forceinline__ RowScore row_score(const A& a, int m, int head) {
     r.cap2 = a.softcap * kLog2e;
     r.rcap = 1.f / r.cap2;
   }
-  if (a.slopes) r.slope = a.slopes[head] * kLog2e;
+  r.sloped = a.slopes != nullptr;
+  if (r.sloped) r.slope = a.slopes[head] * kLog2e;
   return r;
 }
 

@@ -1492,7 +1492,9 @@ __device__ __forceinline__ void load_v(const float* p, float* x) {
     x[0] = *p;
   }
 }
-template <int R, int V>
+// SOME: rows may have fewer splits than the launch, or be done (prefill_tile.hpp,
+// block_splits): the statistics first, then the partials that count.
+template <int R, int V, bool SOME = false>
 __global__ __launch_bounds__(kCombWaveThreads) void combine_rows_kernel(CombArgs a, int64_t units) {
   const int D = a.d;
   const int spans = D / (64 * V);
@@ -1504,11 +1506,21 @@ __global__ __launch_bounds__(kCombWaveThreads) void combine_rows_kernel(CombArgs
   const float* po = a.part_o + slot * a.nchunks * D + pair;
   const float* pml = a.part_ml + slot * a.nchunks * 2;
   float ov[R][V];
+  if constexpr (!SOME) {
 #pragma unroll
-  for (int u = 0; u < R; ++u) load_v<V>(po + (int64_t)min(u, a.nchunks - 1) * D, ov[u]);
+    for (int u = 0; u < R; ++u) load_v<V>(po + (int64_t)min(u, a.nchunks - 1) * D, ov[u]);
+  }
   const int cl = min(lane, a.nchunks - 1);
   const f32x2 ml = *reinterpret_cast<const f32x2*>(pml + 2 * cl);
-  const int nch = a.nchunks;
+  int nch = a.nchunks;
+  if constexpr (SOME) {
+    if (__int_as_float(__builtin_amdgcn_readlane(__float_as_int(ml[1]), 0)) < 0.f) return;
+    // (splits without a key, the ones past a block's among them, weigh nothing and come
+    // last but for a row's own: those before them have finite partials)
+    nch = 64 - __builtin_clzll(__builtin_amdgcn_ballot_w64(lane < nch && ml[1] != 0.f) | 1ull);
+#pragma unroll
+    for (int u = 0; u < R; ++u) load_v<V>(po + (int64_t)min(u, nch - 1) * D, ov[u]);
+  }
   const bool live = lane < nch;
   const float M = wave_reduce<true>(live ? ml[0] : -INFINITY);
   const float wc = live && M != -INFINITY ? softmax_exp(ml[0] - M) : 0.f;
@@ -3085,7 +3097,13 @@ static int launch_prefill(PfFn pk, int64_t wgs, int threads, const PfArgs& a, in
   const int cv = D % 256 == 0 ? 4 : (D % 128 == 0 ? 2 : 1);
   const int64_t cunits = (int64_t)a.M * a.nq * (D / (64 * cv));
   using RowsFn = void (*)(CombArgs, int64_t);
-  const RowsFn rk = nsplit <= 4 ? (cv == 4 ? combine_rows_kernel<4, 4>
+  const RowsFn rk = a.some ? (nsplit <= 4 ? (cv == 4 ? combine_rows_kernel<4, 4, true>
+                                           : cv == 2 ? combine_rows_kernel<4, 2, true>
+                                                     : combine_rows_kernel<4, 1, true>)
+                                        : (cv == 4 ? combine_rows_kernel<8, 4, true>
+                                           : cv == 2 ? combine_rows_kernel<8, 2, true>
+                                                     : combine_rows_kernel<8, 1, true>))
+                  : nsplit <= 4 ? (cv == 4 ? combine_rows_kernel<4, 4>
                                   : cv == 2 ? combine_rows_kernel<4, 2> : combine_rows_kernel<4, 1>)
                                 : (cv == 4 ? combine_rows_kernel<8, 4>
                                   : cv == 2 ? combine_rows_kernel<8, 2> : combine_rows_kernel<8, 1>);
@@ -3317,6 +3335,7 @@ static int prefill_on_pieces(const float* Qm, const void* K, const void* V, floa
     }
   }
   if (nqb * nkv * a.nsplit > (int64_t)0x7FFFFFFF) return MOLOT_ENOTSUP;
+  a.some = sc.on && a.nsplit > 1 && a.nsplit <= 8;  // (more splits: combine_kernel, which reads all)
   a.Rsplit = split_rows < 0 ? a.R : std::min(split_rows, a.R);
   if (a.Rsplit > 0) {
     const int64_t units = (a.Rsplit == a.R ? wide_padded_rows(a.R) : a.Rsplit) * (D / 8);

@@ -36,6 +36,7 @@ struct PfArgs {
   const float* slopes;
   const int32_t* key_lo;
   const int32_t* key_hi;
+  int some;  // a block of few tiles takes fewer than nsplit splits (block_splits)
 };
 
 using PfFn = void (*)(PfArgs);

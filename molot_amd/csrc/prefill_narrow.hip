@@ -85,8 +85,16 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
   int kt_lo, kt_hi;
   block_keys<SC>(a, r0 / G, rl / G, kt_lo, kt_hi);
   const int ntile_all = kt_hi > kt_lo ? (kt_hi - kt_lo + KT - 1) / KT : 0;
-  const int tb0 = (int)((int64_t)sp * ntile_all / a.nsplit);
-  const int ntile = (int)((int64_t)(sp + 1) * ntile_all / a.nsplit) - tb0;
+  const int nsplit = block_splits<SC>(a, ntile_all);
+  if constexpr (SC) {
+    if (sp >= nsplit) {  // (the whole workgroup)
+      mark_split<QB>(a, h, r0, sp, 0.f);
+      return;
+    }
+    if (nsplit == 1 && a.nsplit > 1) mark_split<QB>(a, h, r0, sp, -1.f);
+  }
+  const int tb0 = (int)((int64_t)sp * ntile_all / nsplit);
+  const int ntile = (int)((int64_t)(sp + 1) * ntile_all / nsplit) - tb0;
   const int kt_s = kt_lo + tb0 * KT;
   const int nint = (ntile + 1) / 2;
 
@@ -372,7 +380,7 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
   const f32x4 st = ml[c32];
   if constexpr (OWN) {
     if (redo + st[3] != 0.f) {  // wave-uniform
-      own_rows<D, SC>(own_args(), h, r0 + 32 * rg, 32, kt_s, kt_s + ntile * KT, sp);
+      own_rows<D, SC>(own_args(), h, r0 + 32 * rg, 32, kt_s, kt_s + ntile * KT, sp, nsplit > 1);
       return;
     }
   }
@@ -382,7 +390,7 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
   const float f0 = exp2_hw(rs.m - M), f1 = exp2_hw(st[1] - M);
   const int e0 = -rs.wsh, e1 = -(int)st[2];
   const float l = fmaf(rs.l, f0, st[0] * f1);
-  const bool part = a.nsplit > 1;
+  const bool part = nsplit > 1;
   const float inv = l > 0.f ? 1.f / l : 0.f;  // no key: O = 0 (gemm.h:438)
   const int64_t ps = slot * a.nsplit + sp;
   float* po = part ? a.part_o + ps * D : a.o + slot * a.dh;

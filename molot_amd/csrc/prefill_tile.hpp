@@ -194,32 +194,65 @@ __device__ __forceinline__ void block_keys(const PfArgs& a, int m0, int m1, int&
   hi = __builtin_amdgcn_readfirstlane(h);
 }
 
+// Splits of a query block of `tiles` key tiles (SC launches that say so: the host knows
+// neither the ranges nor how uneven the blocks are): none below kSplitTiles tiles,
+// whose start and merge cost as much as they take.  The workgroups past them leave
+// (-inf, 0) statistics; a block of one split writes O itself and a sum of -1, which
+// ends its rows' merge.  us a pass by kSplitTiles (8q/4kv/d256 bf16; 8q/2kv/d512 fp32),
+// every block split alike first:
+//   2048 tokens in documents of 37 to 592   61; 95    4: 60.6; 81.3   6: 49.7; 80.0   8: 53.6; 84.2
+//   causal, 2048; 1999 tokens               97; 165   4: 95.7; 162.7  6: 96.0; 163.5  8: 100; 167
+constexpr int kSplitTiles = 6;
+template <bool SC>
+__device__ __forceinline__ int block_splits(const PfArgs& a, int tiles) {
+  if (!SC || !a.some) return a.nsplit;
+  return max(1, min(a.nsplit, (tiles + kSplitTiles - 1) / kSplitTiles));
+}
+// The statistics of split sp of the rows r0 .. of a block of QB, where the split has no
+// part in them (l = 0) or the block wrote its output itself (l = -1).
+template <int QB>
+__device__ __forceinline__ void mark_split(const PfArgs& a, int h, int r0, int sp, float l) {
+  const int G = a.nq / a.nkv, row = r0 + (int)threadIdx.x;
+  if (threadIdx.x >= QB || row >= a.M * G) return;
+  const int m = row / G;
+  const int64_t ps = ((int64_t)m * a.nq + h * G + (row - m * G)) * a.nsplit + sp;
+  *reinterpret_cast<f32x2*>(a.part_ml + 2 * ps) = f32x2{-INFINITY, l};
+}
+
 // A scored launch's scores of one query row: N of them in base-2 units at slots
 // t(e), to the capped and biased ones.
 struct RowScore {
   float cap2 = 0.f, rcap = 0.f, slope = 0.f;
   int pos = 0;
-  bool sloped = false;
   template <int N, typename SLOT>
   __device__ __forceinline__ void apply(float (&s)[N], SLOT&& slot) const {
-    if (cap2 > 0.f) cap_scores<N>(s, cap2, rcap);  // wave-uniform, as the next
-    if (sloped) {
+    if (cap2 > 0.f) cap_scores<N>(s, cap2, rcap);           // wave-uniform, as the next
+    if (__builtin_amdgcn_ballot_w64(slope != 0.f) != 0) {  // (a flag would be one more register)
 #pragma unroll
       for (int e = 0; e < N; ++e) s[e] = fmaf(-slope, fabsf((float)(pos - slot(e))), s[e]);
     }
   }
 };
 template <typename A>
-__device__ __forceinline__ RowScore row_score(const A& a, int m, int head) {
+__device__ __forceinline__ RowScore row_score_of(const A& a, float slope, int pos) {
   RowScore r;
-  r.pos = a.pos0 + m;
+  r.pos = pos;
+  r.slope = slope;
   if (a.softcap > 0.f) {
     r.cap2 = a.softcap * kLog2e;
     r.rcap = 1.f / r.cap2;
   }
-  r.sloped = a.slopes != nullptr;
-  if (r.sloped) r.slope = a.slopes[head] * kLog2e;
   return r;
+}
+template <typename A>
+__device__ __forceinline__ RowScore row_score(const A& a, int m, int head) {
+  return row_score_of(a, a.slopes ? a.slopes[head] * kLog2e : 0.f, a.pos0 + m);
+}
+
+// Lane K of each quad's value, in all four.
+template <int K>
+__device__ __forceinline__ int quad_lane(int x) {
+  return __builtin_amdgcn_mov_dpp(x, K * 0x55, 0xF, 0xF, true);
 }
 
 // The address of the kernel's arguments (a PfArgs, its only parameter), to be
@@ -233,13 +266,13 @@ __device__ __forceinline__ uint64_t own_args() {
 
 // Query rows [row0, row0 + n) of KV head h over their own keys of [k_lo, k_hi),
 // a row at a time (every lane of the wave takes part), for the launch's split
-// sp.  Meant for caches that hold non-finite values; two keys in flight.  The
+// sp (part: to the splits' partials, else to O).  Meant for caches that hold non-finite values; two keys in flight.  The
 // arguments are read again from args (own_args), where the compiler cannot move
 // the loads ahead: kept in registers through the kernel's loop they would
 // spill.
 template <int D, bool SC = false>
 __device__ __forceinline__ void own_rows(uint64_t args, int h, int row0, int n, int k_lo, int k_hi,
-                                         int sp) {
+                                         int sp, bool part) {
   const auto* ka = (const __attribute__((address_space(4))) PfArgs*)args;
   PfArgs a{};
   a.q = ka->q, a.k = ka->k, a.v = ka->v, a.o = ka->o, a.block_table = ka->block_table;
@@ -310,7 +343,6 @@ __device__ __forceinline__ void own_rows(uint64_t args, int h, int row0, int n, 
         for (int i = 0; i < EPL; ++i) o[i] = fmaf(p, v[u][i], o[i]);
       }
     }
-    const bool part = a.nsplit > 1;
     const int64_t ps = slot * a.nsplit + sp;
     const float inv = part ? 1.f : l == 0.f ? 0.f : 1.f / l;  // no key: O = 0 (gemm.h:438)
 #pragma unroll

@@ -135,8 +135,16 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   int kt_lo, kt_hi;
   block_keys<SC>(a, r0 / G, rl / G, kt_lo, kt_hi);
   const int ntile_all = kt_hi > kt_lo ? (kt_hi - kt_lo + KT - 1) / KT : 0;
-  const int tb0 = (int)((int64_t)sp * ntile_all / a.nsplit);
-  const int ntile = (int)((int64_t)(sp + 1) * ntile_all / a.nsplit) - tb0;
+  const int nsplit = block_splits<SC>(a, ntile_all);
+  if constexpr (SC) {
+    if (sp >= nsplit) {  // (the whole workgroup)
+      mark_split<QB>(a, h, r0, sp, 0.f);
+      return;
+    }
+    if (nsplit == 1 && a.nsplit > 1) mark_split<QB>(a, h, r0, sp, -1.f);
+  }
+  const int tb0 = (int)((int64_t)sp * ntile_all / nsplit);
+  const int ntile = (int)((int64_t)(sp + 1) * ntile_all / nsplit) - tb0;
   const int kt_s = kt_lo + tb0 * KT;
 
   const int64_t Rp = wide_padded_rows(a.R);
@@ -146,13 +154,14 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   // K or V of the tile at key tk into LDS: 1 KB blocks of 1024/RB rows, wave
   // w blocks w, w + 8, ...; lane l's 16 bytes land at block + 16*l, so it
   // loads the unit the swizzle keeps there
+  constexpr int UPR = D / 8, RPB = 64 / UPR, BPP = KT / RPB;  // units of a row, rows and blocks of a copy
+  // (f(rb + r_in) = f(rb) ^ f(r_in): rb is a multiple of RPB)
+  uint32_t kofs = lane / UPR * RB + 16 * (lane % UPR ^ wk_f<D>(lane / UPR));
+  uint32_t vofs = lane / UPR * RB + 16 * (lane % UPR ^ wv_f<D>(lane / UPR));
   auto copy1 = [&](int t, int tk, char* buf, const uint16_t* head, bool isv) {
-    constexpr int UPR = D / 8, RPB = 64 / UPR, BPP = KT / RPB;
-    const int r_in = lane / UPR, jpos = lane % UPR;
     const int bi = w + 8 * t;  // wave-uniform
     const int pc = bi / BPP, rb = (bi % BPP) * RPB;
-    const int ch = jpos ^ (isv ? wv_f<D>(rb + r_in) : wk_f<D>(rb + r_in));
-    dma16(head + (pc * Rp + (tk - a.T0) + rb) * D, (uint32_t)(r_in * RB + 16 * ch),
+    dma16(head + (pc * Rp + (tk - a.T0) + rb) * D, isv ? vofs ^ 16 * wv_f<D>(rb) : kofs ^ 16 * wk_f<D>(rb),
           (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(buf + bi * 1024));
   };
   auto stage = [&](int tk, char* buf, const uint16_t* head, bool isv) {
@@ -224,14 +233,17 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   const int orr = lane / LPR, oc = lane % LPR;
   int rt0, rnn;
   float qunit;
-  [[maybe_unused]] RowScore rsc;
+  [[maybe_unused]] int rcon;  // SC: the row's rt0, rnn, slope and position, in lanes 0 .. 3 of a quad
   {
     const int row = r0 + 32 * rg + RPO * sl + orr;
     const bool orv = row < rows;
     const int m = orv ? row / G : 0;
     rt0 = orv ? t0_of(m) : 0;  // a row past the last: any keys (not stored)
     rnn = orv ? nn_of(m) : 0x7FFFFFFF;
-    if constexpr (SC) rsc = row_score(a, m, h * G + (orv ? row - m * G : 0));
+    if constexpr (SC) {
+      const RowScore r = row_score(a, m, h * G + (orv ? row - m * G : 0));
+      rcon = (oc & 3) == 0 ? rt0 : (oc & 3) == 1 ? rnn : (oc & 3) == 2 ? __float_as_int(r.slope) : r.pos;
+    }
     const float* qmx = reinterpret_cast<const float*>(sx);
     float qm = 0.f;
 #pragma unroll
@@ -263,14 +275,14 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   const char* p_ld = region(my_ow) + (NSL == 4 ? (my_ow & 1) * 128 : 0) + my_rr * 16;
   char* p_st = region(sl) + (NSL == 4 ? (sl & 1) * 128 : 0) + orr * 16;
 
-  const float* kun = reinterpret_cast<const float*>(khead + NP * Rp * D) - a.T0 + KPL * oc;
-  const float* vun = reinterpret_cast<const float*>(vhead + NP * Rp * D) - a.T0 + KPL * oc;
+  const float* kun = reinterpret_cast<const float*>(khead + NP * Rp * D) - a.T0;
+  const float* vun = reinterpret_cast<const float*>(vhead + NP * Rp * D) - a.T0;
   float ku[KPL], vu[KPL];
   auto load_units = [&](int tk) {
 #pragma unroll
     for (int q = 0; q < KPL; q += 4) {
-      const f32x4_u x = *reinterpret_cast<const f32x4_u*>(kun + tk + q);
-      const f32x4_u y = *reinterpret_cast<const f32x4_u*>(vun + tk + q);
+      const f32x4_u x = *reinterpret_cast<const f32x4_u*>(kun + tk + (uint32_t)(KPL * oc + q));
+      const f32x4_u y = *reinterpret_cast<const f32x4_u*>(vun + tk + (uint32_t)(KPL * oc + q));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         ku[q + e] = x[e];
@@ -288,6 +300,7 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
     const bool more = it + 1 < ntile;
     const char* kb = kbuf[DB ? (it & 1) : 0];
     const char* vb = vbuf[DB ? (it & 1) : 0];
+    asm volatile("" : "+v"(kofs), "+v"(vofs));  // a register each, not one for each copy
     {  // 1. this slice's share of the scores
       f32x16 s2[2];
 #pragma unroll
@@ -360,6 +373,15 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
         for (int e = 0; e < 4; ++e) sv[q + e] = t[e];
       }
       const int k0 = tk + KPL * oc;
+      // A register each would spill, and a spill's load waits for the copies ahead of it:
+      // a row's constants share one.  (Causal, with a cap; us: 2048 tokens of 8q/4kv/d256
+      // bf16 107 -> 99, 1999 of 8q/2kv/d512 fp32 192 -> 163.)
+      [[maybe_unused]] RowScore rsc;
+      if constexpr (SC) {
+        asm volatile("" : "+v"(rcon));  // (taken apart here, not before the loop)
+        rt0 = quad_lane<0>(rcon), rnn = quad_lane<1>(rcon);
+        rsc = row_score_of(a, __int_as_float(quad_lane<2>(rcon)), quad_lane<3>(rcon));
+      }
       const bool full = __builtin_amdgcn_ballot_w64(tk < rt0 || tk + KT > rnn) == 0;
       next_k(1);
 #pragma unroll
@@ -376,17 +398,16 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
         fac = softmax_tile<KPL>(sv, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
       next_k(2);
       next_k(3);
+      char* d = p_st + (KPL == 4 ? (oc >> 1) * 256 + (oc & 1) * 8 : oc * 256);
       if constexpr (KPL == 4) {
-        char* d = p_st + (oc >> 1) * 256 + (oc & 1) * 8;
         *reinterpret_cast<u32x2*>(d) = u32x2{yh[0], yh[1]};
         *reinterpret_cast<u32x2*>(d + 1024) = u32x2{yl[0], yl[1]};
       } else {
-        char* d = p_st + oc * 256;
         *reinterpret_cast<u32x4*>(d) = u32x4{yh[0], yh[1], yh[KPL / 2 - 2], yh[KPL / 2 - 1]};
         *reinterpret_cast<u32x4*>(d + 1024) = u32x4{yl[0], yl[1], yl[KPL / 2 - 2], yl[KPL / 2 - 1]};
       }
-      if (oc == 0)
-        *reinterpret_cast<f32x4*>(region(sl) + 2048 + 16 * orr) = f32x4{fac, 0.f, 0.f, 0.f};
+      if (oc == 0)  // (d is p_st)
+        *reinterpret_cast<f32x4*>(d + 2048) = f32x4{fac, 0.f, 0.f, 0.f};
     }
     if constexpr (!DB) {  // V of this tile is in LDS; K of the next may be in flight
       if (more)
@@ -398,7 +419,7 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
     {  // 3. O^T += V^T . P^T of this slice
       if (more) load_units(tk + KT);  // waited for where the copies are, below
       __builtin_amdgcn_sched_barrier(0);
-      const float fac = (*reinterpret_cast<const f32x4*>(region(my_ow) + 2048 + 16 * my_rr))[0];
+      const float fac = (*reinterpret_cast<const f32x4*>(p_ld + 2048))[0];
       f16x8_t yh[2], yl[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -462,7 +483,7 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
 
   // (every wave met the same units: the workgroup decides alike)
   if (__builtin_amdgcn_ballot_w64(mark != 0.f) != 0) {
-    own_rows<D, SC>(own_args(), h, r0 + (QB / 8) * w, QB / 8, kt_s, kt_s + ntile * KT, sp);
+    own_rows<D, SC>(own_args(), h, r0 + (QB / 8) * w, QB / 8, kt_s, kt_s + ntile * KT, sp, nsplit > 1);
     return;
   }
   // the rows' (l, m, wsh) from their owners to the waves that hold their o
@@ -476,7 +497,7 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
   const int m = row / G, g = row - m * G;
   const int64_t slot = (int64_t)m * a.nq + h * G + g;
   const int sh = -(int)st[2];
-  if (a.nsplit > 1) {
+  if (nsplit > 1) {
     const int64_t ps = slot * a.nsplit + sp;
     float* po = a.part_o + ps * D + 128 * sl + 4 * hh;
 #pragma unroll

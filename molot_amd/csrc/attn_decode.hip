@@ -3260,11 +3260,28 @@ static bool prefill_takes_pieces(int d, int M, int N, int nq, int nkv, int kv_dt
   return true;
 }
 
-// The same of a scored prefill, whose other path is prefill_rows at every head dim:
-// TODO thresholds.
-static bool prefill_scored_pieces(int d, int M, int N, int nq, int nkv, int window, int presplit) {
+// The same of a scored prefill, whose other path is prefill_rows at every head dim: below
+// 64 query rows a KV head that streams the keys a few times, the pieces are two launches
+// before the attention.  Causal with a cap, (tokens, cached), us on rows / on pieces; where
+// the two meet:
+//   16q/4kv/d64    fp32 (300, 0) 18.8 / 20.8, (32, 4000) 38.9 / 26.6; bf16 (16, 4000) 18.6 /
+//                  20.8, (300, 0) 22.9 / 19.0; Q8 (32, 0) 10.8 / 12.1, (128, 0) 19.4 / 14.1
+//   32q/8kv/d128   fp32 (32, 500) 17.8 / 26.2, (200, 0) 34.7 / 23.2; bf16 (128, 0) 16.7 /
+//                  19.2, (200, 0) 28.9 / 21.4; Q8 (16, 300) 16.5 / 21.7, (77, 0) 29.2 / 17.2
+//   8q/4kv/d256    fp32 (300, 0) 33.6 / 39.7, (32, 4000) 71.3 / 46.2; bf16 36.3 / 42.0, 45.7 /
+//                  38.2; Q8 (77, 500) 32.5 / 37.1, (300, 0) 49.6 / 41.9
+//   8q/2kv/d512    fp32 (200, 0) 32.1 / 35.8, (77, 500) 54.6 / 41.2; bf16 (128, 0) 17.0 / 26.1,
+//                  (200, 0) 32.8 / 31.3; Q8 17.5 / 26.4, 33.7 / 31.1
+//   few rows       (2, 65536): rows by 1.4 to 4 times; (4, 16384): d128 fp32 61 / 86, bf16 50 /
+//                  56, Q8 76 / 59
+static bool prefill_scored_pieces(int d, int M, int N, int nq, int nkv, int window, int kv_dtype,
+                                  int presplit) {
+  static constexpr int kPairs[3][4] = {  // thousands of (query row, key), by cache and padded head dim
+      {1800, 800, 900, 340}, {1200, 800, 900, 300}, {150, 180, 500, 300}};
   const int64_t span = window > 0 && window < N ? window : N;
-  return presplit && M <= 65535 && (int64_t)M * nq * span >= 1;
+  const int D = prefill_D(d), cache = kv_dtype == MOLOT_KV_F32 ? 0 : kv_dtype == MOLOT_KV_BF16 ? 1 : 2;
+  return presplit && M <= 65535 && (int64_t)M * (nq / nkv) >= 64 &&
+         (int64_t)M * nq * span >= 1000ll * kPairs[cache][D == 64 ? 0 : D == 128 ? 1 : D == 256 ? 2 : 3];
 }
 
 // Their workspace for the attended keys [T0, N).
@@ -3379,7 +3396,7 @@ static int attn_prefill_impl(const float* Qm, const void* K, const void* V, floa
   if (N == 0) return zero_out(Om, (int64_t)M * nq * d, (hipStream_t)stream);
   if (!K || !V || !aligned16(K) || !aligned16(V) || !aligned16(Qm) || !aligned16(Om))
     return MOLOT_EINVAL;
-  if (sc.on ? prefill_scored_pieces(d, M, N, nq, nkv, window, presplit)
+  if (sc.on ? prefill_scored_pieces(d, M, N, nq, nkv, window, kv_dtype, presplit)
             : prefill_takes_pieces(d, M, N, nq, nkv, kv_dtype, window, presplit)) {
     st = prefill_on_pieces(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype, block_row,
                            page, sc, stream, split_rows);
@@ -3573,7 +3590,7 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   int T0 = 0;
   int split_rows = -1;
   const int presplit = g_presplit.load(std::memory_order_relaxed);
-  if (sc.on ? prefill_scored_pieces(d, M, slot0 + M, nq, nkv, window, presplit)
+  if (sc.on ? prefill_scored_pieces(d, M, slot0 + M, nq, nkv, window, kv_dtype, presplit)
             : prefill_takes_pieces(d, M, slot0 + M, nq, nkv, kv_dtype, window, presplit)) {
     // at d = 512 the split of all rows is as fast (8q/2kv, 1999 tokens: 29 + 7
     // us against 49 for a RoPE/append that leaves the pieces)

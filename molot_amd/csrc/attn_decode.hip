@@ -1570,8 +1570,15 @@ struct WeightArgs {
   int blocked;  // the scores in the matrix-core kernel's order
 };
 constexpr int kWeightThreads = 256;
+constexpr int kWeightAhead = 8;  // heads whose scores a thread has in flight through the merge
 
-// Rows kWeightThreads * rb .. of (sequence b, KV head h); wsm: 2 * G floats.
+// Rows kWeightThreads * rb .. of (sequence b, KV head h).  A short chain of loads (the
+// statistics, the scores, the page's number and the sum that it leads to) bounds a block,
+// so they go out together; us a step with weights, one after the other against
+// together (32q/8kv/d128): 16384 bf16 rows 20.4 -> 20.0, 301 fp32 rows 10.6 -> 10.2; 131072
+// rows of 64q/8kv 130 -> 126.  (Scores read a unit of 4 rows a lane, and turned in LDS, are
+// whole lines a load, and 1 us slower: a block's next waits were not hidden.)
+// wsm: 2 * G floats.
 __device__ __forceinline__ void weigh_rows(const WeightArgs& w, int rb, int h, int b, float* wsm) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int G = w.c.nq / w.c.nkv, gh = w.c.gh;
@@ -1599,15 +1606,37 @@ __device__ __forceinline__ void weigh_rows(const WeightArgs& w, int rb, int h, i
   }
   if (row0 >= span) return;
   const int slot0 = b * w.c.nkv * w.c.nsub + h * w.c.nsub;
+  const int row = row0 + tid, t = t0 + row;
+  const bool in = row < span, set = w.fresh && t == n - 1;
+  const float* s = w.scores + ((int64_t)b * w.c.nkv + h) * w.sc_rows * G;
+  const bool quads = !w.blocked && (G & 3) == 0;
+  const float* x = s + (w.blocked ? (int64_t)(row & ~3) * G + (row & 3) : (int64_t)row * G);
+  const int step = w.blocked ? 4 : 1;
+  float ahead[kWeightAhead];
+#pragma unroll
+  for (int g = 0; g < kWeightAhead; g += 4) {
+    if (quads) {
+      const f32x4 y = in && g < G ? *reinterpret_cast<const f32x4*>(x + g) : f32x4{};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ahead[g + e] = y[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ahead[g + e] = in && g + e < G ? x[step * (g + e)] : 0.f;
+    }
+  }
+  const int64_t i = in ? index(t) : 0;
+  const float old = in && !set ? w.acc[i] : 0.f;
   float *mx = wsm, *inv = wsm + G;
   for (int g = tid >> 6; g < G; g += kWeightThreads / 64) {  // a wave a head
     const float* st = w.stats + ((int64_t)(slot0 + g / gh) * w.c.nchunks * gh + g % gh) * 2;
-    float m = -INFINITY, l = 0.f;
-    for (int c = lane; c < nch; c += 64) m = fmaxf(m, st[(int64_t)c * gh * 2]);
+    auto ml = [&](int c) { return *reinterpret_cast<const f32x2*>(st + (int64_t)c * gh * 2); };
+    const f32x2 first = lane < nch ? ml(lane) : f32x2{-INFINITY, 0.f};
+    float m = first[0], l = 0.f;
+    for (int c = lane + 64; c < nch; c += 64) m = fmaxf(m, ml(c)[0]);
     m = group_max<64>(m);
     for (int c = lane; c < nch; c += 64) {
-      const float mc = st[(int64_t)c * gh * 2];
-      l += mc == -INFINITY ? 0.f : st[(int64_t)c * gh * 2 + 1] * exp2_hw(mc - m);
+      const f32x2 x = c == lane ? first : ml(c);
+      l += x[0] == -INFINITY ? 0.f : x[1] * exp2_hw(x[0] - m);
     }
     l = group_sum<64>(l);
     if (lane == 0) {
@@ -1616,27 +1645,16 @@ __device__ __forceinline__ void weigh_rows(const WeightArgs& w, int rb, int h, i
     }
   }
   __syncthreads();
-  if (row0 + tid >= span) return;
-  const int t = t0 + row0 + tid;
-  const float* s = w.scores + ((int64_t)b * w.c.nkv + h) * w.sc_rows * G;
-  const int row = row0 + tid;
   float sum = 0.f;
-  if (w.blocked) {
-    const float* x = s + (int64_t)(row & ~3) * G + (row & 3);
-#pragma unroll 8
-    for (int g = 0; g < G; ++g) sum = fmaf(exp2_hw(x[4 * g] - mx[g]), inv[g], sum);
-  } else if ((G & 3) == 0) {
-    for (int g = 0; g < G; g += 4) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(s + (int64_t)row * G + g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum = fmaf(exp2_hw(x[e] - mx[g + e]), inv[g + e], sum);
-    }
-  } else {
-    for (int g = 0; g < G; ++g) sum = fmaf(exp2_hw(s[(int64_t)row * G + g] - mx[g]), inv[g], sum);
+  for (int g = 0; g < kWeightAhead; ++g)
+    if (g < G) sum = fmaf(exp2_hw(ahead[g] - mx[g]), inv[g], sum);
+  if (in) {
+#pragma unroll 4
+    for (int g = kWeightAhead; g < G; ++g) sum = fmaf(exp2_hw(x[step * g] - mx[g]), inv[g], sum);
   }
-  const int64_t i = index(t);
-  const bool set = w.fresh && t == n - 1;
-  w.acc[i] = set ? sum : w.acc[i] + sum;
+  if (!in) return;
+  w.acc[i] = set ? sum : old + sum;
   if (set && w.slot_pos) w.slot_pos[i] = pos;
 }
 __global__ __launch_bounds__(kWeightThreads) void attn_weights_kernel(WeightArgs w) {
@@ -1647,7 +1665,8 @@ __global__ __launch_bounds__(kWeightThreads) void attn_weights_kernel(WeightArgs
 // The merge of a split launch and its weights, side by side in one launch (neither
 // needs the other): workgroups below ncomb merge as combine_wave_kernel<R> or, R = 0,
 // combine_kernel, the others weigh.  us a pass, two launches against one: 16001 bf16
-// rows of 32q/8kv/d128 25.1 against 22.6; 13 paged sequences, Q8, 27.2 against 22.9.
+// rows of 32q/8kv/d128 25.1 against 22.6; 13 paged sequences, Q8, 27.2 against 22.9 (now
+// 20.0 and 23.4).
 template <int R>
 __global__ __launch_bounds__(kCombThreads) void combine_weights_kernel(WeightArgs w, int ncomb,
                                                                        int slots) {
@@ -2031,7 +2050,7 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
   if (a.nchunks == 1 && !stats) return 0;  // single chunk: written directly, no combine
   if ((long)rows > kMaxSlots) return MOLOT_ENOTSUP;
   if (stats) {  // the scores of every attended row, for the weights
-    if (B > 65535) return MOLOT_ENOTSUP;  // attn_weights_kernel's grid
+    if (B > 65535 || a.nq / a.nkv > 4096) return MOLOT_ENOTSUP;  // attn_weights_kernel's grid, its LDS
     a.sc_rows = (std::max(span, 0) + 4) & ~3;  // (and the appended row)
     const size_t bytes = sizeof(float) * (size_t)B * a.nq * a.sc_rows;
     if (bytes > kMaxPiecesBytes) return MOLOT_ENOTSUP;
@@ -2149,7 +2168,7 @@ int launch_weights(const CombArgs& cb, const AttnArgs& a, int B, void* stream) {
   const WeightArgs w = weight_args(cb, a);
   const dim3 grid((unsigned)((a.sc_rows + kWeightThreads - 1) / kWeightThreads), a.nkv, B);
   hipLaunchKernelGGL(attn_weights_kernel, grid, dim3(kWeightThreads),
-                     2 * sizeof(float) * (a.nq / a.nkv), (hipStream_t)stream, w);
+                     2 * sizeof(float) * (size_t)(a.nq / a.nkv), (hipStream_t)stream, w);
   return (int)hipGetLastError();
 }
 

@@ -350,6 +350,18 @@ __device__ __forceinline__ unsigned long long arrive_word(int x) {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t l2_rsrc(const float* base) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, 0x7FFFFFFF, 0x00020000);
 }
+// The scores of KV head h of sequence b (AttnArgs::scores), none of a step that keeps none.
+// Stores past the end are dropped, so the kernels' loops store at every tile, a lane without
+// a score at offset -1: with a store under a branch the wait for the next tile's rows, which
+// counts what was issued after them, would wait for the stores as well.  us a step, 64q/8kv/
+// d128 bf16, 131072 keys: 137 with the branch, 130 without; 16384: 21.9, 20.4 (a step that
+// keeps no scores pays 0.2).
+template <typename A>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t score_rsrc(const A& a, int b, int h) {
+  const int64_t rows = a.sc_rows * (a.nq / a.nkv);
+  return __builtin_amdgcn_make_buffer_rsrc(a.scores + ((int64_t)b * a.nkv + h) * rows, 0,
+                                           a.scores ? (int)(4 * rows) : 0, 0x00020000);
+}
 // Loads at a byte offset of a resource, missing the L1 (cache policy sc0).
 __device__ __forceinline__ f32x4 ld_l2x4(__amdgpu_buffer_rsrc_t r, int off) {
   return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 1));
@@ -1081,12 +1093,12 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
   static_assert(!SC || (LPR >= GH && LPR % GH == 0), "a lane of a row for every head");
   [[maybe_unused]] float slope = 0.f, cap2 = 0.f, rcap = 0.f;  // of head s % GH
   [[maybe_unused]] float m_own = -INFINITY;                    // and its running max
-  [[maybe_unused]] float* swr = nullptr;
+  [[maybe_unused]] __amdgpu_buffer_rsrc_t swr;
   if constexpr (SC) {
     if (a.slopes) slope = a.slopes[hq0 + s % GH] * kLog2e;
     cap2 = a.softcap * kLog2e;
     rcap = a.softcap > 0.f ? 1.f / cap2 : 0.f;
-    if (a.scores) swr = a.scores + ((int64_t)b * a.nkv + h) * a.sc_rows * G + sub * GH;
+    swr = score_rsrc(a, b, h);
   }
 
   // ---- 2. streaming blocks with a per-wave online softmax ----
@@ -1146,7 +1158,7 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
     if constexpr (SC) {
       // Every lane of a row holds the row's GH sums; from here on lane s takes head
       // s % GH alone: one cap, bias, comparison and exponential a row instead of GH
-      // (32q/8kv/d128 fp32, 16385 rows, cap and slopes: SCORED_FIGURES).
+      // (32q/8kv/d128 fp32, 16385 rows, cap and slopes: 30.0 -> 27.2 us, the plain step 25.9).
       const int g0 = s % GH;
       float x[KS];
 #pragma unroll
@@ -1165,12 +1177,12 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
         x[k] = rbase + k * RPS + rr < nrows ? y : -INFINITY;
         top = fmaxf(top, x[k]);
       }
-      if (swr && s < GH) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const int at = t_lane + k * RPS - t0;
-          if (rbase + k * RPS + rr < nrows && at < a.sc_rows) swr[(int64_t)at * G + s] = x[k];
-        }
+      for (int k = 0; k < KS; ++k) {
+        const int at = t_lane + k * RPS - t0;
+        const bool mine = s < GH && rbase + k * RPS + rr < nrows;
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[k]), swr,
+                                              mine ? 4 * (at * G + sub * GH + s) : -1, 0, 0);
       }
       if (__builtin_amdgcn_ballot_w64(top > m_own + kLazyMax) != 0) {  // wave-uniform
         auto top_off = [&](auto OFFC) {
@@ -1366,7 +1378,8 @@ __global__ __launch_bounds__(C::NT) void attn_kernel(AttnArgs a) {
       for (int g = 0; g < GH; ++g) {
         const float sl = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(slope), g));
         part[g] = fmaf(-sl, dist, part[g]);
-        if (swr && lane == 0 && n - 1 - t0 < a.sc_rows) swr[(int64_t)(n - 1 - t0) * G + g] = part[g];
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(part[g]), swr,
+                                              lane == 0 ? 4 * ((n - 1 - t0) * G + sub * GH + g) : -1, 0, 0);
       }
     }
 #pragma unroll
@@ -1989,13 +2002,13 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
 
   // SC, as attn_kernel; the lane's head is m16
   [[maybe_unused]] float slope = 0.f, cap2 = 0.f, rcap = 0.f;
-  [[maybe_unused]] float* swr = nullptr;
+  [[maybe_unused]] __amdgpu_buffer_rsrc_t swr;
+  [[maybe_unused]] const int swo = 4 * (sub * GH + m16);
   if constexpr (SC) {
     if (a.slopes && m16 < GH) slope = a.slopes[hq0 + m16] * kLog2e;
     cap2 = a.softcap * kLog2e;
     rcap = a.softcap > 0.f ? 1.f / cap2 : 0.f;
-    if (a.scores && m16 < GH)
-      swr = a.scores + ((int64_t)b * a.nkv + h) * a.sc_rows * G + 4 * (sub * GH + m16);
+    swr = score_rsrc(a, b, h);
   }
 
   // ---- stream ----
@@ -2094,18 +2107,23 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
         sv[i / 4][i % 4] = row < rlim ? y : -INFINITY;
         tmax = fmaxf(tmax, sv[i / 4][i % 4]);
       }
-      if (swr) {  // rows 16u + 4*g4 .. +3 of a head side by side (chunks start at multiples of 4)
+      // rows 16u + 4*g4 .. +3 of a head side by side (chunks start at multiples of 4)
+      bool part = false;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int row = tile_row(tile) + 16 * u + 4 * g4, at = rfirst - t0 + row;
-          float* to = swr + (int64_t)at * G;
-          if (at + 4 > a.sc_rows) continue;
-          if (row + 4 <= rlim)
-            *reinterpret_cast<f32x4*>(to) = f32x4{sv[u][0], sv[u][1], sv[u][2], sv[u][3]};
-          else
+      for (int u = 0; u < 2; ++u) {
+        const int row = tile_row(tile) + 16 * u + 4 * g4, at = rfirst - t0 + row;
+        part = part || (row < rlim && row + 4 > rlim);
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(u32x4, f32x4{sv[u][0], sv[u][1], sv[u][2], sv[u][3]}), swr,
+            m16 < GH && row + 4 <= rlim ? 4 * (at * G + swo) : -1, 0, 0);
+      }
+      if (__builtin_amdgcn_ballot_w64(part) != 0) {  // the rows' end, once: another wave may own the next
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (row + r < rlim) to[r] = sv[u][r];
+        for (int i = 0; i < 8; ++i) {
+          const int u = i / 4, row = tile_row(tile) + 16 * u + 4 * g4, at = rfirst - t0 + row;
+          __builtin_amdgcn_raw_buffer_store_b32(
+              __float_as_uint(sv[u][i % 4]), swr,
+              m16 < GH && row + 4 > rlim && row + i % 4 < rlim ? 4 * (at * G + swo + i % 4) : -1, 0, 0);
         }
       }
     } else
@@ -2207,7 +2225,9 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void attn_mfma_kernel(AttnArgs a) 
       if (a.softcap > 0.f) cap_scores<1>(x, cap2, rcap);
       snew = fmaf(-slope, fabsf((float)(pos - (n - 1))), x[0]);
       const int at = n - 1 - t0;
-      if (swr && g4 == 0 && at < a.sc_rows) swr[(int64_t)(at & ~3) * G + (at & 3)] = snew;
+      __builtin_amdgcn_raw_buffer_store_b32(
+          __float_as_uint(snew), swr,
+          g4 == 0 && m16 < GH ? 4 * ((at & ~3) * G + swo + (at & 3)) : -1, 0, 0);
     }
     const float mn = fmaxf(m_run, snew);
     const float alpha = exp2_hw(m_run - mn);

@@ -375,6 +375,22 @@ PREFILL = [
     ("f32", 32, 8, 128, 1, 0, 0, 50.0, True, "causal"),
     ("bf16", 32, 8, 128, 2, 1000, 0, 50.0, True, "causal"),
     ("q8", 8, 8, 64, 3, 40, 0, 50.0, True, "ranges"),
+    # enough query rows for the pieces; several key splits, and blocks of few keys with one
+    ("f32", 16, 4, 64, 345, 0, 0, 50.0, True, "docs"),
+    ("q8", 8, 8, 64, 150, 0, 0, 50.0, True, "ranges"),
+    ("q8", 4, 2, 36, 211, 0, 0, 30.0, True, "prefix"),
+    ("f32", 6, 2, 34, 601, 0, 0, 5.0, True, "docs"),
+    ("bf16", 32, 8, 128, 175, 0, 0, 50.0, True, "ranges"),
+    ("q8", 32, 8, 128, 101, 0, 0, 50.0, False, "prefix"),
+    ("f32", 12, 4, 96, 301, 0, 0, 30.0, True, "ranges"),
+    ("f32", 8, 4, 256, 351, 0, 0, 0.0, True, "docs"),
+    ("bf16", 8, 4, 256, 700, 0, 0, 50.0, True, "docs"),
+    ("bf16", 8, 4, 256, 65, 2000, 0, 50.0, False, "causal"),
+    ("q8", 8, 4, 256, 301, 0, 0, 50.0, True, "ranges"),
+    ("f32", 8, 2, 512, 401, 0, 0, 50.0, True, "docs"),
+    ("bf16", 8, 2, 512, 699, 0, 0, 50.0, True, "docs"),
+    ("bf16", 8, 2, 512, 33, 2000, 700, 50.0, True, "causal"),
+    ("q8", 8, 2, 512, 399, 0, 0, 50.0, True, "ranges"),
 ]
 
 
@@ -431,15 +447,16 @@ def test_prefill(gpu, kv, nq, nkv, d, m, n0, window, softcap, alibi, mask, presp
 @pytest.mark.parametrize("d", [64, 96, 128, 256, 512])
 @pytest.mark.parametrize("kv", ["f32", "bf16"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, "lowest"])
-def test_prefill_masked_rows_count_for_nothing(gpu, kv, d, bad):
+@pytest.mark.parametrize("m", [96, 500])  # rows streamed one by one; the pieces
+def test_prefill_masked_rows_count_for_nothing(gpu, kv, d, bad, m):
     """What a masked key holds, in K, V or both, reaches no row that does not see it."""
-    nq, nkv, m = 8, 4, 96
+    nq, nkv = 8, 4
     g = gen(43)
     q = randn(g, m, nq, d, sigma=3.0)
     xk, xv = randn(g, m, nkv, d), randn(g, m, nkv, d)
     if bad == "lowest":
         bad = float(torch.finfo(torch.float32 if kv == "f32" else torch.bfloat16).min)
-    starts = attn.document_starts([30, 41, 25])
+    starts = attn.document_starts([30, 41, m - 71])
     for t in (33, 70):  # rows of the second document
         xk[t, 1] = bad
         xv[t, :, ::2] = bad

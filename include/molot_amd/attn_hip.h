@@ -305,7 +305,7 @@ int molot_hip_attn_prefill_paged(const float* Qm, const void* K, const void* V, 
  *   softcap > 0:   s = softcap * tanh(s / softcap)      (0: no cap; else
  *                  within [1e-30, 1e30], MOLOT_EINVAL otherwise)
  *   slopes:        s = s - slopes[h] * |i - t|          (device [nq], one a
- *                  query head; NULL: none)
+ *                  query head; NULL: none; |slopes[h] * (i - t)| below 1e29)
  * and the softmax over the attended slots; an empty range yields o = 0.
  * i is pos_cur, pos or pos0 + m as the entry's window takes it, t the slot.
  * Same kernels, layouts, cache types, head dims, workspaces and accuracy as
@@ -315,11 +315,13 @@ int molot_hip_attn_prefill_paged(const float* Qm, const void* K, const void* V, 
  * attended slot t and KV head g, the softmax weights of the query heads of
  * g's group are added to acc of (g, t) in fp32, heads in order.  Token-major
  * caches: acc[nkv][acc_cap], acc_cap >= the slots; paged ones: pages
- * [num_blocks][nkv][page] through the same block table.  A step that appends
+ * [num_blocks][nkv][page] through the same block table, where no two sequences
+ * of a call share a block (every slot has one writer).  A step that appends
  * a row sets that slot's acc instead, and its position in slot_pos (int32,
  * same layout; NULL: none; only with acc).  The scores of a call with acc are
  * kept for its second launch: 4 * B * nq * (attended rows + 1) bytes of the
- * stream's prefill workspace, at most 1 GiB (MOLOT_ENOTSUP past it). */
+ * stream's prefill workspace, at most 1 GiB (MOLOT_ENOTSUP past it, and past
+ * 4096 query heads a KV head or 65535 sequences). */
 int molot_hip_attn_decode_scored(const float* Q, const void* K, const void* V, float* O, int nq,
                                  int nkv, int n, int d, float scale, int pos_cur, int window,
                                  float softcap, const float* slopes, float* acc, int acc_cap,

@@ -489,9 +489,15 @@ def _acc_cap(acc, slot_pos, nkv, rows):
     return acc.numel() // nkv
 
 
-def _need_acc_pages(acc, slot_pos, nblocks, nkv, page):
+def _need_acc_pages(acc, slot_pos, nblocks, nkv, page, block_table, seq_lens, B, max_blocks):
     if acc is not None:
         _need(acc, "acc", torch.float32, nblocks * nkv * page)
+        # every slot has one writer a call
+        used = (seq_lens.view(-1)[:B].cpu() + page - 1) // page
+        bt = block_table.view(-1)[:B * max_blocks].view(B, max_blocks).cpu()
+        ids = bt[torch.arange(max_blocks)[None, :] < used[:, None]]
+        if ids.unique().numel() != ids.numel():
+            raise ValueError("block_table: with acc, a block belongs to one sequence, once")
     if slot_pos is not None:
         if acc is None:
             raise ValueError("slot_pos needs acc")
@@ -553,7 +559,8 @@ def attn_decode_paged_scored(Q, K, V, O, block_table, seq_lens, pos, B, max_bloc
     _need(O, "O", torch.float32, B * nq * d)
     max_len = _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V)
     _need_scoring(slopes, nq)
-    _need_acc_pages(acc, None, K.numel() // _block_units(kvd, nkv, d, page), nkv, page)
+    _need_acc_pages(acc, None, K.numel() // _block_units(kvd, nkv, d, page), nkv, page,
+                    block_table, seq_lens, B, max_blocks)
     check(_lib.load().molot_hip_attn_decode_paged_scored(
         _ptr(Q), _ptr(K), _ptr(V), _ptr(O), _ptr(block_table), _ptr(seq_lens), _ptr(pos), B,
         max_blocks, max_len, nq, nkv, d, page, float(scale), int(window), float(softcap),
@@ -578,7 +585,8 @@ def decode_step_paged_scored(q, k_new, v_new, K, V, O, block_table, seq_lens, po
     if B and int(seq_lens.min()) < 1:
         raise ValueError("decode_step_paged_scored: every sequence needs seq_lens >= 1")
     _need_scoring(slopes, nq)
-    _need_acc_pages(acc, slot_pos, K.numel() // _block_units(kvd, nkv, d, page), nkv, page)
+    _need_acc_pages(acc, slot_pos, K.numel() // _block_units(kvd, nkv, d, page), nkv, page,
+                    block_table, seq_lens, B, max_blocks)
     check(_lib.load().molot_hip_decode_step_paged_scored(
         _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(K), _ptr(V), _ptr(O), _ptr(block_table),
         _ptr(seq_lens), _ptr(pos), B, max_blocks, max_len, nq, nkv, d, page, _ptr(q_norm),
@@ -688,6 +696,7 @@ def prefill_step_paged_scored(q, k_new, v_new, K, V, O, block_row, max_blocks, p
 
 def kv_track(acc, slot_pos, nkv, n, M, pos):
     """The last M of n slots are new: acc [nkv][cap] 0, slot_pos pos-M+1 .. pos."""
+    _need(acc, "acc", torch.float32)
     cap = _acc_cap(acc, slot_pos, nkv, n)
     check(_lib.load().molot_hip_kv_track(_ptr(acc), _ptr(slot_pos), nkv, int(n), int(M), int(pos),
                                          cap, _stream()), "kv_track")
@@ -712,9 +721,10 @@ def _check_slot_pages(block_table, seq_lens, pos, B, max_blocks, nblocks, page):
 def kv_track_paged(acc, slot_pos, block_table, seq_lens, pos, B, max_blocks, M, nkv, page):
     """kv_track of the last min(M, seq_lens[b]) slots of every sequence, the newest
     at pos[b] (None: seq_lens[b] - 1); acc and slot_pos [blocks][nkv][page]."""
+    _need(acc, "acc", torch.float32)
     nblocks = acc.numel() // (nkv * page)
-    _need_acc_pages(acc, slot_pos, nblocks, nkv, page)
     max_len = _check_slot_pages(block_table, seq_lens, pos, B, max_blocks, nblocks, page)
+    _need_acc_pages(acc, slot_pos, nblocks, nkv, page, block_table, seq_lens, B, max_blocks)
     check(_lib.load().molot_hip_kv_track_paged(
         _ptr(acc), _ptr(slot_pos), _ptr(block_table), _ptr(seq_lens), _ptr(pos), B, max_blocks,
         max_len, int(M), nkv, page, _stream()), "kv_track_paged")
@@ -745,7 +755,8 @@ def kv_evict_paged(K, V, acc, slot_pos, block_table, seq_lens, pos, B, max_block
     if acc is None or slot_pos is None:
         raise ValueError("kv_evict_paged needs acc and slot_pos")
     max_len = _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V)
-    _need_acc_pages(acc, slot_pos, K.numel() // _block_units(kvd, nkv, d, page), nkv, page)
+    _need_acc_pages(acc, slot_pos, K.numel() // _block_units(kvd, nkv, d, page), nkv, page,
+                    block_table, seq_lens, B, max_blocks)
     check(_lib.load().molot_hip_kv_evict_paged(
         _ptr(K), _ptr(V), _ptr(acc), _ptr(slot_pos), _ptr(block_table), _ptr(seq_lens), _ptr(pos),
         B, max_blocks, max_len, nkv, d, page, int(keep), int(recent), kvd, _stream()),

@@ -48,6 +48,10 @@ __device__ __forceinline__ int rows_of(const SlotArgs& a, int b) {
 __device__ __forceinline__ int newest_of(const SlotArgs& a, int b, int n) {
   return !a.block_table ? a.pos : a.pos_arr ? a.pos_arr[b] : n - 1;
 }
+// The newest position that is not recent.
+__device__ __forceinline__ int64_t oldest_of(const SlotArgs& a, int b, int n, int recent) {
+  return (int64_t)newest_of(a, b, n) - recent;
+}
 // Index of slot t of KV head h in acc and slot_pos.
 __device__ __forceinline__ int64_t slot_index(const SlotArgs& a, int b, int h, int t) {
   if (!a.block_table) return (int64_t)h * a.acc_cap + t;
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(SlotArgs a, i
   extern __shared__ uint32_t key_lds[];  // [key_each(longest) * kSelThreads]
   __shared__ SelectLds L;
   __shared__ int32_t own[FUSE ? 2 * kFuseMoves : 1];
-  const int oldest = newest_of(a, b, n) - recent;  // recent: past it
+  const int64_t oldest = oldest_of(a, b, n, recent);  // recent: past it
   const Keys keys{key_lds, key_each(n)};
   for (int t0 = threadIdx.x; t0 < keys.each * kSelThreads; t0 += 8 * kSelThreads) {
     float x[8];
@@ -503,7 +507,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_keys_kernel(LongArgs g) {
   const int64_t pair = (int64_t)b * a.nkv + h;
   __shared__ __attribute__((aligned(16))) int hist[kBins];
   reinterpret_cast<u32x4*>(hist)[tid] = u32x4{0u, 0u, 0u, 0u};
-  const int oldest = newest_of(a, b, n) - g.recent;
+  const int64_t oldest = oldest_of(a, b, n, g.recent);
   float x[kChunkK];
   int32_t p[kChunkK];
 #pragma unroll

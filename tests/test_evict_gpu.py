@@ -26,6 +26,8 @@ def weights(g, kind, nkv, cap):
         return torch.randint(0, 4, (nkv, cap), device="cuda", generator=g).float()
     if kind == "equal":
         return torch.full((nkv, cap), 0.25, device="cuda")
+    if kind == "near":  # equal in their first 20 bits, some in all
+        return 1 + torch.randint(0, 4000, (nkv, cap), device="cuda", generator=g) * 2.0 ** -23
     x = torch.exp(2 * torch.randn(nkv, cap, device="cuda", generator=g))
     if kind == "odd":
         r = torch.rand(nkv, cap, device="cuda", generator=g)
@@ -83,7 +85,7 @@ def test_rule(gpu, n, keep, recent, kind):
         assert torch.equal(raw(got), raw(exp))
 
 
-@pytest.mark.parametrize("kind", ["smooth", "ties", "equal", "odd", "zeros"])
+@pytest.mark.parametrize("kind", ["smooth", "ties", "equal", "odd", "zeros", "near"])
 @pytest.mark.parametrize("n,keep,recent", [(16384, 16000, 500), (16385, 16000, 500), (20001, 8192, 3),
                                            (40000, 39999, 0), (40000, 1, 0), (60000, 24576, 40000),
                                            (33333, 30000, 2500)])
@@ -110,6 +112,50 @@ def test_rule_long(gpu, n, keep, recent, kind):
     attn.kv_evict(K, V, acc, sp, nkv, n, d, keep, recent, pos)
     for got, exp in zip((K, V, acc, sp), want):
         assert torch.equal(raw(got), raw(exp))
+
+
+@pytest.mark.parametrize("pos,recent", [(-5, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31 - 1, 3),
+                                        (-2 ** 31, 7)])
+def test_extreme_positions(gpu, pos, recent):
+    nkv, n, keep = 2, 50, 40
+    acc = weights(gen(4), "smooth", nkv, n)
+    sp = torch.tensor([-2 ** 31, -2 ** 31 + 1, -5, 0, 2 ** 31 - 1] * 10, device="cuda").int().repeat(nkv, 1)
+    K, V = (torch.randn(n, nkv * 2, device="cuda", generator=gen(i)) for i in (5, 6))
+    want = acc.clone()
+    for h, moves in enumerate(ref.evict(acc.cpu(), sp.cpu(), n, keep, recent, pos)):
+        for to, at in moves:
+            want[h, to] = acc[h, at]
+    attn.kv_evict(K, V, acc, sp, nkv, n, 2, keep, recent, pos)
+    assert torch.equal(acc, want)
+
+
+def test_shared_blocks_are_refused(gpu):
+    """Every slot's acc has one writer: two sequences of a call, or one of them twice
+    over, may not name the same block."""
+    nkv, d, page, blocks = 2, 4, 8, 6
+    K, V = (torch.zeros(blocks, nkv * page * d, device="cuda") for _ in range(2))
+    acc = torch.zeros(blocks, nkv, page, device="cuda")
+    sp = torch.zeros(blocks, nkv, page, dtype=torch.int32, device="cuda")
+    q, o = torch.zeros(2, 4, d, device="cuda"), torch.zeros(2, 4, d, device="cuda")
+    new = torch.zeros(2, nkv, d, device="cuda")
+    inv = torch.ones(d // 2, device="cuda")
+    for rows in ([[0, 1], [2, 0]], [[3, 3], [1, 2]]):
+        table = torch.tensor(rows, dtype=torch.int32, device="cuda")
+        lens = torch.tensor([16, 9], dtype=torch.int32, device="cuda")
+        for call in (
+                lambda: attn.attn_decode_paged_scored(q, K, V, o, table, lens, None, 2, 2, 4, nkv, d, page,
+                                                      1.0, acc=acc),
+                lambda: attn.decode_step_paged_scored(q, new, new, K, V, o, table, lens, None, 2, 2, 4, nkv,
+                                                      d, page, inv, 1.0, acc=acc, slot_pos=sp),
+                lambda: attn.kv_track_paged(acc, sp, table, lens, None, 2, 2, 3, nkv, page),
+                lambda: attn.kv_evict_paged(K, V, acc, sp, table, lens, None, 2, 2, nkv, d, page, 5, 1)):
+            with pytest.raises(ValueError):
+                call()
+        # without acc a block may serve several, as in the plain attention
+        attn.attn_decode_paged_scored(q, K, V, o, table, lens, None, 2, 2, 4, nkv, d, page, 1.0)
+    table = torch.tensor([[0, 1], [2, 0]], dtype=torch.int32, device="cuda")  # (its second entry unused)
+    lens = torch.tensor([16, 8], dtype=torch.int32, device="cuda")
+    attn.kv_track_paged(acc, sp, table, lens, None, 2, 2, 3, nkv, page)
 
 
 def test_paged_long(gpu):

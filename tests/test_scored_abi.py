@@ -141,3 +141,19 @@ def test_status(status, cases):
     for fn, kw in cases:
         got = fn(**kw)
         assert got == status, f"{fn.__name__}({kw}): {got}"
+
+
+def test_alibi_slopes():
+    from molot_amd import attn
+    assert attn.alibi_slopes(8).tolist() == [2.0 ** -(h + 1) for h in range(8)]
+    got = attn.alibi_slopes(12)
+    assert got.dtype.is_floating_point and got.tolist() == pytest.approx(
+        [2.0 ** (-8 * (h + 1) / 12) for h in range(12)], rel=2.0 ** -23)
+
+
+def test_document_starts():
+    from molot_amd import attn
+    assert attn.document_starts([3, 0, 1, 2], 10).tolist() == [10, 10, 10, 13, 14, 14]
+    assert attn.document_starts([]).tolist() == []
+    with pytest.raises(ValueError):
+        attn.document_starts([2, -1])

@@ -64,6 +64,8 @@ DECODE = [
     ("q8", 8, 4, 256, 1500, 512, 50.0, True),
     ("q8", 8, 2, 512, 300, 0, 0.0, True),
     ("q8", 4, 2, 36, 70, 0, 50.0, True),
+    ("bf16", 16, 2, 128, 131075, 0, 50.0, False),
+    ("q8", 4, 1, 64, 131072, 0, 50.0, True),
 ]
 
 

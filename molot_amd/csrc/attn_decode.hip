@@ -70,6 +70,7 @@ struct RopeArgs {
   // pieces per value in the layout of prefill_wide.hpp (0: the three-slot
   // layout of pf_split_kernel)
   int pc_np;
+  int own;  // with pc_np: mark the rows that PfArgs::own launches form again
 };
 
 // One workgroup per (head of q or k, sequence); one thread per rotation pair.
@@ -401,16 +402,31 @@ __global__ __launch_bounds__(kRopeTokThreads) void rope_append_tok_kernel(RopeAr
           vpm = fmaxf(vpm, fmaxf(fabsf(cached(v0[k], vs)), fabsf(cached(v1[k], vs))));
         }
       }
-      const int kshift = f16_row_shift(group_max<64>(kpm));
+      kpm = group_max<64>(kpm);
+      const int kshift = f16_row_shift(kpm);
       vpm = group_max<64>(vpm);
+      const bool q8u = np && a.kv_dtype == MOLOT_KV_Q8;
+      const float ksc = q8u ? ks : 1.f, vsc = q8u ? vs : 1.f;
+      float mk = 0.f, mv = 0.f;  // wide_split_kernel's marks
+      if (P32 && a.own) {
+#pragma unroll
+        for (int k = 0; k < KMAX; ++k) {
+          if (k >= nk) break;
+          if (lane + 64 * k < half) {
+            mk = fmaf(cached(r0[k], ks) * ksc, 0.f, fmaf(cached(r1[k], ks) * ksc, 0.f, mk));
+            mv = fmaf(cached(v0[k], vs) * vsc, 0.f, fmaf(cached(v1[k], vs) * vsc, 0.f, mv));
+          }
+        }
+        mk = own_mark(kpm * ksc, group_sum<64>(mk), 0);
+        mv = own_mark(vpm * vsc, group_sum<64>(mv), 1);
+      }
       const int vshift = f16_vrow_shift(vpm);
       uint16_t* ok = a.pieces + (int64_t)kh * hstride + (int64_t)pr * a.d;
       uint16_t* ov = ok + (int64_t)a.nkv * hstride;
       if (lane == 0) {  // the units of a head's rows side by side after its pieces
         const int64_t uo = (np ? np : 2) * pstride - (int64_t)pr * a.d;
-        const bool q8u = np && a.kv_dtype == MOLOT_KV_Q8;
-        reinterpret_cast<float*>(ok + uo)[pr] = f16_row_unit(kshift) * (q8u ? ks : 1.f);
-        reinterpret_cast<float*>(ov + uo)[pr] = f16_vrow_unit(vpm, vshift) * (q8u ? vs : 1.f);
+        reinterpret_cast<float*>(ok + uo)[pr] = f16_row_unit(kshift) * ksc + mk;
+        reinterpret_cast<float*>(ov + uo)[pr] = f16_vrow_unit(vpm, vshift) * vsc + mv;
       }
 #pragma unroll
       for (int k = 0; k < KMAX; ++k) {
@@ -3609,17 +3625,24 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   int T0 = 0;
   int split_rows = -1;
   const int presplit = g_presplit.load(std::memory_order_relaxed);
+  // (scored: a row never sees the rows appended after it, whatever positions a cache
+  // that rows were evicted from has)
+  const int apos = sc.on ? std::min(pos0, slot0) : pos0;
   if (sc.on ? prefill_scored_pieces(d, M, slot0 + M, nq, nkv, window, kv_dtype, presplit)
             : prefill_takes_pieces(d, M, slot0 + M, nq, nkv, kv_dtype, window, presplit)) {
     // at d = 512 the split of all rows is as fast (8q/2kv, 1999 tokens: 29 + 7
-    // us against 49 for a RoPE/append that leaves the pieces)
-    if (!sc.on && (d == 64 || d == 128)) {
+    // us against 49 for a RoPE/append that leaves the pieces), and a scored step's of Q8
+    // rows, whose marks cost the append as much (2048 tokens with a cap, split of all /
+    // left by the append: 32q/8kv/d128 fp32 150.5 / 147.5, bf16 122.6 / 120.3, Q8 123.0 /
+    // 124.1; 16q/4kv/d64 86.2 / 84.7, 76.2 / 75.5, 77.4 / 77.1)
+    if ((d == 64 || d == 128) && !(sc.on && kv_dtype == MOLOT_KV_Q8)) {
       int R = 0;
-      st = pieces32_workspace(nkv, slot0 + M, d, pos0, window, kv_dtype, stream, &pws, &T0, &R);
+      st = pieces32_workspace(nkv, slot0 + M, d, apos, window, kv_dtype, stream, &pws, &T0, &R);
       if (st && st != MOLOT_ENOWS) return st;
       if (!st) {
         r.pc_R = R;
         r.pc_np = wide_pieces(kv_dtype == MOLOT_KV_F32);
+        r.own = sc.on;
       }
     }
   } else if (supported_d(d) && !sc.on) {
@@ -3639,11 +3662,8 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   }
   st = launch_rope_tok(r, M, stream);
   if (st) return st;
-  // (scored: a row never sees the rows appended after it, whatever positions a cache
-  // that rows were evicted from has)
-  return attn_prefill_impl(q, K, V, O, nq, nkv, M, slot0 + M, d, scale,
-                           sc.on ? std::min(pos0, slot0) : pos0, window, kv_dtype, block_row, page,
-                           sc, stream, presplit, split_rows);
+  return attn_prefill_impl(q, K, V, O, nq, nkv, M, slot0 + M, d, scale, apos, window, kv_dtype,
+                           block_row, page, sc, stream, presplit, split_rows);
 }
 
 int molot_hip_prefill_step(float* q, const float* k_new, const float* v_new, void* K, void* V,

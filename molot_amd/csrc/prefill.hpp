@@ -2,6 +2,9 @@
 #ifndef MOLOT_AMD_CSRC_PREFILL_HPP_
 #define MOLOT_AMD_CSRC_PREFILL_HPP_
 
+#include <hip/hip_runtime.h>
+
+#include <cmath>
 #include <cstdint>
 
 struct PfArgs {
@@ -15,7 +18,7 @@ struct PfArgs {
   int page_shift;
   float scale;
   // 32-row kernels: a query row's output depends on the keys it attends alone
-  // (own_rows below); the cache type then says how to read them
+  // (own_mark, below); the cache type then says how to read them
   int own, kv_dtype;
   // the attended keys [T0, T0 + R) of every KV head split into 16-bit pieces
   // once for the launch (pf_split_kernel): [K, V][nkv][3 pieces][R][D]; NULL:
@@ -41,5 +44,24 @@ struct PfArgs {
 
 using PfFn = void (*)(PfArgs);
 using SplitFn = void (*)(PfArgs, uint16_t*);
+
+namespace {
+
+// Rows that the pieces cannot hold for every query row alike.  A product over a
+// tile takes each of its keys for all its query rows, a masked one times zero:
+// a non-finite V row reaches rows that do not attend it, and a K row's infinity
+// leaves no score of its sign.  Where each query row used to read its own keys
+// alone (head dims above 256 and those that are not multiples of 8, Q8 at any
+// padded one: PfArgs::own) the split marks such rows, and those out of the
+// units' range, by a NaN unit, and a workgroup that met one forms its rows'
+// results again from the cache (own_rows, prefill_tile.hpp).
+constexpr float kOwnMaxK = 3.0e23f;   // 2^78: past it a raw score times its unit may overflow
+constexpr float kOwnMinV = 7.9e-31f;  // 2^-100: below it a V row's unit keeps fewer bits
+__device__ __forceinline__ float own_mark(float xmax, float nonfinite, int kv) {
+  const bool out = kv ? xmax > 0.f && xmax < kOwnMinV : xmax > kOwnMaxK;
+  return out ? NAN : nonfinite;  // 0, or NaN
+}
+
+}  // namespace
 
 #endif  // MOLOT_AMD_CSRC_PREFILL_HPP_

@@ -120,21 +120,6 @@ __device__ __forceinline__ float wide_load8(const PfArgs& a, int kv, int h, int 
   return 1.f;
 }
 
-// Rows that the pieces cannot hold for every query row alike.  A product over a
-// tile takes each of its keys for all its query rows, a masked one times zero:
-// a non-finite V row reaches rows that do not attend it, and a K row's infinity
-// leaves no score of its sign.  Where each query row used to read its own keys
-// alone (head dims above 256 and those that are not multiples of 8, Q8 at any
-// padded one: PfArgs::own) the split marks such rows, and those out of the
-// units' range, by a NaN unit, and a workgroup that met one forms its rows'
-// results again from the cache (own_rows).
-constexpr float kOwnMaxK = 3.0e23f;   // 2^78: past it a raw score times its unit may overflow
-constexpr float kOwnMinV = 7.9e-31f;  // 2^-100: below it a V row's unit keeps fewer bits
-__device__ __forceinline__ float own_mark(float xmax, float nonfinite, int kv) {
-  const bool out = kv ? xmax > 0.f && xmax < kOwnMinV : xmax > kOwnMaxK;
-  return out ? NAN : nonfinite;  // 0, or NaN
-}
-
 // Element e of the row at off (wide_row_off's unit), not yet times a Q8 scale.
 __device__ __forceinline__ float own_elem(const PfArgs& a, const char* base, int64_t off, int e) {
   if (a.kv_dtype == MOLOT_KV_Q8) return (float)reinterpret_cast<const int8_t*>(base)[off + e];

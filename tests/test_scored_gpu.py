@@ -477,10 +477,11 @@ def test_prefill_masked_rows_count_for_nothing(gpu, kv, d, bad, m):
 
 @pytest.mark.parametrize("kv,d", [("f32", 128), ("bf16", 64), ("q8", 256), ("f32", 80), ("q8", 512)])
 @pytest.mark.parametrize("slot0", [0, 21])
-def test_prefill_steps(gpu, kv, d, slot0):
+@pytest.mark.parametrize("m", [70, 500])  # rows streamed one by one; the pieces
+def test_prefill_steps(gpu, kv, d, slot0, m):
     """The appending steps, contiguous and paged: rows and q as the unscored steps
     leave them, the attention of the rows stored."""
-    nq, nkv, m, page = 8, 4, 70, 16
+    nq, nkv, page = 8, 4, 16
     g = gen(45)
     N, scale = slot0 + m, 1 / math.sqrt(d)
     q, k, v = randn(g, m, nq, d, sigma=3.0), randn(g, m, nkv, d), randn(g, m, nkv, d)
@@ -515,6 +516,40 @@ def test_prefill_steps(gpu, kv, d, slot0):
     attn.attn_prefill_paged_scored(q3, Kp, Vp, O4, table.cuda(), blocks, page, nq, nkv, m, N, d, scale,
                                    slot0, 0, 50.0, sl, lo, None)
     check_out(O4, want, tol)
+
+
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("slot0,behind,window", [(0, 0, 0), (21, 0, 300), (21, 400, 0), (130, 400, 200)])
+def test_prefill_step_pieces(gpu, kv, d, slot0, behind, window):
+    """A step whose append leaves the attention's operands gives what the attention over
+    the stored rows does, rows among them that no operand holds: not finite, and past
+    the operands' range.  behind: positions past the slots (rows were evicted)."""
+    nq, nkv, m = 8, 4, 520
+    g = gen(48)
+    N, scale = slot0 + m, 1 / math.sqrt(d)
+    q, k, v = randn(g, m, nq, d, sigma=3.0), randn(g, m, nkv, d), randn(g, m, nkv, d)
+    if kv != "q8":
+        k[100, 1] *= 1e25
+        v[200, 2] *= 1e-33
+        k[333, 0, 5] = math.nan
+        v[333, 0, 7] = math.inf
+    inv = attn.rope_inv_freq(10000.0, d).cuda()
+    sl = slopes_of(nq)
+    lo = attn.document_starts([90, 200, 100, m - 390], slot0).cuda()
+    Kc, Vc = (ref.make_cache(randn(g, N, nkv, d), kv)[0] for _ in range(2))
+    O, O2 = torch.empty(m, nq, d, device="cuda"), torch.empty(m, nq, d, device="cuda")
+    _lib.load().molot_hip_set_block_order(0)  # (the small windows' rows are streamed: in one order both times)
+    try:
+        attn.prefill_step_scored(q, k, v, Kc, Vc, O, nq, nkv, d, m, slot0, slot0 + behind, inv, scale,
+                                 window, 50.0, sl, lo)
+        attn.attn_prefill_scored(q, Kc, Vc, O2, nq, nkv, m, N, d, scale, slot0, window, 50.0, sl, lo)
+    finally:
+        _lib.load().molot_hip_set_block_order(1)
+    assert torch.equal(O.view(torch.int32), O2.view(torch.int32))
+    clean = torch.ones(m, dtype=torch.bool, device="cuda")
+    clean[90:290] = clean[333:390] = False  # documents with the rows that are not ordinary, from there on
+    assert bool(torch.isfinite(O[clean]).all())
 
 
 def test_prefill_step_behind_its_positions(gpu):

@@ -1,19 +1,19 @@
 // MI355X (gfx950) fused RoPE + GQA decode attention.
 //
-// Kernels:
+// This file: the C ABI, the host's plans and the kernels around the attention:
 //   rope_append_kernel   RoPE of q (in place) and of the new k, append of the
 //                        rotated k and v into the cache slot
-//                        (include/molot/forward.h:556-575).
-//   split_kernel         flash-decoding split-K attention: one workgroup per
-//                        (KV head, GQA head subgroup, context chunk, sequence).
-//                        Each K/V row is fetched from HBM once with 16-byte
-//                        coalesced loads and consumed by every query head of
-//                        the group held in registers; chunk scores live in
-//                        LDS; the chunk's (max, sum, unnormalised o) partial
-//                        is written for the combine
-//                        (include/molot/attn.h:125-177 computes the same
-//                        softmax(qK^T*scale)V in three passes per head).
-//   combine_kernel       log-sum-exp merge of the chunk partials.
+//                        (include/molot/forward.h:556-575);
+//   combine_kernel       log-sum-exp merge of a split context's chunk partials
+//                        (combine_wave_kernel: of few chunks; combine_rows_kernel:
+//                        of a prefill's key splits);
+//   attn_weights_kernel  the softmax weights of a scored launch, summed a KV head
+//                        (combine_weights_kernel: beside the merge);
+//   prefill_mfma16_kernel, pf_split_kernel.
+// The decode attention's kernels are in attn_kernels.hpp, its instances in
+// attn_flat.hip, attn_paged.hip and, scored, attn_flat_scored.hip and
+// attn_paged_scored.hip; the prefill's others in prefill_narrow.hip and
+// prefill_wide.hip; a cache's eviction in kv_evict.hip.
 //
 // All shapes are validated on the host before any launch.
 #include <hip/hip_ext.h>

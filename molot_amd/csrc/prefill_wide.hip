@@ -44,6 +44,15 @@
 // the vector-ALU kernel (prefill_rows), 196 us here; of the kernel trace's 215
 // this kernel 159, the RoPE/append 33, the merge of the key splits 16, the
 // split 7.
+//
+// Scored (SC; also built for D = 256, whose unscored prompts run on
+// prefill_mfma16_kernel: two slices of the head dim, four row groups): 1999 tokens
+// of 8q/2kv/d512 fp32, us, the attention with its split and merge: 165 unscored,
+// 163 with nothing to score, 164 with a cap, 168 with slopes, 171 with both, 80 in
+// documents of 37 to 592 with a cap; 2048 of 8q/4kv/d256 bf16 96, 100, 98, 102 and
+// 50.  A tile there takes 3.8 us against the 0.9 of its products: scores 1.2 and
+// 0.5 at their barrier, softmax 0.95, PV 1.0; the first comes 7.5 us after the
+// start (ranges, then rows).
 #include <hip/hip_runtime.h>
 
 #include "device_util.hpp"

@@ -320,8 +320,10 @@ int molot_hip_attn_prefill_paged(const float* Qm, const void* K, const void* V, 
  * a row sets that slot's acc instead, and its position in slot_pos (int32,
  * same layout; NULL: none; only with acc).  The scores of a call with acc are
  * kept for its second launch: 4 * B * nq * (attended rows + 1) bytes of the
- * stream's prefill workspace, at most 1 GiB (MOLOT_ENOTSUP past it, and past
- * 4096 query heads a KV head or 65535 sequences). */
+ * stream's prefill workspace, at most 8 GiB and 2 GiB a KV head
+ * (MOLOT_ENOTSUP past it, and past 4096 query heads a KV head or 65535
+ * sequences).  The workspaces are the stream's: graphs captured on one stream
+ * replay one after the other. */
 int molot_hip_attn_decode_scored(const float* Q, const void* K, const void* V, float* O, int nq,
                                  int nkv, int n, int d, float scale, int pos_cur, int window,
                                  float softcap, const float* slopes, float* acc, int acc_cap,
@@ -471,7 +473,8 @@ void molot_hip_set_merge(int in_launch);
  * row, each row scaled by a power of two, into a per-stream workspace of 4
  * (bf16, Q8) or 8 (fp32) bytes * nkv * (N - t0) * d (at most 1 GiB; it grows
  * outside stream capture only, and the buffers it outgrows stay allocated,
- * under 1 GiB in all).  Smaller prompts over fp32 and Q8 caches take K and V
+ * under 1 GiB in all; scored prompts take the pieces at every head dim, from
+ * sizes of their own, and up to 8 GiB of them).  Smaller prompts over fp32 and Q8 caches take K and V
  * as two such pieces too: at d = 256, where one step appends all the keys it
  * attends, and at d <= 128 where that is faster, made once per launch (12 bytes
  * * nkv * (N - t0) * d of the same workspace), else by the attention kernel from

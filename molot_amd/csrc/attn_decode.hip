@@ -1857,8 +1857,9 @@ int molot_host::pieces_workspace(void* stream, size_t bytes, void** out) {
     e = hipStreamIsCapturing((hipStream_t)stream, &cap);
     if (e != hipSuccess) return (int)e;
     if (cap != hipStreamCaptureStatusNone) return MOLOT_ENOWS;
-    // at most kMaxPiecesBytes (bytes never exceeds it), so the live buffer
-    // and the retired ones a captured graph may still hold stay under 2 GiB
+    // twice the size up to kMaxPiecesBytes, past it what is asked for: without
+    // scored calls the live buffer and the retired ones a captured graph may
+    // still hold stay under 2 GiB
     const size_t want = std::min(std::max(bytes, 2 * w.bytes), std::max(bytes, kMaxPiecesBytes));
     void* p = nullptr;
     e = hipMalloc(&p, want);
@@ -2069,7 +2070,8 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
     if (B > 65535 || a.nq / a.nkv > 4096) return MOLOT_ENOTSUP;  // attn_weights_kernel's grid, its LDS
     a.sc_rows = (std::max(span, 0) + 4) & ~3;  // (and the appended row)
     const size_t bytes = sizeof(float) * (size_t)B * a.nq * a.sc_rows;
-    if (bytes > kMaxPiecesBytes) return MOLOT_ENOTSUP;
+    // (a KV head's own by 31-bit offsets: score_rsrc)
+    if (bytes > kMaxScoredBytes || 4 * a.sc_rows * (a.nq / a.nkv) > 0x7FFFFF00) return MOLOT_ENOTSUP;
     void* sc = nullptr;
     const int st = pieces_workspace(stream, bytes, &sc);
     if (st) return st;
@@ -3320,12 +3322,12 @@ static bool prefill_scored_pieces(int d, int M, int N, int nq, int nkv, int wind
 }
 
 // Their workspace for the attended keys [T0, N).
-static int pieces32_workspace(int nkv, int N, int d, int pos0, int window, int kv_dtype,
+static int pieces32_workspace(int nkv, int N, int d, int pos0, int window, int kv_dtype, bool scored,
                               void* stream, void** ws, int* T0, int* R) {
   *T0 = window > 0 && pos0 - window + 1 > 0 ? std::min(pos0 - window + 1, N) : 0;
   *R = N - *T0;
   const size_t need = wide_bytes(nkv, prefill_D(d), wide_pieces(kv_dtype == MOLOT_KV_F32), *R);
-  if (need > kMaxPiecesBytes) return MOLOT_ENOWS;
+  if (need > (scored ? kMaxScoredBytes : kMaxPiecesBytes)) return MOLOT_ENOWS;
   return without_memory(pieces_workspace(stream, need, ws));
 }
 
@@ -3365,7 +3367,7 @@ static int prefill_on_pieces(const float* Qm, const void* K, const void* V, floa
     while ((1 << a.page_shift) < page) ++a.page_shift;
   }
   void* pieces = nullptr;
-  int st = pieces32_workspace(nkv, N, d, pos0, window, kv_dtype, stream, &pieces, &a.T0, &a.R);
+  int st = pieces32_workspace(nkv, N, d, pos0, window, kv_dtype, sc.on, stream, &pieces, &a.T0, &a.R);
   if (st) return st;
   if (a.R == 0) return zero_out(Om, (int64_t)M * nq * d, (hipStream_t)stream);  // no key attended
   a.pieces = reinterpret_cast<const uint16_t*>(pieces);
@@ -3431,6 +3433,21 @@ static int attn_prefill_impl(const float* Qm, const void* K, const void* V, floa
   if (N == 0) return zero_out(Om, (int64_t)M * nq * d, (hipStream_t)stream);
   if (!K || !V || !aligned16(K) || !aligned16(V) || !aligned16(Qm) || !aligned16(Om))
     return MOLOT_EINVAL;
+  if (sc.on && M > 65535) {  // (the launches' grids) by parts
+    constexpr int kPart = 32768;
+    for (int m0 = 0; m0 < M; m0 += kPart) {
+      Scoring part = sc;
+      if (sc.key_lo) part.key_lo += m0;
+      if (sc.key_hi) part.key_hi += m0;
+      const int Mp = std::min(kPart, M - m0);
+      const int Np = sc.key_hi ? N : (int)std::min<int64_t>(N, (int64_t)pos0 + m0 + Mp);
+      const int64_t at = (int64_t)m0 * nq * d;
+      st = attn_prefill_impl(Qm + at, K, V, Om + at, nq, nkv, Mp, Np, d, scale, pos0 + m0, window,
+                             kv_dtype, block_row, page, part, stream, presplit, -1);
+      if (st) return st;
+    }
+    return 0;
+  }
   if (sc.on ? prefill_scored_pieces(d, M, N, nq, nkv, window, kv_dtype, presplit)
             : prefill_takes_pieces(d, M, N, nq, nkv, kv_dtype, window, presplit)) {
     st = prefill_on_pieces(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype, block_row,
@@ -3637,7 +3654,8 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
     // 124.1; 16q/4kv/d64 86.2 / 84.7, 76.2 / 75.5, 77.4 / 77.1)
     if ((d == 64 || d == 128) && !(sc.on && kv_dtype == MOLOT_KV_Q8)) {
       int R = 0;
-      st = pieces32_workspace(nkv, slot0 + M, d, apos, window, kv_dtype, stream, &pws, &T0, &R);
+      st = pieces32_workspace(nkv, slot0 + M, d, apos, window, kv_dtype, sc.on, stream, &pws, &T0,
+                              &R);
       if (st && st != MOLOT_ENOWS) return st;
       if (!st) {
         r.pc_R = R;

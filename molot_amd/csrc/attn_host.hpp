@@ -36,7 +36,9 @@ inline int pick_gh(int G) {
 // share.  MOLOT_ENOWS: a capture that would have to grow one.
 int workspace(void* stream, size_t bytes, unsigned long long** ctr, void** out);
 int pieces_workspace(void* stream, size_t bytes, void** out);
-constexpr size_t kMaxPiecesBytes = (size_t)1 << 30;  // the most that pieces_workspace is asked for
+constexpr size_t kMaxPiecesBytes = (size_t)1 << 30;  // the most that pieces_workspace is asked for,
+constexpr size_t kMaxScoredBytes = (size_t)8 << 30;  // and by scored calls, which have no other path
+                                                     // for long prompts, and none for the weights
 
 // Chunking and workspace of one launch.
 int plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int B, int align, int wpc,

@@ -552,6 +552,40 @@ def test_prefill_step_pieces(gpu, kv, d, slot0, behind, window):
     assert bool(torch.isfinite(O[clean]).all())
 
 
+def test_prefill_of_more_rows_than_a_grid(gpu):
+    """70001 rows in one call: every row its own keys, on either side of the parts' ends."""
+    nq, nkv, d, m = 2, 1, 64, 70001
+    g = gen(49)
+    q = randn(g, m, nq, d, sigma=3.0)
+    Kc, K = ref.make_cache(randn(g, m, nkv, d), "bf16")
+    Vc, V = ref.make_cache(randn(g, m, nkv, d), "bf16")
+    lo = attn.document_starts([700] * 100 + [1]).cuda()
+    hi = (torch.arange(m, device="cuda") + 30).int()
+    sl = slopes_of(nq)
+    O = torch.full((m, nq, d), math.nan, device="cuda")
+    attn.attn_prefill_scored(q, Kc, Vc, O, nq, nkv, m, m, d, 0.125, 0, 0, 50.0, sl, lo, hi)
+    assert bool(torch.isfinite(O).all())
+    some = torch.tensor([0, 1, 699, 700, *range(32760, 32776), *range(65528, 65544), m - 2, m - 1],
+                        device="cuda")
+    want, _ = ref.attend(q[some], K, V, 0.125, some, lo[some].long(), hi[some].long().clamp(max=m), 50.0, sl)
+    check_out(O[some], want, ref.tolerance(q[some], K, V, 0.125, 50.0, sl, m))
+
+
+def test_prefill_pieces_past_a_gigabyte(gpu):
+    """A long fp32 cache: 1.15 GB of pieces."""
+    nq, nkv, d, m, N = 8, 8, 128, 64, 140001
+    g = gen(50)
+    q = randn(g, m, nq, d, sigma=3.0)
+    Kc, K = ref.make_cache(randn(g, N, nkv, d), "f32")
+    Vc, V = ref.make_cache(randn(g, N, nkv, d), "f32")
+    O = torch.empty(m, nq, d, device="cuda")
+    attn.attn_prefill_scored(q, Kc, Vc, O, nq, nkv, m, N, d, 0.09, N - m, 0, 50.0)
+    some = torch.tensor([0, 31, 63], device="cuda")
+    pos = N - m + some
+    want, _ = ref.attend(q[some], K, V, 0.09, pos, torch.zeros_like(pos), pos + 1, 50.0)
+    check_out(O[some], want, ref.tolerance(q[some], K, V, 0.09, 50.0, None, N))
+
+
 def test_prefill_step_behind_its_positions(gpu):
     """slot0 < pos0 (rows were evicted): a row sees no row appended after it."""
     nq, nkv, d, m, slot0, pos0 = 8, 4, 128, 40, 25, 300

@@ -2007,6 +2007,15 @@ int plan_chunk(int span, int rows_of_wgs, int align, int wpc, int split, int wpc
 // 7.9, 8.7, 9.5 against 6.4, 8.2, 9.5.
 constexpr int kOneChunkSpan = 64, kBriefSpan = 2048;
 constexpr long kBriefWork = 1 << 19;
+// How a launch's chunks are merged (g_merge).  A launch that keeps weights has a second
+// one for them in any case, which merges beside it (combine_weights_kernel): left to the
+// library it does, us a step with weights, merged in the launch against beside the
+// weights: fp32 32q/8kv/d128 301 rows 10.3 / 7.7, 16385 29.7 / 26.4; 8q/4kv/d256, window
+// 1024, 12.0 / 8.7.
+int merge_mode(const AttnArgs& a) {
+  const int m = knob(g_merge);
+  return m < 0 && a.acc ? 0 : m;
+}
 }  // namespace
 int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int B, int align, int wpc,
                 void* stream, bool cyclic) {
@@ -2025,7 +2034,7 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
       nch = (target + rows - 1) / rows;
       if (wpcu <= 0 && d <= 256 && span <= kOneChunkSpan) {
         nch = 1;
-      } else if (wpcu <= 0 && d <= 256 && span <= kBriefSpan && knob(g_merge) < 0 &&
+      } else if (wpcu <= 0 && d <= 256 && span <= kBriefSpan && merge_mode(a) < 0 &&
                  (rows % 8 == 0 || (rows >= 4 && rows < 8)) &&
                  (a.matrix || (!a.chunk_fast && (long)span * gh * d <= kBriefWork))) {
         a.brief = 1;
@@ -2109,7 +2118,7 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
   // batches of short paged sequences merge few chunks cheaply in the
   // combine kernel: c4 234.8 against 239.3 us).  The matrix-core kernel
   // keeps the combine kernel (launch_mfma).
-  const int mk = knob(g_merge);
+  const int mk = merge_mode(a);
   const bool want =
       mk > 0 || (mk < 0 && (a.brief || (rows % 8 == 0 && !a.block_table && span >= kMergeAutoSpan)));
   const bool merge = want && !a.chunk_fast && (rows % 8 == 0 || rows < 8) &&

@@ -114,6 +114,25 @@ def test_decode_weights(gpu, kv, nq, nkv, d, n, window, softcap, alibi):
     assert torch.equal(acc[:, n:], before[:, n:]) and torch.equal(acc[:, :int(lo)], before[:, :int(lo)])
 
 
+@pytest.mark.parametrize("merge", [-1, 0, 1])
+@pytest.mark.parametrize("kv,nq,nkv,d,n", [("f32", 32, 8, 128, 300), ("f32", 32, 8, 128, 9001),
+                                           ("bf16", 32, 8, 128, 700), ("q8", 32, 8, 128, 50)])
+def test_decode_weights_by_each_merge(gpu, kv, nq, nkv, d, n, merge):
+    q, Kc, Vc, K, V, sl = decode_problem(kv, nq, nkv, d, n, True)
+    O, acc = torch.empty(1, nq, d, device="cuda"), torch.zeros(nkv, n, device="cuda")
+    _lib.load().molot_hip_set_merge(merge)
+    try:
+        attn.attn_decode_scored(q, Kc, Vc, O, nq, nkv, n, d, 0.09, n - 1, 0, 50.0, sl, acc)
+    finally:
+        _lib.load().molot_hip_set_merge(-1)
+    lo, hi, pos = span(n, n - 1, 0)
+    want, p = ref.attend(q, K, V, 0.09, pos, lo, hi, 50.0, sl)
+    check_out(O, want, ref.tolerance(q, K, V, 0.09, 50.0, sl, n))
+    w = p.view(nkv, nq // nkv, n).sum(1)
+    # (the tolerance of test_two_streams_at_once for one step)
+    assert float((acc.double() - w).abs().max()) < 1e-4 * float(w.max())
+
+
 def test_decode_empty_ranges(gpu):
     """No slot, or a window past them all: o = 0, acc left alone."""
     nq, nkv, d, n = 8, 4, 64, 40

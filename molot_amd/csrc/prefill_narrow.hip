@@ -290,7 +290,7 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
     };
     if constexpr (SC)
       fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl,
-                             [&](float (&s)[16]) { rsc.apply<16>(s, slot); });
+                             [&](float (&s)[16], auto&& again) { rsc.apply<16>(s, slot, again); });
     else
       fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
   };

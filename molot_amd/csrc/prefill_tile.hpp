@@ -209,9 +209,10 @@ __device__ __forceinline__ void mark_split(const PfArgs& a, int h, int r0, int s
 struct RowScore {
   float cap2 = 0.f, rcap = 0.f, slope = 0.f;
   int pos = 0;
-  template <int N, typename SLOT>
-  __device__ __forceinline__ void apply(float (&s)[N], SLOT&& slot) const {
-    if (cap2 > 0.f) cap_scores<N>(s, cap2, rcap);           // wave-uniform, as the next
+  // again: cap_scores
+  template <int N, typename SLOT, typename AGAIN>
+  __device__ __forceinline__ void apply(float (&s)[N], SLOT&& slot, AGAIN&& again) const {
+    if (cap2 > 0.f) cap_scores<N>(s, cap2, rcap, again);    // wave-uniform, as the next
     if (__builtin_amdgcn_ballot_w64(slope != 0.f) != 0) {  // (a flag would be one more register)
 #pragma unroll
       for (int e = 0; e < N; ++e) s[e] = fmaf(-slope, fabsf((float)(pos - slot(e))), s[e]);
@@ -308,7 +309,8 @@ __device__ __forceinline__ void own_rows(uint64_t args, int h, int row0, int n, 
         s[u] = SC || t0 + u < hi ? x : -INFINITY;
       }
       if constexpr (SC) {
-        rsc.apply<2>(s, [&](int u) { return t0 + u; });
+        const float as[2] = {s[0], s[1]};
+        rsc.apply<2>(s, [&](int u) { return t0 + u; }, [&](int u) { return as[u]; });
         if (t0 + 1 >= hi) s[1] = -INFINITY;
       }
       const float mn = fmaxf(mx, fmaxf(s[0], s[1]));
@@ -388,7 +390,7 @@ __device__ __forceinline__ float div_by(float o, float l, float inv) {
 // bits more than needed, so that the next records of 32 rows do not each
 // rescale o.
 //
-// mod(s): the scores in base-2 units past the product (NoMod: as they are).
+// mod(s, again): the scores in base-2 units past the product (NoMod: as they are).
 struct NoMod {};
 template <int NK, typename GMAX, typename DEAD, typename MOD = NoMod>
 __device__ __forceinline__ float softmax_tile(float (&s)[NK], const float (&ku)[NK],
@@ -398,15 +400,21 @@ __device__ __forceinline__ float softmax_tile(float (&s)[NK], const float (&ku)[
                                               MOD&& mod = MOD{}) {
   constexpr bool SC = !std::is_same<typename std::decay<MOD>::type, NoMod>::value;
   const float qunit = SC ? 1.f : unit;
-  constexpr int kRoom = 3;
+  constexpr int kRoom = SC ? 10 : 3;
   constexpr int kNoShift = 1 << 20;
   float ps, zt, z[NK];
-#pragma unroll
-  for (int e = 0; e < NK; ++e) s[e] *= ku[e];
   if constexpr (SC) {
+    float raw[NK];
+    auto again = [&](int e) { return raw[e] * ku[e] * unit; };
 #pragma unroll
-    for (int e = 0; e < NK; ++e) s[e] *= unit;
-    mod(s);
+    for (int e = 0; e < NK; ++e) {
+      raw[e] = s[e];
+      s[e] = again(e);
+    }
+    mod(s, again);
+  } else {
+#pragma unroll
+    for (int e = 0; e < NK; ++e) s[e] *= ku[e];
   }
   if (!full) {
 #pragma unroll

@@ -260,7 +260,7 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
     qunit = f16_row_unit(f16_row_shift(qm));
   }
 
-  f32x16 o[4];
+  float o[4][16];  // (scalars: as vectors they were moved back to their registers every tile)
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -400,9 +400,10 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
       auto gmax = [](float x) { return group_max<LPR>(x); };
       auto dead = [&](int e) { return k0 + e < rt0 || k0 + e >= rnn; };
       if constexpr (SC)
-        fac = softmax_tile<KPL>(sv, ku, vu, qunit, rs, full, gmax, dead, yh, yl, [&](float (&s)[KPL]) {
-          rsc.template apply<KPL>(s, [&](int e) { return k0 + e; });
-        });
+        fac = softmax_tile<KPL>(sv, ku, vu, qunit, rs, full, gmax, dead, yh, yl,
+                                [&](float (&s)[KPL], auto&& again) {
+                                  rsc.template apply<KPL>(s, [&](int e) { return k0 + e; }, again);
+                                });
       else
         fac = softmax_tile<KPL>(sv, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
       next_k(2);
@@ -476,7 +477,9 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
         if (b > 0) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[b - 1][i] = fmaf(o[b - 1][i], fac, t[(b - 1) & 1][i]);
-          asm volatile("" : "+v"(o[b - 1]));  // (else all of them sink to the loop's end)
+          // (else all of them sink to the loop's end)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(o[b - 1][i]));
         }
         __builtin_amdgcn_sched_barrier(0);
       }

@@ -37,11 +37,11 @@
 // 16384 bf16 414 -> 301, Q8 485 -> 298, fp32 497 -> 438 us.
 //
 // Scored (SC; 32q/8kv/d128, 2048 tokens, fp32 / bf16, us, the attention with its
-// split): 133 / 103 unscored, 134 / 107 with nothing to score (rows that are checked
-// for what the pieces cannot hold, ranges), 144 / 118 with a cap, 139 / 112 with
-// slopes, 150 / 123 with both: they lie on the softmax's chain, which the other key
-// group's products hide only in part.  Documents of 37 to 592 with a cap 66 / 60.
-// 240 TFLOP/s of the causal products with a cap over fp32.
+// split): 138 / 101 unscored, 135 / 102 with nothing to score (rows that are checked
+// for what the pieces cannot hold, ranges), 143 / 112 with a cap, 134 / 108 with
+// slopes, 143 / 119 with both: they lie on the softmax's chain, which the other key
+// group's products hide only in part (10 vector instructions a score for the cap,
+// beside 18 of the softmax).  Documents of 37 to 592 with a cap 64 / 60.
 #include <hip/hip_runtime.h>
 
 #include "device_util.hpp"
@@ -290,7 +290,8 @@ __global__ __launch_bounds__(512) void prefill_narrow_kernel(PfArgs a) {
     };
     if constexpr (SC)
       fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl,
-                             [&](float (&s)[16], auto&& again) { rsc.apply<16>(s, slot, again); });
+                             [&](float (&s)[16], auto&& again) { rsc.apply<16>(s, slot, again); },
+                             wide_room(a.R));
     else
       fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
   };

@@ -386,21 +386,27 @@ __device__ __forceinline__ float div_by(float o, float l, float inv) {
 // A tile whose probabilities and y stay in range (the usual one) takes no row
 // maximum: p from the m so far, and two checks.  Otherwise, in any row of the
 // wave, m moves where a score passes it by 4, by a whole number past it; wsh
-// follows o down with it, and is lowered where y would pass 2^14, by kRoom
+// follows o down with it, and is lowered where y would pass 2^14, by `room`
 // bits more than needed, so that the next records of 32 rows do not each
-// rescale o.
+// rescale o.  y's pieces end 2^-(39 - room) below the largest y: a row of N keys
+// loses at most N times that.  Scored: as much room as leaves 2^-20 (wide_room), since
+// capped layers' raw scores spread wide (32q/8kv/d128 fp32, 2048 tokens, us, for 3,
+// 6, 8 and 10 bits: 140.1, 138.7, 137.7, 137.1).
 //
 // mod(s, again): the scores in base-2 units past the product (NoMod: as they are).
 struct NoMod {};
+constexpr int kTileRoom = 3;
+__device__ __forceinline__ int wide_room(int keys) {  // 18 - log2(keys), within 3 .. 10
+  return max(kTileRoom, min(10, __builtin_clz((unsigned)max(keys, 1)) - 13));
+}
 template <int NK, typename GMAX, typename DEAD, typename MOD = NoMod>
 __device__ __forceinline__ float softmax_tile(float (&s)[NK], const float (&ku)[NK],
                                               const float (&vu)[NK], float unit, RowState& st,
                                               bool full, GMAX&& gmax, DEAD&& dead,
                                               uint32_t (&yh)[NK / 2], uint32_t (&yl)[NK / 2],
-                                              MOD&& mod = MOD{}) {
+                                              MOD&& mod = MOD{}, int room = kTileRoom) {
   constexpr bool SC = !std::is_same<typename std::decay<MOD>::type, NoMod>::value;
   const float qunit = SC ? 1.f : unit;
-  constexpr int kRoom = SC ? 10 : 3;
   constexpr int kNoShift = 1 << 20;
   float ps, zt, z[NK];
   if constexpr (SC) {
@@ -452,7 +458,7 @@ __device__ __forceinline__ float softmax_tile(float (&s)[NK], const float (&ku)[
     zt = gmax(zt);
     const int grown = min(st.wsh + gsh, kNoShift);
     const int most = zt > 0.f ? f16_row_shift(zt) : kNoShift;
-    int ns = most < grown ? most - kRoom : grown;
+    int ns = most < grown ? most - room : grown;
     ns = ns == kNoShift ? ns : min(ns, 126);
     fac = ldexpf(1.f, ns - st.wsh - gsh);  // 0 while the row has no key
     st.l *= ldexpf(1.f, -gsh);

@@ -47,11 +47,11 @@
 //
 // Scored (SC; also built for D = 256, whose unscored prompts run on
 // prefill_mfma16_kernel: two slices of the head dim, four row groups): 1999 tokens
-// of 8q/2kv/d512 fp32, us, the attention with its split and merge: 165 unscored,
-// 163 with nothing to score, 164 with a cap, 168 with slopes, 171 with both, 80 in
-// documents of 37 to 592 with a cap; 2048 of 8q/4kv/d256 bf16 96, 100, 98, 102 and
-// 50.  A tile there takes 3.8 us against the 0.9 of its products: scores 1.2 and
-// 0.5 at their barrier, softmax 0.95, PV 1.0; the first comes 7.5 us after the
+// of 8q/2kv/d512 fp32, us, the attention with its split and merge: 159 unscored,
+// 157 with nothing to score, 156 with a cap, 161 with slopes, 163 with both, 77 in
+// documents of 37 to 592 with a cap; 2048 of 8q/4kv/d256 bf16 90, 94, 93, 97 and
+// 49.  A tile there takes 3.7 us against the 0.9 of its products: scores 1.2 and
+// 0.5 at their barrier, softmax 0.9, PV 1.0; the first comes 7.5 us after the
 // start (ranges, then rows).
 #include <hip/hip_runtime.h>
 
@@ -286,17 +286,12 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
 
   const float* kun = reinterpret_cast<const float*>(khead + NP * Rp * D) - a.T0;
   const float* vun = reinterpret_cast<const float*>(vhead + NP * Rp * D) - a.T0;
-  float ku[KPL], vu[KPL];
+  f32x4_u ku4[KPL / 4], vu4[KPL / 4];
   auto load_units = [&](int tk) {
 #pragma unroll
-    for (int q = 0; q < KPL; q += 4) {
-      const f32x4_u x = *reinterpret_cast<const f32x4_u*>(kun + tk + (uint32_t)(KPL * oc + q));
-      const f32x4_u y = *reinterpret_cast<const f32x4_u*>(vun + tk + (uint32_t)(KPL * oc + q));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        ku[q + e] = x[e];
-        vu[q + e] = y[e];
-      }
+    for (int q = 0; q < KPL / 4; ++q) {
+      ku4[q] = *reinterpret_cast<const f32x4_u*>(kun + tk + (uint32_t)(KPL * oc + 4 * q));
+      vu4[q] = *reinterpret_cast<const f32x4_u*>(vun + tk + (uint32_t)(KPL * oc + 4 * q));
     }
   };
   float mark = 0.f;  // NaN once a tile's units held one (a row's lanes hold all its keys)
@@ -393,8 +388,13 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
       }
       const bool full = __builtin_amdgcn_ballot_w64(tk < rt0 || tk + KT > rnn) == 0;
       next_k(1);
+      float ku[KPL], vu[KPL];
 #pragma unroll
-      for (int e = 0; e < KPL; ++e) mark = fmaf(ku[e] + vu[e], 0.f, mark);
+      for (int e = 0; e < KPL; ++e) {
+        ku[e] = ku4[e / 4][e % 4];
+        vu[e] = vu4[e / 4][e % 4];
+        mark = fmaf(ku[e] + vu[e], 0.f, mark);
+      }
       uint32_t yh[KPL / 2], yl[KPL / 2];
       float fac;
       auto gmax = [](float x) { return group_max<LPR>(x); };
@@ -403,7 +403,8 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
         fac = softmax_tile<KPL>(sv, ku, vu, qunit, rs, full, gmax, dead, yh, yl,
                                 [&](float (&s)[KPL], auto&& again) {
                                   rsc.template apply<KPL>(s, [&](int e) { return k0 + e; }, again);
-                                });
+                                },
+                                wide_room(a.R));
       else
         fac = softmax_tile<KPL>(sv, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
       next_k(2);
@@ -487,8 +488,8 @@ __global__ __launch_bounds__(512) void prefill_wide_kernel(PfArgs a) {
       for (int i = 0; i < 16; ++i) o[3][i] = fmaf(o[3][i], fac, t[1][i]);
     }
 #pragma unroll
-    for (int e = 0; e < KPL; ++e)
-      asm volatile("" : "+v"(ku[e]), "+v"(vu[e]));  // the units' wait falls here
+    for (int q = 0; q < KPL / 4; ++q)
+      asm volatile("" : "+v"(ku4[q]), "+v"(vu4[q]));  // the units' wait falls here
     wait_vmcnt<0>();  // the next tile's copies (one buffer: K's) are in LDS
     lds_barrier();    // C: V, P and the shares may be overwritten
   }

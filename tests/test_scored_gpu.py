@@ -571,6 +571,34 @@ def test_prefill_step_pieces(gpu, kv, d, slot0, behind, window):
     assert bool(torch.isfinite(O[clean]).all())
 
 
+@pytest.mark.parametrize("kv,d", [("f32", 128), ("bf16", 64), ("f32", 256), ("bf16", 512)])
+@pytest.mark.parametrize("below", [16.0, 21.0, 24.0])
+def test_prefill_of_one_key_above_a_long_tail(gpu, kv, d, below):
+    """One key, then 16383 that are e^-below of it each and together up to 2e-3 of the
+    output: none of them may be dropped as small."""
+    nq, nkv, m, N = 4, 1, 520, 16384
+    g = gen(52)
+    K, V = torch.zeros(N, nkv, d, device="cuda"), 1 + 0.01 * randn(g, N, nkv, d)
+    K[5, 0, 0], V[5] = 1.0, -1.0
+    q = torch.zeros(m, nq, d, device="cuda")
+    q[:, :, 0] = below
+    Kc, K = ref.make_cache(K, kv)
+    Vc, V = ref.make_cache(V, kv)
+    O = torch.empty(m, nq, d, device="cuda")
+    sl = torch.zeros(nq, device="cuda")
+    attn.attn_prefill_scored(q, Kc, Vc, O, nq, nkv, m, N, d, 1.0, N - m, 0, 0.0, sl)
+    some = torch.tensor([0, 1, 31, 32, 300, 519], device="cuda")
+    pos = N - m + some
+    want, _ = ref.attend(q[some], K, V, 1.0, pos, torch.zeros_like(pos), pos + 1, 0.0)
+    # Every score is one exact product (below * 1, or 0), so what moves is: the one key's
+    # score in base 2 by three roundings of half an ulp of 32, 2^-20 each, and the tail
+    # (mass w of the output, its V 2 away) with it; the sum (test_prefill's 2^-21 and
+    # 8 2^-24 of |V|); and what the pieces drop of 2^14 keys, 2^-20 of |V|.
+    w = N * math.exp(-below)
+    vmax = float(V.abs().max())
+    check_out(O[some], want, 2 * w * 3 * 2.0 ** -20 + (2.0 ** -21 + 8 * ref.EPS32 + 2.0 ** -20) * vmax)
+
+
 def test_prefill_of_more_rows_than_a_grid(gpu):
     """70001 rows in one call: every row its own keys, on either side of the parts' ends."""
     nq, nkv, d, m = 2, 1, 64, 70001

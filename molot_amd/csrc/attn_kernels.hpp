@@ -44,14 +44,14 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
 // the cap and the bias before the softmax, and where the caller keeps weights they
 // are also stored, with each chunk's (max, sum), for attn_weights_kernel.  us a step,
 // unscored | nothing to score, a cap, slopes, both | weights, weights and a cap:
-//   32q/8kv/d128 fp32, 16385 rows   25.9 | 26.2, 26.3, 27.0, 27.2 | 29.6, 29.8
+//   32q/8kv/d128 fp32, 16385 rows   25.9 | 26.2, 26.3, 27.0, 27.2 | 26.5, 26.6
 //   bf16, 16001                     18.9 | 19.3, 19.5, 19.6, 19.7 | 20.0, 20.2
 //   Q8, 16001                       15.9 | 17.1, 17.5, 17.1, 17.6 | 17.5, 18.1
 //   64q/8kv/d128 bf16, 131072       100 | 98, 98, 98, 98 | 126, 126
-//   8q/4kv/d256 fp32, window 1024   8.7 | 8.9, 9.1, 9.6, 9.7 | 11.9, 12.0
+//   8q/4kv/d256 fp32, window 1024   8.7 | 9.0, 9.1, 9.7, 9.8 | 8.9, 8.9
 //   13 paged sequences of 1 to 2999 rows, Q8: 19.3 | 20.3, 20.5 | 23.0, 23.5
 // So a scored step is bounded by what bounds the plain one; the weights by their second
-// launch (1 to 4 us) and, in a long cache, by the stores of the scores between the loads.
+// launch (0.3 to 3 us) and, in a long cache, by the stores of the scores between the loads.
 //
 // Grid (nkv * subgroups, sequences, chunks).  Workgroup (h/sub, b, c) owns
 // chunk c of the context rows of KV head h and the GH query heads

@@ -37,9 +37,9 @@
 // 16384 bf16 414 -> 301, Q8 485 -> 298, fp32 497 -> 438 us.
 //
 // Scored (SC; 32q/8kv/d128, 2048 tokens, fp32 / bf16, us, the attention with its
-// split): 138 / 101 unscored, 135 / 102 with nothing to score (rows that are checked
-// for what the pieces cannot hold, ranges), 143 / 112 with a cap, 134 / 108 with
-// slopes, 143 / 119 with both: they lie on the softmax's chain, which the other key
+// split): 129 / 101 unscored, 129 / 101 with nothing to score (rows that are checked
+// for what the pieces cannot hold, ranges), 137 / 112 with a cap, 132 / 108 with
+// slopes, 142 / 119 with both: they lie on the softmax's chain, which the other key
 // group's products hide only in part (10 vector instructions a score for the cap,
 // beside 18 of the softmax).  Documents of 37 to 592 with a cap 64 / 60.
 #include <hip/hip_runtime.h>

@@ -41,7 +41,7 @@
 // LDS reads and the stores of the shares), the softmax with the next K copies
 // 1900.  The copies go out between products and softmax steps: in a row they
 // held each wave ~500 cycles.  The step: 1468 us with each query row streamed by
-// the vector-ALU kernel (prefill_rows), 196 us here; of the kernel trace's 215
+// the vector-ALU kernel (prefill_rows), 193 us here; of the kernel trace's 215
 // this kernel 159, the RoPE/append 33, the merge of the key splits 16, the
 // split 7.
 //

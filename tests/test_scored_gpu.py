@@ -309,6 +309,27 @@ def test_paged_with_weights(gpu, kv, nq, nkv, d, lens, page, window, alibi):
     assert float((acc.double() - grown).abs().max()) <= tol_w + 2 * ref.EPS32 * (G + 1)
 
 
+def test_paged_weights_past_a_gigabyte(gpu):
+    """64 sequences of 70000 rows under 64 heads: 1.15 GB of scores kept for the weights."""
+    nq, nkv, d, page, B, n = 64, 1, 64, 16, 64, 70000
+    g, G, width = gen(36), nq // nkv, n // page
+    table = torch.randperm(B * width, device="cuda", generator=g).int().view(B, width)
+    K, V = (randn(g, B * width, page * d).bfloat16() for _ in range(2))
+    acc = torch.zeros(B * width, nkv, page, device="cuda")
+    q, O = randn(g, B, nq, d, sigma=3.0), torch.empty(B, nq, d, device="cuda")
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    attn.attn_decode_paged_scored(q, K, V, O, table, lens, None, B, width, nq, nkv, d, page, 0.125, 0,
+                                  50.0, None, acc)
+    lo, hi, pos = span(n, n - 1, 0)
+    for b in (0, 31, B - 1):
+        Kb, Vb = (x[table[b].long()].view(n, nkv, d).double() for x in (K, V))
+        want, p = ref.attend(q[b:b + 1], Kb, Vb, 0.125, pos, lo, hi, 50.0)
+        check_out(O[b], want[0], ref.tolerance(q[b:b + 1], Kb, Vb, 0.125, 50.0, None, n))
+        got = acc[table[b].long()].view(n).double()
+        tol = ref.tolerance(q[b:b + 1], Kb, torch.ones_like(Vb), 0.125, 50.0, None, n) * G
+        assert float((got - p.view(G, n).sum(0)).abs().max()) <= tol
+
+
 @pytest.mark.parametrize("kv", KVS)
 @pytest.mark.parametrize("lag", [0, 3, None])
 def test_paged_step(gpu, kv, lag):

@@ -16,8 +16,8 @@
 // head (load, count, scan, list, move): 4352 bf16 slots of 8 heads (d = 128) cut to 4096
 // in 9.9 us, and kv_track_kernel 2.0, against 0.5 for the bytes; 32 paged sequences of
 // 700 to 1399 Q8 rows cut to 1024 in 12.5.  131072 bf16 slots of 8 heads cut by 8192:
-// keys 10.6, pick 7.3, rank 2.7, list 7.4 us (a launch each, a chunk of 8192 slots a
-// workgroup: half the CUs) and the moves 15.0, which read and write 67 MB at 4.5 TB/s.
+// keys 7.0, pick 8.6, rank 2.7, list 5.3 us (a launch each, a chunk of 4096 slots a
+// workgroup) and the moves 15.0, which read and write 67 MB at 4.5 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -470,7 +470,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(SlotArgs a, int most, c
 }
 
 // ---------------------------------------------------------------------------
-// Longer sequences: chunks of kChunk slots, a workgroup each, on either side of
+// Longer sequences: chunks of 4096 or 8192 slots (CK a thread), a workgroup each, on either side of
 // keep (so that a chunk has holes or moves, never both): nlo of [0, keep), then
 // nhi of [keep, n).
 //   evict_keys_kernel   a chunk's keys, and its counts of their top kTopBits bits;
@@ -480,16 +480,15 @@ __global__ __launch_bounds__(256) void evict_move_kernel(SlotArgs a, int most, c
 //   evict_rank_kernel   a workgroup a (KV head, sequence): T among the listed keys,
 //                       and where each chunk's equals and list entries start;
 //   evict_list_kernel   the chunks' holes and moves.
-constexpr int kChunkK = 8, kChunk = kSelThreads * kChunkK;
 constexpr int kTopBits = 12, kBins = 1 << kTopBits, kLowBits = 32 - kTopBits;
 static_assert(kBins == 4 * kSelThreads, "four bins a thread");
 
 constexpr int kAt = 6;
 struct LongArgs {
   SlotArgs s;
-  int keep, recent, most, nlo, nhi;
-  uint32_t* keys;      // [pair][chunks][kChunk]
-  uint32_t* listed;    // [pair][chunks][kChunk]: the keys of the bin
+  int keep, recent, most, nlo, nhi, chunk;
+  uint32_t* keys;      // [pair][chunks][chunk]
+  uint32_t* listed;    // [pair][chunks][chunk]: the keys of the bin
   uint16_t* bins;      // [pair][chunks][kBins]
   int32_t* chunk_at;   // [pair][chunks][kAt]: keys above the bin, listed; then equals and entries
                        // before; the smallest and largest listed
@@ -501,11 +500,13 @@ struct LongArgs {
 // First slot and end of chunk c of a sequence of n rows.
 __device__ __forceinline__ void chunk_range(const LongArgs& g, int n, int c, int& first, int& end) {
   const bool lo = c < g.nlo;
-  first = lo ? c * kChunk : g.keep + (c - g.nlo) * kChunk;
-  end = min(first + kChunk, lo ? min(g.keep, n) : n);
+  first = lo ? c * g.chunk : g.keep + (c - g.nlo) * g.chunk;
+  end = min(first + g.chunk, lo ? min(g.keep, n) : n);
 }
 
+template <int CK>
 __global__ __launch_bounds__(kSelThreads) void evict_keys_kernel(LongArgs g) {
+  constexpr int kChunkK = CK, kChunk = kSelThreads * CK;
   const SlotArgs& a = g.s;
   const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nc = g.nlo + g.nhi, tid = threadIdx.x;
   const int n = rows_of(a, b);
@@ -540,7 +541,9 @@ __global__ __launch_bounds__(kSelThreads) void evict_keys_kernel(LongArgs g) {
       u32x2{v[0] | v[1] << 16, v[2] | v[3] << 16};
 }
 
+template <int CK>
 __global__ __launch_bounds__(kSelThreads) void evict_pick_kernel(LongArgs g) {
+  constexpr int kChunkK = CK, kChunk = kSelThreads * CK;
   const SlotArgs& a = g.s;
   const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nc = g.nlo + g.nhi, tid = threadIdx.x;
   const int n = rows_of(a, b);
@@ -657,7 +660,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(LongArgs g) {
   int32_t* cn = reinterpret_cast<int32_t*>(rank_lds + kRankMax);  // [nc][3]: listed before the
                                                                   // chunk, its keys past T, equals
   int32_t* ca = g.chunk_at + pair * nc * kAt;
-  const uint32_t* listed = g.listed + pair * nc * kChunk;
+  const uint32_t* listed = g.listed + pair * nc * g.chunk;
   const uint32_t top = (uint32_t)g.rank[pair * 4] << kLowBits;
   const int want = g.rank[pair * 4 + 1];
   // (a chunk past the sequence's end has written no counts)
@@ -695,7 +698,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(LongArgs g) {
 #pragma unroll 1
     for (int c = w; c < nc; c += kSelWaves) {
       const int cnt = count_of(c);
-      const uint32_t* from = listed + (int64_t)c * kChunk;
+      const uint32_t* from = listed + (int64_t)c * g.chunk;
 #pragma unroll 1
       for (int j0 = 0; j0 < cnt; j0 += 256) {
         uint32_t k[4];
@@ -728,7 +731,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(LongArgs g) {
           if (cn[3 * mid] <= j) lo = mid;
           else hi = mid - 1;
         }
-        k[i] = listed[(int64_t)lo * kChunk + j - cn[3 * lo]];
+        k[i] = listed[(int64_t)lo * g.chunk + j - cn[3 * lo]];
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -810,7 +813,9 @@ __global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(LongArgs g) {
   }
 }
 
+template <int CK>
 __global__ __launch_bounds__(kSelThreads) void evict_list_kernel(LongArgs g) {
+  constexpr int kChunkK = CK, kChunk = kSelThreads * CK;
   const SlotArgs& a = g.s;
   const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nc = g.nlo + g.nhi, tid = threadIdx.x;
   const int n = rows_of(a, b);
@@ -874,13 +879,22 @@ int launch_evict(const SlotArgs& a, int n, int keep, int recent, int B, void* st
   g.keep = keep;
   g.recent = recent;
   g.most = most;
-  g.nlo = (keep + kChunk - 1) / kChunk;
-  g.nhi = (n - keep + kChunk - 1) / kChunk;
+  // Chunks of 8192 slots; of 4096 where those would leave CUs idle, up to 2^17 slots (every
+  // chunk sums all chunks' counts).  8 heads, us for 8192 / 4096: 20000 slots 24.0 / 19.1,
+  // 65536 35.9 / 21.4, 131072 37.6 / 38.0 (after other work 46.7 / 42.4), 200000 39.7 / 51.8,
+  // 1048576 138 / 297.
+  auto cut = [&](int chunk) {
+    g.chunk = chunk;
+    g.nlo = (keep + chunk - 1) / chunk;
+    g.nhi = (n - keep + chunk - 1) / chunk;
+  };
+  cut(8 * kSelThreads);
+  if (n <= 1 << 17 && (int64_t)(g.nlo + g.nhi) * (int64_t)pairs < num_cus()) cut(4 * kSelThreads);
   const size_t nc = n <= kSelMax ? 0 : (size_t)g.nlo + g.nhi;
   const size_t lds = sizeof(int32_t) * (kRankMax + 3 * nc);
   if (lds + sizeof(SelectLds) > kMaxLds) return MOLOT_ENOTSUP;  // past 40 million rows
   // [bins | lists | counts | rank, chunk_at | keys | listed]
-  const size_t words = pairs * (2 * (size_t)most + 1 + (nc ? 4 + kAt * nc + 2 * nc * kChunk + nc * (kBins / 2) : 0));
+  const size_t words = pairs * (2 * (size_t)most + 1 + (nc ? 4 + kAt * nc + 2 * nc * g.chunk + nc * (kBins / 2) : 0));
   unsigned long long* ctr = nullptr;
   void* ws = nullptr;
   int st = workspace(stream, sizeof(int32_t) * words, &ctr, &ws);
@@ -895,12 +909,13 @@ int launch_evict(const SlotArgs& a, int n, int keep, int recent, int B, void* st
     g.rank = g.counts + pairs;
     g.chunk_at = g.rank + 4 * pairs;
     g.keys = reinterpret_cast<uint32_t*>(g.chunk_at + kAt * pairs * nc);
-    g.listed = g.keys + pairs * nc * kChunk;
+    g.listed = g.keys + pairs * nc * g.chunk;
     const dim3 chunks((unsigned)nc, a.nkv, B), block(kSelThreads);
-    hipLaunchKernelGGL(evict_keys_kernel, chunks, block, 0, hs, g);
-    hipLaunchKernelGGL(evict_pick_kernel, chunks, block, 0, hs, g);
+    const bool half = g.chunk == 4 * kSelThreads;
+    hipLaunchKernelGGL(half ? evict_keys_kernel<4> : evict_keys_kernel<8>, chunks, block, 0, hs, g);
+    hipLaunchKernelGGL(half ? evict_pick_kernel<4> : evict_pick_kernel<8>, chunks, block, 0, hs, g);
     hipLaunchKernelGGL(evict_rank_kernel, dim3(a.nkv, B), block, lds, hs, g);
-    hipLaunchKernelGGL(evict_list_kernel, chunks, block, 0, hs, g);
+    hipLaunchKernelGGL(half ? evict_list_kernel<4> : evict_list_kernel<8>, chunks, block, 0, hs, g);
   }
   st = (int)hipGetLastError();
   if (st) return st;

@@ -88,7 +88,7 @@ def test_rule(gpu, n, keep, recent, kind):
 @pytest.mark.parametrize("kind", ["smooth", "ties", "equal", "odd", "zeros", "near"])
 @pytest.mark.parametrize("n,keep,recent", [(16384, 16000, 500), (16385, 16000, 500), (20001, 8192, 3),
                                            (40000, 39999, 0), (40000, 1, 0), (60000, 24576, 40000),
-                                           (33333, 30000, 2500)])
+                                           (33333, 30000, 2500), (131073, 120001, 5000)])
 def test_rule_long(gpu, n, keep, recent, kind):
     """Caches past one workgroup's: chunks on both sides of keep, up to one bin of them."""
     nkv, d, pos = 2, 2, n - 1

@@ -309,6 +309,21 @@ def test_paged_with_weights(gpu, kv, nq, nkv, d, lens, page, window, alibi):
     assert float((acc.double() - grown).abs().max()) <= tol_w + 2 * ref.EPS32 * (G + 1)
 
 
+@pytest.mark.parametrize("nq,n", [(4096, 140000), (4097, 10)])
+def test_weights_refused(gpu, nq, n):
+    """Scores of one KV head past 2 GiB, and more than 4096 heads on it: refused, nothing
+    written; the same call without weights runs."""
+    K, V = (torch.ones(n, 2, device="cuda") for _ in range(2))
+    q, O = torch.ones(nq, 2, device="cuda"), torch.zeros(nq, 2, device="cuda")
+    acc = torch.zeros(1, n, device="cuda")
+    with pytest.raises(_lib.MolotHipError):
+        attn.attn_decode_scored(q, K, V, O, nq, 1, n, 2, 1.0, n - 1, 0, 50.0, None, acc)
+    torch.cuda.synchronize()
+    assert torch.count_nonzero(acc) == 0 and torch.count_nonzero(O) == 0
+    attn.attn_decode_scored(q, K, V, O, nq, 1, n, 2, 1.0, n - 1, 0, 50.0)
+    assert float((O - 1).abs().max()) < 1e-5
+
+
 def test_paged_weights_past_a_gigabyte(gpu):
     """64 sequences of 70000 rows under 64 heads: 1.15 GB of scores kept for the weights."""
     nq, nkv, d, page, B, n = 64, 1, 64, 16, 64, 70000

@@ -234,7 +234,10 @@ int molot_hip_attn_prefill_gqa(const float* Qm, const void* K, const void* V, fl
  * layer's norms (as molot_hip_decode_step_norm; NULL weights / v_norm = 0
  * skip them) and RoPE of q (in place, [M][nq][d]) and k_new ([M][nkv][d]),
  * append of k/v at slots slot0 .. slot0+M-1 (positions pos0 ..), then
- * causal prefill attention over N = slot0 + M into O [M][nq][d]. */
+ * causal prefill attention over N = slot0 + M into O [M][nq][d]: as
+ * molot_hip_attn_prefill_gqa with min(pos0, slot0) for pos0, so that no row
+ * sees the rows appended after it where the positions run ahead of the slots
+ * (a cache cut by molot_hip_kv_evict; the window then goes by slots). */
 int molot_hip_prefill_step(float* q, const float* k_new, const float* v_new, void* K, void* V,
                            float* O, int nq, int nkv, int d, int M, int slot0, int pos0,
                            const float* q_norm, const float* k_norm, int v_norm, float eps,
@@ -355,8 +358,8 @@ int molot_hip_decode_step_paged_scored(
  * scored, with the keys of every row as a range: row m attends [lo_m, hi_m),
  *   lo_m = max(the window's start, key_lo[m])    (key_lo NULL: the window's)
  *   hi_m = min(key_hi[m], N)                     (key_hi NULL: pos0 + m + 1)
- * (the steps: min(pos0, slot0) in place of pos0, there and as i, so that no row
- * sees the rows appended after it in a cache that was cut by molot_hip_kv_evict).
+ * (the steps: min(pos0, slot0) in place of pos0, there and as i, as in
+ * molot_hip_prefill_step).
  * key_lo, key_hi: device int32 [M], any values (an empty range gives O = 0).
  * So a packed prompt's documents keep to themselves (key_lo: the first slot
  * of the row's document), a prefix sees itself both ways (key_hi: at least

@@ -302,7 +302,8 @@ def prefill_step(q, k_new, v_new, K, V, O, nq, nkv, d, M, slot0, pos0, inv_freq,
                  window=0, q_norm=None, k_norm=None, v_norm=False, eps=1e-6):
     """forward.h:367-399 for one layer: norms (optional) and RoPE of the M
     prompt tokens' q (in place) and k, append at slots slot0.., then causal
-    prefill attention over slot0 + M."""
+    prefill attention over slot0 + M (by the slots where pos0 is past slot0:
+    a cache that rows were evicted from)."""
     kvd = kv_dtype_of(K)
     row = _row_units(kvd, nkv, d)
     cap = K.numel() // row

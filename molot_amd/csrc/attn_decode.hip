@@ -3651,9 +3651,9 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   int T0 = 0;
   int split_rows = -1;
   const int presplit = g_presplit.load(std::memory_order_relaxed);
-  // (scored: a row never sees the rows appended after it, whatever positions a cache
-  // that rows were evicted from has)
-  const int apos = sc.on ? std::min(pos0, slot0) : pos0;
+  // (a row never sees the rows appended after it: where rows were evicted from the cache
+  // the positions run ahead of the slots, and the attention goes by the slots)
+  const int apos = std::min(pos0, slot0);
   if (sc.on ? prefill_scored_pieces(d, M, slot0 + M, nq, nkv, window, kv_dtype, presplit)
             : prefill_takes_pieces(d, M, slot0 + M, nq, nkv, kv_dtype, window, presplit)) {
     // at d = 512 the split of all rows is as fast (8q/2kv, 1999 tokens: 29 + 7
@@ -3674,7 +3674,7 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
     }
   } else if (supported_d(d) && !sc.on) {
     int64_t R = 0;
-    st = prefill_pieces(nkv, slot0 + M, d, pos0, window, kv_dtype, stream, presplit, &pws, &T0, &R,
+    st = prefill_pieces(nkv, slot0 + M, d, apos, window, kv_dtype, stream, presplit, &pws, &T0, &R,
                         pieces_only);
     if (st) return st;
     r.pc_R = (int)R;

@@ -20,6 +20,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstddef>
 #include <cstring>
@@ -308,13 +309,16 @@ class DeviceKV {
 
   // forward.h:367-399 for a layer without its own KV reading this cache
   // (which already holds the prompt: the source layer ran first): Q
-  // [M][nq][hd] normed and rotated in place, causal attention over this
-  // cache's n slots into AO; device pointers, asynchronous on s.
+  // [M][nq][hd] normed and rotated in place at pos0 + m, causal attention over
+  // this cache's n slots (the last M are the prompt's) into AO; device pointers,
+  // asynchronous on s.
   void prefill_shared(float* Q, float* AO, int nq, int M, int pos0, const float* inv_freq,
                       float scale, int window, const LayerNorms& nm = LayerNorms{},
                       hipStream_t s = nullptr) const {
     check(molot_hip_prefill_q(Q, nq, hd, M, pos0, nm.q_norm, nm.eps, inv_freq, s), "prefill_q");
-    check(molot_hip_attn_prefill_gqa(Q, k, v, AO, nq, nkv, M, n, hd, scale, pos0, window,
+    // (the attention goes by slots, which eviction leaves behind the positions)
+    const int first = M <= n ? std::min(pos0, n - M) : pos0;
+    check(molot_hip_attn_prefill_gqa(Q, k, v, AO, nq, nkv, M, n, hd, scale, first, window,
                                      kv_dtype, s),
           "attn_prefill_gqa");
   }

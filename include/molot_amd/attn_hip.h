@@ -225,7 +225,9 @@ int molot_hip_rope_append_paged(float* q, const float* k_new, const float* v_new
  * [M][nq][d] fp32; K/V the token-major cache [N][nkv*d] holding the M new
  * tokens; query m sits at position pos0 + m and attends slots
  * [t0, min(pos0 + m + 1, N)), t0 = max(0, pos - window + 1) for window > 0.
- * A query with no slot gets O = 0.  scale as given. */
+ * A query with no slot gets O = 0.  scale as given.  pos0 counts slots: over a
+ * cache cut by molot_hip_kv_evict the prompt's first slot, N - M, not its
+ * token's position (which molot_hip_prefill_q takes). */
 int molot_hip_attn_prefill_gqa(const float* Qm, const void* K, const void* V, float* Om, int nq,
                                int nkv, int M, int N, int d, float scale, int pos0, int window,
                                int kv_dtype, void* stream);
@@ -358,8 +360,8 @@ int molot_hip_decode_step_paged_scored(
  * scored, with the keys of every row as a range: row m attends [lo_m, hi_m),
  *   lo_m = max(the window's start, key_lo[m])    (key_lo NULL: the window's)
  *   hi_m = min(key_hi[m], N)                     (key_hi NULL: pos0 + m + 1)
- * (the steps: min(pos0, slot0) in place of pos0, there and as i, as in
- * molot_hip_prefill_step).
+ * (pos0 counts slots, there and as i: over a cut cache N - M; the steps take
+ * min(pos0, slot0) themselves, as molot_hip_prefill_step).
  * key_lo, key_hi: device int32 [M], any values (an empty range gives O = 0).
  * So a packed prompt's documents keep to themselves (key_lo: the first slot
  * of the row's document), a prefix sees itself both ways (key_hi: at least

@@ -198,9 +198,10 @@ class PagedKVCache {
     if (mode_ != Mode::Prefill) throw std::runtime_error("PagedKVCache: prefill outside a step");
     check(molot_hip_prefill_q(q, nq, hd_, prefill_m_, pos0, nm.q_norm, nm.eps, inv_freq, s),
           "prefill_q");
+    const int slot0 = seq(batch_[0]).len;  // (by slots, as DeviceKV::prefill_shared)
     check(molot_hip_attn_prefill_paged(q, k_.at(src), v_.at(src), o, d_table_, maxb_, page_, nq,
-                                       nkv_, prefill_m_, seq(batch_[0]).len + prefill_m_, hd_,
-                                       scale, pos0, window, kv_dtype_, s),
+                                       nkv_, prefill_m_, slot0 + prefill_m_, hd_, scale,
+                                       std::min(pos0, slot0), window, kv_dtype_, s),
           "attn_prefill_paged");
   }
   // prefill() with the layer's Scores and key ranges (device [M]).

@@ -285,7 +285,8 @@ def decode_step_paged(q, k_new, v_new, K, V, O, block_table, seq_lens, pos, B, m
 
 def attn_prefill_gqa(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window=0):
     """gemm.h:409-446: causal prefill attention of M queries [M][nq][d]
-    (positions pos0..) over the token-major cache [N][nkv*d]."""
+    (positions pos0.., as slots: over a cache that rows were evicted from the
+    prompt's first slot, N - M) over the token-major cache [N][nkv*d]."""
     kvd = kv_dtype_of(K)
     row = _row_units(kvd, nkv, d)
     _need(Qm, "Qm", torch.float32, M * nq * d)
@@ -600,7 +601,8 @@ def decode_step_paged_scored(q, k_new, v_new, K, V, O, block_table, seq_lens, po
 def attn_prefill_scored(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window=0, softcap=0.0,
                         slopes=None, key_lo=None, key_hi=None):
     """attn_prefill_gqa with attn_decode_scored's scores and the keys of row m in
-    [max(window's start, key_lo[m]), key_hi[m]) (device int32; None: causal)."""
+    [max(window's start, key_lo[m]), key_hi[m]) (device int32; None: causal);
+    pos0 as attn_prefill_gqa takes it."""
     kvd = kv_dtype_of(K)
     row = _row_units(kvd, nkv, d)
     _need(Qm, "Qm", torch.float32, M * nq * d)

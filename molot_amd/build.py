@@ -98,7 +98,7 @@ def build_cpp_test(name: str = "test_attn_cpp") -> str:
     return out
 
 
-CPP_TESTS = ("test_attn_cpp", "test_paged_kv", "test_kv_budget", "prefill_no_memory", "host_io_time")
+CPP_TESTS = ("test_attn_cpp", "test_paged_kv", "test_kv_budget", "test_kv_cut", "prefill_no_memory", "host_io_time")
 
 
 def build_all() -> None:

@@ -241,7 +241,10 @@ class DeviceKV {
   DeviceKV(const DeviceKV&) = delete;
   DeviceKV& operator=(const DeviceKV&) = delete;
 
-  void reset() { n = 0; }  // molot_chat.cc /reset
+  void reset() {  // molot_chat.cc /reset
+    n = 0;
+    gone = 0;
+  }
 
   // forward.h:556-591 for a layer that owns its KV: q (nq heads) rotated in
   // place, k rotated and appended with v at slot n, n++, then attention into
@@ -259,6 +262,7 @@ class DeviceKV {
               const float* inv_freq, float scale, int window, const LayerNorms& nm,
               hipStream_t s = nullptr) {
     if (n >= cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:570
+    check_window(window, pos);
     const size_t qf = (size_t)nq * hd, kf = (size_t)nkv * hd;
     CallStage view(q, true, ao, qf, qf, s, knew, vnew, kf);
     if (nm.q_norm || nm.k_norm || nm.v_norm)
@@ -284,6 +288,7 @@ class DeviceKV {
                      int window, const LayerNorms& nm = LayerNorms{},
                      hipStream_t s = nullptr) const {
     if (n == 0) throw std::runtime_error("fwd: shared KV empty");  // forward.h:580
+    check_window(window, pos);
     CallStage view(q, true, ao, (size_t)nq * hd, (size_t)nq * hd, s);
     check(molot_hip_decode_step_shared(view.q, k, v, view.o, nq, nkv, hd, n, pos, nm.q_norm,
                                        nm.eps, inv_freq, scale, window, kv_dtype, s),
@@ -299,6 +304,7 @@ class DeviceKV {
                int pos0, const float* inv_freq, float scale, int window,
                const LayerNorms& nm = LayerNorms{}, hipStream_t s = nullptr) {
     if (n + M > cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:385
+    check_window(window, pos0 + M - 1);
     check(molot_hip_prefill_step(Q, K_new, V_new, k, v, AO, nq, nkv, hd, M, n, pos0, nm.q_norm,
                                  nm.k_norm, nm.v_norm ? 1 : 0, nm.eps, inv_freq, scale, window,
                                  kv_dtype, s),
@@ -315,6 +321,7 @@ class DeviceKV {
   void prefill_shared(float* Q, float* AO, int nq, int M, int pos0, const float* inv_freq,
                       float scale, int window, const LayerNorms& nm = LayerNorms{},
                       hipStream_t s = nullptr) const {
+    check_window(window, pos0 + M - 1);
     check(molot_hip_prefill_q(Q, nq, hd, M, pos0, nm.q_norm, nm.eps, inv_freq, s), "prefill_q");
     // (the attention goes by slots, which eviction leaves behind the positions)
     const int first = M <= n ? std::min(pos0, n - M) : pos0;
@@ -327,6 +334,7 @@ class DeviceKV {
   void attend(const float* q, float* ao, int nq, float scale, int pos_cur, int window,
               hipStream_t s = nullptr) const {
     if (n == 0) throw std::runtime_error("fwd: shared KV empty");  // forward.h:580
+    check_window(window, pos_cur);
     CallStage view(const_cast<float*>(q), false, ao, (size_t)nq * hd, (size_t)nq * hd, s);
     check(molot_hip_attn_decode_gqa_cache(view.q, k, v, view.o, nq, nkv, n, hd, scale, pos_cur,
                                           window, kv_dtype, s),
@@ -342,6 +350,7 @@ class DeviceKV {
                      const float* inv_freq, float scale, int window, const LayerNorms& nm,
                      const Scores& sc, hipStream_t s = nullptr) {
     if (n >= cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:570
+    check_window(window, pos);
     const size_t qf = (size_t)nq * hd, kf = (size_t)nkv * hd;
     CallStage view(q, true, ao, qf, qf, s, knew, vnew, kf);
     check(molot_hip_decode_step_scored(view.q, view.k, view.v, k, v, view.o, nq, nkv, hd, n, pos,
@@ -358,6 +367,7 @@ class DeviceKV {
                       int pos0, const float* inv_freq, float scale, int window,
                       const LayerNorms& nm, const Scores& sc, hipStream_t s = nullptr) {
     if (n + M > cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:385
+    check_window(window, pos0 + M - 1);
     check(molot_hip_prefill_step_scored(Q, K_new, V_new, k, v, AO, nq, nkv, hd, M, n, pos0,
                                         nm.q_norm, nm.k_norm, nm.v_norm ? 1 : 0, nm.eps, inv_freq,
                                         scale, window, sc.softcap, sc.slopes, sc.key_lo, sc.key_hi,
@@ -377,18 +387,29 @@ class DeviceKV {
   }
 
   // The cache cut to `keep` slots: the `recent` newest positions (pos: the newest
-  // token's), then the highest weights.
+  // token's), then the highest weights.  The rows left lie in any order, so from then
+  // on until reset() a call whose window would leave a position out throws.
   void evict(int keep, int recent, int pos, hipStream_t s = nullptr) {
     if (!acc) throw std::runtime_error("DeviceKV: evict without track_weights");
     check(molot_hip_kv_evict(k, v, acc, slot_pos, nkv, n, hd, keep, recent, pos, cap, kv_dtype, s),
           "kv_evict");
-    if (keep < n) n = keep;
+    if (keep >= n) return;
+    gone += n - keep;
+    n = keep;
   }
 
   float* acc = nullptr;         // [nkv][cap] (track_weights)
   int32_t* slot_pos = nullptr;  // [nkv][cap]
 
  private:
+  int gone = 0;  // rows evicted
+
+  // A window is a range of slots to the kernels, and of positions to the layer: the same
+  // in a cache that was not cut, or where it holds every position up to pos.
+  void check_window(int window, int pos) const {
+    if (gone > 0 && window > 0 && pos >= window)
+      throw std::runtime_error("DeviceKV: a window over a cache that rows were evicted from");
+  }
   // The last M rows are new, the newest at pos.
   void track(int M, int pos, hipStream_t s) {
     if (acc) check(molot_hip_kv_track(acc, slot_pos, nkv, n, M, pos, cap, s), "kv_track");

@@ -414,7 +414,10 @@ int molot_hip_kv_track_paged(float* acc, int32_t* slot_pos, const int32_t* block
  * Rows hold keys rotated at their own positions, so attention over the cut
  * cache is over the tokens kept, with the next token's slot and position told
  * apart (molot_hip_decode_step_scored's slot and pos, pos[] of the paged
- * steps); windows and slopes go by slots, and no longer hold there.  The
+ * steps).  Windows and slopes go by slots counted from the position given: in a
+ * cut cache those are not the tokens' distances, and nothing here can tell, so
+ * a layer with either keeps its cache whole (DeviceKV and PagedKVCache refuse
+ * such windows).  The
  * paged form cuts every sequence longer than keep (seq_lens is not written; the
  * sequences of a call share no block).
  * K and V 16-byte aligned; every even head dim up to 512. */

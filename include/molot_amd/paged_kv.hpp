@@ -122,6 +122,7 @@ class PagedKVCache {
               const float* inv_freq, float scale, int window, const LayerNorms& nm = LayerNorms{},
               hipStream_t s = nullptr) {
     if (mode_ != Mode::Decode) throw std::runtime_error("PagedKVCache: decode outside a step");
+    check_window(window, cut_pos_);
     check(molot_hip_decode_step_paged_norm(
               q, k, v, k_.at(layer), v_.at(layer), o, d_table_, d_lens_, pos_array(),
               (int)batch_.size(), maxb_, max_len_, nq, nkv_, hd_, page_, nm.q_norm, nm.k_norm,
@@ -137,6 +138,7 @@ class PagedKVCache {
                      int window, const LayerNorms& nm = LayerNorms{},
                      hipStream_t s = nullptr) const {
     if (mode_ != Mode::Decode) throw std::runtime_error("PagedKVCache: decode outside a step");
+    check_window(window, cut_pos_);
     check(molot_hip_decode_step_paged_shared(
               q, k_.at(src), v_.at(src), o, d_table_, d_lens_, pos_array(), (int)batch_.size(),
               maxb_, max_len_, nq, nkv_, hd_, page_, nm.q_norm, nm.eps, inv_freq, scale, window,
@@ -149,6 +151,7 @@ class PagedKVCache {
                      const float* inv_freq, float scale, int window, const LayerNorms& nm,
                      const Scores& sc, hipStream_t s = nullptr) {
     if (mode_ != Mode::Decode) throw std::runtime_error("PagedKVCache: decode outside a step");
+    check_window(window, cut_pos_);
     check(molot_hip_decode_step_paged_scored(
               q, k, v, k_.at(layer), v_.at(layer), o, d_table_, d_lens_, pos_array(),
               (int)batch_.size(), maxb_, max_len_, nq, nkv_, hd_, page_, nm.q_norm, nm.k_norm,
@@ -181,6 +184,7 @@ class PagedKVCache {
                const float* inv_freq, float scale, int window,
                const LayerNorms& nm = LayerNorms{}, hipStream_t s = nullptr) {
     if (mode_ != Mode::Prefill) throw std::runtime_error("PagedKVCache: prefill outside a step");
+    check_window(window, pos0 + prefill_m_ - 1);
     check(molot_hip_prefill_step_paged(q, k, v, k_.at(layer), v_.at(layer), o, d_table_, maxb_,
                                        page_, nq, nkv_, hd_, prefill_m_, seq(batch_[0]).len,
                                        pos0, nm.q_norm, nm.k_norm, nm.v_norm ? 1 : 0, nm.eps,
@@ -196,6 +200,7 @@ class PagedKVCache {
                       float scale, int window, const LayerNorms& nm = LayerNorms{},
                       hipStream_t s = nullptr) const {
     if (mode_ != Mode::Prefill) throw std::runtime_error("PagedKVCache: prefill outside a step");
+    check_window(window, pos0 + prefill_m_ - 1);
     check(molot_hip_prefill_q(q, nq, hd_, prefill_m_, pos0, nm.q_norm, nm.eps, inv_freq, s),
           "prefill_q");
     const int slot0 = seq(batch_[0]).len;  // (by slots, as DeviceKV::prefill_shared)
@@ -209,6 +214,7 @@ class PagedKVCache {
                       int pos0, const float* inv_freq, float scale, int window,
                       const LayerNorms& nm, const Scores& sc, hipStream_t s = nullptr) {
     if (mode_ != Mode::Prefill) throw std::runtime_error("PagedKVCache: prefill outside a step");
+    check_window(window, pos0 + prefill_m_ - 1);
     check(molot_hip_prefill_step_paged_scored(
               q, k, v, k_.at(layer), v_.at(layer), o, d_table_, maxb_, page_, nq, nkv_, hd_,
               prefill_m_, seq(batch_[0]).len, pos0, nm.q_norm, nm.k_norm, nm.v_norm ? 1 : 0, nm.eps,
@@ -238,7 +244,8 @@ class PagedKVCache {
   }
   // Every sequence of ids that is longer than keep is cut to it, in every layer and
   // KV head by itself: its `recent` newest positions, then the highest weights.  The
-  // blocks past the budget return to the pool.
+  // blocks past the budget return to the pool.  The rows left lie in any order, so a call
+  // over such a sequence whose window would leave a position out throws.
   void evict(const std::vector<int>& ids, int keep, int recent, hipStream_t s = nullptr) {
     if (mode_ != Mode::None) throw std::runtime_error("PagedKVCache: a step is in progress");
     if (!acc_[0]) throw std::runtime_error("PagedKVCache: evict without track_weights");
@@ -309,6 +316,12 @@ class PagedKVCache {
   }
   // The batch's positions where a sequence's differ from its slots.
   const int32_t* pos_array() const { return cut_ ? d_pos_ : nullptr; }
+  // A window is a range of slots to the kernels, and of positions to the layer: the same
+  // in a sequence that was not cut, or where it holds every position up to pos.
+  void check_window(int window, int pos) const {
+    if (cut_ && window > 0 && pos >= window)
+      throw std::runtime_error("PagedKVCache: a window over a sequence that rows were evicted from");
+  }
   // Blocks for `tokens` more tokens of sequence id, from the shared pool.
   void reserve(int id, int tokens) {
     Seq& s = seq(id);
@@ -341,10 +354,14 @@ class PagedKVCache {
     std::fill(h_table_, h_table_ + n, 0);
     max_len_ = 0;
     cut_ = false;
+    cut_pos_ = 0;
     for (size_t i = 0; i < B; ++i) {
       const Seq& q = seq(ids[i]);
       h_table_[B * maxb + B + i] = lens[i] - 1 + q.gone;  // the newest token's position
-      cut_ = cut_ || q.gone > 0;
+      if (q.gone > 0) {
+        cut_ = true;
+        cut_pos_ = std::max(cut_pos_, lens[i] - 1 + q.gone);
+      }
       for (size_t j = 0; j < q.blocks.size(); ++j) h_table_[i * maxb + j] = q.blocks[j];
       h_table_[B * maxb + i] = lens[i];
       max_len_ = std::max(max_len_, (int)lens[i]);
@@ -373,7 +390,8 @@ class PagedKVCache {
   hipEvent_t uploaded_ = nullptr;
   int32_t* d_lens_ = nullptr;
   int32_t* d_pos_ = nullptr;
-  bool cut_ = false;
+  bool cut_ = false;  // a sequence of the batch has lost rows
+  int cut_pos_ = 0;   // and the newest position of such
   size_t table_cap_ = 0;
   int maxb_ = 1, max_len_ = 0;
 };

@@ -78,6 +78,16 @@ void check_rows(const std::vector<float>& q, const std::vector<float>& K, const 
   std::printf("%s: error %.2e\n", what, worst);
 }
 
+template <typename F>
+bool throws(F&& fn) {
+  try {
+    fn();
+  } catch (const std::runtime_error&) {
+    return true;
+  }
+  return false;
+}
+
 struct Rows {
   std::vector<float> q, k, v;
   Dev dq, dk, dv, dout;
@@ -166,6 +176,98 @@ void run_paged(int M) {
   kv.end_decode();
 }
 
+// Windows are of positions, the kernels' of slots: refused over a cut cache, in every
+// call, unless they hold every position; as before in one that was not cut.
+void run_windows() {
+  const molot::amd::LayerNorms nm;
+  const molot::amd::Scores sc;
+  Rng rng(13);
+  Rows r(rng, 40), s(rng, 5);
+  molot::amd::DeviceKV kv(64, kNkv, kD, MOLOT_KV_F32);
+  kv.track_weights();
+  auto all = [&](int window, int pos, bool want, const char* what) {
+    const int n = kv.n;
+    auto expect = [&](const char* call, auto&& fn) {
+      CHECK(throws(fn) == want, "%s: %s, window %d", what, call, window);
+      if (want) CHECK(kv.n == n, "%s: %s appended", what, call);
+      kv.n = n;  // (each call at the same length)
+    };
+    expect("decode", [&] { kv.decode(s.dq.p, s.dk.p, s.dv.p, s.dout.p, kNq, pos, nullptr, kScale, window, nm); });
+    expect("decode_scored", [&] {
+      kv.decode_scored(s.dq.p, s.dk.p, s.dv.p, s.dout.p, kNq, pos, nullptr, kScale, window, nm, sc);
+    });
+    expect("decode_shared", [&] { kv.decode_shared(s.dq.p, s.dout.p, kNq, pos, nullptr, kScale, window, nm); });
+    expect("attend", [&] { kv.attend(s.dq.p, s.dout.p, kNq, kScale, pos, window); });
+    expect("prefill", [&] {
+      kv.prefill(s.dq.p, s.dk.p, s.dv.p, s.dout.p, kNq, 5, pos - 4, nullptr, kScale, window, nm);
+    });
+    expect("prefill_scored", [&] {
+      kv.prefill_scored(s.dq.p, s.dk.p, s.dv.p, s.dout.p, kNq, 5, pos - 4, nullptr, kScale, window, nm, sc);
+    });
+    expect("prefill_shared", [&] {
+      kv.prefill_shared(s.dq.p, s.dout.p, kNq, 5, pos - 4, nullptr, kScale, window, nm);
+    });
+  };
+  kv.prefill(r.dq.p, r.dk.p, r.dv.p, r.dout.p, kNq, 40, 0, nullptr, kScale, 16, nm);
+  all(16, 44, false, "not cut");
+  kv.evict(50, 3, 39);
+  all(16, 44, false, "a budget above the length");
+  kv.evict(20, 3, 39);
+  all(44, 44, true, "cut");
+  all(16, 44, true, "cut");
+  all(45, 44, false, "cut, every position in the window");
+  all(0, 44, false, "cut, no window");
+  kv.reset();
+  kv.prefill(r.dq.p, r.dk.p, r.dv.p, r.dout.p, kNq, 40, 0, nullptr, kScale, 16, nm);
+  all(16, 44, false, "reset");
+
+  molot::amd::PagedKVCache pg(1, 32, kNkv, kD, 16, MOLOT_KV_F32);
+  pg.track_weights();
+  const int whole = pg.add_sequence(), cut = pg.add_sequence();
+  auto prompt = [&](int id, Rows& x, int M, int window, bool want, const char* what) {
+    const int pos0 = pg.position(id);
+    pg.begin_prefill(id, M);
+    CHECK(throws([&] {
+            pg.prefill(0, x.dq.p, x.dk.p, x.dv.p, x.dout.p, kNq, pos0, nullptr, kScale, window, nm);
+          }) == want, "%s: prefill, window %d", what, window);
+    CHECK(throws([&] {
+            pg.prefill_scored(0, x.dq.p, x.dk.p, x.dv.p, x.dout.p, kNq, pos0, nullptr, kScale, window, nm, sc);
+          }) == want, "%s: prefill_scored, window %d", what, window);
+    CHECK(throws([&] { pg.prefill_shared(0, x.dq.p, x.dout.p, kNq, pos0, nullptr, kScale, window, nm); }) ==
+              want, "%s: prefill_shared, window %d", what, window);
+    if (want)  // (the step is ended with its rows)
+      pg.prefill(0, x.dq.p, x.dk.p, x.dv.p, x.dout.p, kNq, pos0, nullptr, kScale, 0, nm);
+    pg.end_prefill();
+  };
+  prompt(whole, r, 40, 16, false, "not cut");
+  prompt(cut, r, 40, 16, false, "not cut");
+  pg.evict({cut}, 20, 3);
+  prompt(whole, s, 5, 16, false, "another sequence's cut");
+  prompt(cut, s, 5, 16, true, "cut");
+  prompt(cut, s, 5, 50, false, "cut, every position in the window");
+  Rows t(rng, 2);
+  auto step = [&](const std::vector<int>& ids, int window, bool want, const char* what) {
+    pg.begin_decode(ids);
+    CHECK(throws([&] { pg.decode(0, t.dq.p, t.dk.p, t.dv.p, t.dout.p, kNq, nullptr, kScale, window, nm); }) ==
+              want, "%s: decode, window %d", what, window);
+    CHECK(throws([&] {
+            pg.decode_scored(0, t.dq.p, t.dk.p, t.dv.p, t.dout.p, kNq, nullptr, kScale, window, nm, sc);
+          }) == want, "%s: decode_scored, window %d", what, window);
+    CHECK(throws([&] { pg.decode_shared(0, t.dq.p, t.dout.p, kNq, nullptr, kScale, window, nm); }) == want,
+          "%s: decode_shared, window %d", what, window);
+    if (want) pg.decode(0, t.dq.p, t.dk.p, t.dv.p, t.dout.p, kNq, nullptr, kScale, 0, nm);
+    pg.end_decode();
+  };
+  step({whole}, 16, false, "not cut");                 // positions 45; cut's: 50 next
+  step({whole, cut}, 16, true, "one of them cut");
+  step({cut, whole}, 51, true, "one of them cut");     // its token's position is 51
+  step({cut, whole}, 53, false, "cut, every position in the window");
+  pg.free_sequence(cut);
+  CHECK(pg.add_sequence() == cut, "the id again");
+  prompt(cut, r, 40, 16, false, "a new sequence");
+  check_hip(hipDeviceSynchronize(), "sync");
+}
+
 }  // namespace
 
 int main() {
@@ -176,6 +278,7 @@ int main() {
       run_contiguous(M);
       run_paged(M);
     }
+    run_windows();
   } catch (const std::exception& e) {
     CHECK(false, "%s", e.what());
   }

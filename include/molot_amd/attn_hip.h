@@ -323,7 +323,8 @@ int molot_hip_attn_prefill_paged(const float* Qm, const void* K, const void* V, 
  * [num_blocks][nkv][page] through the same block table, where no two sequences
  * of a call share a block (every slot has one writer).  A step that appends
  * a row sets that slot's acc instead, and its position in slot_pos (int32,
- * same layout; NULL: none; only with acc).  The scores of a call with acc are
+ * same layout; NULL: none; only with acc).  The acc of rows past max_seq_len is
+ * left as it is (an appended row's: set to 0).  The scores of a call with acc are
  * kept for its second launch: 4 * B * nq * (attended rows + 1) bytes of the
  * stream's prefill workspace, at most 8 GiB and 2 GiB a KV head
  * (MOLOT_ENOTSUP past it, and past 4096 query heads a KV head or 65535

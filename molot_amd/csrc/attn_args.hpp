@@ -86,6 +86,7 @@ struct AttnArgs {
   int32_t* slot_pos;
   int64_t sc_rows;
   int acc_cap, fresh;
+  int sc_span;           // rows from t0 that the launch forms scores of, whatever the lengths
 };
 using AttnFn = void (*)(AttnArgs);
 

@@ -1583,6 +1583,7 @@ struct WeightArgs {
   const int32_t* block_table;
   int64_t sc_rows;
   int n, t0, pos, max_blocks, page_shift, acc_cap, fresh;
+  int sc_span;  // AttnArgs::sc_span
   int blocked;  // the scores in the matrix-core kernel's order
 };
 constexpr int kWeightThreads = 256;
@@ -1607,14 +1608,15 @@ __device__ __forceinline__ void weigh_rows(const WeightArgs& w, int rb, int h, i
     if (t0 > n) t0 = n;
     nch = comb_chunks(w.c, b);
   }
-  const int span = (int)min((int64_t)(n - t0), w.sc_rows);
+  const int span = min(n - t0, w.sc_span);
   const int row0 = rb * kWeightThreads;
   auto index = [&](int t) -> int64_t {
     if (!paged) return (int64_t)h * w.acc_cap + t;
     const int64_t blk = w.block_table[(int64_t)b * w.max_blocks + (t >> w.page_shift)];
     return ((blk * w.c.nkv + h) << w.page_shift) + (t & ((1 << w.page_shift) - 1));
   };
-  // a fresh row outside the range (a position behind the cache's end)
+  // a fresh row outside the range (a position behind the cache's end, or past the bound
+  // of the lengths)
   if (w.fresh && n > 0 && n - 1 >= t0 + span && rb == 0 && tid == 0) {
     const int64_t i = index(n - 1);
     w.acc[i] = 0.f;
@@ -2078,6 +2080,8 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
   if (stats) {  // the scores of every attended row, for the weights
     if (B > 65535 || a.nq / a.nkv > 4096) return MOLOT_ENOTSUP;  // attn_weights_kernel's grid, its LDS
     a.sc_rows = (std::max(span, 0) + 4) & ~3;  // (and the appended row)
+    // (a paged span counts it; a sequence's rows past the span may have no scores)
+    a.sc_span = a.block_table ? std::max(span, 0) : (int)a.sc_rows;
     const size_t bytes = sizeof(float) * (size_t)B * a.nq * a.sc_rows;
     // (a KV head's own by 31-bit offsets: score_rsrc)
     if (bytes > kMaxScoredBytes || 4 * a.sc_rows * (a.nq / a.nkv) > 0x7FFFFF00) return MOLOT_ENOTSUP;
@@ -2180,6 +2184,7 @@ WeightArgs weight_args(const CombArgs& cb, const AttnArgs& a) {
   w.slot_pos = a.slot_pos;
   w.block_table = a.block_table;
   w.sc_rows = a.sc_rows;
+  w.sc_span = a.sc_span;
   w.n = a.n;
   w.t0 = a.t0;
   w.pos = a.pos;

@@ -1,0 +1,83 @@
+"""Calls of the scored entries at the limits they document: bounds of the lengths,
+batches and prompts past a launch's grid or a workspace."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import scored_ref as ref
+from molot_amd import attn
+from molot_amd import lib as _lib
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape, sigma=1.0):
+    return torch.randn(*shape, device="cuda", generator=g) * sigma
+
+
+def check_out(got, want, tol):
+    assert torch.isfinite(got).all()
+    err = float((got.double() - want).abs().max())
+    assert err <= tol, f"error {err:.3g}, bound {tol:.3g}"
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("kv,nq,nkv,d", [("f32", 8, 4, 128), ("bf16", 16, 4, 128), ("q8", 16, 4, 128),
+                                         ("q8", 8, 4, 256)])
+@pytest.mark.parametrize("bound,over", [(64, 1), (64, 7), (65, 3), (301, 2)])
+def test_rows_past_the_bound_keep_their_weight(gpu, kv, nq, nkv, d, bound, over, step):
+    """Sequences longer than max_seq_len: what lies past it may be left out, and its acc
+    is left as it is (a step's new row: set); nothing is read from earlier calls' scores."""
+    g, page, B = gen(bound + over), 16, 3
+    n = bound + over
+    width = (n + page - 1) // page
+    table = torch.arange(B * width, dtype=torch.int32).view(B, width)
+    x = randn(g, n, nkv, d)
+    pools = []
+    for _ in range(2):
+        pool = ref.make_pages(randn(g, 0, nkv, d), kv, B * width, [], page)
+        for b in range(B):
+            ref.put_pages(pool, x, kv, table[b].tolist(), page)
+        pools.append(pool)
+    acc = torch.rand(B * width, nkv, page, device="cuda", generator=g)
+    sp = torch.full((B * width, nkv, page), -5, dtype=torch.int32, device="cuda")
+    O = torch.empty(B, nq, d, device="cuda")
+    new = randn(g, B, nkv, d)
+    lens, tb = torch.full((B,), n, dtype=torch.int32, device="cuda"), table.cuda()
+    kvd = {"f32": 0, "bf16": 1, "q8": 2}[kv]
+    P, S = attn._ptr, attn._stream()
+    L = _lib.load()
+
+    def call(q, limit, to):
+        if step:
+            st = L.molot_hip_decode_step_paged_scored(
+                P(q), P(new), P(new), P(pools[0]), P(pools[1]), P(O), P(tb), P(lens), P(None), B, width,
+                limit, nq, nkv, d, page, P(None), P(None), 0, 0.0, P(None), 0.1, 0, 0.0, P(None), P(to),
+                P(sp), kvd, S)
+        else:
+            st = L.molot_hip_attn_decode_paged_scored(
+                P(q), P(pools[0]), P(pools[1]), P(O), P(tb), P(lens), P(None), B, width, limit, nq, nkv, d,
+                page, 0.1, 0, 0.0, P(None), P(to), kvd, S)
+        assert st == 0
+
+    call(randn(g, B, nq, d, sigma=900.0), n, acc.clone())  # scores of another size in the workspace
+    before = acc.clone()
+    call(randn(g, B, nq, d), bound, acc)
+    rows = lambda z: z[tb.long()].permute(0, 2, 1, 3).reshape(B, nkv, -1)[:, :, :n]  # noqa: E731
+    a, b4, G = rows(acc), rows(before), nq // nkv
+    last = n - 1 if step else n
+    assert torch.equal(a[:, :, bound:last], b4[:, :, bound:last])
+    grown = a[:, :, :bound] - b4[:, :, :bound]
+    assert bool((grown >= -1e-6).all()) and float(grown.sum(-1).max()) <= G * (1 + 1e-4)
+    if step:
+        assert bool((a[:, :, n - 1] >= 0).all()) and float(a[:, :, n - 1].max()) <= G * (1 + 1e-4)
+        assert (rows(sp)[:, :, n - 1] == n - 1).all() and (rows(sp)[:, :, :n - 1] == -5).all()

@@ -7,7 +7,9 @@
  * stream), and returns 0 or a non-zero status (molot_hip_strerror() names
  * it): no exceptions cross this ABI.  Device buffers are allocated and owned
  * by the caller; the library never frees or retains them.  The library keeps
- * one internal workspace per device (split-K partials, grown on demand).
+ * internal workspaces per device and stream, grown on demand.  Host threads
+ * may share a stream: no other call's launches come between those of a call
+ * that uses a workspace.
  *
  * Layouts (d = head dim, element type fp32 or bf16 per `kv_dtype`):
  *   q, o            [nq][d] fp32, query head h uses KV head h / (nq/nkv)

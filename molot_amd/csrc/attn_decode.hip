@@ -1740,6 +1740,7 @@ std::atomic<int> g_dynamic{1};      // block order: 1 = claimed by waves as they
 namespace molot_host {
 std::atomic<int> g_bf16_mfma{1};
 std::atomic<int> g_merge{-1};
+std::recursive_mutex g_launch_mu;
 }  // namespace molot_host
 namespace {
 using namespace molot_host;
@@ -1749,11 +1750,11 @@ using namespace molot_host;
 // a stop event per kernel, which HIP stamps from the dispatch itself (the
 // kernel's execution, without the gap before it).  molot_hip_profile_end()
 // waits for the events and returns the summed durations.
+// (g_launch_mu guards the records.)
 struct ProfRec {
   hipEvent_t a0, a1, c0, c1;  // attention kernel, combine kernel
   bool combine;
 };
-std::mutex g_prof_mu;
 bool g_prof_on = false;
 int g_prof_cap = 0;
 std::vector<ProfRec> g_prof;
@@ -2214,7 +2215,7 @@ int molot_host::launch_pair(AttnFn kern, int threads, size_t lds, AttnArgs a, in
   t_last_nchunks = a.nchunks;
   t_last_chunk = a.dyn ? a.dyn_min : a.chunk;
   a.dynamic = knob(g_dynamic);
-  std::lock_guard<std::mutex> plk(g_prof_mu);
+  LaunchLock lock(g_launch_mu);
   const bool prof = !a.ext_ws && prof_active(stream);
   const bool combine = a.nchunks > 1 && !a.ctr;  // a second launch merges the chunks
   ProfRec pr{nullptr, nullptr, nullptr, nullptr, combine};
@@ -2364,6 +2365,7 @@ int zero_out(float* O, int64_t count, hipStream_t st) {
 
 template <bool PAGED, bool ROPE>
 int run_attn(AttnArgs& a, int d, int kv_dtype, int span, int B, void* stream) {
+  LaunchLock lock(g_launch_mu);
   if (a.scored)
     return PAGED ? run_paged_scored(a, ROPE, d, kv_dtype, span, B, stream)
                  : run_flat_scored(a, ROPE, d, kv_dtype, span, B, stream);
@@ -2514,7 +2516,7 @@ void molot_hip_set_bf16_path(int mfma) { g_bf16_mfma = mfma ? 1 : 0; }
 
 int molot_hip_profile_begin(int max_launches) {
   if (max_launches <= 0) return MOLOT_EINVAL;
-  std::lock_guard<std::mutex> lk(g_prof_mu);
+  LaunchLock lock(g_launch_mu);
   for (ProfRec& r : g_prof) prof_destroy(r);
   g_prof.clear();
   g_prof.reserve(max_launches);
@@ -2525,7 +2527,7 @@ int molot_hip_profile_begin(int max_launches) {
 
 int molot_hip_profile_end(float* attn_ms, float* combine_ms, int* launches, int* combines) {
   if (!attn_ms || !combine_ms || !launches || !combines) return MOLOT_EINVAL;
-  std::lock_guard<std::mutex> lk(g_prof_mu);
+  LaunchLock lock(g_launch_mu);
   g_prof_on = false;
   double ta = 0.0, tc = 0.0;
   int n = 0, nc = 0, st = 0;
@@ -3162,7 +3164,7 @@ static int launch_prefill(PfFn pk, int64_t wgs, int threads, const PfArgs& a, in
                            : dim3((unsigned)((int64_t)a.M * a.nq), (unsigned)(D / cb.pairs));
   const dim3 cblock = cwave ? dim3((unsigned)kCombWaveThreads) : dim3(kCombThreads);
   const size_t clds = cwave ? 0 : sizeof(float) * (size_t)comb_lds_floats(nsplit);
-  std::lock_guard<std::mutex> plk(g_prof_mu);
+  LaunchLock lock(g_launch_mu);
   if (prof_active(stream)) {
     ProfRec pr{prof_event(), prof_event(), nullptr, nullptr, nsplit > 1};
     hipExtLaunchKernelGGL(pk, grid, dim3(threads), 0, (hipStream_t)stream, pr.a0, pr.a1, 0, a);
@@ -3444,6 +3446,7 @@ static int attn_prefill_impl(const float* Qm, const void* K, const void* V, floa
   const int D = padded ? (d <= 64 ? 64 : d <= 128 ? 128 : 256) : d;
   if (M < 0 || N < 0 || pos0 < 0 || (M > 0 && (!Qm || !Om))) return MOLOT_EINVAL;
   if (M == 0) return 0;
+  LaunchLock lock(g_launch_mu);
   if (N == 0) return zero_out(Om, (int64_t)M * nq * d, (hipStream_t)stream);
   if (!K || !V || !aligned16(K) || !aligned16(V) || !aligned16(Qm) || !aligned16(Om))
     return MOLOT_EINVAL;
@@ -3621,6 +3624,7 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   if (block_row && ((int64_t)slot0 + M > (int64_t)max_blocks * page || page <= 0 ||
                     (page & (page - 1)) || !q8_pages_ok(nkv, page, kv_dtype)))
     return MOLOT_EINVAL;
+  LaunchLock lock(g_launch_mu);
   RopeArgs r{};
   r.q = q;
   r.k_new = k_new;

@@ -8,6 +8,7 @@
 #include <atomic>
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 
 #include "attn_args.hpp"
 
@@ -30,6 +31,13 @@ inline int pick_gh(int G) {
   if (G % 2 == 0) return 2;
   return 1;
 }
+
+// Held from a call's first use of a workspace to its last launch: its launches hand
+// the workspace on to each other, so those of another host thread on the stream may
+// not come between (an eviction's lists, read after them, would be something else's).
+// Recursive: a prompt's launches include those of its parts.
+extern std::recursive_mutex g_launch_mu;
+using LaunchLock = std::lock_guard<std::recursive_mutex>;
 
 // Per-(device, stream) workspaces: the split-K partials (with the arrival words
 // of the in-launch merge), and the prefill's pieces, which the weights' scores

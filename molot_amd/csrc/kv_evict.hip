@@ -861,6 +861,7 @@ int launch_track(const SlotArgs& a, int M, int B, void* stream) {
 // n: rows of the longest sequence.
 int launch_evict(const SlotArgs& a, int n, int keep, int recent, int B, void* stream) {
   if (n <= keep || keep == 0 || B == 0) return 0;  // nothing moves
+  LaunchLock lock(g_launch_mu);
   const hipStream_t hs = (hipStream_t)stream;
   const int most = std::min(n - keep, keep);
   // units of 16 bytes where every row, head and token starts on one

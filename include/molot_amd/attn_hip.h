@@ -483,8 +483,9 @@ void molot_hip_set_merge(int in_launch);
  * into fp16 pieces once per launch, two of an fp32 row, one of a bf16 or Q8
  * row, each row scaled by a power of two, into a per-stream workspace of 4
  * (bf16, Q8) or 8 (fp32) bytes * nkv * (N - t0) * d (at most 1 GiB; it grows
- * outside stream capture only, and the buffers it outgrows stay allocated,
- * under 1 GiB in all; scored prompts take the pieces at every head dim, from
+ * outside stream capture only, to twice its size or more, and the buffers it
+ * outgrows stay allocated, together less than twice the live one; scored
+ * prompts take the pieces at every head dim, from
  * sizes of their own, and up to 8 GiB of them).  Smaller prompts over fp32 and Q8 caches take K and V
  * as two such pieces too: at d = 256, where one step appends all the keys it
  * attends, and at d <= 128 where that is faster, made once per launch (12 bytes

@@ -39,6 +39,7 @@
 #include "paged_plan.hpp"
 #include "prefill.hpp"
 #include "prefill_wide.hpp"
+#include "ws_growth.hpp"
 
 namespace {
 
@@ -1792,7 +1793,7 @@ struct WsKey {
 // within a step (by the attention kernel, or by it and the combine kernel
 // next on the same stream), so they need no clearing and hold nothing
 // between steps.  An outgrown buffer is retired, never freed: a graph
-// captured earlier on the stream still points at it (workspaces are small).
+// captured earlier on the stream still points at it.
 constexpr size_t kCtrBytes = sizeof(unsigned long long) * (size_t)kMaxSlots;
 struct WsBuf {
   void* ptr = nullptr;
@@ -1804,6 +1805,19 @@ std::vector<void*> g_retired;
 
 __global__ void zero_kernel(float* p, int64_t n);
 bool xcd_map_ok(int dev);
+
+// Allocates `want` bytes, or where there is no memory for them the `bytes` that the call
+// needs; *got is the size.
+hipError_t grow(void** p, size_t bytes, size_t want, size_t* got) {
+  *got = want;
+  hipError_t e = hipMalloc(p, want);
+  if (e == hipErrorOutOfMemory && want > bytes) {
+    (void)hipGetLastError();
+    *got = bytes;
+    e = hipMalloc(p, bytes);
+  }
+  return e;
+}
 
 }  // namespace
 int molot_host::workspace(void* stream, size_t bytes, unsigned long long** ctr, void** out) {
@@ -1820,11 +1834,10 @@ int molot_host::workspace(void* stream, size_t bytes, unsigned long long** ctr, 
     if (e != hipSuccess) return (int)e;
     if (cap != hipStreamCaptureStatusNone) return MOLOT_ENOWS;
     (void)xcd_map_ok(dev);  // the one-time dispatch check, outside any capture
-    if (w.ptr) g_retired.push_back(w.ptr);
-    w = WsBuf{};
-    const size_t want = bytes < ((size_t)1 << 20) ? ((size_t)1 << 20) : bytes;
+    const size_t want = std::max(grown_bytes(bytes, w.bytes, SIZE_MAX), (size_t)1 << 20);
+    size_t got = 0;
     void* p = nullptr;
-    e = hipMalloc(&p, kCtrBytes + want);
+    e = grow(&p, kCtrBytes + bytes, kCtrBytes + want, &got);
     if (e != hipSuccess) return (int)e;
     hipLaunchKernelGGL(zero_kernel, dim3((unsigned)(kCtrBytes / 4 / 256)), dim3(256), 0,
                        (hipStream_t)stream, reinterpret_cast<float*>(p), (int64_t)(kCtrBytes / 4));
@@ -1833,8 +1846,9 @@ int molot_host::workspace(void* stream, size_t bytes, unsigned long long** ctr, 
       (void)hipFree(p);
       return (int)e;
     }
+    if (w.ptr) g_retired.push_back(w.ptr);
     w.ptr = p;
-    w.bytes = want;
+    w.bytes = got - kCtrBytes;
   }
   *ctr = reinterpret_cast<unsigned long long*>(w.ptr);
   *out = reinterpret_cast<char*>(w.ptr) + kCtrBytes;
@@ -1842,10 +1856,9 @@ int molot_host::workspace(void* stream, size_t bytes, unsigned long long** ctr, 
 }
 namespace {
 
-// Per-(device, stream) workspace of the prefill's pre-split K/V pieces,
-// grown to at least twice its last size (so the retired buffers, which a
-// captured graph may still point at, total less than the live one).  Under
-// stream capture it cannot grow: the caller then splits per tile instead.
+// Per-(device, stream) workspace of the prefill's pre-split K/V pieces and of
+// the weights' scores, grown as grown_bytes says.  Under stream capture it
+// cannot grow: the caller then splits per tile instead.
 std::map<WsKey, WsBuf> g_pieces_ws;
 
 }  // namespace
@@ -1860,16 +1873,15 @@ int molot_host::pieces_workspace(void* stream, size_t bytes, void** out) {
     e = hipStreamIsCapturing((hipStream_t)stream, &cap);
     if (e != hipSuccess) return (int)e;
     if (cap != hipStreamCaptureStatusNone) return MOLOT_ENOWS;
-    // twice the size up to kMaxPiecesBytes, past it what is asked for: without
-    // scored calls the live buffer and the retired ones a captured graph may
-    // still hold stay under 2 GiB
-    const size_t want = std::min(std::max(bytes, 2 * w.bytes), std::max(bytes, kMaxPiecesBytes));
+    const size_t want =
+        grown_bytes(bytes, w.bytes, bytes <= kMaxPiecesBytes ? kMaxPiecesBytes : kMaxScoredBytes);
+    size_t got = 0;
     void* p = nullptr;
-    e = hipMalloc(&p, want);
+    e = grow(&p, bytes, want, &got);
     if (e != hipSuccess) return (int)e;
     if (w.ptr) g_retired.push_back(w.ptr);
     w.ptr = p;
-    w.bytes = want;
+    w.bytes = got;
   }
   *out = w.ptr;
   return 0;

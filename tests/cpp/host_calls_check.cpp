@@ -70,13 +70,83 @@ void run_threads() {
   CHECK(several >= kThreads * kCalls, "%d calls of several launches", several);
 }
 
+// A workspace that is asked for a little more at every call is allocated a few times, and
+// what was outgrown, which stays, is less than twice the live buffer.  (least: above the
+// other workspace's sizes.)
+constexpr size_t kMiB = (size_t)1 << 20;
+template <typename F>
+void rising(const char* what, int calls, size_t least, int most_allocations, size_t cap, F&& call) {
+  fake::reset();
+  for (int i = 0; i < calls; ++i) {
+    const int st = call(i);
+    CHECK(st == 0, "%s, call %d: status %d", what, i, st);
+  }
+  size_t live = 0, all = 0;
+  int count = 0;
+  for (size_t bytes : fake::state().mallocs) {
+    if (bytes < least) continue;
+    ++count;
+    live = bytes;
+    all += bytes;
+  }
+  CHECK(count >= 1 && count <= most_allocations, "%s: %d allocations", what, count);
+  CHECK(all - live < 2 * live, "%s: %zu MiB outgrown, %zu live", what, (all - live) / kMiB, live / kMiB);
+  CHECK(live <= cap, "%s: %zu MiB", what, live / kMiB);
+}
+hipStream_t stream(int i) { return reinterpret_cast<hipStream_t>((uintptr_t)0x2000 + 16 * i); }
+
+void run_growth() {
+  // a long prompt by chunks of 2048 over an fp32 cache: pieces of 1 GiB from 131072 rows on
+  rising("scored prompts", 64, 1000 * kMiB, 2, (size_t)8 << 30, [](int i) {
+    return molot_hip_attn_prefill_scored(at<float>(0), at<void>(1), at<void>(2), at<float>(3), 32, 8, 2048,
+                                         131072 + 2048 * i, 128, 0.1f, 129024 + 2048 * i, 0, 50.f, nullptr,
+                                         nullptr, nullptr, MOLOT_KV_F32, stream(0));
+  });
+  // up to the limit of 8 GiB
+  rising("long scored prompts", 40, 1000 * kMiB, 4, (size_t)8 << 30, [](int i) {
+    return molot_hip_attn_prefill_scored(at<float>(0), at<void>(1), at<void>(2), at<float>(3), 32, 8, 256,
+                                         25000 * (i + 1), 128, 0.1f, 25000 * (i + 1) - 256, 0, 50.f, nullptr,
+                                         nullptr, nullptr, MOLOT_KV_F32, stream(1));
+  });
+  // a batch that keeps its weights, four rows more at a time: 1.1 GiB of scores
+  rising("weights", 200, 512 * kMiB, 2, (size_t)8 << 30, [](int i) {
+    return molot_hip_attn_decode_paged_scored(at<float>(0), at<void>(1), at<void>(2), at<float>(3),
+                                              at<int32_t>(4), at<int32_t>(5), nullptr, 64, 8192, 70000 + 4 * i,
+                                              64, 1, 64, 16, 0.1f, 0, 50.f, nullptr, at<float>(6),
+                                              MOLOT_KV_BF16, stream(2));
+  });
+  // plain prompts stay within 1 GiB
+  rising("plain prompts", 60, 78 * kMiB, 5, (size_t)1 << 30, [](int i) {
+    return molot_hip_attn_prefill_gqa(at<float>(0), at<void>(1), at<void>(2), at<float>(3), 32, 8, 200,
+                                      10000 + 2000 * i, 128, 0.1f, 9800 + 2000 * i, 0, MOLOT_KV_F32, stream(3));
+  });
+  // evictions of a growing cache: lists, keys and counts of every slot
+  rising("evictions", 100, kMiB, 6, (size_t)1 << 30,
+         [](int i) { return evict(8, 100000 + 5000 * i, 90000, stream(4)); });
+  // no memory for twice the size: what the call needs
+  const auto prompt_of = [](int N) {
+    return molot_hip_attn_prefill_scored(at<float>(0), at<void>(1), at<void>(2), at<float>(3), 32, 8, 2048, N,
+                                         128, 0.1f, N - 2048, 0, 50.f, nullptr, nullptr, nullptr, MOLOT_KV_F32,
+                                         stream(5));
+  };
+  CHECK(prompt_of(140000) == 0, "the first prompt");
+  fake::reset();
+  fake::state().most = 1300 * kMiB;
+  CHECK(prompt_of(150000) == 0, "a prompt with little memory left");
+  bool pieces = false;
+  for (const auto& l : fake::state().launches) pieces |= l.kernel.find("wide_split") != std::string::npos;
+  CHECK(pieces && fake::state().refused.size() == 1, "a prompt with little memory left: its pieces");
+  CHECK(hipGetLastError() == hipSuccess, "an error was left behind");
+  fake::state().most = SIZE_MAX;
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   const struct {
     const char* name;
     void (*run)();
-  } cases[] = {{"threads", run_threads}};
+  } cases[] = {{"threads", run_threads}, {"growth", run_growth}};
   for (const auto& c : cases)
     if (argc == 2 && !std::strcmp(argv[1], c.name)) {
       c.run();

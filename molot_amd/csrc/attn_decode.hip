@@ -1807,14 +1807,16 @@ __global__ void zero_kernel(float* p, int64_t n);
 bool xcd_map_ok(int dev);
 
 // Allocates `want` bytes, or where there is no memory for them the `bytes` that the call
-// needs; *got is the size.
+// needs; *got is the size.  A failure is the call's status, and not left for the next
+// launch's hipGetLastError.
 hipError_t grow(void** p, size_t bytes, size_t want, size_t* got) {
   *got = want;
   hipError_t e = hipMalloc(p, want);
+  if (e != hipSuccess) (void)hipGetLastError();
   if (e == hipErrorOutOfMemory && want > bytes) {
-    (void)hipGetLastError();
     *got = bytes;
     e = hipMalloc(p, bytes);
+    if (e != hipSuccess) (void)hipGetLastError();
   }
   return e;
 }
@@ -3062,11 +3064,7 @@ static int rope_append_paged_impl(float* q, const float* k_new, const float* v_n
 
 // A workspace that the device has no memory for is one that is unavailable:
 // the path without it runs instead.
-static int without_memory(int st) {
-  if (st != (int)hipErrorOutOfMemory) return st;
-  (void)hipGetLastError();
-  return MOLOT_ENOWS;
-}
+static int without_memory(int st) { return st == (int)hipErrorOutOfMemory ? MOLOT_ENOWS : st; }
 
 // The attended keys of a prefill: [T0, N) with T0 the window start of its
 // first query (pos0), split into 16-bit pieces once per launch for fp32 and

@@ -140,13 +140,40 @@ void run_growth() {
   fake::state().most = SIZE_MAX;
 }
 
+// A call that finds no memory for its workspace says so, and leaves nothing for the
+// next one: its launches are not taken for failed.
+void run_no_memory() {
+  const auto refused = [](const char* what, auto&& call) {
+    fake::reset();
+    fake::state().most = kMiB / 4;
+    const int st = call(true);
+    CHECK(st == (int)hipErrorOutOfMemory, "%s: status %d", what, st);
+    for (const auto& l : fake::state().launches)  // (but for the check of the dispatch, once)
+      CHECK(l.kernel.find("xcc_probe") != std::string::npos, "%s: %s", what, l.kernel.c_str());
+    CHECK(fake::last_error == hipSuccess, "%s: an error was left behind", what);
+    const int next = call(false);
+    CHECK(next == 0, "%s: the next call's status %d", what, next);
+    fake::state().most = SIZE_MAX;
+  };
+  refused("a step", [](bool large) {
+    return molot_hip_decode_step(at<float>(0), at<float>(1), at<float>(2), at<void>(3), at<void>(4),
+                                 at<float>(5), 32, 8, 128, large ? 30000 : 20, 20, nullptr, 0.1f, 0,
+                                 MOLOT_KV_F32, stream(10));
+  });
+  refused("an eviction", [](bool large) { return evict(8, large ? 40000 : 100, 90, stream(11)); });
+  refused("a step's weights", [](bool large) {
+    return large ? scored_step(8, 30000, stream(12))
+                 : molot_hip_kv_track(at<float>(0), nullptr, 8, 10, 1, 9, 10, stream(12));
+  });
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   const struct {
     const char* name;
     void (*run)();
-  } cases[] = {{"threads", run_threads}, {"growth", run_growth}};
+  } cases[] = {{"threads", run_threads}, {"growth", run_growth}, {"no_memory", run_no_memory}};
   for (const auto& c : cases)
     if (argc == 2 && !std::strcmp(argv[1], c.name)) {
       c.run();

@@ -3091,6 +3091,11 @@ static int prefill_pieces(int nkv, int N, int d, int pos0, int window, int kv_dt
   return 0;
 }
 
+// The widest range of keys that a query row may attend.
+static int prefill_span(int N, int window, const Scoring& sc) {
+  return window > 0 && window < N && !sc.key_hi ? window : N;
+}
+
 // The prefill at a head dim the matrix-core prefill does not tile (an even d
 // that is not a multiple of 8; a padded Q8 cache), and above 256 where the
 // prompt is too small for prefill_on_pieces or its workspace cannot be had:
@@ -3126,10 +3131,28 @@ static int prefill_rows(const float* Qm, const void* K, const void* V, float* Om
   a.scale = scale;
   a.pf = 1;
   set_scoring(a, sc, 0);
-  // the widest attended range of any query row
-  const int span = window > 0 && window < N && !sc.key_hi ? window : N;
-  return block_row ? run_attn<true, false>(a, d, kv_dtype, span, M, stream)
-                   : run_attn<false, false>(a, d, kv_dtype, span, M, stream);
+  const int span = prefill_span(N, window, sc);
+  // rows m0 .. m0 + rows - 1
+  auto launch = [&](int m0, int rows) {
+    AttnArgs b = a;
+    b.q += (int64_t)m0 * nq * d;
+    b.o += (int64_t)m0 * nq * d;
+    b.pos += m0;
+    if (b.key_lo) b.key_lo += m0;
+    if (b.key_hi) b.key_hi += m0;
+    return block_row ? run_attn<true, false>(b, d, kv_dtype, span, rows, stream)
+                     : run_attn<false, false>(b, d, kv_dtype, span, rows, stream);
+  };
+  const int st = launch(0, M);
+  // more (row, head group) slots than the merge of their chunks takes: by parts
+  const int64_t groups = (int64_t)nkv * (nq / nkv / std::min(pick_gh(nq / nkv), 4));  // (or fewer)
+  const int part = (int)std::max<int64_t>(1, kMaxSlots / groups);
+  if (st != MOLOT_ENOTSUP || M <= part) return st;
+  for (int m0 = 0; m0 < M; m0 += part) {
+    const int sp = launch(m0, std::min(part, M - m0));
+    if (sp) return sp;
+  }
+  return 0;
 }
 
 // Launches a prefill attention kernel of `wgs` workgroups and, where its key
@@ -3338,10 +3361,10 @@ static bool prefill_takes_pieces(int d, int M, int N, int nq, int nkv, int kv_dt
 //   few rows       (2, 65536): rows by 1.4 to 4 times; (4, 16384): d128 fp32 61 / 86, bf16 50 /
 //                  56, Q8 76 / 59
 static bool prefill_scored_pieces(int d, int M, int N, int nq, int nkv, int window, int kv_dtype,
-                                  int presplit) {
+                                  const Scoring& sc, int presplit) {
   static constexpr int kPairs[3][4] = {  // thousands of (query row, key), by cache and padded head dim
       {1800, 800, 900, 340}, {1200, 800, 900, 300}, {150, 180, 500, 300}};
-  const int64_t span = window > 0 && window < N ? window : N;
+  const int64_t span = prefill_span(N, window, sc);
   const int D = prefill_D(d), cache = kv_dtype == MOLOT_KV_F32 ? 0 : kv_dtype == MOLOT_KV_BF16 ? 1 : 2;
   return presplit && M <= 65535 && (int64_t)M * (nq / nkv) >= 64 &&
          (int64_t)M * nq * span >= 1000ll * kPairs[cache][D == 64 ? 0 : D == 128 ? 1 : D == 256 ? 2 : 3];
@@ -3475,7 +3498,7 @@ static int attn_prefill_impl(const float* Qm, const void* K, const void* V, floa
     }
     return 0;
   }
-  if (sc.on ? prefill_scored_pieces(d, M, N, nq, nkv, window, kv_dtype, presplit)
+  if (sc.on ? prefill_scored_pieces(d, M, N, nq, nkv, window, kv_dtype, sc, presplit)
             : prefill_takes_pieces(d, M, N, nq, nkv, kv_dtype, window, presplit)) {
     st = prefill_on_pieces(Qm, K, V, Om, nq, nkv, M, N, d, scale, pos0, window, kv_dtype, block_row,
                            page, sc, stream, split_rows);
@@ -3673,7 +3696,7 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   // (a row never sees the rows appended after it: where rows were evicted from the cache
   // the positions run ahead of the slots, and the attention goes by the slots)
   const int apos = std::min(pos0, slot0);
-  if (sc.on ? prefill_scored_pieces(d, M, slot0 + M, nq, nkv, window, kv_dtype, presplit)
+  if (sc.on ? prefill_scored_pieces(d, M, slot0 + M, nq, nkv, window, kv_dtype, sc, presplit)
             : prefill_takes_pieces(d, M, slot0 + M, nq, nkv, kv_dtype, window, presplit)) {
     // at d = 512 the split of all rows is as fast (8q/2kv, 1999 tokens: 29 + 7
     // us against 49 for a RoPE/append that leaves the pieces), and a scored step's of Q8

@@ -81,3 +81,38 @@ def test_rows_past_the_bound_keep_their_weight(gpu, kv, nq, nkv, d, bound, over,
     if step:
         assert bool((a[:, :, n - 1] >= 0).all()) and float(a[:, :, n - 1].max()) <= G * (1 + 1e-4)
         assert (rows(sp)[:, :, n - 1] == n - 1).all() and (rows(sp)[:, :, :n - 1] == -5).all()
+
+
+# (kv, nq, nkv, d, m, window, ranges, presplit): past 65536 (row, head group) slots
+ROWS = [("bf16", 8, 8, 128, 10000, 8, True, True), ("bf16", 8, 8, 64, 9000, 0, True, False),
+        ("f32", 8, 4, 34, 17000, 40, False, False), ("q8", 16, 8, 256, 8300, 30, True, True)]
+
+
+@pytest.mark.parametrize("kv,nq,nkv,d,m,window,ranges,presplit", ROWS)
+def test_prompt_rows_past_a_grid(gpu, kv, nq, nkv, d, m, window, ranges, presplit):
+    """Prompts that stream each row's own keys, of more rows than one launch takes: a
+    window with key_hi past it, and the pieces switched off."""
+    g, scale = gen(m), 1 / math.sqrt(d)
+    q = randn(g, m, nq, d, sigma=3.0)
+    Kc, K = ref.make_cache(randn(g, m, nkv, d), kv)
+    Vc, V = ref.make_cache(randn(g, m, nkv, d), kv)
+    i = torch.arange(m, device="cuda")
+    lo = hi = None
+    start, end = (i - window + 1).clamp(min=0) if window else torch.zeros_like(i), i + 1
+    if ranges:
+        lo = (i - 50).clamp(min=0).int()
+        hi = (i + 20).int()
+        start, end = torch.maximum(start, lo.long()), hi.long().clamp(max=m)
+    sl = attn.alibi_slopes(nq).cuda()
+    O = torch.full((m, nq, d), math.nan, device="cuda")
+    attn.set_prefill_presplit(presplit)
+    try:
+        attn.attn_prefill_scored(q, Kc, Vc, O, nq, nkv, m, m, d, scale, 0, window, 50.0, sl, lo, hi)
+    finally:
+        attn.set_prefill_presplit(True)
+    assert bool(torch.isfinite(O).all())
+    part = 65536 // nkv  # (ends of the launches' parts, whatever the heads of a group)
+    some = sorted({t for e in (0, part // 2, part, 2 * part, m) for t in range(e - 4, e + 4) if 0 <= t < m})
+    some = torch.tensor(some, device="cuda")
+    want, _ = ref.attend(q[some], K, V, scale, some, start[some], end[some], 50.0, sl)
+    check_out(O[some], want, ref.tolerance(q[some], K, V, scale, 50.0, sl, 100))

@@ -2091,7 +2091,7 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
   a.mrg = 0;
   const size_t stats = a.acc ? (size_t)rows * a.nchunks * gh * 2 : 0;
   if (a.nchunks == 1 && !stats) return 0;  // single chunk: written directly, no combine
-  if ((long)rows > kMaxSlots) return MOLOT_ENOTSUP;
+  if (a.nchunks > 1 && (long)rows > kMaxSlots) return MOLOT_ENOTSUP;  // (nothing to merge: any number)
   if (stats) {  // the scores of every attended row, for the weights
     if (B > 65535 || a.nq / a.nkv > 4096) return MOLOT_ENOTSUP;  // attn_weights_kernel's grid, its LDS
     a.sc_rows = (std::max(span, 0) + 4) & ~3;  // (and the appended row)

@@ -116,3 +116,25 @@ def test_prompt_rows_past_a_grid(gpu, kv, nq, nkv, d, m, window, ranges, prespli
     some = torch.tensor(some, device="cuda")
     want, _ = ref.attend(q[some], K, V, scale, some, start[some], end[some], 50.0, sl)
     check_out(O[some], want, ref.tolerance(q[some], K, V, scale, 50.0, sl, 100))
+
+
+def test_weights_of_many_short_sequences(gpu):
+    """8200 sequences of 8 KV heads in one launch each: more (sequence, head) pairs than a
+    merge takes, and nothing to merge."""
+    nq, nkv, d, page, B = 8, 8, 4, 4, 8200
+    g = gen(70)
+    K, V = (randn(g, B, nkv, page, d) for _ in range(2))
+    table = torch.randperm(B, device="cuda", generator=g).int().view(B, 1)
+    lens = (torch.arange(B, device="cuda") % 5).int()
+    q, O = randn(g, B, nq, d, sigma=3.0), torch.empty(B, nq, d, device="cuda")
+    acc = torch.zeros(B, nkv, page, device="cuda")
+    attn.attn_decode_paged_scored(q, K.view(B, -1), V.view(B, -1), O, table, lens, None, B, 1, nq, nkv, d,
+                                  page, 0.5, 0, 20.0, None, acc)
+    kb, vb = (z[table[:, 0].long()].double() for z in (K, V))  # [B][head][slot][d]
+    s = 20 * ((q.double()[:, :, None] * kb).sum(-1) * 0.5 / 20).tanh()
+    s.masked_fill_(torch.arange(page, device="cuda") >= lens[:, None, None], -math.inf)
+    p = torch.nan_to_num(s.softmax(-1))
+    tol = ref.tolerance(q[0][None], kb[0].transpose(0, 1), vb[0].transpose(0, 1), 0.5, 20.0, None, page)
+    tol = 4 * tol  # (one sequence's largest |q||k| and |V| stand for all: 8200 of 4 elements each)
+    check_out(O, (p[..., None] * vb).sum(2), tol)
+    assert float((acc[table[:, 0].long()].double() - p).abs().max()) <= tol

@@ -327,11 +327,13 @@ int molot_hip_attn_prefill_paged(const float* Qm, const void* K, const void* V, 
  * a row sets that slot's acc instead, and its position in slot_pos (int32,
  * same layout; NULL: none; only with acc).  The acc of rows past max_seq_len is
  * left as it is (an appended row's: set to 0).  The scores of a call with acc are
- * kept for its second launch: 4 * B * nq * (attended rows + 1) bytes of the
- * stream's prefill workspace, at most 8 GiB and 2 GiB a KV head
- * (MOLOT_ENOTSUP past it, and past 4096 query heads a KV head or 65535
- * sequences).  The workspaces are the stream's: graphs captured on one stream
- * replay one after the other. */
+ * kept for its second launch, in the stream's prefill workspace: 4 * nq * (rows
+ * + 1, rounded up to 4) bytes a sequence, rows the most that a sequence of the
+ * call may attend (max_seq_len; a window's, if shorter and pos is NULL; of a
+ * contiguous cache those attended).  A batch of more than 8 GiB runs by parts;
+ * MOLOT_ENOTSUP past 8 GiB a sequence or 2 GiB a KV head of one, 4096 query
+ * heads a KV head, or 65535 sequences.  The workspaces are the stream's: graphs
+ * captured on one stream replay one after the other. */
 int molot_hip_attn_decode_scored(const float* Q, const void* K, const void* V, float* O, int nq,
                                  int nkv, int n, int d, float scale, int pos_cur, int window,
                                  float softcap, const float* slopes, float* acc, int acc_cap,

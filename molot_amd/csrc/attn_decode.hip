@@ -2033,6 +2033,9 @@ int merge_mode(const AttnArgs& a) {
   const int m = knob(g_merge);
   return m < 0 && a.acc ? 0 : m;
 }
+// Rows of scores kept of a sequence of at most `span` cache rows: those, the appended
+// one, and up to a unit of 4 of the matrix-core kernel's order.
+int64_t score_rows(int span) { return ((int64_t)std::max(span, 0) + 4) & ~3ll; }
 }  // namespace
 int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int B, int align, int wpc,
                 void* stream, bool cyclic) {
@@ -2094,7 +2097,7 @@ int molot_host::plan_launch(AttnArgs& a, int d, int span, int gh, int nsubs, int
   if (a.nchunks > 1 && (long)rows > kMaxSlots) return MOLOT_ENOTSUP;  // (nothing to merge: any number)
   if (stats) {  // the scores of every attended row, for the weights
     if (B > 65535 || a.nq / a.nkv > 4096) return MOLOT_ENOTSUP;  // attn_weights_kernel's grid, its LDS
-    a.sc_rows = (std::max(span, 0) + 4) & ~3;  // (and the appended row)
+    a.sc_rows = score_rows(span);
     // (a paged span counts it; a sequence's rows past the span may have no scores)
     a.sc_span = a.block_table ? std::max(span, 0) : (int)a.sc_rows;
     const size_t bytes = sizeof(float) * (size_t)B * a.nq * a.sc_rows;
@@ -2380,6 +2383,28 @@ int zero_out(float* O, int64_t count, hipStream_t st) {
 template <bool PAGED, bool ROPE>
 int run_attn(AttnArgs& a, int d, int kv_dtype, int span, int B, void* stream) {
   LaunchLock lock(g_launch_mu);
+  if (PAGED && a.acc) {  // the weights' scores within their workspace: sequences by parts
+    const int64_t most = (int64_t)kMaxScoredBytes / (4 * a.nq * score_rows(span));
+    if (most >= 1 && B > most) {
+      for (int b0 = 0; b0 < B; b0 += (int)most) {
+        AttnArgs p = a;
+        const int64_t qf = (int64_t)b0 * a.nq * d, kf = (int64_t)b0 * a.nkv * d;
+        p.q += qf;
+        p.o += qf;
+        if (ROPE) {
+          p.q_out += qf;
+          p.k_new += kf;
+          p.v_new += kf;
+        }
+        p.block_table += (int64_t)b0 * a.max_blocks;
+        p.seq_lens += b0;
+        if (p.pos_arr) p.pos_arr += b0;
+        const int st = run_attn<PAGED, ROPE>(p, d, kv_dtype, span, std::min((int)most, B - b0), stream);
+        if (st) return st;
+      }
+      return 0;
+    }
+  }
   if (a.scored)
     return PAGED ? run_paged_scored(a, ROPE, d, kv_dtype, span, B, stream)
                  : run_flat_scored(a, ROPE, d, kv_dtype, span, B, stream);

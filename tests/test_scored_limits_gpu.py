@@ -138,3 +138,47 @@ def test_weights_of_many_short_sequences(gpu):
     tol = 4 * tol  # (one sequence's largest |q||k| and |V| stand for all: 8200 of 4 elements each)
     check_out(O, (p[..., None] * vb).sum(2), tol)
     assert float((acc[table[:, 0].long()].double() - p).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_weights_of_a_ragged_batch_past_the_workspace(gpu, step):
+    """One sequence of a million rows among 39 short ones under 64 heads: the scores of
+    40 such sequences would be 10 GiB, what the workspace holds at most is 8."""
+    nq, nkv, d, page, B, n = 64, 1, 2, 16, 40, 1 << 20
+    g, width = gen(71), n // page
+    lens = [17 + b for b in range(B)]
+    lens[23] = n
+    table = torch.zeros(B, width, dtype=torch.int32)
+    at = 0
+    for b, m in enumerate(lens):
+        k = (m + page - 1) // page
+        table[b, :k] = torch.arange(at, at + k, dtype=torch.int32)
+        at += k
+    K, V = (randn(g, at, page * d) for _ in range(2))
+    acc, sp = torch.zeros(at, nkv, page, device="cuda"), torch.zeros(at, nkv, page, dtype=torch.int32,
+                                                                     device="cuda")
+    q, O = randn(g, B, nq, d), torch.empty(B, nq, d, device="cuda")
+    new = [randn(g, B, nkv, d) for _ in range(2)]
+    L, tb = torch.tensor(lens, dtype=torch.int32, device="cuda"), table.cuda()
+    pos = (L + 4) if step else None
+    if step:
+        attn.decode_step_paged_scored(q, *new, K, V, O, tb, L, pos, B, width, nq, nkv, d, page, None, 0.7, 0,
+                                      50.0, None, acc, sp)
+    else:
+        attn.attn_decode_paged_scored(q, K, V, O, tb, L, None, B, width, nq, nkv, d, page, 0.7, 0, 50.0,
+                                      None, acc)
+    for b in (0, 22, 23, 24, B - 1):
+        m = lens[b]
+        blk = tb[b, :(m + page - 1) // page].long()
+        Kb, Vb = (z[blk].view(-1, nkv, d)[:m].double() for z in (K, V))
+        if step:
+            assert torch.equal(Kb[-1].float(), new[0][b]) and torch.equal(Vb[-1].float(), new[1][b])
+            assert int(sp[blk[-1], 0, (m - 1) % page]) == m + 4
+        end = torch.tensor([m], device="cuda")
+        want, p = ref.attend(q[b:b + 1], Kb, Vb, 0.7, end - 1, end * 0, end, 50.0)
+        tol = ref.tolerance(q[b:b + 1], Kb, Vb, 0.7, 50.0, None, m)
+        check_out(O[b], want[0], tol)
+        got = acc[blk].view(-1)[:m].double()
+        # (a head's weights each to the bound of an output of V = 1; 64 of them)
+        one = ref.tolerance(q[b:b + 1], Kb, torch.ones_like(Vb), 0.7, 50.0, None, m)
+        assert float((got - p[0].sum(0)).abs().max()) <= nq * one

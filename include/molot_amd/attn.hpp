@@ -41,7 +41,9 @@ inline void check(int status, const char* what) {
 }
 
 inline void check_hip(hipError_t e, const char* what) {
-  if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
+  if (e == hipSuccess) return;
+  (void)hipGetLastError();  // (the exception's, not the next launch's)
+  throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
 }
 
 // True for device (or managed) memory, false for host memory.
@@ -210,6 +212,18 @@ struct Scores {
   const int32_t* key_lo = nullptr;  // prefill: [M]
   const int32_t* key_hi = nullptr;
 };
+
+// A cache's acc and slot_pos of `slots` (attn_hip.h: a budget of rows): both, or an
+// exception and neither.
+inline void alloc_books(size_t slots, float** acc, int32_t** slot_pos) {
+  void *a = nullptr, *p = nullptr;
+  check_hip(hipMalloc(&a, slots * sizeof(float)), "hipMalloc acc");
+  const hipError_t e = hipMalloc(&p, slots * sizeof(int32_t));
+  if (e != hipSuccess) (void)hipFree(a);
+  check_hip(e, "hipMalloc slot_pos");
+  *acc = static_cast<float*>(a);
+  *slot_pos = static_cast<int32_t*>(p);
+}
 
 // Device KV cache of one layer (Runner::KVC, forward.h:48-51) with the
 // decode-attention block of forward.h:554-591 in one fused launch, the
@@ -381,9 +395,7 @@ class DeviceKV {
   void track_weights() {
     if (acc) return;
     if (n) throw std::runtime_error("DeviceKV: track_weights on a cache in use");
-    const size_t slots = (size_t)nkv * cap;
-    check_hip(hipMalloc((void**)&acc, slots * sizeof(float)), "hipMalloc acc");
-    check_hip(hipMalloc((void**)&slot_pos, slots * sizeof(int32_t)), "hipMalloc slot_pos");
+    alloc_books((size_t)nkv * cap, &acc, &slot_pos);
   }
 
   // The cache cut to `keep` slots: the `recent` newest positions (pos: the newest

@@ -237,9 +237,16 @@ class PagedKVCache {
     for (const Seq& s : seqs_)
       if (s.live && s.len) throw std::runtime_error("PagedKVCache: track_weights on a cache in use");
     const size_t slots = (size_t)nblocks_ * nkv_ * page_;
-    for (int l = 0; l < layers_; ++l) {
-      check_hip(hipMalloc((void**)&acc_[l], slots * sizeof(float)), "hipMalloc acc");
-      check_hip(hipMalloc((void**)&slot_pos_[l], slots * sizeof(int32_t)), "hipMalloc slot_pos");
+    try {
+      for (int l = 0; l < layers_; ++l) alloc_books(slots, &acc_[l], &slot_pos_[l]);
+    } catch (...) {  // in every layer or in none
+      for (int l = 0; l < layers_; ++l) {
+        if (acc_[l]) (void)hipFree(acc_[l]);
+        if (slot_pos_[l]) (void)hipFree(slot_pos_[l]);
+        acc_[l] = nullptr;
+        slot_pos_[l] = nullptr;
+      }
+      throw;
     }
   }
   // Every sequence of ids that is longer than keep is cut to it, in every layer and

@@ -9,6 +9,7 @@
 
 #include <chrono>
 #include <cstdint>
+#include <cstdlib>
 #include <cstring>
 #include <map>
 #include <mutex>
@@ -30,7 +31,9 @@ struct State {
   std::vector<Launch> launches;
   std::vector<size_t> mallocs;   // sizes asked for and given
   std::vector<size_t> refused;
-  size_t most = SIZE_MAX;        // allocations past it are refused
+  size_t most = SIZE_MAX;        // allocations past it are refused,
+  int left = INT32_MAX;          // and after so many more
+  int live = 0;                  // allocations not freed
   uintptr_t next = 1ull << 40;
   bool capturing = false;
   int pause_us = 0;              // after every launch
@@ -100,16 +103,39 @@ hipError_t hipExtLaunchKernel(const void* fn, dim3 grid, dim3 block, void**, siz
 hipError_t hipMalloc(void** p, size_t bytes) {
   fake::State& s = fake::state();
   std::lock_guard<std::mutex> lk(s.mu);
-  if (bytes > s.most) {
+  if (bytes > s.most || s.left <= 0) {
     s.refused.push_back(bytes);
     return fake::last_error = hipErrorOutOfMemory;
   }
   s.mallocs.push_back(bytes);
+  --s.left;
+  ++s.live;
   *p = reinterpret_cast<void*>(s.next);
   s.next += (bytes + 255) / 256 * 256;
   return hipSuccess;
 }
-hipError_t hipFree(void*) { return hipSuccess; }
+hipError_t hipFree(void* p) {
+  fake::State& s = fake::state();
+  std::lock_guard<std::mutex> lk(s.mu);
+  s.live -= p != nullptr;
+  return hipSuccess;
+}
+// (what the classes of include/molot_amd use besides)
+hipError_t hipMemset(void*, int, size_t) { return hipSuccess; }
+hipError_t hipMemcpyAsync(void*, const void*, size_t, hipMemcpyKind, hipStream_t) { return hipSuccess; }
+hipError_t hipHostMalloc(void** p, size_t bytes, unsigned) {
+  *p = std::malloc(bytes);
+  return hipSuccess;
+}
+hipError_t hipHostFree(void* p) {
+  std::free(p);
+  return hipSuccess;
+}
+hipError_t hipPointerGetAttributes(hipPointerAttribute_t* attr, const void*) {
+  attr->type = hipMemoryTypeDevice;
+  return hipSuccess;
+}
+hipError_t hipEventRecord(hipEvent_t, hipStream_t) { return hipSuccess; }
 hipError_t hipGetLastError() {
   const hipError_t e = fake::last_error;
   fake::last_error = hipSuccess;
@@ -145,7 +171,7 @@ hipError_t hipGetSymbolAddress(void** p, const void*) {
 }
 hipError_t hipEventCreate(hipEvent_t* e) {
   *e = nullptr;
-  return hipErrorNotSupported;
+  return hipSuccess;
 }
 hipError_t hipEventDestroy(hipEvent_t) { return hipSuccess; }
 hipError_t hipEventSynchronize(hipEvent_t) { return hipSuccess; }

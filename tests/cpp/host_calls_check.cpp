@@ -7,7 +7,9 @@
 #include <set>
 
 #include "check_util.hpp"
+#include "molot_amd/attn.hpp"
 #include "molot_amd/attn_hip.h"
+#include "molot_amd/paged_kv.hpp"
 
 namespace {
 
@@ -167,13 +169,63 @@ void run_no_memory() {
   });
 }
 
+template <typename F>
+bool throws(F&& fn) {
+  try {
+    fn();
+  } catch (const std::runtime_error&) {
+    return true;
+  }
+  return false;
+}
+
+// track_weights without the memory for all of it: none of it is kept, the cache runs on
+// as one that tracks nothing, and a later call gets it all.
+void run_track() {
+  const molot::amd::LayerNorms nm;
+  for (int given = 0; given < 2; ++given) {
+    molot::amd::DeviceKV kv(64, 4, 128, MOLOT_KV_F32);
+    const int live = fake::state().live;
+    fake::state().left = given;
+    CHECK(throws([&] { kv.track_weights(); }), "contiguous: no error");
+    fake::state().left = INT32_MAX;
+    CHECK(fake::state().live == live && !kv.acc && !kv.slot_pos, "contiguous: kept after %d", given);
+    CHECK(!throws([&] {
+            kv.prefill(at<float>(0), at<float>(1), at<float>(2), at<float>(3), 8, 8, 0, nullptr, 0.1f, 0, nm);
+          }), "contiguous: the next prompt");
+    kv.reset();
+    kv.track_weights();
+    CHECK(kv.acc && kv.slot_pos, "contiguous: not allocated");
+  }
+  for (int given = 0; given < 4; ++given) {
+    molot::amd::PagedKVCache kv(2, 8, 4, 128, 16, MOLOT_KV_F32);
+    const int live = fake::state().live;
+    fake::state().left = given;
+    CHECK(throws([&] { kv.track_weights(); }), "paged: no error");
+    fake::state().left = INT32_MAX;
+    CHECK(fake::state().live == live, "paged: %d kept after %d", fake::state().live - live, given);
+    for (int l = 0; l < 2; ++l) CHECK(!kv.acc_pages(l) && !kv.slot_pos_pages(l), "paged: layer %d kept", l);
+    CHECK(throws([&] { kv.evict({kv.add_sequence()}, 4, 1); }), "paged: evicts without books");
+    kv.track_weights();
+    for (int l = 0; l < 2; ++l) CHECK(kv.acc_pages(l) && kv.slot_pos_pages(l), "paged: layer %d without", l);
+    const int id = kv.add_sequence();
+    kv.begin_prefill(id, 20);
+    for (int l = 0; l < 2; ++l)
+      CHECK(!throws([&] {
+              kv.prefill(l, at<float>(0), at<float>(1), at<float>(2), at<float>(3), 8, 0, nullptr, 0.1f, 0, nm);
+            }), "paged: the next prompt");
+    kv.end_prefill();
+    CHECK(!throws([&] { kv.evict({id}, 10, 4); }), "paged: evict");
+  }
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   const struct {
     const char* name;
     void (*run)();
-  } cases[] = {{"threads", run_threads}, {"growth", run_growth}, {"no_memory", run_no_memory}};
+  } cases[] = {{"threads", run_threads}, {"growth", run_growth}, {"no_memory", run_no_memory}, {"track", run_track}};
   for (const auto& c : cases)
     if (argc == 2 && !std::strcmp(argv[1], c.name)) {
       c.run();

@@ -16,8 +16,9 @@
 // head (load, count, scan, list, move): 4352 bf16 slots of 8 heads (d = 128) cut to 4096
 // in 9.9 us, and kv_track_kernel 2.0, against 0.5 for the bytes; 32 paged sequences of
 // 700 to 1399 Q8 rows cut to 1024 in 12.5.  131072 bf16 slots of 8 heads cut by 8192:
-// keys 7.0, pick 8.6, rank 2.7, list 5.3 us (a launch each, a chunk of 4096 slots a
-// workgroup) and the moves 15.0, which read and write 67 MB at 4.5 TB/s.
+// keys 7.8, pick 9.4, rank 3.8, list 5.1 us (a launch each, a chunk of 4096 slots a
+// workgroup; pick reads every chunk's counts in each of them, 67 MB, and so grows with the
+// square of the chunks) and the moves 13.2, which read and write 67 MB at 5.1 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -880,17 +881,22 @@ int launch_evict(const SlotArgs& a, int n, int keep, int recent, int B, void* st
   g.keep = keep;
   g.recent = recent;
   g.most = most;
-  // Chunks of 8192 slots; of 4096 where those would leave CUs idle, up to 2^17 slots (every
-  // chunk sums all chunks' counts).  8 heads, us for 8192 / 4096: 20000 slots 24.0 / 19.1,
-  // 65536 35.9 / 21.4, 131072 37.6 / 38.0 (after other work 46.7 / 42.4), 200000 39.7 / 51.8,
-  // 1048576 138 / 297.
+  // Chunks of 4096 slots where their workgroups fit the CUs in one round, up to 80 a head
+  // (each sums all the chunks' counts); else of 8192.  us a pass of tracking and cutting
+  // 8192 of the bf16 slots (d = 128; the caches' turn about), for 4096 / 8192: 8 heads, 20000
+  // slots 28.0 / 33.4, 65536 30.2 / 34.7, 114688 33.5 / 37.2, 131072 (256 chunks) 33.4 / 36.7;
+  // cut by 5000 (264 chunks) 37.8 / 33.8; 147456 41.0 / 38.5, 200000 45.5 / 40.6.  4 heads,
+  // 200000 34.7 / 36.4, 270000 (272) 46.8 / 37.7.  32 heads, 28000 34.3 / 38.3, 36000 (288) 39.3 /
+  // 39.3.  One head, 65536 26.6 / 31.0, 262144 32.8 / 34.4, 327680 (80) 35.6 / 35.4, 393216 37.6 /
+  // 36.4, 1048576 59.4 / 47.5.
   auto cut = [&](int chunk) {
     g.chunk = chunk;
     g.nlo = (keep + chunk - 1) / chunk;
     g.nhi = (n - keep + chunk - 1) / chunk;
   };
-  cut(8 * kSelThreads);
-  if (n <= 1 << 17 && (int64_t)(g.nlo + g.nhi) * (int64_t)pairs < num_cus()) cut(4 * kSelThreads);
+  cut(4 * kSelThreads);
+  if (g.nlo + g.nhi > 80 || (int64_t)(g.nlo + g.nhi) * (int64_t)pairs > num_cus())
+    cut(8 * kSelThreads);
   const size_t nc = n <= kSelMax ? 0 : (size_t)g.nlo + g.nhi;
   const size_t lds = sizeof(int32_t) * (kRankMax + 3 * nc);
   if (lds + sizeof(SelectLds) > kMaxLds) return MOLOT_ENOTSUP;  // past 40 million rows

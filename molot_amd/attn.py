@@ -454,8 +454,17 @@ def rope_append_paged(q, k_new, v_new, K, V, block_table, seq_lens, pos, B, max_
 # --- scored attention, and a cache held to a budget of rows ------------------
 
 
-def alibi_slopes(nq: int) -> torch.Tensor:
-    """Host fp32 table of geometric slopes 2^(-8 (h + 1) / nq), a query head each."""
+def alibi_slopes(nq: int, interleaved: bool = False) -> torch.Tensor:
+    """Host fp32 table of geometric slopes 2^(-8 (h + 1) / nq), a query head each.
+
+    The published table (Press, Smith and Lewis, "Train Short, Test Long", 2022) is
+    this one where nq is a power of two.  For other counts it has the slopes of p heads,
+    p the power of two below nq, and then the first, third, ... of 2p heads:
+    interleaved=True, for models trained with it (the same for powers of two)."""
+    p = 1 << max(int(nq), 1).bit_length() - 1
+    if interleaved and p < nq:
+        between = alibi_slopes(2 * p)[::2]
+        return torch.cat([alibi_slopes(p), between[:nq - p]])
     return torch.exp2(-8.0 * torch.arange(1, nq + 1, dtype=torch.float64) / nq).float()
 
 

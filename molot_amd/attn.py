@@ -41,11 +41,19 @@ def _ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
+# The current device (a device tensor exists where it is asked for, so without
+# torch.cuda.current_device's look at the initialization: 1 us a call of nine tensors).
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _need(t: torch.Tensor, name: str, dtype=None, min_numel: int = 0) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
-    if t.device.type != "cuda":
+    at = t.get_device()  # (-1: not a device tensor)
+    if at < 0:
         raise ValueError(f"{name}: must be a device tensor, got {t.device}")
+    if at != _device():  # the call runs on the current device's stream
+        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{_device()}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
     if dtype is not None and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):

@@ -235,10 +235,10 @@ def _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V):
     _need(K, "K", _KV_DTYPES, nblocks * bu)
     _need(V, "V", K.dtype, nblocks * bu)
     # host-side bounds check of every block id a kernel can reach
-    lens = seq_lens.cpu()
-    if int(lens.min()) < 0 or int(lens.max()) > max_blocks * page:
+    lens = seq_lens.view(-1)[:B].cpu()
+    if B and (int(lens.min()) < 0 or int(lens.max()) > max_blocks * page):
         raise ValueError("seq_lens outside [0, max_blocks*page]")
-    bt = block_table.view(B, max_blocks).cpu()
+    bt = block_table.view(-1)[:B * max_blocks].view(B, max_blocks).cpu()
     for b in range(B):
         used = (int(lens[b]) + page - 1) // page
         if used and (int(bt[b, :used].min()) < 0 or int(bt[b, :used].max()) >= nblocks):
@@ -274,7 +274,7 @@ def decode_step_paged(q, k_new, v_new, K, V, O, block_table, seq_lens, pos, B, m
     _need(v_new, "v_new", torch.float32, B * nkv * d)
     _need_table(inv_freq, d)
     max_len = _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V)
-    if B and int(seq_lens.min()) < 1:
+    if B and int(seq_lens.view(-1)[:B].min()) < 1:
         raise ValueError("decode_step_paged: every sequence needs seq_lens >= 1")
     if q_norm is None and k_norm is None and not v_norm:
         check(_lib.load().molot_hip_decode_step_paged(
@@ -398,7 +398,7 @@ def decode_step_paged_shared(q, K, V, O, block_table, seq_lens, pos, B, max_bloc
     _need_table(inv_freq, d)
     _need_norms(q_norm, None, d)
     max_len = _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V)
-    if B and int(seq_lens.min()) < 1:
+    if B and int(seq_lens.view(-1)[:B].min()) < 1:
         raise RuntimeError("fwd: shared KV empty")
     check(_lib.load().molot_hip_decode_step_paged_shared(
         _ptr(q), _ptr(K), _ptr(V), _ptr(O), _ptr(block_table), _ptr(seq_lens), _ptr(pos), B,
@@ -451,7 +451,7 @@ def rope_append_paged(q, k_new, v_new, K, V, block_table, seq_lens, pos, B, max_
     _need(v_new, "v_new", torch.float32, B * nkv * d)
     _need_table(inv_freq, d)
     _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V)
-    if B and int(seq_lens.min()) < 1:
+    if B and int(seq_lens.view(-1)[:B].min()) < 1:
         raise ValueError("rope_append_paged: every sequence needs seq_lens >= 1")
     check(_lib.load().molot_hip_rope_append_paged(
         _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(K), _ptr(V), _ptr(block_table), _ptr(seq_lens),
@@ -601,7 +601,7 @@ def decode_step_paged_scored(q, k_new, v_new, K, V, O, block_table, seq_lens, po
     _need_table(inv_freq, d)
     _need_norms(q_norm, k_norm, d)
     max_len = _check_paged(block_table, seq_lens, pos, B, max_blocks, nkv, d, page, K, V)
-    if B and int(seq_lens.min()) < 1:
+    if B and int(seq_lens.view(-1)[:B].min()) < 1:
         raise ValueError("decode_step_paged_scored: every sequence needs seq_lens >= 1")
     _need_scoring(slopes, nq)
     _need_acc_pages(acc, slot_pos, K.numel() // _block_units(kvd, nkv, d, page), nkv, page,
@@ -727,7 +727,7 @@ def _check_slot_pages(block_table, seq_lens, pos, B, max_blocks, nblocks, page):
     _need(seq_lens, "seq_lens", torch.int32, B)
     if pos is not None:
         _need(pos, "pos", torch.int32, B)
-    lens = seq_lens[:B].cpu()
+    lens = seq_lens.view(-1)[:B].cpu()
     if B and (int(lens.min()) < 0 or int(lens.max()) > max_blocks * page):
         raise ValueError("seq_lens outside [0, max_blocks*page]")
     bt = block_table.view(-1)[:B * max_blocks].view(B, max_blocks).cpu()

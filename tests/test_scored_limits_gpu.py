@@ -182,3 +182,25 @@ def test_weights_of_a_ragged_batch_past_the_workspace(gpu, step):
         # (a head's weights each to the bound of an output of V = 1; 64 of them)
         one = ref.tolerance(q[b:b + 1], Kb, torch.ones_like(Vb), 0.7, 50.0, None, m)
         assert float((got - p[0].sum(0)).abs().max()) <= nq * one
+
+
+def test_empty_and_partial_batches(gpu):
+    """No sequence: nothing to do.  Lengths and tables of more sequences than the batch's
+    are not looked at past it."""
+    nq, nkv, d, page, width = 4, 2, 8, 4, 2
+    K, V = (torch.randn(4, nkv * page * d, device="cuda") for _ in range(2))
+    acc, sp = torch.zeros(4, nkv, page, device="cuda"), torch.zeros(4, nkv, page, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([5, -1], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[0, 1], [99, 0]], dtype=torch.int32, device="cuda")
+    q, new = torch.randn(1, nq, d, device="cuda"), torch.randn(1, nkv, d, device="cuda")
+    for B in (0, 1):
+        O = torch.full((1, nq, d), 7.0, device="cuda")
+        attn.attn_decode_paged(q, K, V, O, table, lens, None, B, width, nq, nkv, d, page, 0.3)
+        O2 = torch.full((1, nq, d), 7.0, device="cuda")
+        attn.attn_decode_paged_scored(q, K, V, O2, table, lens, None, B, width, nq, nkv, d, page, 0.3, acc=acc)
+        assert bool((O == 7).all()) == (B == 0) and float((O - O2).abs().max()) < 1e-6
+        attn.decode_step_paged_scored(q.clone(), new, new, K, V, O, table, lens, None, B, width, nq, nkv, d,
+                                      page, None, 0.3, acc=acc, slot_pos=sp)
+        attn.kv_track_paged(acc, sp, table, lens, None, B, width, 3, nkv, page)
+        attn.kv_evict_paged(K, V, acc, sp, table, lens, None, B, width, nkv, d, page, 4, 1)
+    assert torch.isfinite(O).all()

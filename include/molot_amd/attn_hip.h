@@ -227,7 +227,8 @@ int molot_hip_rope_append_paged(float* q, const float* k_new, const float* v_new
  * [M][nq][d] fp32; K/V the token-major cache [N][nkv*d] holding the M new
  * tokens; query m sits at position pos0 + m and attends slots
  * [t0, min(pos0 + m + 1, N)), t0 = max(0, pos - window + 1) for window > 0.
- * A query with no slot gets O = 0.  scale as given.  pos0 counts slots: over a
+ * A query with no slot gets O = 0.  scale as given.  pos0 + M (and a step's
+ * slot0 + M) stay below 2^31 (MOLOT_EINVAL).  pos0 counts slots: over a
  * cache cut by molot_hip_kv_evict the prompt's first slot, N - M, not its
  * token's position (which molot_hip_prefill_q takes). */
 int molot_hip_attn_prefill_gqa(const float* Qm, const void* K, const void* V, float* Om, int nq,

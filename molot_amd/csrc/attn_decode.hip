@@ -3116,6 +3116,9 @@ static int prefill_pieces(int nkv, int N, int d, int pos0, int window, int kv_dt
   return 0;
 }
 
+// The last position or slot of a prompt: pos0 + m + 1 is an int in the kernels.
+constexpr int kMaxPos = 0x7FFFFFFF;
+
 // The widest range of keys that a query row may attend.
 static int prefill_span(int N, int window, const Scoring& sc) {
   return window > 0 && window < N && !sc.key_hi ? window : N;
@@ -3502,7 +3505,8 @@ static int attn_prefill_impl(const float* Qm, const void* K, const void* V, floa
   const bool rows_path = prefill_by_rows(d, kv_dtype);
   const bool pieces_only = kv_dtype == MOLOT_KV_Q8 && d == 256;
   const int D = padded ? (d <= 64 ? 64 : d <= 128 ? 128 : 256) : d;
-  if (M < 0 || N < 0 || pos0 < 0 || (M > 0 && (!Qm || !Om))) return MOLOT_EINVAL;
+  if (M < 0 || N < 0 || pos0 < 0 || pos0 > kMaxPos - M || (M > 0 && (!Qm || !Om)))
+    return MOLOT_EINVAL;
   if (M == 0) return 0;
   LaunchLock lock(g_launch_mu);
   if (N == 0) return zero_out(Om, (int64_t)M * nq * d, (hipStream_t)stream);
@@ -3675,7 +3679,8 @@ static int prefill_step_impl(float* q, const float* k_new, const float* v_new, v
   nm.k = k_norm;
   nm.v = v_norm ? 1 : 0;
   nm.eps = eps;
-  if (!norms_ok(nm) || M < 0 || slot0 < 0 || pos0 < 0) return MOLOT_EINVAL;
+  if (!norms_ok(nm) || M < 0 || slot0 < 0 || pos0 < 0 || slot0 > kMaxPos - M || pos0 > kMaxPos - M)
+    return MOLOT_EINVAL;
   if (M == 0) return 0;
   if (!q || !k_new || !v_new || !K || !V || !O) return MOLOT_EINVAL;
   if ((int64_t)M > 65535) return MOLOT_ENOTSUP;  // one grid row per token
@@ -3809,7 +3814,8 @@ int molot_hip_prefill_step_paged_scored(
 // place, no append (the RoPE/append kernel with its KV part off).
 static int q_prologue(float* q, int nq, int d, int M, int pos0, const float* q_norm, float eps,
                       const float* inv_freq, void* stream) {
-  if (nq < 0 || M < 0 || d <= 0 || (d & 1) || d > 2048 || pos0 < 0) return MOLOT_EINVAL;
+  if (nq < 0 || M < 0 || d <= 0 || (d & 1) || d > 2048 || pos0 < 0 || pos0 > kMaxPos - M)
+    return MOLOT_EINVAL;
   if (!(eps >= 0.f && eps < INFINITY)) return MOLOT_EINVAL;
   if (nq == 0 || M == 0) return 0;
   if (!q) return MOLOT_EINVAL;

@@ -316,8 +316,10 @@ int molot_hip_attn_prefill_paged(const float* Qm, const void* K, const void* V, 
  *                  query head; NULL: none; |slopes[h] * (i - t)| below 1e29)
  * and the softmax over the attended slots; an empty range yields o = 0.
  * i is pos_cur, pos or pos0 + m as the entry's window takes it, t the slot.
- * Same kernels, layouts, cache types, head dims, workspaces and accuracy as
- * the plain entries.
+ * Same kernels, layouts, cache types, head dims and workspaces as the plain
+ * entries.  fp32 accuracy as theirs, but for one figure: a prompt on the pieces
+ * (molot_hip_set_prefill_presplit) may lose 2^-20 of a row's largest |V| to
+ * the ends of the probabilities' pieces, where plain ones lose up to 2^-36 a key.
  *
  * acc (NULL: none) is the weights a cache's eviction goes by: for every
  * attended slot t and KV head g, the softmax weights of the query heads of
@@ -400,8 +402,9 @@ int molot_hip_prefill_step_paged_scored(
  * acc and slot_pos (layouts as above) describe the slots in use: the weight a
  * slot has got so far, and the position of the token it holds.  A scored step
  * with both keeps them for the row it appends; molot_hip_kv_track does for
- * rows appended otherwise (a prompt): the last M of n slots get acc 0 and the
- * positions pos - M + 1 .. pos (slot_pos NULL: none).  The paged form takes
+ * rows appended otherwise (a prompt, whose own attention is not counted): the
+ * last M of n slots get acc 0 and the positions pos - M + 1 .. pos (slot_pos
+ * NULL: none).  The paged form takes
  * the last min(M, seq_lens[b]) slots of every sequence, pos[b] its newest
  * token's position (pos NULL: seq_lens[b] - 1). */
 int molot_hip_kv_track(float* acc, int32_t* slot_pos, int nkv, int n, int M, int pos, int acc_cap,

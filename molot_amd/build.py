@@ -7,6 +7,8 @@
   tests/cpp/test_paged_kv      C++ self-check of the paged-KV manager
                               (include/molot_amd/attn.hpp), linked to the above
                               and to the oracle (its checker)
+  tests/cpp/test_kv_budget     self-checks of caches held to a budget, and of prompts and
+  tests/cpp/test_kv_cut        steps over the caches that rows were evicted from
   tests/cpp/prefill_no_memory  prefill where its workspace's allocation is refused
   tests/cpp/host_io_time       time of the C++ drop-in's decode call with host
                               vectors against device ones (bench.py's host_io)

@@ -276,6 +276,7 @@ class DeviceKV {
               const float* inv_freq, float scale, int window, const LayerNorms& nm,
               hipStream_t s = nullptr) {
     if (n >= cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:570
+    if (n == 0 && pos == 0) gone = 0;  // from the start again
     check_window(window, pos);
     const size_t qf = (size_t)nq * hd, kf = (size_t)nkv * hd;
     CallStage view(q, true, ao, qf, qf, s, knew, vnew, kf);
@@ -318,6 +319,7 @@ class DeviceKV {
                int pos0, const float* inv_freq, float scale, int window,
                const LayerNorms& nm = LayerNorms{}, hipStream_t s = nullptr) {
     if (n + M > cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:385
+    if (n == 0 && pos0 == 0) gone = 0;  // from the start again
     check_window(window, pos0 + M - 1);
     check(molot_hip_prefill_step(Q, K_new, V_new, k, v, AO, nq, nkv, hd, M, n, pos0, nm.q_norm,
                                  nm.k_norm, nm.v_norm ? 1 : 0, nm.eps, inv_freq, scale, window,
@@ -364,6 +366,7 @@ class DeviceKV {
                      const float* inv_freq, float scale, int window, const LayerNorms& nm,
                      const Scores& sc, hipStream_t s = nullptr) {
     if (n >= cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:570
+    if (n == 0 && pos == 0) gone = 0;  // from the start again
     check_window(window, pos);
     const size_t qf = (size_t)nq * hd, kf = (size_t)nkv * hd;
     CallStage view(q, true, ao, qf, qf, s, knew, vnew, kf);
@@ -381,6 +384,7 @@ class DeviceKV {
                       int pos0, const float* inv_freq, float scale, int window,
                       const LayerNorms& nm, const Scores& sc, hipStream_t s = nullptr) {
     if (n + M > cap) throw std::runtime_error("fwd: KV cache full");  // forward.h:385
+    if (n == 0 && pos0 == 0) gone = 0;  // from the start again
     check_window(window, pos0 + M - 1);
     check(molot_hip_prefill_step_scored(Q, K_new, V_new, k, v, AO, nq, nkv, hd, M, n, pos0,
                                         nm.q_norm, nm.k_norm, nm.v_norm ? 1 : 0, nm.eps, inv_freq,
@@ -400,7 +404,8 @@ class DeviceKV {
 
   // The cache cut to `keep` slots: the `recent` newest positions (pos: the newest
   // token's), then the highest weights.  The rows left lie in any order, so from then
-  // on until reset() a call whose window would leave a position out throws.
+  // on until the cache starts again (reset(), or n = 0 and position 0) a call whose
+  // window would leave a position out throws.
   void evict(int keep, int recent, int pos, hipStream_t s = nullptr) {
     if (!acc) throw std::runtime_error("DeviceKV: evict without track_weights");
     check(molot_hip_kv_evict(k, v, acc, slot_pos, nkv, n, hd, keep, recent, pos, cap, kv_dtype, s),

@@ -220,6 +220,16 @@ void run_windows() {
   kv.reset();
   kv.prefill(r.dq.p, r.dk.p, r.dv.p, r.dout.p, kNq, 40, 0, nullptr, kScale, 16, nm);
   all(16, 44, false, "reset");
+  kv.evict(20, 3, 39);
+  all(16, 44, true, "cut again");
+  kv.evict(0, 3, 39);
+  Rows one(rng, 1);
+  CHECK(throws([&] {
+          kv.decode(one.dq.p, one.dk.p, one.dv.p, one.dout.p, kNq, 40, nullptr, kScale, 16, nm);
+        }), "cut to nothing: the next token");
+  kv.n = 0;  // (without reset)
+  kv.prefill(r.dq.p, r.dk.p, r.dv.p, r.dout.p, kNq, 40, 0, nullptr, kScale, 16, nm);
+  all(16, 44, false, "from position 0 again");
 
   molot::amd::PagedKVCache pg(1, 32, kNkv, kD, 16, MOLOT_KV_F32);
   pg.track_weights();

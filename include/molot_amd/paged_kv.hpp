@@ -354,6 +354,7 @@ class PagedKVCache {
       if (h_table_) check_hip(hipHostFree(h_table_), "hipHostFree");
       d_table_ = nullptr;
       h_table_ = nullptr;
+      table_cap_ = 0;
       check_hip(hipMalloc(&d_table_, bytes), "hipMalloc block table");
       check_hip(hipHostMalloc((void**)&h_table_, bytes, hipHostMallocDefault), "hipHostMalloc");
       table_cap_ = bytes;

@@ -219,13 +219,33 @@ void run_track() {
   }
 }
 
+// A batch whose larger block table finds no memory: an error, and the next one runs.
+void run_table() {
+  const molot::amd::LayerNorms nm;
+  molot::amd::PagedKVCache kv(1, 64, 4, 128, 16, MOLOT_KV_F32);
+  std::vector<int> ids;
+  for (int i = 0; i < 8; ++i) ids.push_back(kv.add_sequence());
+  auto step = [&](const std::vector<int>& batch) {
+    kv.begin_decode(batch);
+    kv.decode(0, at<float>(0), at<float>(1), at<float>(2), at<float>(3), 8, nullptr, 0.1f, 0, nm);
+    kv.end_decode();
+  };
+  step({ids[0]});
+  fake::state().left = 0;
+  CHECK(throws([&] { step(ids); }), "no error");
+  fake::state().left = INT32_MAX;
+  CHECK(!throws([&] { step({ids[0]}); }), "the small batch again");
+  CHECK(!throws([&] { step(ids); }), "the large one");
+  CHECK(kv.length(ids[0]) == 3 && kv.length(ids[7]) == 1, "lengths");
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   const struct {
     const char* name;
     void (*run)();
-  } cases[] = {{"threads", run_threads}, {"growth", run_growth}, {"no_memory", run_no_memory}, {"track", run_track}};
+  } cases[] = {{"threads", run_threads}, {"growth", run_growth}, {"no_memory", run_no_memory}, {"track", run_track}, {"table", run_table}};
   for (const auto& c : cases)
     if (argc == 2 && !std::strcmp(argv[1], c.name)) {
       c.run();

@@ -31,7 +31,7 @@ def program(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("case", ["threads", "growth", "no_memory", "track"])
+@pytest.mark.parametrize("case", ["threads", "growth", "no_memory", "track", "table"])
 def test_host_calls(program, case):
     r = subprocess.run([program, case], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "PASSED" in r.stdout, r.stdout[-4000:] + r.stderr

@@ -1616,9 +1616,9 @@ __device__ __forceinline__ void weigh_rows(const WeightArgs& w, int rb, int h, i
     const int64_t blk = w.block_table[(int64_t)b * w.max_blocks + (t >> w.page_shift)];
     return ((blk * w.c.nkv + h) << w.page_shift) + (t & ((1 << w.page_shift) - 1));
   };
-  // a fresh row outside the range (a position behind the cache's end, or past the bound
-  // of the lengths)
-  if (w.fresh && n > 0 && n - 1 >= t0 + span && rb == 0 && tid == 0) {
+  // a fresh row outside the range (before its window, whose start is n at most, or past
+  // the bound of the lengths)
+  if (w.fresh && n > 0 && (n - 1 < t0 || n - 1 >= t0 + span) && rb == 0 && tid == 0) {
     const int64_t i = index(n - 1);
     w.acc[i] = 0.f;
     if (w.slot_pos) w.slot_pos[i] = pos;

@@ -204,3 +204,37 @@ def test_empty_and_partial_batches(gpu):
         attn.kv_track_paged(acc, sp, table, lens, None, B, width, 3, nkv, page)
         attn.kv_evict_paged(K, V, acc, sp, table, lens, None, B, width, nkv, d, page, 4, 1)
     assert torch.isfinite(O).all()
+
+
+@pytest.mark.parametrize("kv,nq,nkv,d", [("f32", 8, 4, 128), ("bf16", 16, 4, 128), ("q8", 16, 4, 128),
+                                         ("q8", 8, 4, 256), ("f32", 6, 2, 34)])
+def test_paged_step_outside_its_window(gpu, kv, nq, nkv, d):
+    """New rows outside the windows of their positions, beside others inside: appended,
+    o = 0, their acc 0 and their positions kept."""
+    page, window, lens, pos = 16, 9, (40, 1, 17, 300, 33), (48, 9, 25, 400, 33)
+    B, width = len(lens), (max(lens) + page - 1) // page
+    g = gen(72)
+    table = torch.randperm(B * width, generator=torch.Generator().manual_seed(3)).int().view(B, width)
+    pools = [ref.make_pages(randn(g, 0, nkv, d), kv, B * width, [], page) for _ in range(2)]
+    for pool in pools:
+        for b, n in enumerate(lens):
+            ref.put_pages(pool, randn(g, n, nkv, d), kv, table[b].tolist(), page)
+    acc = torch.rand(B * width, nkv, page, device="cuda", generator=g)
+    sp = torch.full((B * width, nkv, page), -5, dtype=torch.int32, device="cuda")
+    before, tb = acc.clone(), table.cuda()
+    q, O = randn(g, B, nq, d), torch.full((B, nq, d), 7.0, device="cuda")
+    new = [randn(g, B, nkv, d) for _ in range(2)]
+    L, P = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lens, pos))
+    attn.decode_step_paged_scored(q, *new, *pools, O, tb, L, P, B, width, nq, nkv, d, page, None, 0.1, window,
+                                  50.0, None, acc, sp)
+    rows = lambda z, b: z[tb[b].long()].permute(1, 0, 2).reshape(nkv, -1)[:, :lens[b]]  # noqa: E731
+    for b, (n, p) in enumerate(zip(lens, pos)):
+        a, a0, s = rows(acc, b), rows(before, b), rows(sp, b)
+        assert (s[:, -1] == p).all() and (s[:, :-1] == -5).all()
+        inside = p - window + 1 < n  # the window still holds slot n - 1
+        assert bool((O[b] != 0).any()) == inside
+        first = max(0, p - window + 1)
+        assert torch.equal(a[:, :min(first, n - 1)], a0[:, :min(first, n - 1)])
+        G = nq // nkv
+        grown = a[:, -1] + (a[:, :-1] - a0[:, :-1]).sum(-1)  # (fp32 sums of at most 9 rows of weights up to G)
+        assert float((grown - (G if inside else 0)).abs().max()) <= (2e-5 * G if inside else 0.0)

@@ -238,3 +238,22 @@ def test_paged_step_outside_its_window(gpu, kv, nq, nkv, d):
         G = nq // nkv
         grown = a[:, -1] + (a[:, :-1] - a0[:, :-1]).sum(-1)  # (fp32 sums of at most 9 rows of weights up to G)
         assert float((grown - (G if inside else 0)).abs().max()) <= (2e-5 * G if inside else 0.0)
+
+
+def test_plain_prompt_rows_past_a_grid(gpu):
+    """The same path without scores, at a head dim that no prefill kernel tiles."""
+    nq, nkv, d, m = 8, 4, 34, 17000
+    g, scale = gen(73), 1 / math.sqrt(d)
+    q = randn(g, m, nq, d, sigma=3.0)
+    Kc, K = ref.make_cache(randn(g, m, nkv, d), "f32")
+    Vc, V = ref.make_cache(randn(g, m, nkv, d), "f32")
+    O = torch.full((m, nq, d), math.nan, device="cuda")
+    attn.set_prefill_presplit(False)
+    try:
+        attn.attn_prefill_gqa(q, Kc, Vc, O, nq, nkv, m, m, d, scale, 0)
+    finally:
+        attn.set_prefill_presplit(True)
+    assert bool(torch.isfinite(O).all())
+    some = torch.tensor([0, 1, 16383, 16384, 16385, m - 1], device="cuda")
+    want, _ = ref.attend(q[some], K, V, scale, some, torch.zeros_like(some), some + 1)
+    check_out(O[some], want, ref.tolerance(q[some], K, V, scale, 0.0, None, m))

@@ -437,6 +437,81 @@ int molot_hip_kv_evict_paged(void* K, void* V, float* acc, int32_t* slot_pos,
                              const int32_t* pos, int B, int max_blocks, int max_seq_len, int nkv,
                              int d, int page, int keep, int recent, int kv_dtype, void* stream);
 
+/* ---- Ragged batches: packed rows of sequences of different lengths ----
+ * (no reference counterpart: a Runner has one sequence, forward.h:48-51.)  One
+ * call takes sequences that bring one new row, a few or a prompt: the rows of all
+ * are packed, sequence after sequence, row_start[b] .. row_start[b + 1] - 1 those of
+ * sequence b, and kv_lens[b] counts them.  All index arrays are device int32; what
+ * they hold is known to the device alone, so that a serving loop needs no copy to the
+ * host and can be captured in a graph.  T is a bound of the rows (the arrays' length):
+ * rows from row_start[B] on are left as they are.  num_blocks: blocks of the pool;
+ * ids outside it are never followed (such a row is not stored, and attention over it
+ * unspecified).
+ *
+ * molot_hip_ragged_plan makes those arrays from the requests' lengths.  Sequence b has
+ * seq_lens[b] rows cached and brings counts[b] >= 0.
+ *   kv_lens[b]      rows with the new ones (may be seq_lens itself);
+ *   row_start       [B + 1], as above;
+ *   row_seq         [max_rows] the row's sequence (-1 past the last);
+ *   row_pos         its position: pos[b] + i of the sequence's row i (pos NULL: its
+ *                   slot seq_lens[b] + i; 0 past the last row);
+ *   row_slot        its place in the pool: block * page + slot % page (-1 past the last
+ *                   row, or where the table's entry is no block of the pool);
+ *   status          [1] 0, or why the batch was not planned: MOLOT_EINVAL (a negative
+ *                   count or length, more rows than max_blocks * page, a free list
+ *                   that is none), MOLOT_E2BIG (more rows than max_rows), MOLOT_ENOSPC
+ *                   (not enough blocks).  Then kv_lens = seq_lens, free_left =
+ *                   free_count, the table is as it was, and the batch has no rows.
+ * free_blocks [num_blocks] is the free list, a stack of free_count[0] ids: new blocks
+ * come off its top, sequence after sequence, and go into block_table[B][max_blocks];
+ * free_left[0] (may be free_count itself) is what is left.  done (NULL: none): where
+ * done[b] != 0 the sequence is finished: its blocks go on the stack first (in
+ * order), and counts[b] rows start it anew.  Entries of the stack past free_left, and
+ * of the table past a sequence's blocks, hold anything.  With kv_lens and free_left of
+ * their own a plan commits nothing until the caller takes them for the next one's
+ * seq_lens and free_count.  free_blocks NULL (then done too): the table holds the new
+ * rows' blocks already, and only the maps are made.
+ * B, max_rows and max_blocks up to 2^20 (MOLOT_ENOTSUP past it). */
+int molot_hip_ragged_plan(const int32_t* counts, const int32_t* done, const int32_t* pos,
+                          const int32_t* seq_lens, int32_t* kv_lens, int32_t* block_table,
+                          int32_t* free_blocks, const int32_t* free_count, int32_t* free_left,
+                          int B, int max_blocks, int page, int num_blocks, int max_rows,
+                          int32_t* row_start, int32_t* row_seq, int32_t* row_pos,
+                          int32_t* row_slot, int32_t* status, void* stream);
+
+/* Norms (as molot_hip_decode_step_norm: NULL weights and v_norm = 0 skip them), RoPE and
+ * append of the packed rows: row r of q[T][nq][d] in place and of k_new[T][nkv][d] at
+ * row_pos[r], k and v stored at row_slot[r] of the pages.  A row whose slot is not
+ * in the pool is left as it is.  k_new and v_new NULL: q alone (a layer that reads another
+ * layer's KV).  No two rows of a call have one slot. */
+int molot_hip_rope_append_ragged(float* q, const float* k_new, const float* v_new, void* K, void* V,
+                                 const int32_t* row_pos, const int32_t* row_slot, int T,
+                                 int num_blocks, int nq, int nkv, int d, int page,
+                                 const float* q_norm, const float* k_norm, int v_norm, float eps,
+                                 const float* inv_freq, int kv_dtype, void* stream);
+
+/* Attention of the packed rows over the paged cache, causal by slots: row i of sequence
+ * b is at slot s = kv_lens[b] - count + i, count its rows, and attends slots [t0, s],
+ * t0 = max(0, s - window + 1) for window > 0 (else 0).  softcap and slopes as the scored
+ * entries take them (0 and NULL: plain scores), i the slot.  Q and O [T][nq][d], O not Q.
+ * max_len: a bound of every kv_lens[b] (the longest, or a table's capacity); slots past
+ * it are left out. */
+int molot_hip_attn_ragged(const float* Q, const void* K, const void* V, float* O,
+                          const int32_t* block_table, const int32_t* kv_lens,
+                          const int32_t* row_start, int T, int B, int max_blocks, int num_blocks,
+                          int max_len, int nq, int nkv, int d, int page, float scale, int window,
+                          float softcap, const float* slopes, int kv_dtype, void* stream);
+
+/* One layer of a ragged batch: molot_hip_rope_append_ragged, then molot_hip_attn_ragged
+ * of the rotated q into O. */
+int molot_hip_step_ragged(float* q, const float* k_new, const float* v_new, void* K, void* V,
+                          float* O, const int32_t* block_table, const int32_t* kv_lens,
+                          const int32_t* row_start, const int32_t* row_pos, const int32_t* row_slot,
+                          int T, int B, int max_blocks, int num_blocks, int max_len, int nq, int nkv,
+                          int d, int page, const float* q_norm, const float* k_norm, int v_norm,
+                          float eps, const float* inv_freq, float scale, int window, float softcap,
+                          const float* slopes, int kv_dtype, void* stream);
+
 /* The exponential of the split-K merges (the chunk weights e^(m_c - M),
  * the device expf), applied elementwise (x, y device [n]).  Counterpart of
  * exp_avx512_ps, include/molot/norm.h:35-47, exposed so its accuracy can be

@@ -29,6 +29,7 @@ __all__ = [
     "decode_step_paged_scored", "attn_prefill_scored", "attn_prefill_paged_scored",
     "prefill_step_scored", "prefill_step_paged_scored", "kv_track", "kv_track_paged", "kv_evict",
     "kv_evict_paged", "alibi_slopes", "document_starts",
+    "ragged_plan", "rope_append_ragged", "attn_ragged", "step_ragged",
     "last_plan", "set_split_chunk", "attn_prefill_gqa", "prefill_step", "KVCache", "kv_dtype_of",
 ]
 
@@ -781,6 +782,124 @@ def kv_evict_paged(K, V, acc, slot_pos, block_table, seq_lens, pos, B, max_block
         _ptr(K), _ptr(V), _ptr(acc), _ptr(slot_pos), _ptr(block_table), _ptr(seq_lens), _ptr(pos),
         B, max_blocks, max_len, nkv, d, page, int(keep), int(recent), kvd, _stream()),
         "kv_evict_paged")
+
+
+# --- ragged batches: packed rows of sequences of different lengths -----------
+
+
+def ragged_plan(counts, seq_lens, kv_lens, block_table, B, max_blocks, page, num_blocks, max_rows,
+                row_start, row_seq, row_pos, row_slot, status, free_blocks=None, free_count=None,
+                free_left=None, done=None, pos=None):
+    """The index arrays of a ragged batch from how many rows every sequence brings
+    (counts) and has cached (seq_lens), all device int32: the blocks of finished
+    sequences (done) back on the free list and new ones off it, the tables, lengths
+    and the rows' maps; see molot_hip_ragged_plan.  Whether the batch fits is known to
+    the device alone: status [1] holds 0 or the reason, and a batch that does not fit
+    has no rows.  Without free_blocks the table holds the rows' blocks already."""
+    i32 = torch.int32
+    for t, name, n in ((counts, "counts", B), (seq_lens, "seq_lens", B), (kv_lens, "kv_lens", B),
+                       (block_table, "block_table", B * max_blocks), (row_start, "row_start", B + 1),
+                       (row_seq, "row_seq", max_rows), (row_pos, "row_pos", max_rows),
+                       (row_slot, "row_slot", max_rows), (status, "status", 1)):
+        _need(t, name, i32, n)
+    if free_blocks is None:
+        if done is not None or free_count is not None or free_left is not None:
+            raise ValueError("done, free_count and free_left need free_blocks")
+    else:
+        _need(free_blocks, "free_blocks", i32, num_blocks)
+        _need(free_count, "free_count", i32, 1)
+        _need(free_left, "free_left", i32, 1)
+    for t, name in ((done, "done"), (pos, "pos")):
+        if t is not None:
+            _need(t, name, i32, B)
+    check(_lib.load().molot_hip_ragged_plan(
+        _ptr(counts), _ptr(done), _ptr(pos), _ptr(seq_lens), _ptr(kv_lens), _ptr(block_table),
+        _ptr(free_blocks), _ptr(free_count), _ptr(free_left), int(B), int(max_blocks), int(page),
+        int(num_blocks), int(max_rows), _ptr(row_start), _ptr(row_seq), _ptr(row_pos),
+        _ptr(row_slot), _ptr(status), _stream()), "ragged_plan")
+
+
+def _need_pool(K, V, num_blocks, nkv, d, page):
+    kvd = kv_dtype_of(K)
+    _need(K, "K", _KV_DTYPES, num_blocks * _block_units(kvd, nkv, d, page))
+    _need(V, "V", K.dtype, num_blocks * _block_units(kvd, nkv, d, page))
+    return kvd
+
+
+def _need_ragged(block_table, kv_lens, row_start, B, max_blocks):
+    _need(block_table, "block_table", torch.int32, B * max_blocks)
+    _need(kv_lens, "kv_lens", torch.int32, B)
+    _need(row_start, "row_start", torch.int32, B + 1)
+
+
+def rope_append_ragged(q, k_new, v_new, K, V, row_pos, row_slot, T, num_blocks, nq, nkv, d, page,
+                       inv_freq, q_norm=None, k_norm=None, v_norm=False, eps=1e-6):
+    """Norms, RoPE and append of T packed rows: q [T][nq][d] in place, k_new and v_new
+    [T][nkv][d] into the pool's slots row_slot, at the positions row_pos (ragged_plan's).
+    k_new, v_new, K and V None: q alone (a layer that reads another layer's KV)."""
+    if k_new is None:
+        if v_new is not None or K is not None or V is not None:
+            raise ValueError("rope_append_ragged: k_new, v_new, K and V go together")
+        kvd = KV_F32
+    else:
+        kvd = _need_pool(K, V, num_blocks, nkv, d, page)
+        _need(k_new, "k_new", torch.float32, T * nkv * d)
+        _need(v_new, "v_new", torch.float32, T * nkv * d)
+    _need(q, "q", torch.float32, T * nq * d)
+    _need(row_pos, "row_pos", torch.int32, T)
+    _need(row_slot, "row_slot", torch.int32, T)
+    _need_table(inv_freq, d)
+    _need_norms(q_norm, k_norm, d)
+    check(_lib.load().molot_hip_rope_append_ragged(
+        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(K), _ptr(V), _ptr(row_pos), _ptr(row_slot), int(T),
+        int(num_blocks), nq, nkv, d, page, _ptr(q_norm), _ptr(k_norm), int(bool(v_norm)), float(eps),
+        _ptr(inv_freq), kvd, _stream()), "rope_append_ragged")
+    return q
+
+
+def attn_ragged(Q, K, V, O, block_table, kv_lens, row_start, T, B, max_blocks, num_blocks, max_len,
+                nq, nkv, d, page, scale, window=0, softcap=0.0, slopes=None):
+    """Attention of the packed rows Q [T][nq][d] of B sequences over their pages, causal
+    by slots; sequences of one row, a few or a prompt in one call.  max_len bounds
+    kv_lens.  Nothing is copied to the host; see molot_hip_attn_ragged."""
+    kvd = _need_pool(K, V, num_blocks, nkv, d, page)
+    _need(Q, "Q", torch.float32, T * nq * d)
+    _need(O, "O", torch.float32, T * nq * d)
+    _need_ragged(block_table, kv_lens, row_start, B, max_blocks)
+    _need_scoring(slopes, nq)
+    check(_lib.load().molot_hip_attn_ragged(
+        _ptr(Q), _ptr(K), _ptr(V), _ptr(O), _ptr(block_table), _ptr(kv_lens), _ptr(row_start), int(T),
+        int(B), int(max_blocks), int(num_blocks), int(max_len), nq, nkv, d, page, float(scale),
+        int(window), float(softcap), _ptr(slopes), kvd, _stream()), "attn_ragged")
+    return O
+
+
+def step_ragged(q, k_new, v_new, K, V, O, block_table, kv_lens, row_start, row_pos, row_slot, T, B,
+                max_blocks, num_blocks, max_len, nq, nkv, d, page, inv_freq, scale, window=0,
+                softcap=0.0, slopes=None, q_norm=None, k_norm=None, v_norm=False, eps=1e-6):
+    """One layer of a ragged batch: rope_append_ragged, then attn_ragged (k_new, v_new
+    None: nothing appended, the pages are another layer's)."""
+    kvd = _need_pool(K, V, num_blocks, nkv, d, page)
+    if (k_new is None) != (v_new is None):
+        raise ValueError("step_ragged: k_new and v_new go together")
+    if k_new is not None:
+        _need(k_new, "k_new", torch.float32, T * nkv * d)
+        _need(v_new, "v_new", torch.float32, T * nkv * d)
+    _need(q, "q", torch.float32, T * nq * d)
+    _need(O, "O", torch.float32, T * nq * d)
+    _need(row_pos, "row_pos", torch.int32, T)
+    _need(row_slot, "row_slot", torch.int32, T)
+    _need_ragged(block_table, kv_lens, row_start, B, max_blocks)
+    _need_table(inv_freq, d)
+    _need_norms(q_norm, k_norm, d)
+    _need_scoring(slopes, nq)
+    check(_lib.load().molot_hip_step_ragged(
+        _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(K), _ptr(V), _ptr(O), _ptr(block_table),
+        _ptr(kv_lens), _ptr(row_start), _ptr(row_pos), _ptr(row_slot), int(T), int(B),
+        int(max_blocks), int(num_blocks), int(max_len), nq, nkv, d, page, _ptr(q_norm), _ptr(k_norm),
+        int(bool(v_norm)), float(eps), _ptr(inv_freq), float(scale), int(window), float(softcap),
+        _ptr(slopes), kvd, _stream()), "step_ragged")
+    return O
 
 
 def vexp(x: torch.Tensor, y: torch.Tensor | None = None) -> torch.Tensor:

@@ -59,6 +59,14 @@ _SIGS = {
     "molot_hip_kv_track_paged": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "molot_hip_kv_evict": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "molot_hip_kv_evict_paged": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
+    "molot_hip_ragged_plan": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P,
+                              _P, _P],
+    "molot_hip_rope_append_ragged": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I,
+                                     _F, _P, _I, _P],
+    "molot_hip_attn_ragged": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I,
+                              _F, _P, _I, _P],
+    "molot_hip_step_ragged": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
+                              _I, _I, _P, _P, _I, _F, _P, _F, _I, _F, _P, _I, _P],
     "molot_hip_rope_apply": [_P, _I, _I, _I, _P, _P],
     "molot_hip_rope_append": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P],
     "molot_hip_attn_decode_gqa_cache": [_P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P],

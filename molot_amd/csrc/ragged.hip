@@ -639,8 +639,6 @@ struct Layout {
   }
 };
 
-using RaggedFn = void (*)(RaggedArgs);
-
 int launch_attention(RaggedArgs a, void* stream) {
   LaunchLock lock(g_launch_mu);
   const int cus = num_cus();
@@ -652,17 +650,30 @@ int launch_attention(RaggedArgs a, void* stream) {
                    : D == 128 ? ragged_merge_kernel<2>
                    : D == 256 ? ragged_merge_kernel<4> : ragged_merge_kernel<8>;
   int threads = 64 * kValuWaves;
-  a.qs = a.ql = kValuWaves;
+  a.qs = a.ql = a.slot_rows = kValuWaves;
   a.few = 0x7FFFFFFF;
   a.min_keys = 256;
-  a.target = (8 * cus + a.nkv - 1) / a.nkv;
-  a.slot_rows = a.qs;
-  // Bounds: at most rows / ql + 1 tiles of a sequence with wide ones, few / qs + 1 of the
-  // others; a tile's splits add target in all, and each split tile has at most twice its
-  // share of them (ragged_units_kernel).
+  int per_cu = 8;
+  // (the matrix-core kernel's offsets within a block are of 32 bits)
+  const int64_t block = ((int64_t)a.nkv << a.page_shift) * (4 * a.d);
+  if (a.d <= 256 && a.d % 8 == 0 && block <= 0x7FFFFFFF) {
+    const RaggedTile t = ragged_tile(a.d, a.kv_dtype, a.softcap > 0.f || a.slopes);
+    attend = t.fn;
+    threads = t.threads;
+    a.qs = kRaggedNarrow;
+    a.ql = kRaggedWide;
+    a.few = 2 * kRaggedNarrow;
+    // (a tile holds no more rows than the batch)
+    a.slot_rows = (int64_t)a.T * a.G <= a.few ? kRaggedNarrow : kRaggedWide;
+    per_cu = 2;
+  }
+  a.target = (per_cu * cus + a.nkv - 1) / a.nkv;
+  // Bounds: a sequence of R rows r has at most R / ql + 1 wide tiles, or R / qs + 1 narrow
+  // ones where R <= few; its splits add at most its share of target, and a split tile has
+  // at most twice that (ragged_units_kernel).
   const int64_t R = (int64_t)a.T * a.G;
-  const int seqs = std::min(a.T, a.B);
-  const int64_t tiles = R / std::min(a.qs, a.ql) + seqs;
+  const int64_t seqs = std::min(a.T, a.B);
+  const int64_t tiles = std::min(R / a.qs, R / a.ql + seqs * (a.few / a.qs)) + seqs;
   if (R > 0x3FFFFFFF || (tiles + a.target) * a.nkv > 0x7FFFFFFF) return MOLOT_ENOTSUP;
   a.max_units = (int)(tiles + a.target);
   a.max_parts = a.cap > a.min_keys ? 2 * a.target : 0;  // (else no tile is split)

@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "device_util.hpp"
 #include "molot_amd/attn_hip.h"
@@ -55,6 +56,16 @@ struct RaggedArgs {
   int max_units, max_parts;
 };
 
+// The matrix-core kernel of a head dim (a multiple of 8 up to 256) and cache type, and
+// the threads of its workgroups: ragged_tile.hip.
+using RaggedFn = void (*)(RaggedArgs);
+struct RaggedTile {
+  RaggedFn fn;
+  int threads;
+};
+constexpr int kRaggedWide = 128, kRaggedNarrow = 32;  // rows of its tiles
+RaggedTile ragged_tile(int d, int kv_dtype, bool scored) __attribute__((visibility("hidden")));
+
 namespace {
 
 // The new rows of sequence b as the kernels take them, whatever the arrays hold: first
@@ -81,13 +92,20 @@ __device__ __forceinline__ int ragged_block(const RaggedArgs& a, int b, int t) {
   return (unsigned)id < (unsigned)a.num_blocks ? id : 0;
 }
 // Elements (Q8: bytes) of row t of KV head h from the pool's start, and a Q8 row's scale.
-__device__ __forceinline__ int64_t ragged_row(const RaggedArgs& a, int blk, int h, int t,
-                                              int64_t& scale) {
+template <typename T>
+__device__ __forceinline__ int64_t ragged_row_of(const RaggedArgs& a, int blk, int h, int t,
+                                                 int64_t& scale) {
   const int page = 1 << a.page_shift, sl = t & (page - 1);
-  if (a.kv_dtype != MOLOT_KV_Q8) return (((int64_t)blk * a.nkv + h) * page + sl) * a.d;
+  if constexpr (!std::is_same<T, q8_t>::value)
+    return (((int64_t)blk * a.nkv + h) * page + sl) * a.d;
   const int64_t rows = (int64_t)a.nkv * page, b0 = (int64_t)blk * rows * (a.d + 4);
   scale = b0 + rows * a.d + 4 * ((int64_t)h * page + sl);
   return b0 + ((int64_t)h * page + sl) * a.d;
+}
+__device__ __forceinline__ int64_t ragged_row(const RaggedArgs& a, int blk, int h, int t,
+                                              int64_t& scale) {
+  return a.kv_dtype == MOLOT_KV_Q8 ? ragged_row_of<q8_t>(a, blk, h, t, scale)
+                                   : ragged_row_of<float>(a, blk, h, t, scale);
 }
 
 // The scores past the product of query row r (head h*G + g) at its slot.

@@ -1,0 +1,629 @@
+// Attention of ragged batches on the matrix cores, head dims up to 256 that are
+// multiples of 8.
+//
+// A workgroup takes one unit (ragged.hpp) of one KV head: 32 query rows a wave on the
+// 32 columns of v_mfma_f32_32x32x16_f16, S^T = K . Q^T, the softmax in registers (a lane
+// holds one row and 16 keys of a tile of 32, its row's other 16 in lane ^ 32), and
+// O^T += V^T . P^T with P where the score accumulator left it (V^T by transposed LDS
+// reads in the same key order).  q and p are two fp16 pieces, K and V row-scaled pieces
+// (two of an fp32 row, one of a bf16 or Q8 row): the products of prefill_narrow.hip.  There
+// the pieces come from a launch of their own over one sequence's keys; here the keys of a
+// batch are many sequences', most of them read by few rows, so every workgroup makes
+// the pieces of its own tiles on their way from the pages to LDS.
+//
+// Wide tiles (prompts): 128 rows, 4 row groups of waves by KG key groups that take the
+// tiles of 32 keys in turn; the workgroup stages an interval of KG tiles together, double
+// buffered, the next interval's loads in flight while one is used.
+// Narrow tiles (one row, drafts): 32 rows, every wave a key group by itself with
+// its own LDS, so no wave waits for another: a tile's K, then its V, take the same place.
+// The key groups' (m, l, o) are merged through LDS at the end.
+#include "ragged.hpp"
+
+#include <type_traits>
+
+#include "prefill_wide.hpp"
+
+namespace {
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Maximum over aligned groups of N lanes (8, 16 or 32), as group_max.
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_u(unsigned x) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false);
+}
+template <int N>
+__device__ __forceinline__ unsigned group_umax(unsigned v) {
+  v = max(v, dpp_u<0xB1>(v));
+  v = max(v, dpp_u<0x4E>(v));
+  v = max(v, dpp_u<0x141>(v));
+  if constexpr (N >= 16) v = max(v, dpp_u<0x140>(v));
+  if constexpr (N >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(r[0], r[1]);
+  }
+  return v;
+}
+
+// Eight elements of a cached row as loaded, and (Q8) the row's scale in every lane of it.
+template <typename T>
+struct Raw;
+template <>
+struct Raw<float> {
+  f32x4 x[2];
+};
+template <>
+struct Raw<bf16_t> {
+  u32x4 x;
+};
+template <>
+struct Raw<q8_t> {
+  u32x2 x;
+  float scale;
+};
+
+// The pieces of eight elements, and the unit of their row: x = piece * unit.  LPR lanes
+// hold the row.  A NaN unit marks a row that the pieces cannot hold (own_mark).
+template <int NP>
+struct Pieces {
+  u32x4 p[NP];
+  float unit;
+};
+template <int LPR>
+__device__ __forceinline__ Pieces<2> make_pieces(const Raw<float>& r, int kv) {
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(r.x[i][e]) & 0x7FFFFFFFu);
+  m = group_umax<LPR>(m);
+  const float top = __uint_as_float(m);
+  const int shift = kv ? f16_vrow_shift(top) : f16_row_shift(top);
+  const float sc = ldexpf(1.f, shift);
+  Pieces<2> out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t hi, lo;
+    mix_split(r.x[i >> 1][2 * (i & 1)], r.x[i >> 1][2 * (i & 1) + 1], sc, hi, lo);
+    out.p[0][i] = hi;
+    out.p[1][i] = lo;
+  }
+  out.unit = (kv ? f16_vrow_unit(top, shift) : f16_row_unit(shift)) +
+             own_mark(top, m >= 0x7F800000u ? NAN : 0.f, kv);
+  return out;
+}
+// bf16 to fp16 by its bits: with the row's largest exponent field e, off = max(e - 30, 0)
+// is taken from every exponent (fp16's 1 .. 30 then hold 30 binades, each value with
+// all its 8 bits; smaller ones, 2^-29 of the largest, go to 0 or near it) and the
+// mantissa moves up by 3: 2.5 instructions a pair where a conversion through fp32 takes 7.
+template <int LPR>
+__device__ __forceinline__ Pieces<1> make_pieces(const Raw<bf16_t>& r, int kv) {
+  uint32_t t[4];  // (scalars: a bit cast of a vector's element would take the first)
+  u16x2 m2 = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[i] = r.x[i] & 0x7FFF7FFFu;
+    m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(u16x2, t[i]));
+  }
+  const unsigned m = group_umax<LPR>(max((unsigned)m2[0], (unsigned)m2[1]));
+  const int e = (int)(m >> 7);
+  const unsigned off = (unsigned)max(e - 30, 0);
+  const unsigned short sub = (unsigned short)(off << 7);
+  const u16x2 sub2 = {sub, sub};
+  Pieces<1> out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    u16x2 y = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, t[i]), sub2);
+    y = y << (unsigned short)3;
+    out.p[0][i] = (r.x[i] & 0x80008000u) | __builtin_bit_cast(uint32_t, y);
+  }
+  const float top = __uint_as_float(m << 16);
+  const float unit = kv && m == 0 ? 0.f : __uint_as_float((off + 15u) << 23);  // 2^(off - 112)
+  out.unit = unit + own_mark(top, e == 255 ? NAN : 0.f, kv);
+  return out;
+}
+// Codes are exact in fp16: 0x6400 + (code ^ 0x80) is 1152 + code.
+template <int LPR>
+__device__ __forceinline__ Pieces<1> make_pieces(const Raw<q8_t>& r, int kv) {
+  Pieces<1> out;
+  const f16x2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = r.x[i >> 1] ^ 0x80808080u;
+    const uint32_t b = __builtin_amdgcn_perm(0x64646464u, x, i & 1 ? 0x04030402u : 0x04010400u);
+    out.p[0][i] = __builtin_bit_cast(uint32_t, (f16x2)(__builtin_bit_cast(f16x2, b) - bias));
+  }
+  float unit = r.scale;
+  if (kv) {  // a row of zeros weighs nothing whatever its scale
+    const unsigned any = group_umax<LPR>(min(r.x[0] | r.x[1], 1u));
+    unit = any ? unit : 0.f;
+  }
+  const bool out_of = !(unit >= 0.f) || unit > kOwnMaxK * 0.0078125f || (kv && unit > 0.f && unit < kOwnMinV);
+  out.unit = unit + (out_of ? NAN : 0.f);
+  return out;
+}
+
+// SC: scores past the product (a cap, slopes).
+template <int D, typename T, bool SC>
+struct Tile {
+  static constexpr int NW = D <= 128 ? 8 : 4;  // waves: at d = 256 one a SIMD, with its registers
+  static constexpr int NT = 64 * NW;
+  static constexpr int NP = sizeof(T) == 4 ? 2 : 1;
+  static constexpr int KT = 32;
+  static constexpr int RGW = 4, KGW = NW / 4;  // wide tiles: row and key groups
+  static constexpr int RB = 2 * D;             // bytes of a staged row of one piece
+  static constexpr int PB = KT * RB;           // of a tile's piece
+  static constexpr int TB = NP * PB;           // of a tile
+  static constexpr int LPR = D / 8;            // lanes of a row
+  static constexpr int CW = KGW * KT * LPR / NT;  // chunks of 8 elements a thread, wide
+  static constexpr int CN = KT * LPR / 64;        // and a lane, narrow
+  static constexpr int kTiles = 4 * KGW * TB;  // = NW * TB: the narrow tiles' places
+  static constexpr int kMerge = NW / 2 * KT * D * 4;
+  static constexpr int kData = kTiles > kMerge ? kTiles : kMerge;
+  static constexpr int kUnits = NW * 2 * KT * 4;  // narrow: [wave][K, V][32]; wide: 4 * KGW * 32
+  static constexpr int kStats = NW / 2 * KT * 16;
+  static constexpr int LDS = kData + (kUnits > kStats ? kUnits : kStats);
+  static_assert(kTiles == NW * TB && 4 * KGW * KT * 4 <= kUnits, "both kinds share the LDS");
+
+  using raw_t = Raw<T>;
+
+  // Where rows lie, in bytes: block blk at blk * block, row sl of KV head h of it at
+  // head + sl * row, and a Q8 row's scale at scales + 4 * sl.  (The host takes the blocks
+  // that fit 31 bits.)
+  struct Pages {
+    unsigned block, head, row, scales;
+    int mask;
+  };
+  __device__ static __forceinline__ Pages pages(const RaggedArgs& a, int h) {
+    constexpr bool Q8 = std::is_same<T, q8_t>::value;
+    const unsigned page = 1u << a.page_shift, rows = a.nkv * page;
+    Pages p;
+    p.row = a.d * (unsigned)sizeof(T);
+    p.block = rows * (p.row + (Q8 ? 4 : 0));
+    p.head = h * page * p.row;
+    p.scales = rows * a.d + 4 * h * page;
+    p.mask = (int)page - 1;
+    return p;
+  }
+  // Eight elements at byte `at` of row t in block blk.  (Lanes past d take the row's first:
+  // they meet zeros of q, or columns that are not stored.)  once: no other workgroup
+  // reads the row soon.
+  __device__ static __forceinline__ void load(const Pages& p, const char* pool, int blk, int t, unsigned at,
+                                              bool once, raw_t& r) {
+    const unsigned sl = (unsigned)(t & p.mask);
+    const char* b = pool + (uint64_t)(unsigned)blk * p.block;
+    const char* x = b + (p.head + sl * p.row + at);
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x4* v = reinterpret_cast<const f32x4*>(x) + i;
+        r.x[i] = once ? __builtin_nontemporal_load(v) : *v;
+      }
+    } else if constexpr (std::is_same<T, bf16_t>::value) {
+      const u32x4* v = reinterpret_cast<const u32x4*>(x);
+      r.x = once ? __builtin_nontemporal_load(v) : *v;
+    } else {
+      r.x = *reinterpret_cast<const u32x2*>(x);
+      r.scale = *reinterpret_cast<const float*>(b + (p.scales + 4 * sl));
+    }
+  }
+  // N chunks of a thread into LDS: chunk i is unit j of row r + STEP*i (STEP a power of two
+  // past r) of the tile, at(i) the tile's place; the lanes with j = 0 leave the rows' units.
+  template <int N, int STEP, typename AT, typename UNITS>
+  __device__ static __forceinline__ void store(const raw_t (&raw)[N], int kv, int r, int j, AT&& at,
+                                               UNITS&& units) {
+    const int base = r * RB + 16 * (j ^ (kv ? wv_f<D>(r) : wk_f<D>(r)));
+    float unit[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const Pieces<NP> x = make_pieces<LPR>(raw[i], kv);
+      unit[i] = x.unit;
+      // (the swizzle of row r + STEP*i is r's and STEP*i's by exclusive or)
+      char* to = at(i) + ((base ^ (16 * (kv ? wv_f<D>(STEP * i) : wk_f<D>(STEP * i)))) + STEP * i * RB);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) *reinterpret_cast<u32x4*>(to + p * PB) = x.p[p];
+    }
+    if (j == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) units(i)[r + STEP * i] = unit[i];
+    }
+  }
+};
+
+// A wave's rows over its tiles.
+template <int D, typename T, bool SC>
+struct Rows {
+  using C = Tile<D, T, SC>;
+  static constexpr int QS = D / 16, DB = D / 32, NP = C::NP, RB = C::RB, PB = C::PB;
+  f16x8_t qh[QS], ql[QS];
+  float qunit;
+  f32x16 o[DB], s;
+  RowState rs;
+  uint32_t yh[8], yl[8];
+  float fac, mark;
+  RowScore score;
+  int lo, hi;  // the row's keys of this unit
+  int room;
+
+  __device__ __forceinline__ void init(const RaggedArgs& a, const RaggedUnit& u, const RaggedSeq& sq, int h,
+                                       int r, int hh) {
+    const bool rv = r < sq.rows * a.G;
+    const int m = rv ? r / a.G : 0, g = rv ? r - m * a.G : 0, slot = sq.slot0 + m;
+    // (a row past the last: any keys, not stored)
+    lo = rv ? max(ragged_lo(a, slot), u.lo) : 0;
+    hi = rv ? min(ragged_hi(a, slot), u.hi) : 0x7FFFFFFF;
+    const float* qr = a.q + (((int64_t)sq.start + m) * a.nq + h * a.G + g) * a.d;
+    const float qsc = a.scale * kLog2e;
+    // (read twice, the largest first: all of the row at once would take 4 * QS registers)
+    auto eight = [&](int k, float (&x)[8]) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int e0 = 16 * k + 8 * hh + 4 * i;
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+        if (rv && e0 < a.d) y = *reinterpret_cast<const f32x4*>(qr + e0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e] * qsc;
+      }
+    };
+    float qm = 0.f;
+#pragma unroll
+    for (int k = 0; k < QS; ++k) {
+      float x[8];
+      eight(k, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qm = fmaxf(qm, fabsf(x[e]));
+    }
+    asm volatile("" : "+v"(qr));
+    const int shift = f16_row_shift(max_xor32(qm));
+    qunit = f16_row_unit(shift);
+#pragma unroll
+    for (int k = 0; k < QS; ++k) {
+      float x[8];
+      eight(k, x);
+      uint32_t h4[4], l4[4];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) split2h(x[e], x[e + 1], shift, h4[e / 2], l4[e / 2]);
+      qh[k] = __builtin_bit_cast(f16x8_t, u32x4{h4[0], h4[1], h4[2], h4[3]});
+      ql[k] = __builtin_bit_cast(f16x8_t, u32x4{l4[0], l4[1], l4[2], l4[3]});
+    }
+    if constexpr (SC) score = ragged_score(a, h * a.G + g, slot);
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+    fac = 1.f;
+    mark = 0.f;
+    room = wide_room(u.hi - u.lo);
+  }
+
+  // S^T of a tile: keys 8*(i/4) + 4*hh + i%4.  The products with a low piece have a sum of
+  // their own: small beside the others', which alone then rounds at the scores' size.
+  __device__ __forceinline__ void scores(const char* tile, int c32, int hh) {
+    const char* kr = tile + c32 * RB;
+    const int kx = 16 * (hh ^ wk_f<D>(c32));
+    f32x16 low;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = low[i] = 0.f;
+    f16x8_t k[2][2][NP];
+    auto read_k = [&](int k0) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          k[(k0 >> 1) & 1][j][p] =
+              *reinterpret_cast<const f16x8_t*>(kr + p * PB + (kx ^ (32 * (k0 + j))));
+    };
+    read_k(0);
+#pragma unroll
+    for (int k0 = 0; k0 < QS; k0 += 2) {
+      if (k0 + 2 < QS) read_k(k0 + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      auto& c = k[(k0 >> 1) & 1];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        s = mfma32_f16(c[j][0], qh[k0 + j], s);
+        low = mfma32_f16(c[j][0], ql[k0 + j], low);
+        if constexpr (NP == 2) low = mfma32_f16(c[j][1], qh[k0 + j], low);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] += low[i];
+  }
+
+  __device__ __forceinline__ void softmax(const float* ku_, const float* vu_, int tk, int c32, int hh) {
+    float x[16], ku[16], vu[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(ku_ + 4 * hh + 8 * i);
+      const f32x4 z = *reinterpret_cast<const f32x4*>(vu_ + 4 * hh + 8 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[4 * i + e] = s[4 * i + e];
+        ku[4 * i + e] = y[e];
+        vu[4 * i + e] = z[e];
+      }
+    }
+    mark = fmaf(ku_[c32] + vu_[c32], 0.f, mark);
+    const bool full = __builtin_amdgcn_ballot_w64(tk < lo || tk + C::KT > hi) == 0;
+    auto slot = [&](int e) { return tk + 8 * (e >> 2) + 4 * hh + (e & 3); };
+    auto gmax = [](float v) { return max_xor32(v); };
+    auto dead = [&](int e) {
+      const int t = slot(e);
+      return t < lo || t >= hi;
+    };
+    if constexpr (SC)
+      fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl,
+                             [&](float (&z)[16], auto&& again) { score.template apply<16>(z, slot, again); },
+                             room);
+    else
+      fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
+  }
+
+  // O^T += V^T . P^T.  A transposed read's 16-lane group (2*hh + x) takes keys 16j + 8u +
+  // 4hh .. +3 of the block's 16 columns 16x ..: slots 4u + i of the A operand, P's order.
+  __device__ __forceinline__ void pv(char* tile, int lane, int hh) {
+    if (__builtin_amdgcn_ballot_w64(fac != 1.f) != 0) {
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= fac;
+    }
+    const int l16 = lane & 15, rr = 4 * hh + (l16 >> 2);
+    char* vr = tile + rr * RB + 32 * ((lane >> 4) & 1) + 16 * ((l16 & 3) >> 1) + 8 * (l16 & 1);
+    const int vx = 16 * wv_f<D>(rr);
+    f16x8_t av[2][2][NP];
+    auto read_v = [&](int q) {  // step q: key half j, output blocks b0 and b0 + 1
+      const int j = q / (DB / 2), b0 = 2 * (q % (DB / 2));
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          i16x4_t t2[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            t2[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) i16x4_t*)(vr + p * PB + (16 * j + 8 * u) * RB +
+                                                             ((64 * (b0 + b)) ^ vx)));
+          av[q & 1][b][p] =
+              __builtin_bit_cast(f16x8_t, __builtin_shufflevector(t2[0], t2[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    };
+    read_v(0);
+#pragma unroll
+    for (int q = 0; q < DB; ++q) {
+      if (q + 1 < DB) read_v(q + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      const int j = q / (DB / 2), b0 = 2 * (q % (DB / 2));
+      const f16x8_t ph =
+          __builtin_bit_cast(f16x8_t, u32x4{yh[4 * j], yh[4 * j + 1], yh[4 * j + 2], yh[4 * j + 3]});
+      const f16x8_t pl =
+          __builtin_bit_cast(f16x8_t, u32x4{yl[4 * j], yl[4 * j + 1], yl[4 * j + 2], yl[4 * j + 3]});
+      auto& vc = av[q & 1];
+      if constexpr (NP == 2) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) o[b0 + b] = mfma32_f16(vc[b][1], ph, o[b0 + b]);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) o[b0 + b] = mfma32_f16(vc[b][0], pl, o[b0 + b]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) o[b0 + b] = mfma32_f16(vc[b][0], ph, o[b0 + b]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
+template <int D, typename T, bool SC>
+__global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(RaggedArgs a) {
+  using C = Tile<D, T, SC>;
+  constexpr int KT = C::KT, LPR = C::LPR, DB = D / 32;
+  __shared__ __attribute__((aligned(16))) char lds[C::LDS];
+  float* const units = reinterpret_cast<float*>(lds + C::kData);
+
+  const int ui = blockIdx.x / a.nkv, h = blockIdx.x - ui * a.nkv;
+  if (ui >= a.head->nunits) return;
+  const RaggedUnit u = a.units[ui];
+  const RaggedSeq sq = ragged_seq(a, u.seq);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c32 = lane & 31, hh = lane >> 5;
+  const bool wide = u.wide;
+  const int rg = wide ? w & 3 : 0, kg = wide ? w >> 2 : w;
+  const int r = u.r0 + 32 * rg + c32;
+  const int ntile = (u.hi - u.lo + KT - 1) / KT;
+  const int last = u.hi - 1;  // rows past it read it again (masked)
+  const int32_t* table = a.block_table + (int64_t)u.seq * a.max_blocks;
+  auto block_of = [&](int t) {
+    const int id = table[min(t, last) >> a.page_shift];
+    return (unsigned)id < (unsigned)a.num_blocks ? id : 0;
+  };
+
+  const typename C::Pages pg = C::pages(a, h);
+  Rows<D, T, SC> x;
+  x.init(a, u, sq, h, r, hh);
+
+  if (wide) {
+    const int nint = (ntile + C::KGW - 1) / C::KGW;
+    auto tile_buf = [&](int kv, int bf, int g) { return lds + ((kv * 2 + bf) * C::KGW + g) * C::TB; };
+    auto unit_buf = [&](int kv, int bf, int g) { return units + ((kv * 2 + bf) * C::KGW + g) * KT; };
+    typename C::raw_t kr[C::CW], vr[C::CW];
+    int blk[C::CW];
+    // chunk i of this thread: unit j of row r0 + STEP*i of the interval's KGW tiles in a row
+    constexpr int STEP = C::NT / LPR;
+    const int rr = tid / LPR, j = tid % LPR;
+    const unsigned at = 8 * j < a.d ? 8 * j * (unsigned)sizeof(T) : 0;
+    auto key = [&](int it, int i) { return u.lo + C::KGW * KT * it + rr + STEP * i; };
+    auto blocks = [&](int it) {
+#pragma unroll
+      for (int i = 0; i < C::CW; ++i) blk[i] = block_of(key(it, i));
+    };
+    auto fetch = [&](int it) {
+#pragma unroll
+      for (int i = 0; i < C::CW; ++i) {
+        const int t = min(key(it, i), last);
+        C::load(pg, a.k, blk[i], t, at, false, kr[i]);
+        C::load(pg, a.v, blk[i], t, at, false, vr[i]);
+      }
+    };
+    auto stage = [&](int it) {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        constexpr int N = STEP < KT ? C::CW : 1;  // chunks of a tile
+        if constexpr (STEP < KT) {
+          static_assert(C::KGW == 1, "one tile");
+          C::template store<N, STEP>(kv ? vr : kr, kv, rr, j, [&](int) { return tile_buf(kv, it & 1, 0); },
+                                     [&](int) { return unit_buf(kv, it & 1, 0); });
+        } else {  // a tile or more a chunk
+#pragma unroll
+          for (int i = 0; i < C::CW; ++i) {
+            const typename C::raw_t one[1] = {kv ? vr[i] : kr[i]};
+            const int g = STEP / KT * i + rr / KT;
+            C::template store<1, KT>(one, kv, rr % KT, j, [&](int) { return tile_buf(kv, it & 1, g); },
+                                     [&](int) { return unit_buf(kv, it & 1, g); });
+          }
+        }
+      }
+    };
+    if (nint > 0) {
+      blocks(0);
+      fetch(0);
+      if (nint > 1) blocks(1);
+      stage(0);
+    }
+    __syncthreads();
+    for (int it = 0; it < nint; ++it) {
+      const bool more = it + 1 < nint;
+      if (more) {
+        fetch(it + 1);
+        if (it + 2 < nint) blocks(it + 2);
+      }
+      const int bf = it & 1;
+      x.scores(tile_buf(0, bf, kg), c32, hh);
+      x.softmax(unit_buf(0, bf, kg), unit_buf(1, bf, kg), u.lo + (C::KGW * it + kg) * KT, c32, hh);
+      x.pv(tile_buf(1, bf, kg), lane, hh);
+      if (more) stage(it + 1);
+      lds_barrier();
+    }
+  } else {
+    char* const buf = lds + w * C::TB;
+    float* const ub = units + w * 2 * KT;
+    typename C::raw_t raw[C::CN];
+    const int r_in = lane / LPR, j = lane % LPR;
+    constexpr int RPI = 64 / LPR;  // rows of a load
+    const unsigned at = 8 * j < a.d ? 8 * j * (unsigned)sizeof(T) : 0;
+    auto ids = [&](int t) { return block_of(u.lo + t * KT + c32); };
+    auto fetch = [&](const char* pool, int t, int id) {
+#pragma unroll
+      for (int i = 0; i < C::CN; ++i) {
+        const int rr = r_in + RPI * i;
+        C::load(pg, pool, __shfl(id, rr), min(u.lo + t * KT + rr, last), at, true, raw[i]);
+      }
+    };
+    auto stage = [&](int kv) {
+      C::template store<C::CN, RPI>(raw, kv, r_in, j, [&](int) { return buf; },
+                                    [&](int) { return ub + kv * KT; });
+      asm volatile("" ::: "memory");  // the wave's own LDS: in order
+    };
+    int id = 0, idn = 0;
+    if (w < ntile) {
+      id = ids(w);
+      fetch(a.k, w, id);
+      idn = ids(w + C::NW);
+    }
+    for (int t = w; t < ntile; t += C::NW) {
+      stage(0);
+      fetch(a.v, t, id);
+      x.scores(buf, c32, hh);
+      asm volatile("" ::: "memory");
+      stage(1);
+      id = idn;
+      if (t + C::NW < ntile) {
+        fetch(a.k, t + C::NW, id);
+        idn = ids(t + 2 * C::NW);
+      }
+      x.softmax(ub, ub + KT, u.lo + t * KT, c32, hh);
+      x.pv(buf, lane, hh);
+      asm volatile("" ::: "memory");
+    }
+  }
+
+  // a row that the pieces cannot hold: the unit's rows again, each over its own keys
+  if (__syncthreads_or(x.mark != 0.f)) {
+    const int rows = wide ? 32 * C::RGW : 32;
+    for (int i = w; i < rows; i += C::NW) ragged_own_row<D / 64>(a, u, h, u.r0 + i);
+    return;
+  }
+
+  // the key groups' merge, halves at a time: o in units of 2^m
+  float l = sum_xor32(x.rs.l), m = x.rs.m;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x.o[b][i] = ldexpf(x.o[b][i], -x.rs.wsh);
+  const int rgs = wide ? C::RGW : 1;
+  for (int half = (wide ? C::KGW : C::NW) / 2; half > 0; half /= 2) {
+    const int at = (kg % half) * rgs + rg;
+    f32x4* mo = reinterpret_cast<f32x4*>(lds) + at * DB * 4 * 64 + lane;
+    f32x2* ml = reinterpret_cast<f32x2*>(lds + C::kData) + at * 64 + lane;
+    if (kg >= half && kg < 2 * half) {
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mo[(b * 4 + i) * 64] =
+              f32x4{x.o[b][4 * i], x.o[b][4 * i + 1], x.o[b][4 * i + 2], x.o[b][4 * i + 3]};
+      *ml = f32x2{m, l};
+    }
+    __syncthreads();
+    if (kg < half) {
+      const f32x2 st = *ml;
+      const float M = fmaxf(m, st[0]), f0 = exp2_hw(m - M), f1 = exp2_hw(st[0] - M);
+      m = M;
+      l = l * f0 + st[1] * f1;
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 z = mo[(b * 4 + i) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x.o[b][4 * i + e] = x.o[b][4 * i + e] * f0 + z[e] * f1;
+        }
+    }
+    __syncthreads();
+  }
+  if (kg > 0 || r >= sq.rows * a.G) return;
+  const bool part = u.part >= 0;
+  const int64_t ps = ((int64_t)u.part * a.nkv + h) * a.slot_rows + (r - u.r0);
+  const int mm = r / a.G, g = r - mm * a.G;
+  float* out = part ? a.part_o + ps * D : a.o + (((int64_t)sq.start + mm) * a.nq + h * a.G + g) * a.d;
+  const int dh = part ? D : a.d;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // no key: O = 0
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e0 = 32 * b + 8 * i + 4 * hh;
+      f32x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = part ? x.o[b][4 * i + e] : div_by(x.o[b][4 * i + e], l, inv);
+      if (e0 < dh) *reinterpret_cast<f32x4*>(out + e0) = y;
+    }
+  if (part && hh == 0)
+    *reinterpret_cast<f32x2*>(a.part_ml + 2 * ps) = f32x2{l == 0.f ? -INFINITY : m, l};
+}
+
+template <int D, bool SC>
+RaggedTile tile_of(int kv_dtype) {
+  if (kv_dtype == MOLOT_KV_F32) return {ragged_tile_kernel<D, float, SC>, Tile<D, float, SC>::NT};
+  if (kv_dtype == MOLOT_KV_BF16) return {ragged_tile_kernel<D, bf16_t, SC>, Tile<D, bf16_t, SC>::NT};
+  return {ragged_tile_kernel<D, q8_t, SC>, Tile<D, q8_t, SC>::NT};
+}
+
+}  // namespace
+
+RaggedTile ragged_tile(int d, int kv_dtype, bool scored) {
+  if (d <= 64) return scored ? tile_of<64, true>(kv_dtype) : tile_of<64, false>(kv_dtype);
+  if (d <= 128) return scored ? tile_of<128, true>(kv_dtype) : tile_of<128, false>(kv_dtype);
+  return scored ? tile_of<256, true>(kv_dtype) : tile_of<256, false>(kv_dtype);
+}

@@ -63,7 +63,7 @@ struct RaggedTile {
   RaggedFn fn;
   int threads;
 };
-constexpr int kRaggedWide = 128, kRaggedNarrow = 32;  // rows of its tiles
+constexpr int kRaggedWide = 128, kRaggedNarrow = 16;  // rows of its tiles
 RaggedTile ragged_tile(int d, int kv_dtype, bool scored) __attribute__((visibility("hidden")));
 
 namespace {

@@ -1,21 +1,25 @@
 // Attention of ragged batches on the matrix cores, head dims up to 256 that are
 // multiples of 8.
 //
-// A workgroup takes one unit (ragged.hpp) of one KV head: 32 query rows a wave on the
-// 32 columns of v_mfma_f32_32x32x16_f16, S^T = K . Q^T, the softmax in registers (a lane
-// holds one row and 16 keys of a tile of 32, its row's other 16 in lane ^ 32), and
-// O^T += V^T . P^T with P where the score accumulator left it (V^T by transposed LDS
-// reads in the same key order).  q and p are two fp16 pieces, K and V row-scaled pieces
-// (two of an fp32 row, one of a bf16 or Q8 row): the products of prefill_narrow.hip.  There
-// the pieces come from a launch of their own over one sequence's keys; here the keys of a
-// batch are many sequences', most of them read by few rows, so every workgroup makes
-// the pieces of its own tiles on their way from the pages to LDS.
+// A workgroup takes one unit (ragged.hpp) of one KV head: S^T = K . Q^T with a query row a
+// column of the matrix instructions, the softmax in registers (a lane holds one row and
+// some keys of a tile of 32, the lanes around it the others), and O^T += V^T . P^T with P
+// where the score accumulator left it (V^T by transposed LDS reads in the same key order).
+// q and p are two fp16 pieces, K and V row-scaled pieces (two of an fp32 row, one of a
+// bf16 or Q8 row): the products of prefill_narrow.hip.  There the pieces come from a launch
+// of their own over one sequence's keys; here the keys of a batch are many
+// sequences', most of them read by few rows, so every workgroup makes the pieces of its
+// own tiles on their way from the pages to LDS.
 //
-// Wide tiles (prompts): 128 rows, 4 row groups of waves by KG key groups that take the
-// tiles of 32 keys in turn; the workgroup stages an interval of KG tiles together, double
-// buffered, the next interval's loads in flight while one is used.
-// Narrow tiles (one row, drafts): 32 rows, every wave a key group by itself with
-// its own LDS, so no wave waits for another: a tile's K, then its V, take the same place.
+// Wide tiles (prompts): 128 rows, 32 a wave (16 at d = 256, whose 32 would take 256
+// registers for q and o) and KG key groups that take the tiles of 32 keys in turn.  The
+// workgroup stages an interval of KG tiles together, double buffered.  Waves w and w + 4
+// share a SIMD: the first half of the waves stages the next interval after its products,
+// the second before them, so that one's conversions meet the other's products; the
+// interval after next is in flight meanwhile.
+// Narrow tiles (one row, drafts): 16 rows, every wave a key group by itself with
+// its own LDS, so no wave waits for another: a tile's K, then its V, take the same place,
+// and the next tile's are in flight.
 // The key groups' (m, l, o) are merged through LDS at the end.
 #include "ragged.hpp"
 
@@ -147,24 +151,25 @@ __device__ __forceinline__ Pieces<1> make_pieces(const Raw<q8_t>& r, int kv) {
 // SC: scores past the product (a cap, slopes).
 template <int D, typename T, bool SC>
 struct Tile {
-  static constexpr int NW = D <= 128 ? 8 : 4;  // waves: at d = 256 one a SIMD, with its registers
-  static constexpr int NT = 64 * NW;
+  static constexpr int NW = 8, NT = 64 * NW;
   static constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   static constexpr int KT = 32;
-  static constexpr int RGW = 4, KGW = NW / 4;  // wide tiles: row and key groups
-  static constexpr int RB = 2 * D;             // bytes of a staged row of one piece
-  static constexpr int PB = KT * RB;           // of a tile's piece
-  static constexpr int TB = NP * PB;           // of a tile
-  static constexpr int LPR = D / 8;            // lanes of a row
+  static constexpr int WR = D <= 128 ? 32 : 16;  // wide tiles: rows a wave,
+  static constexpr int RGW = kRaggedWide / WR;   // row groups
+  static constexpr int KGW = NW / RGW;           // and key groups
+  static constexpr int RB = 2 * D;               // bytes of a staged row of one piece
+  static constexpr int PB = KT * RB;             // of a tile's piece
+  static constexpr int TB = NP * PB;             // of a tile
+  static constexpr int NWN = TB <= 16384 ? NW : NW / 2;  // narrow tiles: waves whose tiles fit
+  static constexpr int LPR = D / 8;              // lanes of a row
   static constexpr int CW = KGW * KT * LPR / NT;  // chunks of 8 elements a thread, wide
   static constexpr int CN = KT * LPR / 64;        // and a lane, narrow
-  static constexpr int kTiles = 4 * KGW * TB;  // = NW * TB: the narrow tiles' places
-  static constexpr int kMerge = NW / 2 * KT * D * 4;
-  static constexpr int kData = kTiles > kMerge ? kTiles : kMerge;
-  static constexpr int kUnits = NW * 2 * KT * 4;  // narrow: [wave][K, V][32]; wide: 4 * KGW * 32
-  static constexpr int kStats = NW / 2 * KT * 16;
-  static constexpr int LDS = kData + (kUnits > kStats ? kUnits : kStats);
-  static_assert(kTiles == NW * TB && 4 * KGW * KT * 4 <= kUnits, "both kinds share the LDS");
+  static constexpr int max2(int x, int y) { return x > y ? x : y; }
+  static constexpr int kMergeW = KGW / 2 * kRaggedWide * D * 4, kMergeN = NWN / 2 * 16 * D * 4;
+  static constexpr int kData = max2(max2(4 * KGW * TB, NWN * TB), max2(kMergeW, kMergeN));
+  static constexpr int kUnits = max2(NWN * 2, 4 * KGW) * KT * 4;  // narrow: [wave][K, V][32]
+  static constexpr int LDS = kData + max2(kUnits, NW / 2 * 64 * 8);
+  static_assert(LDS <= 160 * 1024, "fits a CU");
 
   using raw_t = Raw<T>;
 
@@ -231,23 +236,21 @@ struct Tile {
   }
 };
 
-// A wave's rows over its tiles.
+// What the rows of a wave share whatever their number: the row of this lane.
 template <int D, typename T, bool SC>
-struct Rows {
+struct RowsBase {
   using C = Tile<D, T, SC>;
-  static constexpr int QS = D / 16, DB = D / 32, NP = C::NP, RB = C::RB, PB = C::PB;
-  f16x8_t qh[QS], ql[QS];
-  float qunit;
-  f32x16 o[DB], s;
+  float qunit, fac, mark;
   RowState rs;
-  uint32_t yh[8], yl[8];
-  float fac, mark;
   RowScore score;
   int lo, hi;  // the row's keys of this unit
   int room;
 
+  // q's pieces, N steps: step k the elements STEP*k + 8*part .. +7 of row r, as an operand.
+  // gmax: the maximum over the row's lanes.
+  template <int N, int STEP, typename GMAX>
   __device__ __forceinline__ void init(const RaggedArgs& a, const RaggedUnit& u, const RaggedSeq& sq, int h,
-                                       int r, int hh) {
+                                       int r, int part, GMAX&& gmax, f16x8_t (&qh)[N], f16x8_t (&ql)[N]) {
     const bool rv = r < sq.rows * a.G;
     const int m = rv ? r / a.G : 0, g = rv ? r - m * a.G : 0, slot = sq.slot0 + m;
     // (a row past the last: any keys, not stored)
@@ -255,11 +258,11 @@ struct Rows {
     hi = rv ? min(ragged_hi(a, slot), u.hi) : 0x7FFFFFFF;
     const float* qr = a.q + (((int64_t)sq.start + m) * a.nq + h * a.G + g) * a.d;
     const float qsc = a.scale * kLog2e;
-    // (read twice, the largest first: all of the row at once would take 4 * QS registers)
+    // (read twice, the largest first: all of the row at once would take 8 * N registers)
     auto eight = [&](int k, float (&x)[8]) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int e0 = 16 * k + 8 * hh + 4 * i;
+        const int e0 = STEP * k + 8 * part + 4 * i;
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
         if (rv && e0 < a.d) y = *reinterpret_cast<const f32x4*>(qr + e0);
 #pragma unroll
@@ -268,17 +271,17 @@ struct Rows {
     };
     float qm = 0.f;
 #pragma unroll
-    for (int k = 0; k < QS; ++k) {
+    for (int k = 0; k < N; ++k) {
       float x[8];
       eight(k, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) qm = fmaxf(qm, fabsf(x[e]));
     }
     asm volatile("" : "+v"(qr));
-    const int shift = f16_row_shift(max_xor32(qm));
+    const int shift = f16_row_shift(gmax(qm));
     qunit = f16_row_unit(shift);
 #pragma unroll
-    for (int k = 0; k < QS; ++k) {
+    for (int k = 0; k < N; ++k) {
       float x[8];
       eight(k, x);
       uint32_t h4[4], l4[4];
@@ -288,18 +291,69 @@ struct Rows {
       ql[k] = __builtin_bit_cast(f16x8_t, u32x4{l4[0], l4[1], l4[2], l4[3]});
     }
     if constexpr (SC) score = ragged_score(a, h * a.G + g, slot);
-#pragma unroll
-    for (int b = 0; b < DB; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
     fac = 1.f;
     mark = 0.f;
     room = wide_room(u.hi - u.lo);
   }
+  // The tile's probabilities of this lane's N keys, slot(e) their slots.
+  template <int N, typename SLOT, typename GMAX>
+  __device__ __forceinline__ void tile(float (&x)[N], const float (&ku)[N], const float (&vu)[N], int tk,
+                                       SLOT&& slot, GMAX&& gmax, uint32_t (&yh)[N / 2],
+                                       uint32_t (&yl)[N / 2]) {
+    const bool full = __builtin_amdgcn_ballot_w64(tk < lo || tk + C::KT > hi) == 0;
+    auto dead = [&](int e) {
+      const int t = slot(e);
+      return t < lo || t >= hi;
+    };
+    if constexpr (SC)
+      fac = softmax_tile<N>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl,
+                            [&](float (&z)[N], auto&& again) { score.template apply<N>(z, slot, again); },
+                            room);
+    else
+      fac = softmax_tile<N>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
+  }
+};
+
+// 32 rows of a wave over its tiles (v_mfma_f32_32x32x16_f16).
+template <int D, typename T, bool SC>
+struct Rows32 : RowsBase<D, T, SC> {
+  using B = RowsBase<D, T, SC>;
+  using C = typename B::C;
+  using B::fac, B::mark;
+  static constexpr int NR = 32, NV = D / 8;  // rows; vectors of 4 outputs a lane
+  static constexpr int QS = D / 16, DB = D / 32, NP = C::NP, RB = C::RB, PB = C::PB;
+  f16x8_t qh[QS], ql[QS];
+  f32x16 o[DB], s;
+  uint32_t yh[8], yl[8];
+
+  __device__ static __forceinline__ float gmax(float v) { return max_xor32(v); }
+  __device__ static __forceinline__ float gsum(float v) { return sum_xor32(v); }
+  __device__ __forceinline__ void init(const RaggedArgs& a, const RaggedUnit& u, const RaggedSeq& sq, int h,
+                                       int r, int lane) {
+    B::template init<QS, 16>(a, u, sq, h, r, lane >> 5, gmax, qh, ql);
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+  }
+  // Output vector v of this lane, and where its four elements lie in the row.
+  __device__ __forceinline__ f32x4 get(int v) const {
+    const auto& x = o[v >> 2];
+    const int i = 4 * (v & 3);
+    return f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+  }
+  __device__ __forceinline__ void put(int v, f32x4 y) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[v >> 2][4 * (v & 3) + e] = y[e];
+  }
+  __device__ static __forceinline__ int place(int v, int lane) {
+    return 32 * (v >> 2) + 8 * (v & 3) + 4 * (lane >> 5);
+  }
 
   // S^T of a tile: keys 8*(i/4) + 4*hh + i%4.  The products with a low piece have a sum of
   // their own: small beside the others', which alone then rounds at the scores' size.
-  __device__ __forceinline__ void scores(const char* tile, int c32, int hh) {
+  __device__ __forceinline__ void scores(const char* tile, int lane) {
+    const int c32 = lane & 31, hh = lane >> 5;
     const char* kr = tile + c32 * RB;
     const int kx = 16 * (hh ^ wk_f<D>(c32));
     f32x16 low;
@@ -332,7 +386,8 @@ struct Rows {
     for (int i = 0; i < 16; ++i) s[i] += low[i];
   }
 
-  __device__ __forceinline__ void softmax(const float* ku_, const float* vu_, int tk, int c32, int hh) {
+  __device__ __forceinline__ void softmax(const float* ku_, const float* vu_, int tk, int lane) {
+    const int hh = lane >> 5;
     float x[16], ku[16], vu[16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -345,25 +400,15 @@ struct Rows {
         vu[4 * i + e] = z[e];
       }
     }
-    mark = fmaf(ku_[c32] + vu_[c32], 0.f, mark);
-    const bool full = __builtin_amdgcn_ballot_w64(tk < lo || tk + C::KT > hi) == 0;
-    auto slot = [&](int e) { return tk + 8 * (e >> 2) + 4 * hh + (e & 3); };
-    auto gmax = [](float v) { return max_xor32(v); };
-    auto dead = [&](int e) {
-      const int t = slot(e);
-      return t < lo || t >= hi;
-    };
-    if constexpr (SC)
-      fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl,
-                             [&](float (&z)[16], auto&& again) { score.template apply<16>(z, slot, again); },
-                             room);
-    else
-      fac = softmax_tile<16>(x, ku, vu, qunit, rs, full, gmax, dead, yh, yl);
+    mark = fmaf(ku_[lane & 31] + vu_[lane & 31], 0.f, mark);
+    B::template tile<16>(x, ku, vu, tk, [&](int e) { return tk + 8 * (e >> 2) + 4 * hh + (e & 3); }, gmax, yh,
+                         yl);
   }
 
   // O^T += V^T . P^T.  A transposed read's 16-lane group (2*hh + x) takes keys 16j + 8u +
   // 4hh .. +3 of the block's 16 columns 16x ..: slots 4u + i of the A operand, P's order.
-  __device__ __forceinline__ void pv(char* tile, int lane, int hh) {
+  __device__ __forceinline__ void pv(char* tile, int lane) {
+    const int hh = lane >> 5;
     if (__builtin_amdgcn_ballot_w64(fac != 1.f) != 0) {
 #pragma unroll
       for (int b = 0; b < DB; ++b)
@@ -414,10 +459,209 @@ struct Rows {
   }
 };
 
+__device__ __forceinline__ f32x4 mfma16_f16(f16x8_t a, f16x8_t b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// 16 rows of a wave (v_mfma_f32_16x16x32_f16): half the registers.  A lane holds the keys
+// 16*b + 4*(lane / 16) + i of row lane % 16, e = 4*b + i.
+template <int D, typename T, bool SC>
+struct Rows16 : RowsBase<D, T, SC> {
+  using B = RowsBase<D, T, SC>;
+  using C = typename B::C;
+  using B::fac, B::mark;
+  static constexpr int NR = 16, NV = D / 16;
+  static constexpr int QS = D / 32, NP = C::NP, RB = C::RB, PB = C::PB;
+  f16x8_t qh[QS], ql[QS];
+  f32x4 o[NV], s[2];
+  uint32_t yh[4], yl[4];
+
+  __device__ static __forceinline__ float gmax(float v) { return max_xor32(max_xor16(v)); }
+  __device__ static __forceinline__ float gsum(float v) { return sum_xor32(sum_xor16(v)); }
+  __device__ __forceinline__ void init(const RaggedArgs& a, const RaggedUnit& u, const RaggedSeq& sq, int h,
+                                       int r, int lane) {
+    B::template init<QS, 32>(a, u, sq, h, r, lane >> 4, gmax, qh, ql);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ f32x4 get(int v) const { return o[v]; }
+  __device__ __forceinline__ void put(int v, f32x4 y) { o[v] = y; }
+  __device__ static __forceinline__ int place(int v, int lane) { return 16 * v + 4 * (lane >> 4); }
+
+  __device__ __forceinline__ void scores(const char* tile, int lane) {
+    const int r = lane & 15;  // (rows r and 16 + r have one swizzle)
+    const char* kr = tile + r * RB;
+    const int kx = 16 * ((lane >> 4) ^ wk_f<D>(r));
+    f32x4 low[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) s[b] = low[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f16x8_t k[2][2][NP];
+    auto read_k = [&](int q) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          k[q & 1][b][p] = *reinterpret_cast<const f16x8_t*>(kr + 16 * b * RB + p * PB + (kx ^ (64 * q)));
+    };
+    read_k(0);
+#pragma unroll
+    for (int q = 0; q < QS; ++q) {
+      if (q + 1 < QS) read_k(q + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) s[b] = mfma16_f16(k[q & 1][b][0], qh[q], s[b]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) low[b] = mfma16_f16(k[q & 1][b][0], ql[q], low[b]);
+      if constexpr (NP == 2) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) low[b] = mfma16_f16(k[q & 1][b][1], qh[q], low[b]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[b][i] += low[b][i];
+  }
+
+  __device__ __forceinline__ void softmax(const float* ku_, const float* vu_, int tk, int lane) {
+    const int g = lane >> 4;
+    float x[8], ku[8], vu[8];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(ku_ + 16 * b + 4 * g);
+      const f32x4 z = *reinterpret_cast<const f32x4*>(vu_ + 16 * b + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[4 * b + i] = s[b][i];
+        ku[4 * b + i] = y[i];
+        vu[4 * b + i] = z[i];
+      }
+    }
+    mark = fmaf(ku_[lane & 31] + vu_[lane & 31], 0.f, mark);
+    B::template tile<8>(x, ku, vu, tk, [&](int e) { return tk + 16 * (e >> 2) + 4 * g + (e & 3); }, gmax, yh, yl);
+  }
+
+  // A transposed read's 16-lane group g takes keys 16b + 4g .. +3 of 16 columns: P's order.
+  __device__ __forceinline__ void pv(char* tile, int lane) {
+    if (__builtin_amdgcn_ballot_w64(fac != 1.f) != 0) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[v][i] *= fac;
+    }
+    const int l16 = lane & 15, rr = 4 * (lane >> 4) + (l16 >> 2);
+    char* vr = tile + rr * RB + 8 * (l16 & 1);
+    const int vx = 16 * (((l16 & 3) >> 1) ^ wv_f<D>(rr));  // (rows rr and 16 + rr alike)
+    const f16x8_t ph = __builtin_bit_cast(f16x8_t, u32x4{yh[0], yh[1], yh[2], yh[3]});
+    const f16x8_t pl = __builtin_bit_cast(f16x8_t, u32x4{yl[0], yl[1], yl[2], yl[3]});
+    f16x8_t av[2][2][NP];
+    auto read_v = [&](int v0) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          i16x4_t t2[2];
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            t2[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) i16x4_t*)(vr + p * PB + 16 * b * RB +
+                                                             (vx ^ (32 * (v0 + j)))));
+          av[(v0 >> 1) & 1][j][p] =
+              __builtin_bit_cast(f16x8_t, __builtin_shufflevector(t2[0], t2[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    };
+    read_v(0);
+#pragma unroll
+    for (int v0 = 0; v0 < NV; v0 += 2) {
+      if (v0 + 2 < NV) read_v(v0 + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      auto& vc = av[(v0 >> 1) & 1];
+      if constexpr (NP == 2) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) o[v0 + j] = mfma16_f16(vc[j][1], ph, o[v0 + j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) o[v0 + j] = mfma16_f16(vc[j][0], pl, o[v0 + j]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) o[v0 + j] = mfma16_f16(vc[j][0], ph, o[v0 + j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
+// The end of a unit: x the rows of this wave, group rg of RG of key group kg of KG.
+template <int RG, int KG, typename X>
+__device__ __forceinline__ void finish(const RaggedArgs& a, const RaggedUnit& u, const RaggedSeq& sq, int h,
+                                       X& x, int rg, int kg, char* lds) {
+  using C = typename X::C;
+  constexpr int D = X::NV * 4 * (64 / X::NR);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int r = u.r0 + X::NR * rg + (lane & (X::NR - 1));
+  // a row that the pieces cannot hold: the unit's rows again, each over its own keys
+  if (__syncthreads_or(x.mark != 0.f)) {
+    for (int i = w; i < RG * X::NR; i += C::NW) ragged_own_row<D / 64>(a, u, h, u.r0 + i);
+    return;
+  }
+  // the key groups' merge, halves at a time: o in units of 2^m
+  float l = X::gsum(x.rs.l), m = x.rs.m;
+#pragma unroll
+  for (int v = 0; v < X::NV; ++v) {
+    f32x4 y = x.get(v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = ldexpf(y[e], -x.rs.wsh);
+    x.put(v, y);
+  }
+#pragma unroll
+  for (int half = KG / 2; half > 0; half /= 2) {
+    const int at = (kg & (half - 1)) * RG + rg;
+    f32x4* mo = reinterpret_cast<f32x4*>(lds) + at * X::NV * 64 + lane;
+    f32x2* ml = reinterpret_cast<f32x2*>(lds + C::kData) + at * 64 + lane;
+    if (kg >= half && kg < 2 * half) {
+#pragma unroll
+      for (int v = 0; v < X::NV; ++v) mo[v * 64] = x.get(v);
+      *ml = f32x2{m, l};
+    }
+    __syncthreads();
+    if (kg < half) {
+      const f32x2 st = *ml;
+      const float M = fmaxf(m, st[0]), f0 = exp2_hw(m - M), f1 = exp2_hw(st[0] - M);
+      m = M;
+      l = l * f0 + st[1] * f1;
+#pragma unroll
+      for (int v = 0; v < X::NV; ++v) {
+        const f32x4 z = mo[v * 64];
+        f32x4 y = x.get(v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = y[e] * f0 + z[e] * f1;
+        x.put(v, y);
+      }
+    }
+    if (half > 1) __syncthreads();
+  }
+  if (kg > 0 || r >= sq.rows * a.G) return;
+  const bool part = u.part >= 0;
+  const int64_t ps = ((int64_t)u.part * a.nkv + h) * a.slot_rows + (r - u.r0);
+  const int mm = r / a.G, g = r - mm * a.G;
+  float* out = part ? a.part_o + ps * D : a.o + (((int64_t)sq.start + mm) * a.nq + h * a.G + g) * a.d;
+  const int dh = part ? D : a.d;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // no key: O = 0
+#pragma unroll
+  for (int v = 0; v < X::NV; ++v) {
+    const int e0 = X::place(v, lane);
+    f32x4 y = x.get(v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = part ? y[e] : div_by(y[e], l, inv);
+    if (e0 < dh) *reinterpret_cast<f32x4*>(out + e0) = y;
+  }
+  if (part && lane < X::NR)
+    *reinterpret_cast<f32x2*>(a.part_ml + 2 * ps) = f32x2{l == 0.f ? -INFINITY : m, l};
+}
+
 template <int D, typename T, bool SC>
 __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(RaggedArgs a) {
   using C = Tile<D, T, SC>;
-  constexpr int KT = C::KT, LPR = C::LPR, DB = D / 32;
+  constexpr int KT = C::KT, LPR = C::LPR;
   __shared__ __attribute__((aligned(16))) char lds[C::LDS];
   float* const units = reinterpret_cast<float*>(lds + C::kData);
 
@@ -427,10 +671,6 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
   const RaggedSeq sq = ragged_seq(a, u.seq);
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c32 = lane & 31, hh = lane >> 5;
-  const bool wide = u.wide;
-  const int rg = wide ? w & 3 : 0, kg = wide ? w >> 2 : w;
-  const int r = u.r0 + 32 * rg + c32;
   const int ntile = (u.hi - u.lo + KT - 1) / KT;
   const int last = u.hi - 1;  // rows past it read it again (masked)
   const int32_t* table = a.block_table + (int64_t)u.seq * a.max_blocks;
@@ -438,18 +678,19 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
     const int id = table[min(t, last) >> a.page_shift];
     return (unsigned)id < (unsigned)a.num_blocks ? id : 0;
   };
-
   const typename C::Pages pg = C::pages(a, h);
-  Rows<D, T, SC> x;
-  x.init(a, u, sq, h, r, hh);
 
-  if (wide) {
+  if (u.wide) {
+    using X = typename std::conditional<C::WR == 32, Rows32<D, T, SC>, Rows16<D, T, SC>>::type;
+    const int rg = w % C::RGW, kg = w / C::RGW;
+    X x;
+    x.init(a, u, sq, h, u.r0 + X::NR * rg + (lane & (X::NR - 1)), lane);
     const int nint = (ntile + C::KGW - 1) / C::KGW;
     auto tile_buf = [&](int kv, int bf, int g) { return lds + ((kv * 2 + bf) * C::KGW + g) * C::TB; };
     auto unit_buf = [&](int kv, int bf, int g) { return units + ((kv * 2 + bf) * C::KGW + g) * KT; };
     typename C::raw_t kr[C::CW], vr[C::CW];
     int blk[C::CW];
-    // chunk i of this thread: unit j of row r0 + STEP*i of the interval's KGW tiles in a row
+    // chunk i of this thread: unit j of row rr + STEP*i of the interval's KGW tiles in a row
     constexpr int STEP = C::NT / LPR;
     const int rr = tid / LPR, j = tid % LPR;
     const unsigned at = 8 * j < a.d ? 8 * j * (unsigned)sizeof(T) : 0;
@@ -458,6 +699,7 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
 #pragma unroll
       for (int i = 0; i < C::CW; ++i) blk[i] = block_of(key(it, i));
     };
+    // the rows of interval it, and the blocks of the one after it (its rows' clamp: any it)
     auto fetch = [&](int it) {
 #pragma unroll
       for (int i = 0; i < C::CW; ++i) {
@@ -465,16 +707,17 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
         C::load(pg, a.k, blk[i], t, at, false, kr[i]);
         C::load(pg, a.v, blk[i], t, at, false, vr[i]);
       }
+      blocks(it + 1);
     };
     auto stage = [&](int it) {
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        constexpr int N = STEP < KT ? C::CW : 1;  // chunks of a tile
-        if constexpr (STEP < KT) {
-          static_assert(C::KGW == 1, "one tile");
-          C::template store<N, STEP>(kv ? vr : kr, kv, rr, j, [&](int) { return tile_buf(kv, it & 1, 0); },
-                                     [&](int) { return unit_buf(kv, it & 1, 0); });
-        } else {  // a tile or more a chunk
+        if constexpr (STEP < KT) {  // part of a tile a chunk
+          static_assert(STEP >= KT || C::KGW == 1, "one tile");
+          C::template store<C::CW, STEP>(kv ? vr : kr, kv, rr, j,
+                                         [&](int) { return tile_buf(kv, it & 1, 0); },
+                                         [&](int) { return unit_buf(kv, it & 1, 0); });
+        } else {  // a tile or more
 #pragma unroll
           for (int i = 0; i < C::CW; ++i) {
             const typename C::raw_t one[1] = {kv ? vr[i] : kr[i]};
@@ -488,129 +731,82 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
     if (nint > 0) {
       blocks(0);
       fetch(0);
-      if (nint > 1) blocks(1);
       stage(0);
+      fetch(1);
     }
     __syncthreads();
+    const bool first = w < C::NW / 2;
     for (int it = 0; it < nint; ++it) {
-      const bool more = it + 1 < nint;
-      if (more) {
-        fetch(it + 1);
-        if (it + 2 < nint) blocks(it + 2);
-      }
       const int bf = it & 1;
-      x.scores(tile_buf(0, bf, kg), c32, hh);
-      x.softmax(unit_buf(0, bf, kg), unit_buf(1, bf, kg), u.lo + (C::KGW * it + kg) * KT, c32, hh);
-      x.pv(tile_buf(1, bf, kg), lane, hh);
-      if (more) stage(it + 1);
+      const bool more = it + 1 < nint;
+      if (!first && more) {
+        stage(it + 1);
+        fetch(it + 2);
+      }
+      x.scores(tile_buf(0, bf, kg), lane);
+      x.softmax(unit_buf(0, bf, kg), unit_buf(1, bf, kg), u.lo + (C::KGW * it + kg) * KT, lane);
+      x.pv(tile_buf(1, bf, kg), lane);
+      if (first && more) {
+        stage(it + 1);
+        fetch(it + 2);
+      }
       lds_barrier();
     }
-  } else {
+    finish<C::RGW, C::KGW>(a, u, sq, h, x, rg, kg, lds);
+    return;
+  }
+
+  Rows16<D, T, SC> x;
+  x.init(a, u, sq, h, u.r0 + (lane & 15), lane);
+  if (w < C::NWN) {
     char* const buf = lds + w * C::TB;
     float* const ub = units + w * 2 * KT;
-    typename C::raw_t raw[C::CN];
-    const int r_in = lane / LPR, j = lane % LPR;
+    // K and V each have their registers where those are few enough
+    constexpr bool BOTH = C::CN * (int)sizeof(typename C::raw_t) <= 128;
+    typename C::raw_t raw[BOTH ? 2 : 1][C::CN];
     constexpr int RPI = 64 / LPR;  // rows of a load
+    const int r_in = lane / LPR, j = lane % LPR;
     const unsigned at = 8 * j < a.d ? 8 * j * (unsigned)sizeof(T) : 0;
-    auto ids = [&](int t) { return block_of(u.lo + t * KT + c32); };
-    auto fetch = [&](const char* pool, int t, int id) {
+    auto ids = [&](int t) { return block_of(u.lo + t * KT + (lane & 31)); };
+    auto fetch = [&](int kv, int t, int id) {
 #pragma unroll
       for (int i = 0; i < C::CN; ++i) {
         const int rr = r_in + RPI * i;
-        C::load(pg, pool, __shfl(id, rr), min(u.lo + t * KT + rr, last), at, true, raw[i]);
+        C::load(pg, kv ? a.v : a.k, __shfl(id, rr), min(u.lo + t * KT + rr, last), at, true,
+                raw[BOTH ? kv : 0][i]);
       }
     };
     auto stage = [&](int kv) {
-      C::template store<C::CN, RPI>(raw, kv, r_in, j, [&](int) { return buf; },
+      C::template store<C::CN, RPI>(raw[BOTH ? kv : 0], kv, r_in, j, [&](int) { return buf; },
                                     [&](int) { return ub + kv * KT; });
       asm volatile("" ::: "memory");  // the wave's own LDS: in order
     };
     int id = 0, idn = 0;
     if (w < ntile) {
       id = ids(w);
-      fetch(a.k, w, id);
-      idn = ids(w + C::NW);
+      fetch(0, w, id);
+      if (BOTH) fetch(1, w, id);
+      idn = ids(w + C::NWN);
     }
-    for (int t = w; t < ntile; t += C::NW) {
+    for (int t = w; t < ntile; t += C::NWN) {
+      const bool more = t + C::NWN < ntile;
       stage(0);
-      fetch(a.v, t, id);
-      x.scores(buf, c32, hh);
+      if (!BOTH) fetch(1, t, id);
+      else if (more) fetch(0, t + C::NWN, idn);
+      x.scores(buf, lane);
       asm volatile("" ::: "memory");
       stage(1);
-      id = idn;
-      if (t + C::NW < ntile) {
-        fetch(a.k, t + C::NW, id);
-        idn = ids(t + 2 * C::NW);
+      if (more) {
+        id = idn;
+        fetch(BOTH ? 1 : 0, t + C::NWN, id);
+        idn = ids(t + 2 * C::NWN);
       }
-      x.softmax(ub, ub + KT, u.lo + t * KT, c32, hh);
-      x.pv(buf, lane, hh);
+      x.softmax(ub, ub + KT, u.lo + t * KT, lane);
+      x.pv(buf, lane);
       asm volatile("" ::: "memory");
     }
   }
-
-  // a row that the pieces cannot hold: the unit's rows again, each over its own keys
-  if (__syncthreads_or(x.mark != 0.f)) {
-    const int rows = wide ? 32 * C::RGW : 32;
-    for (int i = w; i < rows; i += C::NW) ragged_own_row<D / 64>(a, u, h, u.r0 + i);
-    return;
-  }
-
-  // the key groups' merge, halves at a time: o in units of 2^m
-  float l = sum_xor32(x.rs.l), m = x.rs.m;
-#pragma unroll
-  for (int b = 0; b < DB; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x.o[b][i] = ldexpf(x.o[b][i], -x.rs.wsh);
-  const int rgs = wide ? C::RGW : 1;
-  for (int half = (wide ? C::KGW : C::NW) / 2; half > 0; half /= 2) {
-    const int at = (kg % half) * rgs + rg;
-    f32x4* mo = reinterpret_cast<f32x4*>(lds) + at * DB * 4 * 64 + lane;
-    f32x2* ml = reinterpret_cast<f32x2*>(lds + C::kData) + at * 64 + lane;
-    if (kg >= half && kg < 2 * half) {
-#pragma unroll
-      for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mo[(b * 4 + i) * 64] =
-              f32x4{x.o[b][4 * i], x.o[b][4 * i + 1], x.o[b][4 * i + 2], x.o[b][4 * i + 3]};
-      *ml = f32x2{m, l};
-    }
-    __syncthreads();
-    if (kg < half) {
-      const f32x2 st = *ml;
-      const float M = fmaxf(m, st[0]), f0 = exp2_hw(m - M), f1 = exp2_hw(st[0] - M);
-      m = M;
-      l = l * f0 + st[1] * f1;
-#pragma unroll
-      for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 z = mo[(b * 4 + i) * 64];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x.o[b][4 * i + e] = x.o[b][4 * i + e] * f0 + z[e] * f1;
-        }
-    }
-    __syncthreads();
-  }
-  if (kg > 0 || r >= sq.rows * a.G) return;
-  const bool part = u.part >= 0;
-  const int64_t ps = ((int64_t)u.part * a.nkv + h) * a.slot_rows + (r - u.r0);
-  const int mm = r / a.G, g = r - mm * a.G;
-  float* out = part ? a.part_o + ps * D : a.o + (((int64_t)sq.start + mm) * a.nq + h * a.G + g) * a.d;
-  const int dh = part ? D : a.d;
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // no key: O = 0
-#pragma unroll
-  for (int b = 0; b < DB; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e0 = 32 * b + 8 * i + 4 * hh;
-      f32x4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = part ? x.o[b][4 * i + e] : div_by(x.o[b][4 * i + e], l, inv);
-      if (e0 < dh) *reinterpret_cast<f32x4*>(out + e0) = y;
-    }
-  if (part && hh == 0)
-    *reinterpret_cast<f32x2*>(a.part_ml + 2 * ps) = f32x2{l == 0.f ? -INFINITY : m, l};
+  finish<1, C::NWN>(a, u, sq, h, x, 0, w, lds);
 }
 
 template <int D, bool SC>

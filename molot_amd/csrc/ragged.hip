@@ -408,6 +408,14 @@ __global__ __launch_bounds__(kAppendThreads) void ragged_append_kernel(AppendArg
 // the others.
 constexpr int kUnitThreads = kPlanThreads;
 
+// Tiles of a sequence of R rows r: wide ones as long as more than `few` rows are left, then
+// narrow ones.
+__device__ __forceinline__ int wide_tiles(const RaggedArgs& a, int R) {
+  return R / a.ql + (R % a.ql > a.few ? 1 : 0);
+}
+__device__ __forceinline__ int slim_tiles(const RaggedArgs& a, int R) {
+  return R % a.ql > a.few ? 0 : (R % a.ql + a.qs - 1) / a.qs;
+}
 struct UnitTile {
   int seq, r0, lo, hi, wide;
 };
@@ -417,8 +425,9 @@ __device__ __forceinline__ UnitTile unit_tile(const RaggedArgs& a, int t, int nw
   const int b = plan_find(a.B, i, [&](int s) { return before(s, kind); });
   const RaggedSeq s = ragged_seq(a, b);
   const int R = s.rows * a.G, rows = kind ? a.qs : a.ql;
-  const int n = (R + rows - 1) / rows;
-  const int r0 = (n - 1 - (i - before(b, kind))) * rows, r1 = min(r0 + rows, R) - 1;
+  const int n = kind ? slim_tiles(a, R) : wide_tiles(a, R);
+  const int r0 = (kind ? R / a.ql * a.ql : 0) + (n - 1 - (i - before(b, kind))) * rows;
+  const int r1 = min(r0 + rows, R) - 1;
   const int lo = ragged_lo(a, s.slot0 + r0 / a.G);
   return {b, r0, lo, max(lo, ragged_hi(a, s.slot0 + r1 / a.G)), !kind};
 }
@@ -433,11 +442,9 @@ __global__ __launch_bounds__(kUnitThreads) void ragged_units_kernel(RaggedArgs a
   for (int b0 = 0; b0 < a.B; b0 += kUnitThreads) {
     const int b = b0 + tid;
     const int R = b < a.B ? ragged_seq(a, b).rows * a.G : 0;
-    const bool wide = R > a.few;
-    const int n = R == 0 ? 0 : wide ? (R + a.ql - 1) / a.ql : (R + a.qs - 1) / a.qs;
     int t0, t1;
-    const int w = nwide + block_scan(wide ? n : 0, sh, t0);
-    const int s = nslim + block_scan(wide ? 0 : n, sh, t1);
+    const int w = nwide + block_scan(wide_tiles(a, R), sh, t0);
+    const int s = nslim + block_scan(slim_tiles(a, R), sh, t1);
     nwide += t0;
     nslim += t1;
     if (b < a.B) {
@@ -651,7 +658,7 @@ int launch_attention(RaggedArgs a, void* stream) {
                    : D == 256 ? ragged_merge_kernel<4> : ragged_merge_kernel<8>;
   int threads = 64 * kValuWaves;
   a.qs = a.ql = a.slot_rows = kValuWaves;
-  a.few = 0x7FFFFFFF;
+  a.few = 0;  // every tile a wide one
   a.min_keys = 256;
   int per_cu = 8;
   // (the matrix-core kernel's offsets within a block are of 32 bits)
@@ -660,20 +667,20 @@ int launch_attention(RaggedArgs a, void* stream) {
     const RaggedTile t = ragged_tile(a.d, a.kv_dtype, a.softcap > 0.f || a.slopes);
     attend = t.fn;
     threads = t.threads;
-    a.qs = kRaggedNarrow;
-    a.ql = kRaggedWide;
-    a.few = 2 * kRaggedNarrow;
+    a.qs = t.narrow;
+    a.ql = t.wide;
+    a.few = 2 * a.qs;
     // (a tile holds no more rows than the batch)
-    a.slot_rows = (int64_t)a.T * a.G <= a.few ? kRaggedNarrow : kRaggedWide;
+    a.slot_rows = (int64_t)a.T * a.G <= a.few ? a.qs : a.ql;
     per_cu = 2;
   }
   a.target = (per_cu * cus + a.nkv - 1) / a.nkv;
-  // Bounds: a sequence of R rows r has at most R / ql + 1 wide tiles, or R / qs + 1 narrow
-  // ones where R <= few; its splits add at most its share of target, and a split tile has
-  // at most twice that (ragged_units_kernel).
+  // Bounds: a sequence of R rows r has at most R / ql wide tiles and one more, or narrow
+  // ones for up to `few` rows; its splits add at most its share of target, and a split tile
+  // has at most twice that (ragged_units_kernel).
   const int64_t R = (int64_t)a.T * a.G;
   const int64_t seqs = std::min(a.T, a.B);
-  const int64_t tiles = std::min(R / a.qs, R / a.ql + seqs * (a.few / a.qs)) + seqs;
+  const int64_t tiles = R / a.ql + seqs * std::max(1, (a.few + a.qs - 1) / a.qs);
   if (R > 0x3FFFFFFF || (tiles + a.target) * a.nkv > 0x7FFFFFFF) return MOLOT_ENOTSUP;
   a.max_units = (int)(tiles + a.target);
   a.max_parts = a.cap > a.min_keys ? 2 * a.target : 0;  // (else no tile is split)

@@ -57,13 +57,12 @@ struct RaggedArgs {
 };
 
 // The matrix-core kernel of a head dim (a multiple of 8 up to 256) and cache type, and
-// the threads of its workgroups: ragged_tile.hip.
+// the threads of its workgroups.
 using RaggedFn = void (*)(RaggedArgs);
 struct RaggedTile {
   RaggedFn fn;
-  int threads;
+  int threads, wide, narrow;  // (rows of its tiles)
 };
-constexpr int kRaggedWide = 128, kRaggedNarrow = 16;  // rows of its tiles
 RaggedTile ragged_tile(int d, int kv_dtype, bool scored) __attribute__((visibility("hidden")));
 
 namespace {

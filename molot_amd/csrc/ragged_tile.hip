@@ -11,10 +11,9 @@
 // sequences', most of them read by few rows, so every workgroup makes the pieces of its
 // own tiles on their way from the pages to LDS.
 //
-// Wide tiles (prompts): 128 rows, 32 a wave (16 at d = 256, whose 32 would take 256
-// registers for q and o) and KG key groups that take the tiles of 32 keys in turn.  The
-// workgroup stages an interval of KG tiles together, double buffered.  Waves w and w + 4
-// share a SIMD: the first half of the waves stages the next interval after its products,
+// Wide tiles (prompts): 256 rows, 32 a wave (at d = 256, where those would take 256
+// registers for q and o, 16).  The workgroup stages an interval of one or two tiles of 32
+// keys together, double buffered.  Waves w and w + 4 share a SIMD: the first half of the waves stages the next interval after its products,
 // the second before them, so that one's conversions meet the other's products; the
 // interval after next is in flight meanwhile.
 // Narrow tiles (one row, drafts): 16 rows, every wave a key group by itself with
@@ -155,19 +154,19 @@ struct Tile {
   static constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   static constexpr int KT = 32;
   static constexpr int WR = D <= 128 ? 32 : 16;  // wide tiles: rows a wave,
-  static constexpr int RGW = kRaggedWide / WR;   // row groups
-  static constexpr int KGW = NW / RGW;           // and key groups
+  static constexpr int QL = NW * WR;             // and of the tile;
+  static constexpr int IT = D <= 128 ? 2 : 1;    // tiles of keys an interval
   static constexpr int RB = 2 * D;               // bytes of a staged row of one piece
   static constexpr int PB = KT * RB;             // of a tile's piece
   static constexpr int TB = NP * PB;             // of a tile
   static constexpr int NWN = TB <= 16384 ? NW : NW / 2;  // narrow tiles: waves whose tiles fit
   static constexpr int LPR = D / 8;              // lanes of a row
-  static constexpr int CW = KGW * KT * LPR / NT;  // chunks of 8 elements a thread, wide
+  static constexpr int CW = IT * KT * LPR / NT;   // chunks of 8 elements a thread, wide
   static constexpr int CN = KT * LPR / 64;        // and a lane, narrow
   static constexpr int max2(int x, int y) { return x > y ? x : y; }
-  static constexpr int kMergeW = KGW / 2 * kRaggedWide * D * 4, kMergeN = NWN / 2 * 16 * D * 4;
-  static constexpr int kData = max2(max2(4 * KGW * TB, NWN * TB), max2(kMergeW, kMergeN));
-  static constexpr int kUnits = max2(NWN * 2, 4 * KGW) * KT * 4;  // narrow: [wave][K, V][32]
+  static constexpr int kMerge = NWN / 2 * 16 * D * 4;
+  static constexpr int kData = max2(max2(4 * IT * TB, NWN * TB), kMerge);
+  static constexpr int kUnits = max2(NWN * 2, 4 * IT) * KT * 4;  // narrow: [wave][K, V][32]
   static constexpr int LDS = kData + max2(kUnits, NW / 2 * 64 * 8);
   static_assert(LDS <= 160 * 1024, "fits a CU");
 
@@ -213,25 +212,23 @@ struct Tile {
       r.scale = *reinterpret_cast<const float*>(b + (p.scales + 4 * sl));
     }
   }
-  // N chunks of a thread into LDS: chunk i is unit j of row r + STEP*i (STEP a power of two
-  // past r) of the tile, at(i) the tile's place; the lanes with j = 0 leave the rows' units.
-  template <int N, int STEP, typename AT, typename UNITS>
-  __device__ static __forceinline__ void store(const raw_t (&raw)[N], int kv, int r, int j, AT&& at,
-                                               UNITS&& units) {
+  // N chunks of a thread into LDS: chunk i is unit j of row r + STEP*i of the tile (rows
+  // past it: of the next), r < KT, STEP a power of two past r or a multiple of KT.  units:
+  // the rows' units, the same in all their lanes.
+  template <int N, int STEP>
+  __device__ static __forceinline__ void pieces(const raw_t (&raw)[N], int kv, int r, int j, char* tile,
+                                                float (&units)[N]) {
     const int base = r * RB + 16 * (j ^ (kv ? wv_f<D>(r) : wk_f<D>(r)));
-    float unit[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const Pieces<NP> x = make_pieces<LPR>(raw[i], kv);
-      unit[i] = x.unit;
+      units[i] = x.unit;
       // (the swizzle of row r + STEP*i is r's and STEP*i's by exclusive or)
-      char* to = at(i) + ((base ^ (16 * (kv ? wv_f<D>(STEP * i) : wk_f<D>(STEP * i)))) + STEP * i * RB);
+      constexpr int M = KT - 1;
+      const int up = STEP * i & M;
+      char* to = tile + STEP * i / KT * TB + ((base ^ (16 * (kv ? wv_f<D>(up) : wk_f<D>(up)))) + up * RB);
 #pragma unroll
       for (int p = 0; p < NP; ++p) *reinterpret_cast<u32x4*>(to + p * PB) = x.p[p];
-    }
-    if (j == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) units(i)[r + STEP * i] = unit[i];
     }
   }
 };
@@ -350,15 +347,14 @@ struct Rows32 : RowsBase<D, T, SC> {
     return 32 * (v >> 2) + 8 * (v & 3) + 4 * (lane >> 5);
   }
 
-  // S^T of a tile: keys 8*(i/4) + 4*hh + i%4.  The products with a low piece have a sum of
-  // their own: small beside the others', which alone then rounds at the scores' size.
+  // S^T of a tile: keys 8*(i/4) + 4*hh + i%4.  Of each step the products with a low piece
+  // first: they are small beside the others, whose sum alone then rounds at its size.
   __device__ __forceinline__ void scores(const char* tile, int lane) {
     const int c32 = lane & 31, hh = lane >> 5;
     const char* kr = tile + c32 * RB;
     const int kx = 16 * (hh ^ wk_f<D>(c32));
-    f32x16 low;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = low[i] = 0.f;
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
     f16x8_t k[2][2][NP];
     auto read_k = [&](int k0) {
 #pragma unroll
@@ -376,14 +372,13 @@ struct Rows32 : RowsBase<D, T, SC> {
       auto& c = k[(k0 >> 1) & 1];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        s = mfma32_f16(c[j][0], qh[k0 + j], s);
-        low = mfma32_f16(c[j][0], ql[k0 + j], low);
-        if constexpr (NP == 2) low = mfma32_f16(c[j][1], qh[k0 + j], low);
+        if constexpr (NP == 2) s = mfma32_f16(c[j][1], qh[k0 + j], s);
+        s = mfma32_f16(c[j][0], ql[k0 + j], s);
       }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s = mfma32_f16(c[j][0], qh[k0 + j], s);
       __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] += low[i];
   }
 
   __device__ __forceinline__ void softmax(const float* ku_, const float* vu_, int tk, int lane) {
@@ -674,27 +669,29 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
   const int ntile = (u.hi - u.lo + KT - 1) / KT;
   const int last = u.hi - 1;  // rows past it read it again (masked)
   const int32_t* table = a.block_table + (int64_t)u.seq * a.max_blocks;
-  auto block_of = [&](int t) {
-    const int id = table[min(t, last) >> a.page_shift];
-    return (unsigned)id < (unsigned)a.num_blocks ? id : 0;
-  };
+  // The table's entry for row t; whether it is a block of the pool is asked where it is
+  // used, an interval later (here it would wait for every load in flight).
+  auto block_of = [&](int t) { return table[min(t, last) >> a.page_shift]; };
+  auto valid = [&](int id) { return (unsigned)id < (unsigned)a.num_blocks ? id : 0; };
   const typename C::Pages pg = C::pages(a, h);
 
   if (u.wide) {
     using X = typename std::conditional<C::WR == 32, Rows32<D, T, SC>, Rows16<D, T, SC>>::type;
-    const int rg = w % C::RGW, kg = w / C::RGW;
     X x;
-    x.init(a, u, sq, h, u.r0 + X::NR * rg + (lane & (X::NR - 1)), lane);
-    const int nint = (ntile + C::KGW - 1) / C::KGW;
-    auto tile_buf = [&](int kv, int bf, int g) { return lds + ((kv * 2 + bf) * C::KGW + g) * C::TB; };
-    auto unit_buf = [&](int kv, int bf, int g) { return units + ((kv * 2 + bf) * C::KGW + g) * KT; };
+    x.init(a, u, sq, h, u.r0 + X::NR * w + (lane & (X::NR - 1)), lane);
+    const bool rows = u.r0 + X::NR * w < sq.rows * a.G;  // else this wave only stages
+    constexpr int KI = C::IT * KT;                       // keys an interval
+    const int nint = (ntile + C::IT - 1) / C::IT;
+    auto tile_buf = [&](int kv, int bf, int g) { return lds + ((kv * 2 + bf) * C::IT + g) * C::TB; };
+    auto unit_buf = [&](int kv, int bf, int g) { return units + ((kv * 2 + bf) * C::IT + g) * KT; };
     typename C::raw_t kr[C::CW], vr[C::CW];
     int blk[C::CW];
-    // chunk i of this thread: unit j of row rr + STEP*i of the interval's KGW tiles in a row
+    // chunk i of this thread: unit j of row rr + STEP*i of the interval's tiles in a row
     constexpr int STEP = C::NT / LPR;
+    static_assert(STEP % KT == 0 || C::IT == 1, "chunks of a thread: of tiles, or of one tile");
     const int rr = tid / LPR, j = tid % LPR;
     const unsigned at = 8 * j < a.d ? 8 * j * (unsigned)sizeof(T) : 0;
-    auto key = [&](int it, int i) { return u.lo + C::KGW * KT * it + rr + STEP * i; };
+    auto key = [&](int it, int i) { return u.lo + KI * it + rr + STEP * i; };
     auto blocks = [&](int it) {
 #pragma unroll
       for (int i = 0; i < C::CW; ++i) blk[i] = block_of(key(it, i));
@@ -703,28 +700,23 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
     auto fetch = [&](int it) {
 #pragma unroll
       for (int i = 0; i < C::CW; ++i) {
-        const int t = min(key(it, i), last);
-        C::load(pg, a.k, blk[i], t, at, false, kr[i]);
-        C::load(pg, a.v, blk[i], t, at, false, vr[i]);
+        const int t = min(key(it, i), last), b = valid(blk[i]);
+        C::load(pg, a.k, b, t, at, false, kr[i]);
+        C::load(pg, a.v, b, t, at, false, vr[i]);
       }
       blocks(it + 1);
     };
+    // (an interval's tiles lie one after the other, and their units)
     auto stage = [&](int it) {
+      float ku[C::CW], vu[C::CW];
+      const int r0 = rr % KT, g0 = rr / KT;
+      C::template pieces<C::CW, STEP>(kr, 0, r0, j, tile_buf(0, it & 1, g0), ku);
+      C::template pieces<C::CW, STEP>(vr, 1, r0, j, tile_buf(1, it & 1, g0), vu);
+      if (j == 0) {
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        if constexpr (STEP < KT) {  // part of a tile a chunk
-          static_assert(STEP >= KT || C::KGW == 1, "one tile");
-          C::template store<C::CW, STEP>(kv ? vr : kr, kv, rr, j,
-                                         [&](int) { return tile_buf(kv, it & 1, 0); },
-                                         [&](int) { return unit_buf(kv, it & 1, 0); });
-        } else {  // a tile or more
-#pragma unroll
-          for (int i = 0; i < C::CW; ++i) {
-            const typename C::raw_t one[1] = {kv ? vr[i] : kr[i]};
-            const int g = STEP / KT * i + rr / KT;
-            C::template store<1, KT>(one, kv, rr % KT, j, [&](int) { return tile_buf(kv, it & 1, g); },
-                                     [&](int) { return unit_buf(kv, it & 1, g); });
-          }
+        for (int i = 0; i < C::CW; ++i) {
+          unit_buf(0, it & 1, 0)[rr + STEP * i] = ku[i];
+          unit_buf(1, it & 1, 0)[rr + STEP * i] = vu[i];
         }
       }
     };
@@ -743,16 +735,21 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
         stage(it + 1);
         fetch(it + 2);
       }
-      x.scores(tile_buf(0, bf, kg), lane);
-      x.softmax(unit_buf(0, bf, kg), unit_buf(1, bf, kg), u.lo + (C::KGW * it + kg) * KT, lane);
-      x.pv(tile_buf(1, bf, kg), lane);
+      if (rows) {
+#pragma unroll
+        for (int g = 0; g < C::IT; ++g) {
+          x.scores(tile_buf(0, bf, g), lane);
+          x.softmax(unit_buf(0, bf, g), unit_buf(1, bf, g), u.lo + KI * it + KT * g, lane);
+          x.pv(tile_buf(1, bf, g), lane);
+        }
+      }
       if (first && more) {
         stage(it + 1);
         fetch(it + 2);
       }
       lds_barrier();
     }
-    finish<C::RGW, C::KGW>(a, u, sq, h, x, rg, kg, lds);
+    finish<C::NW, 1>(a, u, sq, h, x, w, 0, lds);
     return;
   }
 
@@ -772,13 +769,17 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
 #pragma unroll
       for (int i = 0; i < C::CN; ++i) {
         const int rr = r_in + RPI * i;
-        C::load(pg, kv ? a.v : a.k, __shfl(id, rr), min(u.lo + t * KT + rr, last), at, true,
+        C::load(pg, kv ? a.v : a.k, valid(__shfl(id, rr)), min(u.lo + t * KT + rr, last), at, true,
                 raw[BOTH ? kv : 0][i]);
       }
     };
     auto stage = [&](int kv) {
-      C::template store<C::CN, RPI>(raw[BOTH ? kv : 0], kv, r_in, j, [&](int) { return buf; },
-                                    [&](int) { return ub + kv * KT; });
+      float unit[C::CN];
+      C::template pieces<C::CN, RPI>(raw[BOTH ? kv : 0], kv, r_in, j, buf, unit);
+      if (j == 0) {
+#pragma unroll
+        for (int i = 0; i < C::CN; ++i) ub[kv * KT + r_in + RPI * i] = unit[i];
+      }
       asm volatile("" ::: "memory");  // the wave's own LDS: in order
     };
     int id = 0, idn = 0;
@@ -811,9 +812,11 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
 
 template <int D, bool SC>
 RaggedTile tile_of(int kv_dtype) {
-  if (kv_dtype == MOLOT_KV_F32) return {ragged_tile_kernel<D, float, SC>, Tile<D, float, SC>::NT};
-  if (kv_dtype == MOLOT_KV_BF16) return {ragged_tile_kernel<D, bf16_t, SC>, Tile<D, bf16_t, SC>::NT};
-  return {ragged_tile_kernel<D, q8_t, SC>, Tile<D, q8_t, SC>::NT};
+  using C = Tile<D, float, SC>;  // (the rows are every type's)
+  return {kv_dtype == MOLOT_KV_F32    ? ragged_tile_kernel<D, float, SC>
+          : kv_dtype == MOLOT_KV_BF16 ? ragged_tile_kernel<D, bf16_t, SC>
+                                      : ragged_tile_kernel<D, q8_t, SC>,
+          C::NT, C::QL, 16};
 }
 
 }  // namespace

@@ -49,20 +49,22 @@ struct PlanArgs {
   int B, max_blocks, page_shift, num_blocks, max_rows;
 };
 
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr int kPlanThreads = 1024;
 // Sequences whose prefix sums fit in LDS: a row's search then takes log2(B) LDS reads.
 constexpr int kPlanSeqs = 4096;
 constexpr int kPlanMost = 1 << 20;  // rows, blocks a sequence: sums of 1024 stay below 2^31
 
 // Exclusive prefix over the workgroup of x, and the total.
+template <int NT>
 __device__ __forceinline__ int block_scan(int x, int* sh, int& total) {
+  constexpr int NW = NT / 64;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int inc = wave_scan(x);
   __syncthreads();  // the last scan's sums are read
   if (lane == 63) sh[w] = inc;
   __syncthreads();
-  const int other = wave_scan(lane < kPlanWaves ? sh[lane] : 0);
-  total = __builtin_amdgcn_readlane(other, kPlanWaves - 1);
+  const int other = wave_scan(lane < NW ? sh[lane] : 0);
+  total = __builtin_amdgcn_readlane(other, NW - 1);
   const int before = w ? __builtin_amdgcn_readlane(other, w - 1) : 0;
   return before + inc - x;
 }
@@ -139,7 +141,7 @@ __device__ __forceinline__ int plan_sum(int x, int y) { return min((unsigned)x +
 
 // One workgroup.  `rows`: it writes the rows' maps too, else ragged_rows_kernel does.
 __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, int rows) {
-  __shared__ int sh[kPlanWaves], s_st;
+  __shared__ int sh[kPlanThreads / 64], s_st;
   __shared__ int s_start[kPlanSeqs + 1], s_taken[kPlanSeqs];
   const int tid = threadIdx.x;
   const bool pool = a.free_blocks != nullptr;
@@ -151,9 +153,9 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, i
     const PlanSeq s = plan_seq(a, b0 + tid);
     if (s.st) st = s.st;
     int t0, t1, t2;
-    (void)block_scan(s.count, sh, t0);
-    (void)block_scan(s.take, sh, t1);
-    (void)block_scan(s.give, sh, t2);
+    (void)block_scan<kPlanThreads>(s.count, sh, t0);
+    (void)block_scan<kPlanThreads>(s.take, sh, t1);
+    (void)block_scan<kPlanThreads>(s.give, sh, t2);
     nrows = plan_sum(nrows, t0);
     take = plan_sum(take, t1);
     give = plan_sum(give, t2);
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, i
     for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
       const PlanSeq s = plan_seq(a, b0 + tid);
       int all;
-      int at = base + block_scan(s.give, sh, all);
+      int at = base + block_scan<kPlanThreads>(s.give, sh, all);
       base += all;
       for (int j = 0; j < s.give; ++j) {
         const int id = a.block_table[(int64_t)(b0 + tid) * a.max_blocks + j];
@@ -194,8 +196,8 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, i
     PlanSeq s = plan_seq(a, b);
     if (st) s = PlanSeq{was, 0, 0, 0, 0};
     int nr, nt;
-    const int rs = row0 + block_scan(s.count, sh, nr);
-    const int tk = taken0 + block_scan(s.take, sh, nt);
+    const int rs = row0 + block_scan<kPlanThreads>(s.count, sh, nr);
+    const int tk = taken0 + block_scan<kPlanThreads>(s.take, sh, nt);
     row0 += nr;
     taken0 += nt;
     if (b < a.B) {
@@ -402,11 +404,12 @@ __global__ __launch_bounds__(kAppendThreads) void ragged_append_kernel(AppendArg
 //
 // The host knows neither the lengths nor the counts, only bounds (rows T, sequences B),
 // so one workgroup forms the attention's work list from them: the tiles of every
-// sequence, the keys each attends, and with their sum the keys a unit takes so that
-// about `target` units a KV head come on top of one a tile: splits go to the tiles that
-// are longer than that.  Wide tiles come first, the last of a sequence (most keys) before
-// the others.
-constexpr int kUnitThreads = kPlanThreads;
+// sequence, the keys each attends, and from their costs (a wide tile's key counts `weight`
+// narrow ones) the share of a CU.  Tiles that cost more than a share (narrow ones, whose
+// partials are small: half of one) are split; so at most `target` = two units a CU come on
+// top of one a tile.  The list goes by cost, the largest first: the workgroups that start
+// last are short.
+constexpr int kUnitBuckets = 64;
 
 // Tiles of a sequence of R rows r: wide ones as long as more than `few` rows are left, then
 // narrow ones.
@@ -416,8 +419,9 @@ __device__ __forceinline__ int wide_tiles(const RaggedArgs& a, int R) {
 __device__ __forceinline__ int slim_tiles(const RaggedArgs& a, int R) {
   return R % a.ql > a.few ? 0 : (R % a.ql + a.qs - 1) / a.qs;
 }
+// A tile's keys: [lo, hi), kt of 32.
 struct UnitTile {
-  int seq, r0, lo, hi, wide;
+  int seq, r0, lo, hi, wide, kt;
 };
 template <typename BEFORE>
 __device__ __forceinline__ UnitTile unit_tile(const RaggedArgs& a, int t, int nwide, BEFORE&& before) {
@@ -425,26 +429,30 @@ __device__ __forceinline__ UnitTile unit_tile(const RaggedArgs& a, int t, int nw
   const int b = plan_find(a.B, i, [&](int s) { return before(s, kind); });
   const RaggedSeq s = ragged_seq(a, b);
   const int R = s.rows * a.G, rows = kind ? a.qs : a.ql;
-  const int n = kind ? slim_tiles(a, R) : wide_tiles(a, R);
-  const int r0 = (kind ? R / a.ql * a.ql : 0) + (n - 1 - (i - before(b, kind))) * rows;
+  const int r0 = (kind ? R / a.ql * a.ql : 0) + (i - before(b, kind)) * rows;
   const int r1 = min(r0 + rows, R) - 1;
   const int lo = ragged_lo(a, s.slot0 + r0 / a.G);
-  return {b, r0, lo, max(lo, ragged_hi(a, s.slot0 + r1 / a.G)), !kind};
+  const int hi = max(lo, ragged_hi(a, s.slot0 + r1 / a.G));
+  return {b, r0, lo, hi, !kind, (hi - lo + 31) >> 5};
 }
 
-__global__ __launch_bounds__(kUnitThreads) void ragged_units_kernel(RaggedArgs a) {
-  __shared__ int sh[kPlanWaves];
-  __shared__ unsigned long long s_sum;
+// NT threads of one workgroup.
+template <int NT>
+__device__ __forceinline__ void make_units(const RaggedArgs& a) {
+  __shared__ int sh[NT / 64], s_bucket[kUnitBuckets];
+  __shared__ unsigned long long s_cost;
   __shared__ int s_tiles[2 * (kPlanSeqs + 1)];
   const int tid = threadIdx.x;
   const bool in_lds = a.B <= kPlanSeqs;
+  if (tid == 0) s_cost = 0;
+  if (tid < kUnitBuckets) s_bucket[tid] = 0;
   int nwide = 0, nslim = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kUnitThreads) {
+  for (int b0 = 0; b0 < a.B; b0 += NT) {
     const int b = b0 + tid;
     const int R = b < a.B ? ragged_seq(a, b).rows * a.G : 0;
     int t0, t1;
-    const int w = nwide + block_scan(wide_tiles(a, R), sh, t0);
-    const int s = nslim + block_scan(slim_tiles(a, R), sh, t1);
+    const int w = nwide + block_scan<NT>(wide_tiles(a, R), sh, t0);
+    const int s = nslim + block_scan<NT>(slim_tiles(a, R), sh, t1);
     nwide += t0;
     nslim += t1;
     if (b < a.B) {
@@ -453,45 +461,81 @@ __global__ __launch_bounds__(kUnitThreads) void ragged_units_kernel(RaggedArgs a
       at[1] = s;
     }
   }
-  if (tid == 0) s_sum = 0;
   __threadfence_block();
   __syncthreads();
   const int ntiles = nwide + nslim;
   auto before = [&](int b, int kind) { return in_lds ? s_tiles[2 * b + kind] : a.tiles[2 * b + kind]; };
-  // keys in tiles of 32, all tiles' together
-  unsigned long long sum = 0;
-  for (int t = tid; t < ntiles; t += kUnitThreads) {
+  // (a batch of at most NT tiles keeps them; a larger one finds each again)
+  const bool once = ntiles <= NT;
+  UnitTile mine{};
+  unsigned long long cost = 0;
+  for (int t = tid; t < ntiles; t += NT) {
     const UnitTile u = unit_tile(a, t, nwide, before);
-    sum += (u.hi - u.lo + 31) >> 5;
+    if (once) mine = u;
+    cost += (unsigned)u.kt * (unsigned)(u.wide ? a.weight : 1);
   }
-  atomicAdd(&s_sum, sum);
+  atomicAdd(&s_cost, cost);
   __syncthreads();
-  const unsigned long long each = (s_sum + a.target - 1) / a.target;
-  const int chunk = max(a.min_keys >> 5, (int)min(each, 1ull << 26));
-  int nunits = 0, nparts = 0;
-  for (int t0 = 0; t0 < ntiles; t0 += kUnitThreads) {
+  // the keys (of 32) a unit takes at most: whole intervals of its kind
+  auto up = [](unsigned long long x, int n) { return (int)((min(x, 1ull << 26) + n - 1) / n * n); };
+  const unsigned long long half = (s_cost + a.target - 1) / a.target;
+  const int most_wide = up(max((2 * half + a.weight - 1) / a.weight, (unsigned long long)a.min_keys >> 5), 2);
+  const int most_slim = up(max(half, (unsigned long long)a.min_keys >> 5), 8);
+  const float top = (float)max(most_wide * a.weight, most_slim);
+  // how a tile is split: n units of `size`
+  auto split = [&](const UnitTile& u, int& size) {
+    const int most = u.wide ? most_wide : most_slim;
+    if (u.kt <= most) {
+      size = u.kt;
+      return 1;
+    }
+    const int n = (u.kt + most - 1) / most;
+    size = up((u.kt + n - 1) / n, u.wide ? 2 : 8);
+    return (u.kt + size - 1) / size;
+  };
+  auto bucket = [&](const UnitTile& u, int size) {
+    const float c = (float)(size * (u.wide ? a.weight : 1));
+    return max(0, kUnitBuckets - 1 - (int)(c / top * (kUnitBuckets - 1)));
+  };
+  for (int t = tid; t < ntiles; t += NT) {
+    const UnitTile u = once ? mine : unit_tile(a, t, nwide, before);
+    int size;
+    const int n = split(u, size);
+    atomicAdd(&s_bucket[bucket(u, size)], n);
+  }
+  __syncthreads();
+  if (tid < 64) {
+    const int n = s_bucket[tid], all = wave_scan(n);
+    s_bucket[tid] = all - n;
+    if (tid == 63) a.head->nunits = min(all, a.max_units);
+  }
+  __syncthreads();
+  int nparts = 0;
+  for (int t0 = 0; t0 < ntiles; t0 += NT) {
     const int t = t0 + tid;
     UnitTile u{};
-    int ns = 0, kt = 0;
+    int n = 0, size = 1;
     if (t < ntiles) {
-      u = unit_tile(a, t, nwide, before);
-      kt = (u.hi - u.lo + 31) >> 5;
-      ns = max(1, (kt + chunk - 1) / chunk);
+      u = once ? mine : unit_tile(a, t, nwide, before);
+      n = split(u, size);
     }
-    int all, parts;
-    const int at = nunits + block_scan(ns, sh, all);
-    const int pt = nparts + block_scan(ns > 1 ? ns : 0, sh, parts);
-    nunits += all;
+    int parts;
+    const int pt = nparts + block_scan<NT>(n > 1 ? n : 0, sh, parts);
     nparts += parts;
-    for (int i = 0; i < ns; ++i) {
-      if (at + i >= a.max_units || (ns > 1 && pt + i >= a.max_parts)) break;  // (never: the bounds hold)
-      const int lo = u.lo + (int)((int64_t)kt * i / ns) * 32;
-      const int hi = i + 1 < ns ? u.lo + (int)((int64_t)kt * (i + 1) / ns) * 32 : u.hi;
-      a.units[at + i] = RaggedUnit{u.seq, u.r0, lo, hi, ns > 1 ? pt + i : -1, i, ns, u.wide};
-      if (ns > 1) a.part_unit[pt + i] = at + i;
+    // (the order within a bucket is any: a unit's results do not depend on its place)
+    const int at = n ? atomicAdd(&s_bucket[bucket(u, size)], n) : 0;
+    for (int i = 0; i < n; ++i) {
+      if (at + i >= a.max_units || (n > 1 && pt + i >= a.max_parts)) break;  // (never: the bounds hold)
+      const int lo = u.lo + size * i * 32, hi = i + 1 < n ? lo + size * 32 : u.hi;
+      a.units[at + i] = RaggedUnit{u.seq, u.r0, lo, hi, n > 1 ? pt + i : -1, i, n, u.wide};
+      if (n > 1) a.part_unit[pt + i] = at + i;
     }
   }
-  if (tid == 0) *a.head = RaggedHead{min(nunits, a.max_units), min(nparts, a.max_parts), {0, 0}};
+  if (tid == 0) a.head->nparts = min(nparts, a.max_parts);
+}
+
+__global__ __launch_bounds__(kPlanThreads) void ragged_units_kernel(RaggedArgs a) {
+  make_units<kPlanThreads>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -646,6 +690,11 @@ struct Layout {
   }
 };
 
+// A wide tile's key against a narrow one's, us a key and CU at 32q/8kv/d128 bf16, fp32 and
+// Q8: 0.097, 0.117 and 0.085 (512 rows after 16384) against 0.032, 0.051 and 0.025 (64
+// sequences of one row).
+constexpr int kWideWeight = 3;
+
 int launch_attention(RaggedArgs a, void* stream) {
   LaunchLock lock(g_launch_mu);
   const int cus = num_cus();
@@ -660,6 +709,7 @@ int launch_attention(RaggedArgs a, void* stream) {
   a.qs = a.ql = a.slot_rows = kValuWaves;
   a.few = 0;  // every tile a wide one
   a.min_keys = 256;
+  a.weight = 1;
   int per_cu = 8;
   // (the matrix-core kernel's offsets within a block are of 32 bits)
   const int64_t block = ((int64_t)a.nkv << a.page_shift) * (4 * a.d);
@@ -670,6 +720,7 @@ int launch_attention(RaggedArgs a, void* stream) {
     a.qs = t.narrow;
     a.ql = t.wide;
     a.few = 2 * a.qs;
+    a.weight = kWideWeight;
     // (a tile holds no more rows than the batch)
     a.slot_rows = (int64_t)a.T * a.G <= a.few ? a.qs : a.ql;
     per_cu = 2;
@@ -696,7 +747,7 @@ int launch_attention(RaggedArgs a, void* stream) {
   a.part_unit = reinterpret_cast<int32_t*>(w + l.part_unit);
   a.part_ml = reinterpret_cast<float*>(w + l.part_ml);
   a.part_o = reinterpret_cast<float*>(w + l.part_o);
-  hipLaunchKernelGGL(ragged_units_kernel, dim3(1), dim3(kUnitThreads), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(ragged_units_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
   hipLaunchKernelGGL(attend, dim3((unsigned)(a.max_units * a.nkv)), dim3(threads), 0,
                      (hipStream_t)stream, a);
   if (a.max_parts)

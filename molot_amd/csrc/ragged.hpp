@@ -49,10 +49,10 @@ struct RaggedArgs {
   float* part_o;    // [part][nkv][slot_rows][D] unnormalised o
   float* part_ml;   // [part][nkv][slot_rows][2] (max in base 2, sum)
   int slot_rows;    // rows of a partial's slot
-  // Tiles: sequences of at most `few` rows r in tiles of qs rows, others of ql.
-  // Units: `target` of them (a KV head) beyond one a tile, of at least min_keys keys
-  // (multiples of 32).
-  int qs, ql, few, target, min_keys;
+  // Tiles: of ql rows r, and of qs for the last `few` of a sequence.
+  // Units: up to `target` of them (a KV head) beyond one a tile, of at least min_keys keys;
+  // a key costs a wide tile `weight` times a narrow one's.
+  int qs, ql, few, target, min_keys, weight;
   int max_units, max_parts;
 };
 

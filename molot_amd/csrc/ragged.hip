@@ -711,9 +711,10 @@ int launch_attention(RaggedArgs a, void* stream) {
   a.min_keys = 256;
   a.weight = 1;
   int per_cu = 8;
-  // (the matrix-core kernel's offsets within a block are of 32 bits)
-  const int64_t block = ((int64_t)a.nkv << a.page_shift) * (4 * a.d);
-  if (a.d <= 256 && a.d % 8 == 0 && block <= 0x7FFFFFFF) {
+  // (the matrix-core kernel's offsets are of 31 bits within a block, and of 35 in a pool)
+  const int64_t block = ((int64_t)a.nkv << a.page_shift) *
+                        (a.kv_dtype == MOLOT_KV_Q8 ? a.d + 4 : a.d * (a.kv_dtype == MOLOT_KV_BF16 ? 2 : 4));
+  if (a.d <= 256 && a.d % 8 == 0 && block <= 0x7FFFFFFF && a.num_blocks * block <= (8ll << 32)) {
     const RaggedTile t = ragged_tile(a.d, a.kv_dtype, a.softcap > 0.f || a.slopes);
     attend = t.fn;
     threads = t.threads;

@@ -49,7 +49,7 @@ __device__ __forceinline__ unsigned group_umax(unsigned v) {
   return v;
 }
 
-// Eight elements of a cached row as loaded, and (Q8) the row's scale in every lane of it.
+// Eight elements of a cached row as loaded.
 template <typename T>
 struct Raw;
 template <>
@@ -63,15 +63,15 @@ struct Raw<bf16_t> {
 template <>
 struct Raw<q8_t> {
   u32x2 x;
-  float scale;
 };
 
-// The pieces of eight elements, and the unit of their row: x = piece * unit.  LPR lanes
-// hold the row.  A NaN unit marks a row that the pieces cannot hold (own_mark).
+// The pieces of eight elements, and what the unit of their row (x = piece * unit) follows
+// from: the bits of its largest |x|, of Q8 rows whether it has a code but zero.  LPR lanes
+// hold the row.
 template <int NP>
 struct Pieces {
   u32x4 p[NP];
-  float unit;
+  unsigned top;
 };
 template <int LPR>
 __device__ __forceinline__ Pieces<2> make_pieces(const Raw<float>& r, int kv) {
@@ -92,9 +92,15 @@ __device__ __forceinline__ Pieces<2> make_pieces(const Raw<float>& r, int kv) {
     out.p[0][i] = hi;
     out.p[1][i] = lo;
   }
-  out.unit = (kv ? f16_vrow_unit(top, shift) : f16_row_unit(shift)) +
-             own_mark(top, m >= 0x7F800000u ? NAN : 0.f, kv);
+  out.top = m;
   return out;
+}
+// A NaN unit marks a row that the pieces cannot hold (own_mark).
+__device__ __forceinline__ float unit_of(float, unsigned m, int kv) {
+  const float top = __uint_as_float(m);
+  const int shift = kv ? f16_vrow_shift(top) : f16_row_shift(top);
+  return (kv ? f16_vrow_unit(top, shift) : f16_row_unit(shift)) +
+         own_mark(top, m >= 0x7F800000u ? NAN : 0.f, kv);
 }
 // bf16 to fp16 by its bits: with the row's largest exponent field e, off = max(e - 30, 0)
 // is taken from every exponent (fp16's 1 .. 30 then hold 30 binades, each value with
@@ -121,10 +127,13 @@ __device__ __forceinline__ Pieces<1> make_pieces(const Raw<bf16_t>& r, int kv) {
     y = y << (unsigned short)3;
     out.p[0][i] = (r.x[i] & 0x80008000u) | __builtin_bit_cast(uint32_t, y);
   }
-  const float top = __uint_as_float(m << 16);
-  const float unit = kv && m == 0 ? 0.f : __uint_as_float((off + 15u) << 23);  // 2^(off - 112)
-  out.unit = unit + own_mark(top, e == 255 ? NAN : 0.f, kv);
+  out.top = m;
   return out;
+}
+__device__ __forceinline__ float unit_of(bf16_t, unsigned m, int kv) {
+  const int e = (int)(m >> 7);
+  const float unit = kv && m == 0 ? 0.f : __uint_as_float((unsigned)(max(e - 30, 0) + 15) << 23);  // 2^(off - 112)
+  return unit + own_mark(__uint_as_float(m << 16), e == 255 ? NAN : 0.f, kv);
 }
 // Codes are exact in fp16: 0x6400 + (code ^ 0x80) is 1152 + code.
 template <int LPR>
@@ -137,14 +146,15 @@ __device__ __forceinline__ Pieces<1> make_pieces(const Raw<q8_t>& r, int kv) {
     const uint32_t b = __builtin_amdgcn_perm(0x64646464u, x, i & 1 ? 0x04030402u : 0x04010400u);
     out.p[0][i] = __builtin_bit_cast(uint32_t, (f16x2)(__builtin_bit_cast(f16x2, b) - bias));
   }
-  float unit = r.scale;
-  if (kv) {  // a row of zeros weighs nothing whatever its scale
-    const unsigned any = group_umax<LPR>(min(r.x[0] | r.x[1], 1u));
-    unit = any ? unit : 0.f;
-  }
-  const bool out_of = !(unit >= 0.f) || unit > kOwnMaxK * 0.0078125f || (kv && unit > 0.f && unit < kOwnMinV);
-  out.unit = unit + (out_of ? NAN : 0.f);
+  out.top = 1;
+  if (kv) out.top = group_umax<LPR>(min(r.x[0] | r.x[1], 1u));
   return out;
+}
+// (a row of zeros weighs nothing whatever its scale)
+__device__ __forceinline__ float q8_unit(float scale, unsigned any, int kv) {
+  const float unit = any ? scale : 0.f;
+  const bool out_of = !(unit >= 0.f) || unit > kOwnMaxK * 0.0078125f || (kv && unit > 0.f && unit < kOwnMinV);
+  return unit + (out_of ? NAN : 0.f);
 }
 
 // SC: scores past the product (a cap, slopes).
@@ -190,14 +200,16 @@ struct Tile {
     p.mask = (int)page - 1;
     return p;
   }
-  // Eight elements at byte `at` of row t in block blk.  (Lanes past d take the row's first:
-  // they meet zeros of q, or columns that are not stored.)  once: no other workgroup
-  // reads the row soon.
-  __device__ static __forceinline__ void load(const Pages& p, const char* pool, int blk, int t, unsigned at,
-                                              bool once, raw_t& r) {
-    const unsigned sl = (unsigned)(t & p.mask);
-    const char* b = pool + (uint64_t)(unsigned)blk * p.block;
-    const char* x = b + (p.head + sl * p.row + at);
+  // Where row t of block blk starts in a pool, and its Q8 scale.
+  __device__ static __forceinline__ uint64_t row_at(const Pages& p, int blk, int t) {
+    return (uint64_t)(unsigned)blk * p.block + (p.head + (unsigned)(t & p.mask) * p.row);
+  }
+  __device__ static __forceinline__ float scale_at(const Pages& p, const char* pool, int blk, int t) {
+    return *reinterpret_cast<const float*>(pool + (uint64_t)(unsigned)blk * p.block +
+                                           (p.scales + 4 * (unsigned)(t & p.mask)));
+  }
+  // Eight elements.  once: no other workgroup reads the row soon.
+  __device__ static __forceinline__ void load(const char* x, bool once, raw_t& r) {
     if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -209,20 +221,19 @@ struct Tile {
       r.x = once ? __builtin_nontemporal_load(v) : *v;
     } else {
       r.x = *reinterpret_cast<const u32x2*>(x);
-      r.scale = *reinterpret_cast<const float*>(b + (p.scales + 4 * sl));
     }
   }
   // N chunks of a thread into LDS: chunk i is unit j of row r + STEP*i of the tile (rows
-  // past it: of the next), r < KT, STEP a power of two past r or a multiple of KT.  units:
-  // the rows' units, the same in all their lanes.
+  // past it: of the next), r < KT, STEP a power of two past r or a multiple of KT.  tops:
+  // Pieces::top.
   template <int N, int STEP>
   __device__ static __forceinline__ void pieces(const raw_t (&raw)[N], int kv, int r, int j, char* tile,
-                                                float (&units)[N]) {
+                                                unsigned (&tops)[N]) {
     const int base = r * RB + 16 * (j ^ (kv ? wv_f<D>(r) : wk_f<D>(r)));
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const Pieces<NP> x = make_pieces<LPR>(raw[i], kv);
-      units[i] = x.unit;
+      tops[i] = x.top;
       // (the swizzle of row r + STEP*i is r's and STEP*i's by exclusive or)
       constexpr int M = KT - 1;
       const int up = STEP * i & M;
@@ -684,12 +695,15 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
     const int nint = (ntile + C::IT - 1) / C::IT;
     auto tile_buf = [&](int kv, int bf, int g) { return lds + ((kv * 2 + bf) * C::IT + g) * C::TB; };
     auto unit_buf = [&](int kv, int bf, int g) { return units + ((kv * 2 + bf) * C::IT + g) * KT; };
+    constexpr bool Q8 = std::is_same<T, q8_t>::value;
     typename C::raw_t kr[C::CW], vr[C::CW];
+    float ks[C::CW], vs[C::CW];  // (Q8)
     int blk[C::CW];
     // chunk i of this thread: unit j of row rr + STEP*i of the interval's tiles in a row
     constexpr int STEP = C::NT / LPR;
     static_assert(STEP % KT == 0 || C::IT == 1, "chunks of a thread: of tiles, or of one tile");
     const int rr = tid / LPR, j = tid % LPR;
+    // (lanes past d take the row's first: they meet zeros of q, or columns that are not stored)
     const unsigned at = 8 * j < a.d ? 8 * j * (unsigned)sizeof(T) : 0;
     auto key = [&](int it, int i) { return u.lo + KI * it + rr + STEP * i; };
     auto blocks = [&](int it) {
@@ -701,22 +715,35 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
 #pragma unroll
       for (int i = 0; i < C::CW; ++i) {
         const int t = min(key(it, i), last), b = valid(blk[i]);
-        C::load(pg, a.k, b, t, at, false, kr[i]);
-        C::load(pg, a.v, b, t, at, false, vr[i]);
+        const uint64_t row = C::row_at(pg, b, t) + at;
+        C::load(a.k + row, false, kr[i]);
+        C::load(a.v + row, false, vr[i]);
+        if constexpr (Q8) {
+          ks[i] = C::scale_at(pg, a.k, b, t);
+          vs[i] = C::scale_at(pg, a.v, b, t);
+        }
       }
       blocks(it + 1);
     };
     // (an interval's tiles lie one after the other, and their units)
     auto stage = [&](int it) {
-      float ku[C::CW], vu[C::CW];
+      unsigned ku[C::CW], vu[C::CW];
       const int r0 = rr % KT, g0 = rr / KT;
       C::template pieces<C::CW, STEP>(kr, 0, r0, j, tile_buf(0, it & 1, g0), ku);
       C::template pieces<C::CW, STEP>(vr, 1, r0, j, tile_buf(1, it & 1, g0), vu);
       if (j == 0) {
 #pragma unroll
         for (int i = 0; i < C::CW; ++i) {
-          unit_buf(0, it & 1, 0)[rr + STEP * i] = ku[i];
-          unit_buf(1, it & 1, 0)[rr + STEP * i] = vu[i];
+          float k, v;
+          if constexpr (Q8) {
+            k = q8_unit(ks[i], 1, 0);
+            v = q8_unit(vs[i], vu[i], 1);
+          } else {
+            k = unit_of(T{}, ku[i], 0);
+            v = unit_of(T{}, vu[i], 1);
+          }
+          unit_buf(0, it & 1, 0)[rr + STEP * i] = k;
+          unit_buf(1, it & 1, 0)[rr + STEP * i] = v;
         }
       }
     };
@@ -760,48 +787,64 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
     float* const ub = units + w * 2 * KT;
     // K and V each have their registers where those are few enough
     constexpr bool BOTH = C::CN * (int)sizeof(typename C::raw_t) <= 128;
+    constexpr bool Q8 = std::is_same<T, q8_t>::value;
     typename C::raw_t raw[BOTH ? 2 : 1][C::CN];
+    float scale[2];          // (Q8: of key lane % 32)
     constexpr int RPI = 64 / LPR;  // rows of a load
-    const int r_in = lane / LPR, j = lane % LPR;
+    const int r_in = lane / LPR, j = lane % LPR, key = lane & 31;
     const unsigned at = 8 * j < a.d ? 8 * j * (unsigned)sizeof(T) : 0;
-    auto ids = [&](int t) { return block_of(u.lo + t * KT + (lane & 31)); };
-    auto fetch = [&](int kv, int t, int id) {
+    const char *kp = a.k + at, *vp = a.v + at;
+    // A lane forms the place of one key, in units of 8 bytes, and the key's lanes take it
+    // from there.
+    auto ids = [&](int t) { return block_of(u.lo + t * KT + key); };
+    auto slot_of = [&](int t) { return min(u.lo + t * KT + key, last); };
+    auto place = [&](int t, int id) { return (unsigned)(C::row_at(pg, valid(id), slot_of(t)) >> 3); };
+    auto fetch = [&](int kv, int t, int id, unsigned off) {
 #pragma unroll
-      for (int i = 0; i < C::CN; ++i) {
-        const int rr = r_in + RPI * i;
-        C::load(pg, kv ? a.v : a.k, valid(__shfl(id, rr)), min(u.lo + t * KT + rr, last), at, true,
+      for (int i = 0; i < C::CN; ++i)
+        C::load((kv ? vp : kp) + ((uint64_t)(unsigned)__shfl((int)off, r_in + RPI * i) << 3), true,
                 raw[BOTH ? kv : 0][i]);
-      }
+      if constexpr (Q8) scale[kv] = C::scale_at(pg, kv ? a.v : a.k, valid(id), slot_of(t));
     };
     auto stage = [&](int kv) {
-      float unit[C::CN];
-      C::template pieces<C::CN, RPI>(raw[BOTH ? kv : 0], kv, r_in, j, buf, unit);
+      unsigned top[C::CN];
+      C::template pieces<C::CN, RPI>(raw[BOTH ? kv : 0], kv, r_in, j, buf, top);
+      float* const to = ub + kv * KT;
       if (j == 0) {
 #pragma unroll
-        for (int i = 0; i < C::CN; ++i) ub[kv * KT + r_in + RPI * i] = unit[i];
+        for (int i = 0; i < C::CN; ++i) to[r_in + RPI * i] = __uint_as_float(top[i]);
       }
       asm volatile("" ::: "memory");  // the wave's own LDS: in order
+      const unsigned mine = __float_as_uint(to[key]);
+      float unit;
+      if constexpr (Q8) unit = q8_unit(scale[kv], mine, kv);
+      else unit = unit_of(T{}, mine, kv);
+      to[key] = unit;  // (both lanes of a key the same)
+      asm volatile("" ::: "memory");
     };
     int id = 0, idn = 0;
+    unsigned off = 0;
     if (w < ntile) {
       id = ids(w);
-      fetch(0, w, id);
-      if (BOTH) fetch(1, w, id);
+      off = place(w, id);
+      fetch(0, w, id, off);
+      if (BOTH) fetch(1, w, id, off);
       idn = ids(w + C::NWN);
     }
     for (int t = w; t < ntile; t += C::NWN) {
       const bool more = t + C::NWN < ntile;
       stage(0);
-      if (!BOTH) fetch(1, t, id);
-      else if (more) fetch(0, t + C::NWN, idn);
+      if (!BOTH) fetch(1, t, id, off);
+      if (more) {
+        id = idn;
+        off = place(t + C::NWN, id);
+        idn = ids(t + 2 * C::NWN);
+        if (BOTH) fetch(0, t + C::NWN, id, off);
+      }
       x.scores(buf, lane);
       asm volatile("" ::: "memory");
       stage(1);
-      if (more) {
-        id = idn;
-        fetch(BOTH ? 1 : 0, t + C::NWN, id);
-        idn = ids(t + 2 * C::NWN);
-      }
+      if (more) fetch(BOTH ? 1 : 0, t + C::NWN, id, off);
       x.softmax(ub, ub + KT, u.lo + t * KT, lane);
       x.pv(buf, lane);
       asm volatile("" ::: "memory");

@@ -171,17 +171,24 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, i
   }
   const int top = count0 + give;
   // finished sequences' blocks above the stack's top (unused places if the plan fails)
+  // (a sequence's blocks by a wave: their number is uneven, and a lane each would wait for
+  // the longest)
   if (st == 0 && give > 0) {
     int base = count0;
     for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
       const PlanSeq s = plan_seq(a, b0 + tid);
       int all;
-      int at = base + block_scan<kPlanThreads>(s.give, sh, all);
+      const int at = base + block_scan<kPlanThreads>(s.give, sh, all);
       base += all;
-      for (int j = 0; j < s.give; ++j) {
-        const int id = a.block_table[(int64_t)(b0 + tid) * a.max_blocks + j];
-        if ((unsigned)id >= (unsigned)a.num_blocks) atomicMin(&s_st, MOLOT_EINVAL);
-        a.free_blocks[at + j] = id;
+      for (uint64_t left = __builtin_amdgcn_ballot_w64(s.give > 0); left; left &= left - 1) {
+        const int l = __builtin_ctzll(left);
+        const int n = __builtin_amdgcn_readlane(s.give, l), to = __builtin_amdgcn_readlane(at, l);
+        const int32_t* from = a.block_table + (int64_t)(b0 + (tid & ~63) + l) * a.max_blocks;
+        for (int j = tid & 63; j < n; j += 64) {
+          const int id = from[j];
+          if ((unsigned)id >= (unsigned)a.num_blocks) atomicMin(&s_st, MOLOT_EINVAL);
+          a.free_blocks[to + j] = id;
+        }
       }
     }
     __threadfence_block();
@@ -240,163 +247,6 @@ __global__ __launch_bounds__(256) void ragged_rows_kernel(PlanArgs a) {
   const int b = plan_find(a.B, r, [&](int i) { return a.row_start[i]; });
   const int start = a.row_start[b];
   plan_row(a, r, b, start, a.kv_lens[b] - (a.row_start[b + 1] - start), a.taken[b], a.taken[a.B]);
-}
-
-// ---------------------------------------------------------------------------
-// Norms, RoPE and append of the packed rows: row r's heads normed and rotated at
-// row_pos[r], k and v stored at row_slot[r] (< 0: the row is left as it is).  A
-// workgroup takes some heads of a row, its waves a head at a time, lane l the pairs
-// l, l + 64, ...; angles, sums and roundings are those of rope_append_tok_kernel.
-struct AppendArgs {
-  float* q;
-  const float* k_new;  // NULL: q alone
-  const float* v_new;
-  char* K;
-  char* V;
-  const int32_t* row_pos;
-  const int32_t* row_slot;
-  const float* q_norm;
-  const float* k_norm;
-  const float* inv_freq;
-  int nq, nkv, d, page_shift, v_norm, kv_dtype;
-  int64_t slots;  // of the pool
-  float eps;
-};
-constexpr int kAppendThreads = 256, kAppendWaves = kAppendThreads / 64;
-
-template <int KMAX>
-__global__ __launch_bounds__(kAppendThreads) void ragged_append_kernel(AppendArgs a) {
-  __shared__ float cs_s[64 * KMAX], sn_s[64 * KMAX];
-  const int r = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int half = a.d >> 1;
-  const int64_t at = a.row_slot[r];
-  if (at < 0 || at >= a.slots) return;  // (the whole workgroup)
-  const int pos = a.row_pos[r];
-  const bool rot = a.inv_freq != nullptr;
-  for (int i = tid; rot && i < half; i += kAppendThreads) {
-    const float ang = (float)pos * a.inv_freq[i];
-    double sd, cd;
-    sincos((double)ang, &sd, &cd);
-    cs_s[i] = (float)cd;
-    sn_s[i] = (float)sd;
-  }
-  __syncthreads();
-  auto rms_inv = [&](float ss, int n) { return 1.0f / sqrtf(ss / (float)n + a.eps); };
-  const int heads = a.nq + (a.k_new ? a.nkv : 0);
-  const int step = kAppendWaves * gridDim.y;
-  for (int hh = blockIdx.y * kAppendWaves + w; hh < heads; hh += step) {
-    const bool isq = hh < a.nq;
-    const int kh = hh - a.nq;
-    const float* x = isq ? a.q + ((int64_t)r * a.nq + hh) * a.d
-                         : a.k_new + ((int64_t)r * a.nkv + kh) * a.d;
-    const float* weight = isq ? a.q_norm : a.k_norm;
-    const float* vx = a.v_new + ((int64_t)r * a.nkv + kh) * a.d;  // (not read for q)
-    float x0[KMAX], x1[KMAX], v0[KMAX], v1[KMAX];
-#pragma unroll
-    for (int k = 0; k < KMAX; ++k) {
-      const int j = lane + 64 * k;
-      const bool in = j < half;
-      x0[k] = in ? x[j] : 0.f;
-      x1[k] = in ? x[j + half] : 0.f;
-      v0[k] = in && !isq ? vx[j] : 0.f;
-      v1[k] = in && !isq ? vx[j + half] : 0.f;
-    }
-    if (weight) {
-      float ss = 0.f;
-#pragma unroll
-      for (int k = 0; k < KMAX; ++k)
-        if (64 * k < half) ss += group_sum<64>(x0[k] * x0[k] + x1[k] * x1[k]);
-      const float inv = rms_inv(ss, a.d);
-#pragma unroll
-      for (int k = 0; k < KMAX; ++k) {
-        const int j = min(lane + 64 * k, half - 1);
-        x0[k] = x0[k] * inv * weight[j];
-        x1[k] = x1[k] * inv * weight[j + half];
-      }
-    }
-    float r0[KMAX], r1[KMAX];
-#pragma unroll
-    for (int k = 0; k < KMAX; ++k) {
-      const int j = min(lane + 64 * k, half - 1);
-      r0[k] = rot ? x0[k] * cs_s[j] - x1[k] * sn_s[j] : x0[k];
-      r1[k] = rot ? x0[k] * sn_s[j] + x1[k] * cs_s[j] : x1[k];
-    }
-    if (isq) {
-      float* y = a.q + ((int64_t)r * a.nq + hh) * a.d;
-#pragma unroll
-      for (int k = 0; k < KMAX; ++k) {
-        const int j = lane + 64 * k;
-        if (j < half) {
-          y[j] = r0[k];
-          y[j + half] = r1[k];
-        }
-      }
-      continue;
-    }
-    if (a.v_norm) {  // one RMS over the row's nkv*d values
-      const float* vall = a.v_new + (int64_t)r * a.nkv * a.d;
-      float part = 0.f;
-      for (int j = lane; j < a.nkv * a.d; j += 64) part = fmaf(vall[j], vall[j], part);
-      const float inv = rms_inv(group_sum<64>(part), a.nkv * a.d);
-#pragma unroll
-      for (int k = 0; k < KMAX; ++k) {
-        v0[k] *= inv;
-        v1[k] *= inv;
-      }
-    }
-    const int page = 1 << a.page_shift, sl = (int)(at & (page - 1));
-    const int64_t blk = at >> a.page_shift, rows = (int64_t)a.nkv * page;
-    const int64_t in_block = ((int64_t)kh * page + sl) * a.d;
-    if (a.kv_dtype == MOLOT_KV_Q8) {
-      float kmax = 0.f, vmax = 0.f;
-#pragma unroll
-      for (int k = 0; k < KMAX; ++k) {
-        if (lane + 64 * k >= half) continue;
-        kmax = fmaxf(kmax, fmaxf(fabsf(r0[k]), fabsf(r1[k])));
-        vmax = fmaxf(vmax, fmaxf(fabsf(v0[k]), fabsf(v1[k])));
-      }
-      const float ks = q8_scale(group_max<64>(kmax)), vs = q8_scale(group_max<64>(vmax));
-      const int64_t b0 = blk * rows * (a.d + 4), so = b0 + rows * a.d + 4 * ((int64_t)kh * page + sl);
-      int8_t* kd = reinterpret_cast<int8_t*>(a.K) + b0 + in_block;
-      int8_t* vd = reinterpret_cast<int8_t*>(a.V) + b0 + in_block;
-#pragma unroll
-      for (int k = 0; k < KMAX; ++k) {
-        const int j = lane + 64 * k;
-        if (j >= half) continue;
-        kd[j] = (int8_t)q8_code(r0[k], ks);
-        kd[j + half] = (int8_t)q8_code(r1[k], ks);
-        vd[j] = (int8_t)q8_code(v0[k], vs);
-        vd[j + half] = (int8_t)q8_code(v1[k], vs);
-      }
-      if (lane == 0) {
-        *reinterpret_cast<float*>(a.K + so) = ks;
-        *reinterpret_cast<float*>(a.V + so) = vs;
-      }
-      continue;
-    }
-    const int64_t off = blk * rows * a.d + in_block;
-#pragma unroll
-    for (int k = 0; k < KMAX; ++k) {
-      const int j = lane + 64 * k;
-      if (j >= half) continue;
-      if (a.kv_dtype == MOLOT_KV_F32) {
-        float* kd = reinterpret_cast<float*>(a.K) + off;
-        float* vd = reinterpret_cast<float*>(a.V) + off;
-        kd[j] = r0[k];
-        kd[j + half] = r1[k];
-        vd[j] = v0[k];
-        vd[j + half] = v1[k];
-      } else {
-        uint16_t* kd = reinterpret_cast<uint16_t*>(a.K) + off;
-        uint16_t* vd = reinterpret_cast<uint16_t*>(a.V) + off;
-        kd[j] = f32_to_bf16(r0[k]);
-        kd[j + half] = f32_to_bf16(r1[k]);
-        vd[j] = f32_to_bf16(v0[k]);
-        vd[j + half] = f32_to_bf16(v1[k]);
-      }
-    }
-  }
 }
 
 // ---------------------------------------------------------------------------
@@ -539,6 +389,168 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_units_kernel(RaggedArgs a
 }
 
 // ---------------------------------------------------------------------------
+// Norms, RoPE and append of the packed rows: row r's heads normed and rotated at
+// row_pos[r], k and v stored at row_slot[r] (< 0: the row is left as it is).  A
+// workgroup takes some heads of a row, its waves a head at a time, lane l the pairs
+// l, l + 64, ...; angles, sums and roundings are those of rope_append_tok_kernel.
+struct AppendArgs {
+  float* q;
+  const float* k_new;  // NULL: q alone
+  const float* v_new;
+  char* K;
+  char* V;
+  const int32_t* row_pos;
+  const int32_t* row_slot;
+  const float* q_norm;
+  const float* k_norm;
+  const float* inv_freq;
+  int nq, nkv, d, page_shift, v_norm, kv_dtype;
+  int64_t slots;  // of the pool
+  float eps;
+};
+constexpr int kAppendThreads = 256, kAppendWaves = kAppendThreads / 64;
+
+// UNITS: a step's; one more workgroup forms the attention's units meanwhile.
+template <int KMAX, bool UNITS>
+__global__ __launch_bounds__(kAppendThreads) void ragged_append_kernel(AppendArgs a, RaggedArgs u) {
+  __shared__ float cs_s[64 * KMAX], sn_s[64 * KMAX];
+  if (UNITS && blockIdx.x == 0) {
+    if (blockIdx.y == 0) make_units<kAppendThreads>(u);
+    return;
+  }
+  const int r = UNITS ? (int)blockIdx.x - 1 : (int)blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int half = a.d >> 1;
+  const int64_t at = a.row_slot[r];
+  if (at < 0 || at >= a.slots) return;  // (the whole workgroup)
+  const int pos = a.row_pos[r];
+  const bool rot = a.inv_freq != nullptr;
+  for (int i = tid; rot && i < half; i += kAppendThreads) {
+    const float ang = (float)pos * a.inv_freq[i];
+    double sd, cd;
+    sincos((double)ang, &sd, &cd);
+    cs_s[i] = (float)cd;
+    sn_s[i] = (float)sd;
+  }
+  __syncthreads();
+  auto rms_inv = [&](float ss, int n) { return 1.0f / sqrtf(ss / (float)n + a.eps); };
+  const int heads = a.nq + (a.k_new ? a.nkv : 0);
+  const int step = kAppendWaves * gridDim.y;
+  for (int hh = blockIdx.y * kAppendWaves + w; hh < heads; hh += step) {
+    const bool isq = hh < a.nq;
+    const int kh = hh - a.nq;
+    const float* x = isq ? a.q + ((int64_t)r * a.nq + hh) * a.d
+                         : a.k_new + ((int64_t)r * a.nkv + kh) * a.d;
+    const float* weight = isq ? a.q_norm : a.k_norm;
+    const float* vx = a.v_new + ((int64_t)r * a.nkv + kh) * a.d;  // (not read for q)
+    float x0[KMAX], x1[KMAX], v0[KMAX], v1[KMAX];
+#pragma unroll
+    for (int k = 0; k < KMAX; ++k) {
+      const int j = lane + 64 * k;
+      const bool in = j < half;
+      x0[k] = in ? x[j] : 0.f;
+      x1[k] = in ? x[j + half] : 0.f;
+      v0[k] = in && !isq ? vx[j] : 0.f;
+      v1[k] = in && !isq ? vx[j + half] : 0.f;
+    }
+    if (weight) {
+      float ss = 0.f;
+#pragma unroll
+      for (int k = 0; k < KMAX; ++k)
+        if (64 * k < half) ss += group_sum<64>(x0[k] * x0[k] + x1[k] * x1[k]);
+      const float inv = rms_inv(ss, a.d);
+#pragma unroll
+      for (int k = 0; k < KMAX; ++k) {
+        const int j = min(lane + 64 * k, half - 1);
+        x0[k] = x0[k] * inv * weight[j];
+        x1[k] = x1[k] * inv * weight[j + half];
+      }
+    }
+    float r0[KMAX], r1[KMAX];
+#pragma unroll
+    for (int k = 0; k < KMAX; ++k) {
+      const int j = min(lane + 64 * k, half - 1);
+      r0[k] = rot ? x0[k] * cs_s[j] - x1[k] * sn_s[j] : x0[k];
+      r1[k] = rot ? x0[k] * sn_s[j] + x1[k] * cs_s[j] : x1[k];
+    }
+    if (isq) {
+      float* y = a.q + ((int64_t)r * a.nq + hh) * a.d;
+#pragma unroll
+      for (int k = 0; k < KMAX; ++k) {
+        const int j = lane + 64 * k;
+        if (j < half) {
+          y[j] = r0[k];
+          y[j + half] = r1[k];
+        }
+      }
+      continue;
+    }
+    if (a.v_norm) {  // one RMS over the row's nkv*d values
+      const float* vall = a.v_new + (int64_t)r * a.nkv * a.d;
+      float part = 0.f;
+      for (int j = lane; j < a.nkv * a.d; j += 64) part = fmaf(vall[j], vall[j], part);
+      const float inv = rms_inv(group_sum<64>(part), a.nkv * a.d);
+#pragma unroll
+      for (int k = 0; k < KMAX; ++k) {
+        v0[k] *= inv;
+        v1[k] *= inv;
+      }
+    }
+    const int page = 1 << a.page_shift, sl = (int)(at & (page - 1));
+    const int64_t blk = at >> a.page_shift, rows = (int64_t)a.nkv * page;
+    const int64_t in_block = ((int64_t)kh * page + sl) * a.d;
+    if (a.kv_dtype == MOLOT_KV_Q8) {
+      float kmax = 0.f, vmax = 0.f;
+#pragma unroll
+      for (int k = 0; k < KMAX; ++k) {
+        if (lane + 64 * k >= half) continue;
+        kmax = fmaxf(kmax, fmaxf(fabsf(r0[k]), fabsf(r1[k])));
+        vmax = fmaxf(vmax, fmaxf(fabsf(v0[k]), fabsf(v1[k])));
+      }
+      const float ks = q8_scale(group_max<64>(kmax)), vs = q8_scale(group_max<64>(vmax));
+      const int64_t b0 = blk * rows * (a.d + 4), so = b0 + rows * a.d + 4 * ((int64_t)kh * page + sl);
+      int8_t* kd = reinterpret_cast<int8_t*>(a.K) + b0 + in_block;
+      int8_t* vd = reinterpret_cast<int8_t*>(a.V) + b0 + in_block;
+#pragma unroll
+      for (int k = 0; k < KMAX; ++k) {
+        const int j = lane + 64 * k;
+        if (j >= half) continue;
+        kd[j] = (int8_t)q8_code(r0[k], ks);
+        kd[j + half] = (int8_t)q8_code(r1[k], ks);
+        vd[j] = (int8_t)q8_code(v0[k], vs);
+        vd[j + half] = (int8_t)q8_code(v1[k], vs);
+      }
+      if (lane == 0) {
+        *reinterpret_cast<float*>(a.K + so) = ks;
+        *reinterpret_cast<float*>(a.V + so) = vs;
+      }
+      continue;
+    }
+    const int64_t off = blk * rows * a.d + in_block;
+#pragma unroll
+    for (int k = 0; k < KMAX; ++k) {
+      const int j = lane + 64 * k;
+      if (j >= half) continue;
+      if (a.kv_dtype == MOLOT_KV_F32) {
+        float* kd = reinterpret_cast<float*>(a.K) + off;
+        float* vd = reinterpret_cast<float*>(a.V) + off;
+        kd[j] = r0[k];
+        kd[j + half] = r1[k];
+        vd[j] = v0[k];
+        vd[j + half] = v1[k];
+      } else {
+        uint16_t* kd = reinterpret_cast<uint16_t*>(a.K) + off;
+        uint16_t* vd = reinterpret_cast<uint16_t*>(a.V) + off;
+        kd[j] = f32_to_bf16(r0[k]);
+        kd[j + half] = f32_to_bf16(r1[k]);
+        vd[j] = f32_to_bf16(v0[k]);
+        vd[j + half] = f32_to_bf16(v1[k]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Attention of any head dim and cache type: a unit's rows a wave each (ragged_own_row).
 // What bounds it: the latency of a key's rows and of the wave's sum, two keys at a time;
 // the units' splits fill the chip.
@@ -657,15 +669,18 @@ int check_ragged(int nq, int nkv, int d, int page, int num_blocks, int kv_dtype)
   return 0;
 }
 
-int launch_append(AppendArgs a, int T, void* stream) {
+// units: a step's attention, whose units the launch forms too (NULL: none).
+int launch_append(AppendArgs a, int T, const RaggedArgs* units, void* stream) {
   const int heads = a.nq + (a.k_new ? a.nkv : 0);
   const int most = (heads + kAppendWaves - 1) / kAppendWaves;
   // workgroups a row: enough for the chip where the rows are few
   const int y = std::max(1, std::min({most, 1024 / T, 64}));
   const int half = a.d / 2;
-  auto k = half <= 64 ? ragged_append_kernel<1>
-           : half <= 128 ? ragged_append_kernel<2> : ragged_append_kernel<4>;
-  hipLaunchKernelGGL(k, dim3(T, y), dim3(kAppendThreads), 0, (hipStream_t)stream, a);
+  auto k = half <= 64    ? units ? ragged_append_kernel<1, true> : ragged_append_kernel<1, false>
+           : half <= 128 ? units ? ragged_append_kernel<2, true> : ragged_append_kernel<2, false>
+           : units       ? ragged_append_kernel<4, true> : ragged_append_kernel<4, false>;
+  hipLaunchKernelGGL(k, dim3(T + (units ? 1 : 0), y), dim3(kAppendThreads), 0, (hipStream_t)stream, a,
+                     units ? *units : RaggedArgs{});
   return (int)hipGetLastError();
 }
 
@@ -695,7 +710,8 @@ struct Layout {
 // sequences of one row).
 constexpr int kWideWeight = 3;
 
-int launch_attention(RaggedArgs a, void* stream) {
+// append, T rows: a step's, before the attention.
+int launch_attention(RaggedArgs a, const AppendArgs* append, void* stream) {
   LaunchLock lock(g_launch_mu);
   const int cus = num_cus();
   const int D = a.d <= 64 ? 64 : a.d <= 128 ? 128 : a.d <= 256 ? 256 : 512;
@@ -721,6 +737,7 @@ int launch_attention(RaggedArgs a, void* stream) {
     a.qs = t.narrow;
     a.ql = t.wide;
     a.few = 2 * a.qs;
+    a.min_keys = 512;
     a.weight = kWideWeight;
     // (a tile holds no more rows than the batch)
     a.slot_rows = (int64_t)a.T * a.G <= a.few ? a.qs : a.ql;
@@ -748,7 +765,12 @@ int launch_attention(RaggedArgs a, void* stream) {
   a.part_unit = reinterpret_cast<int32_t*>(w + l.part_unit);
   a.part_ml = reinterpret_cast<float*>(w + l.part_ml);
   a.part_o = reinterpret_cast<float*>(w + l.part_o);
-  hipLaunchKernelGGL(ragged_units_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
+  if (append) {
+    const int sa = launch_append(*append, a.T, &a, stream);
+    if (sa) return sa;
+  } else {
+    hipLaunchKernelGGL(ragged_units_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
+  }
   hipLaunchKernelGGL(attend, dim3((unsigned)(a.max_units * a.nkv)), dim3(threads), 0,
                      (hipStream_t)stream, a);
   if (a.max_parts)
@@ -875,7 +897,7 @@ int molot_hip_rope_append_ragged(float* q, const float* k_new, const float* v_ne
   const int st = append_args(a, q, k_new, v_new, K, V, row_pos, row_slot, T, num_blocks, nq, nkv, d,
                              page, q_norm, k_norm, v_norm, eps, inv_freq, kv_dtype);
   if (st || T == 0) return st;
-  return launch_append(a, T, stream);
+  return launch_append(a, T, nullptr, stream);
 }
 
 int molot_hip_attn_ragged(const float* Q, const void* K, const void* V, float* O,
@@ -888,7 +910,7 @@ int molot_hip_attn_ragged(const float* Q, const void* K, const void* V, float* O
                                 num_blocks, max_len, nq, nkv, d, page, scale, window, softcap,
                                 slopes, kv_dtype);
   if (st || T == 0 || B == 0) return st;
-  return launch_attention(a, stream);
+  return launch_attention(a, nullptr, stream);
 }
 
 int molot_hip_step_ragged(float* q, const float* k_new, const float* v_new, void* K, void* V,
@@ -907,9 +929,7 @@ int molot_hip_step_ragged(float* q, const float* k_new, const float* v_new, void
   st = append_args(r, q, k_new, v_new, K, V, row_pos, row_slot, T, num_blocks, nq, nkv, d, page,
                    q_norm, k_norm, v_norm, eps, inv_freq, kv_dtype);
   if (st || T == 0 || B == 0) return st;
-  LaunchLock lock(g_launch_mu);
-  st = launch_append(r, T, stream);
-  return st ? st : launch_attention(a, stream);
+  return launch_attention(a, &r, stream);
 }
 
 }  // extern "C"

@@ -75,27 +75,26 @@ struct PlanSeq {
   int len, count, take, give, st;
 };
 __device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int b) {
-  PlanSeq s{};
-  if (b >= a.B) return s;
-  const int len = a.seq_lens[b], count = a.counts[b];
-  const bool done = a.done && a.done[b] != 0;
+  const bool in = b < a.B;
+  const int i = in ? b : 0;  // (B > 0)
+  const int len = a.seq_lens[i], count = in ? a.counts[i] : 0;
+  const bool done = a.done && a.done[i] != 0;
   const int64_t cap = (int64_t)a.max_blocks << a.page_shift;
-  const int64_t from = done ? 0 : len;
-  if (len < 0 || count < 0 || len > cap || from + count > cap) {
-    s.st = MOLOT_EINVAL;
-    return s;
-  }
-  if (count > a.max_rows) {
-    s.st = MOLOT_E2BIG;
-    return s;
-  }
+  const int64_t from = done || !in ? 0 : len;
   const int r = (1 << a.page_shift) - 1;
   auto blocks = [&](int64_t n) { return (int)((n + r) >> a.page_shift); };
-  s.len = (int)from;
-  s.count = count;
-  if (a.free_blocks) {
-    s.take = blocks(from + count) - blocks(from);
-    s.give = done ? blocks(len) : 0;
+  PlanSeq s{};
+  if (in && (len < 0 || count < 0 || len > cap || from + count > cap)) {
+    s.st = MOLOT_EINVAL;
+  } else if (count > a.max_rows) {
+    s.st = MOLOT_E2BIG;
+  } else {
+    s.len = (int)from;
+    s.count = count;
+    if (a.free_blocks) {
+      s.take = blocks(from + count) - blocks(from);
+      s.give = in && done ? blocks(len) : 0;
+    }
   }
   return s;
 }
@@ -136,40 +135,61 @@ __device__ __forceinline__ int plan_find(int B, int r, START&& start) {
   return lo;
 }
 
-// Sums that saturate (each at most 2^30).
-__device__ __forceinline__ int plan_sum(int x, int y) { return min((unsigned)x + (unsigned)y, 1u << 30); }
+// Sequences b0 + tid, b0 + kPlanThreads + tid, ...: their loads in flight together.
+constexpr int kPlanBatch = 5;  // (of a batch of more than kPlanThreads)
+template <int N>
+__device__ __forceinline__ void plan_batch(const PlanArgs& a, int b0, PlanSeq (&s)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = plan_seq(a, b0 + kPlanThreads * i + (int)threadIdx.x);
+}
 
 // One workgroup.  `rows`: it writes the rows' maps too, else ragged_rows_kernel does.
+template <int N>
 __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, int rows) {
   __shared__ int sh[kPlanThreads / 64], s_st;
+  __shared__ unsigned long long s_sum[3];
   __shared__ int s_start[kPlanSeqs + 1], s_taken[kPlanSeqs];
   const int tid = threadIdx.x;
   const bool pool = a.free_blocks != nullptr;
   const int count0 = pool ? *a.free_count : 0;
+  if (tid < 3) s_sum[tid] = 0;
   if (tid == 0) s_st = 0;
   // totals, and whether the batch fits
-  int nrows = 0, take = 0, give = 0, st = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
-    const PlanSeq s = plan_seq(a, b0 + tid);
-    if (s.st) st = s.st;
-    int t0, t1, t2;
-    (void)block_scan<kPlanThreads>(s.count, sh, t0);
-    (void)block_scan<kPlanThreads>(s.take, sh, t1);
-    (void)block_scan<kPlanThreads>(s.give, sh, t2);
-    nrows = plan_sum(nrows, t0);
-    take = plan_sum(take, t1);
-    give = plan_sum(give, t2);
+  unsigned long long nrows = 0, take = 0, give = 0;  // (lane 63's are the wave's)
+  int st = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads * N) {
+    PlanSeq s[N];
+    plan_batch(a, b0, s);
+    int x = 0, y = 0, z = 0;  // (each at most N * kPlanMost: a wave's sum stays below 2^31)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (s[i].st) st = s[i].st;
+      x += s[i].count;
+      y += s[i].take;
+      z += s[i].give;
+    }
+    nrows += wave_scan(x);
+    take += wave_scan(y);
+    give += wave_scan(z);
   }
   __syncthreads();
   if (st) atomicMin(&s_st, st);  // of several, the same one whatever the order
-  __syncthreads();
-  st = s_st;
-  if (st == 0 && nrows > a.max_rows) st = MOLOT_E2BIG;
-  if (pool && st == 0) {
-    if (count0 < 0 || give > a.num_blocks || count0 > a.num_blocks - give) st = MOLOT_EINVAL;
-    else if (take > count0 + give) st = MOLOT_ENOSPC;
+  if ((tid & 63) == 63) {
+    atomicAdd(&s_sum[0], nrows);
+    atomicAdd(&s_sum[1], take);
+    atomicAdd(&s_sum[2], give);
   }
-  const int top = count0 + give;
+  __syncthreads();
+  nrows = s_sum[0], take = s_sum[1], give = s_sum[2];
+  st = s_st;
+  if (st == 0 && nrows > (unsigned long long)a.max_rows) st = MOLOT_E2BIG;
+  if (pool && st == 0) {
+    if (count0 < 0 || give > (unsigned long long)a.num_blocks || count0 > a.num_blocks - (int)give)
+      st = MOLOT_EINVAL;
+    else if (take > (unsigned long long)count0 + give)
+      st = MOLOT_ENOSPC;
+  }
+  const int top = count0 + (int)(st ? 0 : give);
   // finished sequences' blocks above the stack's top (unused places if the plan fails)
   // (a sequence's blocks by a wave: their number is uneven, and a lane each would wait for
   // the longest)
@@ -197,23 +217,28 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, i
   }
   // the batch as it will be
   int row0 = 0, taken0 = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
-    const int b = b0 + tid;
-    const int was = b < a.B ? a.seq_lens[b] : 0;
-    PlanSeq s = plan_seq(a, b);
-    if (st) s = PlanSeq{was, 0, 0, 0, 0};
-    int nr, nt;
-    const int rs = row0 + block_scan<kPlanThreads>(s.count, sh, nr);
-    const int tk = taken0 + block_scan<kPlanThreads>(s.take, sh, nt);
-    row0 += nr;
-    taken0 += nt;
-    if (b < a.B) {
-      a.row_start[b] = rs;
-      a.kv_lens[b] = s.len + s.count;
-      if (!rows) a.taken[b] = tk;
-      if (rows && b < kPlanSeqs) {
-        s_start[b] = rs;
-        s_taken[b] = tk;
+  for (int b1 = 0; b1 < a.B; b1 += kPlanThreads * N) {
+    PlanSeq all[N];
+    plan_batch(a, b1, all);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int b = b1 + kPlanThreads * i + tid;
+      if (b1 + kPlanThreads * i >= a.B) break;  // (the whole workgroup)
+      PlanSeq s = all[i];
+      if (st) s = PlanSeq{b < a.B ? a.seq_lens[b] : 0, 0, 0, 0, 0};
+      int nr, nt;
+      const int rs = row0 + block_scan<kPlanThreads>(s.count, sh, nr);
+      const int tk = taken0 + block_scan<kPlanThreads>(s.take, sh, nt);
+      row0 += nr;
+      taken0 += nt;
+      if (b < a.B) {
+        a.row_start[b] = rs;
+        a.kv_lens[b] = s.len + s.count;
+        if (!rows) a.taken[b] = tk;
+        if (rows && b < kPlanSeqs) {
+          s_start[b] = rs;
+          s_taken[b] = tk;
+        }
       }
     }
   }
@@ -272,6 +297,7 @@ __device__ __forceinline__ int slim_tiles(const RaggedArgs& a, int R) {
 // A tile's keys: [lo, hi), kt of 32.
 struct UnitTile {
   int seq, r0, lo, hi, wide, kt;
+  RaggedSeq s;
 };
 template <typename BEFORE>
 __device__ __forceinline__ UnitTile unit_tile(const RaggedArgs& a, int t, int nwide, BEFORE&& before) {
@@ -283,7 +309,7 @@ __device__ __forceinline__ UnitTile unit_tile(const RaggedArgs& a, int t, int nw
   const int r1 = min(r0 + rows, R) - 1;
   const int lo = ragged_lo(a, s.slot0 + r0 / a.G);
   const int hi = max(lo, ragged_hi(a, s.slot0 + r1 / a.G));
-  return {b, r0, lo, hi, !kind, (hi - lo + 31) >> 5};
+  return {b, r0, lo, hi, !kind, (hi - lo + 31) >> 5, s};
 }
 
 // NT threads of one workgroup.
@@ -377,7 +403,7 @@ __device__ __forceinline__ void make_units(const RaggedArgs& a) {
     for (int i = 0; i < n; ++i) {
       if (at + i >= a.max_units || (n > 1 && pt + i >= a.max_parts)) break;  // (never: the bounds hold)
       const int lo = u.lo + size * i * 32, hi = i + 1 < n ? lo + size * 32 : u.hi;
-      a.units[at + i] = RaggedUnit{u.seq, u.r0, lo, hi, n > 1 ? pt + i : -1, i, n, u.wide};
+      a.units[at + i] = RaggedUnit{u.seq, u.r0, lo, hi, n > 1 ? pt + i : -1, i, n, u.wide, u.s, 0};
       if (n > 1) a.part_unit[pt + i] = at + i;
     }
   }
@@ -391,8 +417,8 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_units_kernel(RaggedArgs a
 // ---------------------------------------------------------------------------
 // Norms, RoPE and append of the packed rows: row r's heads normed and rotated at
 // row_pos[r], k and v stored at row_slot[r] (< 0: the row is left as it is).  A
-// workgroup takes some heads of a row, its waves a head at a time, lane l the pairs
-// l, l + 64, ...; angles, sums and roundings are those of rope_append_tok_kernel.
+// wave takes some heads of a row, lane l the pairs l, l + 64, ...; angles, sums and
+// roundings are those of rope_append_tok_kernel.
 struct AppendArgs {
   float* q;
   const float* k_new;  // NULL: q alone
@@ -405,54 +431,76 @@ struct AppendArgs {
   const float* k_norm;
   const float* inv_freq;
   int nq, nkv, d, page_shift, v_norm, kv_dtype;
+  int each;  // heads a wave
   int64_t slots;  // of the pool
   float eps;
 };
-constexpr int kAppendThreads = 256, kAppendWaves = kAppendThreads / 64;
+constexpr int kAppendThreads = 256, kAppendWaves = kAppendThreads / 64, kAppendHeads = 10;
 
 // UNITS: a step's; one more workgroup forms the attention's units meanwhile.
 template <int KMAX, bool UNITS>
 __global__ __launch_bounds__(kAppendThreads) void ragged_append_kernel(AppendArgs a, RaggedArgs u) {
-  __shared__ float cs_s[64 * KMAX], sn_s[64 * KMAX];
   if (UNITS && blockIdx.x == 0) {
     if (blockIdx.y == 0) make_units<kAppendThreads>(u);
     return;
   }
   const int r = UNITS ? (int)blockIdx.x - 1 : (int)blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int half = a.d >> 1;
   const int64_t at = a.row_slot[r];
   if (at < 0 || at >= a.slots) return;  // (the whole workgroup)
   const int pos = a.row_pos[r];
   const bool rot = a.inv_freq != nullptr;
-  for (int i = tid; rot && i < half; i += kAppendThreads) {
-    const float ang = (float)pos * a.inv_freq[i];
-    double sd, cd;
-    sincos((double)ang, &sd, &cd);
-    cs_s[i] = (float)cd;
-    sn_s[i] = (float)sd;
-  }
-  __syncthreads();
-  auto rms_inv = [&](float ss, int n) { return 1.0f / sqrtf(ss / (float)n + a.eps); };
   const int heads = a.nq + (a.k_new ? a.nkv : 0);
-  const int step = kAppendWaves * gridDim.y;
-  for (int hh = blockIdx.y * kAppendWaves + w; hh < heads; hh += step) {
+  const int h0 = (blockIdx.y * kAppendWaves + w) * a.each, h1 = min(h0 + a.each, heads);
+  if (h0 >= h1) return;
+  // a head's x (q's or k's) and v, the next one's in flight while one is used
+  float n0[KMAX], n1[KMAX], nv0[KMAX], nv1[KMAX];
+  auto load = [&](int hh) {
     const bool isq = hh < a.nq;
-    const int kh = hh - a.nq;
     const float* x = isq ? a.q + ((int64_t)r * a.nq + hh) * a.d
-                         : a.k_new + ((int64_t)r * a.nkv + kh) * a.d;
-    const float* weight = isq ? a.q_norm : a.k_norm;
-    const float* vx = a.v_new + ((int64_t)r * a.nkv + kh) * a.d;  // (not read for q)
-    float x0[KMAX], x1[KMAX], v0[KMAX], v1[KMAX];
+                         : a.k_new + ((int64_t)r * a.nkv + (hh - a.nq)) * a.d;
+    const float* vx = a.v_new + ((int64_t)r * a.nkv + (hh - a.nq)) * a.d;  // (not read for q)
 #pragma unroll
     for (int k = 0; k < KMAX; ++k) {
       const int j = lane + 64 * k;
       const bool in = j < half;
-      x0[k] = in ? x[j] : 0.f;
-      x1[k] = in ? x[j + half] : 0.f;
-      v0[k] = in && !isq ? vx[j] : 0.f;
-      v1[k] = in && !isq ? vx[j + half] : 0.f;
+      n0[k] = in ? x[j] : 0.f;
+      n1[k] = in ? x[j + half] : 0.f;
+      nv0[k] = in && !isq ? vx[j] : 0.f;
+      nv1[k] = in && !isq ? vx[j + half] : 0.f;
     }
+  };
+  load(h0);
+  // a lane's pairs are the same in every head: its angles in registers
+  float cs[KMAX], sn[KMAX];
+#pragma unroll
+  for (int k = 0; k < KMAX; ++k) {
+    cs[k] = 1.f;
+    sn[k] = 0.f;
+    if (rot && 64 * k < half) {
+      const float ang = (float)pos * a.inv_freq[min(lane + 64 * k, half - 1)];
+      double sd, cd;
+      sincos((double)ang, &sd, &cd);
+      cs[k] = (float)cd;
+      sn[k] = (float)sd;
+    }
+  }
+  auto rms_inv = [&](float ss, int n) { return 1.0f / sqrtf(ss / (float)n + a.eps); };
+  for (int hh = h0; hh < h1; ++hh) {
+    const bool isq = hh < a.nq;
+    const int kh = hh - a.nq;
+    const float* weight = isq ? a.q_norm : a.k_norm;
+    float x0[KMAX], x1[KMAX], v0[KMAX], v1[KMAX];
+#pragma unroll
+    for (int k = 0; k < KMAX; ++k) {
+      x0[k] = n0[k];
+      x1[k] = n1[k];
+      v0[k] = nv0[k];
+      v1[k] = nv1[k];
+    }
+    if (hh + 1 < h1) load(hh + 1);
     if (weight) {
       float ss = 0.f;
 #pragma unroll
@@ -469,9 +517,8 @@ __global__ __launch_bounds__(kAppendThreads) void ragged_append_kernel(AppendArg
     float r0[KMAX], r1[KMAX];
 #pragma unroll
     for (int k = 0; k < KMAX; ++k) {
-      const int j = min(lane + 64 * k, half - 1);
-      r0[k] = rot ? x0[k] * cs_s[j] - x1[k] * sn_s[j] : x0[k];
-      r1[k] = rot ? x0[k] * sn_s[j] + x1[k] * cs_s[j] : x1[k];
+      r0[k] = rot ? x0[k] * cs[k] - x1[k] * sn[k] : x0[k];
+      r1[k] = rot ? x0[k] * sn[k] + x1[k] * cs[k] : x1[k];
     }
     if (isq) {
       float* y = a.q + ((int64_t)r * a.nq + hh) * a.d;
@@ -576,7 +623,7 @@ __global__ __launch_bounds__(kMergeThreads) void ragged_merge_kernel(RaggedArgs 
   const int p = blockIdx.x / a.nkv, h = blockIdx.x - p * a.nkv;
   if (p >= a.head->nparts) return;
   const RaggedUnit t = a.units[a.part_unit[p]];
-  const RaggedSeq s = ragged_seq(a, t.seq);
+  const RaggedSeq& s = t.s;
   const int n = t.nsplit, p0 = p - t.split;
   const int rows = min(t.wide ? a.ql : a.qs, s.rows * a.G - t.r0);
   const bool shared = n > kMergeFew;  // uniform
@@ -672,9 +719,9 @@ int check_ragged(int nq, int nkv, int d, int page, int num_blocks, int kv_dtype)
 // units: a step's attention, whose units the launch forms too (NULL: none).
 int launch_append(AppendArgs a, int T, const RaggedArgs* units, void* stream) {
   const int heads = a.nq + (a.k_new ? a.nkv : 0);
-  const int most = (heads + kAppendWaves - 1) / kAppendWaves;
-  // workgroups a row: enough for the chip where the rows are few
-  const int y = std::max(1, std::min({most, 1024 / T, 64}));
+  // heads a wave: enough waves for the chip, and then more for each angle
+  a.each = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)T * heads / 8192, kAppendHeads));
+  const int y = (heads + kAppendWaves * a.each - 1) / (kAppendWaves * a.each);
   const int half = a.d / 2;
   auto k = half <= 64    ? units ? ragged_append_kernel<1, true> : ragged_append_kernel<1, false>
            : half <= 128 ? units ? ragged_append_kernel<2, true> : ragged_append_kernel<2, false>
@@ -774,7 +821,7 @@ int launch_attention(RaggedArgs a, const AppendArgs* append, void* stream) {
   hipLaunchKernelGGL(attend, dim3((unsigned)(a.max_units * a.nkv)), dim3(threads), 0,
                      (hipStream_t)stream, a);
   if (a.max_parts)
-    hipLaunchKernelGGL(merge, dim3((unsigned)(a.max_parts * a.nkv), a.slot_rows > 4 ? 4 : 1),
+    hipLaunchKernelGGL(merge, dim3((unsigned)(a.max_parts * a.nkv), std::min(a.slot_rows / kMergeWaves, 8)),
                        dim3(kMergeThreads), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
@@ -880,8 +927,8 @@ int molot_hip_ragged_plan(const int32_t* counts, const int32_t* done, const int3
     if (st) return st;
     a.taken = reinterpret_cast<int32_t*>(ws);
   }
-  hipLaunchKernelGGL(ragged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, a,
-                     rows ? 1 : 0);
+  hipLaunchKernelGGL(B <= kPlanThreads ? ragged_plan_kernel<1> : ragged_plan_kernel<kPlanBatch>, dim3(1),
+                     dim3(kPlanThreads), 0, (hipStream_t)stream, a, rows ? 1 : 0);
   if (!rows && max_rows > 0)
     hipLaunchKernelGGL(ragged_rows_kernel, dim3((max_rows + 255) / 256), dim3(256), 0,
                        (hipStream_t)stream, a);

@@ -21,13 +21,20 @@
 struct RaggedHead {
   int nunits, nparts, pad[2];
 };
+// The new rows of a sequence: first packed row, rows, and the slot of the first.
+struct RaggedSeq {
+  int start, rows, slot0;
+};
 struct RaggedUnit {
   int seq, r0;   // sequence, first row r of the tile
   int lo, hi;    // keys [lo, hi)
   int part;      // of a split tile: the unit's place in the partials (-1: whole)
   int split, nsplit;
   int wide;      // a tile of RaggedArgs::ql rows, else of qs
+  RaggedSeq s;
+  int pad;
 };
+static_assert(sizeof(RaggedUnit) == 48, "16-byte loads");
 
 struct RaggedArgs {
   const float* q;  // [T][nq][d]
@@ -67,11 +74,7 @@ RaggedTile ragged_tile(int d, int kv_dtype, bool scored) __attribute__((visibili
 
 namespace {
 
-// The new rows of sequence b as the kernels take them, whatever the arrays hold: first
-// packed row, rows, and the slot of the first.
-struct RaggedSeq {
-  int start, rows, slot0;
-};
+// The new rows of sequence b as the kernels take them, whatever the arrays hold.
 __device__ __forceinline__ RaggedSeq ragged_seq(const RaggedArgs& a, int b) {
   const int s0 = max(0, min(a.row_start[b], a.T));
   const int s1 = max(s0, min(a.row_start[b + 1], a.T));
@@ -121,7 +124,7 @@ template <int EPL>
 __device__ __forceinline__ void ragged_own_row(const RaggedArgs& a, const RaggedUnit& u, int h, int r) {
   constexpr int D = 64 * EPL;
   const int lane = threadIdx.x & 63;
-  const RaggedSeq s = ragged_seq(a, u.seq);
+  const RaggedSeq& s = u.s;
   if (r >= s.rows * a.G) return;
   const int m = r / a.G, g = r - m * a.G, slot = s.slot0 + m, head = h * a.G + g;
   const int lo = max(ragged_lo(a, slot), u.lo), hi = min(ragged_hi(a, slot), u.hi);

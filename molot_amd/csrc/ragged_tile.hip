@@ -674,7 +674,7 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
   const int ui = blockIdx.x / a.nkv, h = blockIdx.x - ui * a.nkv;
   if (ui >= a.head->nunits) return;
   const RaggedUnit u = a.units[ui];
-  const RaggedSeq sq = ragged_seq(a, u.seq);
+  const RaggedSeq& sq = u.s;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ntile = (u.hi - u.lo + KT - 1) / KT;
@@ -688,8 +688,6 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
 
   if (u.wide) {
     using X = typename std::conditional<C::WR == 32, Rows32<D, T, SC>, Rows16<D, T, SC>>::type;
-    X x;
-    x.init(a, u, sq, h, u.r0 + X::NR * w + (lane & (X::NR - 1)), lane);
     const bool rows = u.r0 + X::NR * w < sq.rows * a.G;  // else this wave only stages
     constexpr int KI = C::IT * KT;                       // keys an interval
     const int nint = (ntile + C::IT - 1) / C::IT;
@@ -750,6 +748,10 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
     if (nint > 0) {
       blocks(0);
       fetch(0);
+    }
+    X x;  // (the first rows on their way)
+    x.init(a, u, sq, h, u.r0 + X::NR * w + (lane & (X::NR - 1)), lane);
+    if (nint > 0) {
       stage(0);
       fetch(1);
     }
@@ -781,8 +783,10 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
   }
 
   Rows16<D, T, SC> x;
-  x.init(a, u, sq, h, u.r0 + (lane & 15), lane);
-  if (w < C::NWN) {
+  const int r = u.r0 + (lane & 15);
+  if (w >= C::NWN) {
+    x.init(a, u, sq, h, r, lane);
+  } else {
     char* const buf = lds + w * C::TB;
     float* const ub = units + w * 2 * KT;
     // K and V each have their registers where those are few enough
@@ -831,6 +835,7 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
       if (BOTH) fetch(1, w, id, off);
       idn = ids(w + C::NWN);
     }
+    x.init(a, u, sq, h, r, lane);  // (the first rows on their way)
     for (int t = w; t < ntile; t += C::NWN) {
       const bool more = t + C::NWN < ntile;
       stage(0);

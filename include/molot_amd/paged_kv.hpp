@@ -1,6 +1,6 @@
 // Paged KV cache with continuous batching: the host side of the paged
 // kernels (include/molot_amd/attn_hip.h: molot_hip_decode_step_paged_norm,
-// molot_hip_prefill_step_paged).
+// molot_hip_prefill_step_paged, molot_hip_step_ragged).
 //
 // No reference counterpart: the reference keeps one contiguous fp32 cache
 // per layer and sequence (Runner::KVC, include/molot/forward.h:48-51, one
@@ -18,7 +18,9 @@
 //     begin_decode uploads that batch's block table and lengths once, every
 //     layer's decode() reuses them, end_decode advances the lengths;
 //   * a prompt is prefilled per sequence the same way (begin_prefill,
-//     prefill() per layer, end_prefill).
+//     prefill() per layer, end_prefill);
+//   * or one step takes both: a ragged batch (begin_batch, step() per layer,
+//     end_batch), in which every sequence brings one row, a few or a prompt.
 // Errors throw std::runtime_error; a full pool is "fwd: KV cache full", as
 // forward.h:570 reports a full contiguous cache.
 #pragma once
@@ -68,6 +70,7 @@ class PagedKVCache {
     for (int32_t* p : slot_pos_)
       if (p) (void)hipFree(p);
     if (d_table_) (void)hipFree(d_table_);
+    if (d_rows_) (void)hipFree(d_rows_);
     if (h_table_) (void)hipHostFree(h_table_);
     if (uploaded_) (void)hipEventDestroy(uploaded_);
   }
@@ -229,6 +232,82 @@ class PagedKVCache {
     mode_ = Mode::None;
   }
 
+  // ---- a ragged batch: each sequence of ids brings counts[i] new rows (0 or more) ----
+  // Their rows are packed in the order of ids: q [T][nq][hd], k/v [T][nkv][hd],
+  // o [T][nq][hd], T = rows().  Reserves their slots and makes the batch's index arrays
+  // on stream s (molot_hip_ragged_plan, over the tables of this class's allocator).
+  // Throws "fwd: KV cache full" before any state of the step is set, and for a cache
+  // held to a budget, whose books go by prefill() and decode_scored().
+  void begin_batch(const std::vector<int>& ids, const std::vector<int>& counts,
+                   hipStream_t s = nullptr) {
+    if (mode_ != Mode::None) throw std::runtime_error("PagedKVCache: a step is in progress");
+    if (acc_[0]) throw std::runtime_error("PagedKVCache: a ragged batch over a cache held to a budget");
+    if (ids.size() != counts.size()) throw std::runtime_error("PagedKVCache: counts of other sequences");
+    const size_t B = ids.size();
+    std::vector<int32_t> after(B), more(2 * B);
+    int maxb = 1;
+    int64_t rows = 0;
+    for (size_t i = 0; i < B; ++i) {
+      if (counts[i] < 0) throw std::runtime_error("PagedKVCache: a negative count");
+      for (size_t j = 0; j < i; ++j)
+        if (ids[j] == ids[i]) throw std::runtime_error("PagedKVCache: a sequence twice");
+      rows += counts[i];
+      more[i] = counts[i];
+      more[B + i] = seq(ids[i]).len;
+    }
+    if (rows == 0 || rows > (1 << 20)) throw std::runtime_error("PagedKVCache: a batch of no rows, or too many");
+    for (size_t i = 0; i < B; ++i) {
+      reserve(ids[i], counts[i]);
+      after[i] = seq(ids[i]).len + counts[i];
+      maxb = std::max(maxb, (int)seq(ids[i]).blocks.size());
+    }
+    upload(ids, maxb, after, s, more);
+    const size_t n = B + 2 + 3 * (size_t)rows;
+    if (n > rows_cap_) {
+      if (d_rows_) check_hip(hipStreamSynchronize(s), "hipStreamSynchronize");
+      if (d_rows_) check_hip(hipFree(d_rows_), "hipFree");
+      d_rows_ = nullptr;
+      rows_cap_ = 0;
+      check_hip(hipMalloc((void**)&d_rows_, n * sizeof(int32_t)), "hipMalloc rows");
+      rows_cap_ = n;
+    }
+    T_ = (int)rows;
+    check(molot_hip_ragged_plan(d_pos_ + B, nullptr, nullptr, d_pos_ + 2 * B, d_lens_, d_table_, nullptr,
+                                nullptr, nullptr, (int)B, maxb_, page_, nblocks_, T_, row_start(),
+                                row_seq(), row_pos(), row_slot(), d_rows_, s),
+          "ragged_plan");
+    batch_ = ids;
+    counts_ = counts;
+    mode_ = Mode::Batch;
+  }
+  int rows() const { return T_; }
+  // One layer over the batch: forward.h:554-591 for every row, q, k, v and o device
+  // pointers (q normed and rotated in place), sc's cap and slopes.
+  void step(int layer, float* q, const float* k, const float* v, float* o, int nq,
+            const float* inv_freq, float scale, int window, const LayerNorms& nm = LayerNorms{},
+            const Scores& sc = Scores{}, hipStream_t s = nullptr) {
+    if (!k || !v) throw std::runtime_error("PagedKVCache: step() needs k and v");
+    ragged(layer, q, k, v, o, nq, inv_freq, scale, window, nm, sc, s);
+  }
+  // The same for a layer without its own KV reading layer `src`'s pages: nothing appended.
+  void step_shared(int src, float* q, float* o, int nq, const float* inv_freq, float scale,
+                   int window, const LayerNorms& nm = LayerNorms{}, const Scores& sc = Scores{},
+                   hipStream_t s = nullptr) {
+    ragged(src, q, nullptr, nullptr, o, nq, inv_freq, scale, window, nm, sc, s);
+  }
+  void end_batch() {
+    if (mode_ != Mode::Batch) throw std::runtime_error("PagedKVCache: no batch to end");
+    for (size_t i = 0; i < batch_.size(); ++i) seq(batch_[i]).len += counts_[i];
+    batch_.clear();
+    counts_.clear();
+    mode_ = Mode::None;
+  }
+  // The batch's index arrays on the device: [B + 1], [T], [T], [T].
+  int32_t* row_start() const { return d_rows_ + 1; }
+  int32_t* row_seq() const { return d_rows_ + (rows_cap_ ? rows_cap_ - 3 * (size_t)T_ : 0); }
+  int32_t* row_pos() const { return row_seq() + T_; }
+  int32_t* row_slot() const { return row_seq() + 2 * T_; }
+
   // ---- a budget of rows a sequence ----
   // Keep every slot's weight and position from here on, in every layer (call it
   // before the first sequence's rows).
@@ -302,7 +381,7 @@ class PagedKVCache {
     int gone = 0;  // rows evicted: the next token's position is len + gone
     std::vector<int> blocks;
   };
-  enum class Mode { None, Decode, Prefill };
+  enum class Mode { None, Decode, Prefill, Batch };
 
   Seq& seq(int id) {
     if (id < 0 || id >= (int)seqs_.size() || !seqs_[id].live)
@@ -313,6 +392,17 @@ class PagedKVCache {
     if (id < 0 || id >= (int)seqs_.size() || !seqs_[id].live)
       throw std::runtime_error("PagedKVCache: no such sequence");
     return seqs_[id];
+  }
+  void ragged(int layer, float* q, const float* k, const float* v, float* o, int nq,
+              const float* inv_freq, float scale, int window, const LayerNorms& nm, const Scores& sc,
+              hipStream_t s) {
+    if (mode_ != Mode::Batch) throw std::runtime_error("PagedKVCache: step outside a batch");
+    if (sc.key_lo || sc.key_hi) throw std::runtime_error("PagedKVCache: key ranges in a ragged batch");
+    check(molot_hip_step_ragged(q, k, v, k_.at(layer), v_.at(layer), o, d_table_, d_lens_, row_start(),
+                                row_pos(), row_slot(), T_, (int)batch_.size(), maxb_, nblocks_, max_len_,
+                                nq, nkv_, hd_, page_, nm.q_norm, nm.k_norm, nm.v_norm ? 1 : 0, nm.eps,
+                                inv_freq, scale, window, sc.softcap, sc.slopes, kv_dtype_, s),
+          "step_ragged");
   }
   // The batch's last M rows of a layer are new.
   void track(int layer, int M, hipStream_t s) {
@@ -342,10 +432,11 @@ class PagedKVCache {
   }
   // The batch's block table [B][maxb] and lengths to the device, through a
   // pinned staging buffer whose previous copy has finished (event).
+  // (more: further words, after the positions)
   void upload(const std::vector<int>& ids, int maxb, const std::vector<int32_t>& lens,
-              hipStream_t s) {
+              hipStream_t s, const std::vector<int32_t>& more = {}) {
     const size_t B = ids.size();
-    const size_t n = B * maxb + 2 * B, bytes = n * sizeof(int32_t);
+    const size_t n = B * maxb + 2 * B + more.size(), bytes = n * sizeof(int32_t);
     if (uploaded_) check_hip(hipEventSynchronize(uploaded_), "hipEventSynchronize");
     if (bytes > table_cap_) {
       // the previous step's kernels may still read the old table
@@ -374,6 +465,7 @@ class PagedKVCache {
       h_table_[B * maxb + i] = lens[i];
       max_len_ = std::max(max_len_, (int)lens[i]);
     }
+    std::copy(more.begin(), more.end(), h_table_ + B * maxb + 2 * B);
     check_hip(hipMemcpyAsync(d_table_, h_table_, bytes, hipMemcpyHostToDevice, s),
               "H2D block table");
     if (!uploaded_) check_hip(hipEventCreate(&uploaded_), "hipEventCreate");
@@ -402,6 +494,10 @@ class PagedKVCache {
   int cut_pos_ = 0;   // and the newest position of such
   size_t table_cap_ = 0;
   int maxb_ = 1, max_len_ = 0;
+  std::vector<int> counts_;     // a ragged batch's new rows
+  int32_t* d_rows_ = nullptr;   // its status, row_start [B + 1] and, at the end, the rows' maps
+  size_t rows_cap_ = 0;
+  int T_ = 0;
 };
 
 }  // namespace molot::amd

@@ -9,6 +9,7 @@
                               and to the oracle (its checker)
   tests/cpp/test_kv_budget     self-checks of caches held to a budget, and of prompts and
   tests/cpp/test_kv_cut        steps over the caches that rows were evicted from
+  tests/cpp/test_kv_ragged     self-check of ragged batches through the paged-KV manager
   tests/cpp/prefill_no_memory  prefill where its workspace's allocation is refused
   tests/cpp/host_io_time       time of the C++ drop-in's decode call with host
                               vectors against device ones (bench.py's host_io)
@@ -101,7 +102,7 @@ def build_cpp_test(name: str = "test_attn_cpp") -> str:
     return out
 
 
-CPP_TESTS = ("test_attn_cpp", "test_paged_kv", "test_kv_budget", "test_kv_cut", "prefill_no_memory", "host_io_time")
+CPP_TESTS = ("test_attn_cpp", "test_paged_kv", "test_kv_budget", "test_kv_cut", "test_kv_ragged", "prefill_no_memory", "host_io_time")
 
 
 def build_all() -> None:

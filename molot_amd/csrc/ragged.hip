@@ -280,10 +280,9 @@ __global__ __launch_bounds__(256) void ragged_rows_kernel(PlanArgs a) {
 // The host knows neither the lengths nor the counts, only bounds (rows T, sequences B),
 // so one workgroup forms the attention's work list from them: the tiles of every
 // sequence, the keys each attends, and from their costs (a wide tile's key counts `weight`
-// narrow ones) the share of a CU.  Tiles that cost more than a share (narrow ones, whose
-// partials are small: half of one) are split; so at most `target` = two units a CU come on
-// top of one a tile.  The list goes by cost, the largest first: the workgroups that start
-// last are short.
+// narrow ones) the share of a workgroup that the chip holds at once.  Tiles that cost more are
+// split; so at most `target` units, one such workgroup each, come on top of one a tile.  The
+// list goes by cost, the largest first: the workgroups that start last are short.
 constexpr int kUnitBuckets = 64;
 
 // Tiles of a sequence of R rows r: wide ones as long as more than `few` rows are left, then
@@ -354,9 +353,9 @@ __device__ __forceinline__ void make_units(const RaggedArgs& a) {
   __syncthreads();
   // the keys (of 32) a unit takes at most: whole intervals of its kind
   auto up = [](unsigned long long x, int n) { return (int)((min(x, 1ull << 26) + n - 1) / n * n); };
-  const unsigned long long half = (s_cost + a.target - 1) / a.target;
-  const int most_wide = up(max((2 * half + a.weight - 1) / a.weight, (unsigned long long)a.min_keys >> 5), 2);
-  const int most_slim = up(max(half, (unsigned long long)a.min_keys >> 5), 8);
+  const unsigned long long share = (s_cost + a.target - 1) / a.target;
+  const int most_wide = up(max((share + a.weight - 1) / a.weight, (unsigned long long)a.min_keys >> 5), 2);
+  const int most_slim = up(max(share, (unsigned long long)a.min_keys >> 5), 8);
   const float top = (float)max(most_wide * a.weight, most_slim);
   // how a tile is split: n units of `size`
   auto split = [&](const UnitTile& u, int& size) {
@@ -752,10 +751,12 @@ struct Layout {
   }
 };
 
-// A wide tile's key against a narrow one's, us a key and CU at 32q/8kv/d128 bf16, fp32 and
-// Q8: 0.097, 0.117 and 0.085 (512 rows after 16384) against 0.032, 0.051 and 0.025 (64
-// sequences of one row).
-constexpr int kWideWeight = 3;
+// A wide tile's key against a narrow one's.  Alone the two take 3 to 1 (us a key and CU at
+// 32q/8kv/d128 bf16, fp32 and Q8: 0.097, 0.117 and 0.085 for 512 rows after 16384, 0.032,
+// 0.051 and 0.025 for 64 sequences of one row); mixed, where wide units run beside narrow ones
+// that wait for memory, wide ones that are cut shorter still end sooner: 512 rows beside 63
+// decoding sequences (bf16) 137 us at 3, 130 at 6, 127 at 8 and 10.
+constexpr int kWideWeight = 8;
 
 // append, T rows: a step's, before the attention.
 int launch_attention(RaggedArgs a, const AppendArgs* append, void* stream) {
@@ -773,7 +774,7 @@ int launch_attention(RaggedArgs a, const AppendArgs* append, void* stream) {
   a.few = 0;  // every tile a wide one
   a.min_keys = 256;
   a.weight = 1;
-  int per_cu = 8;
+  int per_cu = 4;
   // (the matrix-core kernel's offsets are of 31 bits within a block, and of 35 in a pool)
   const int64_t block = ((int64_t)a.nkv << a.page_shift) *
                         (a.kv_dtype == MOLOT_KV_Q8 ? a.d + 4 : a.d * (a.kv_dtype == MOLOT_KV_BF16 ? 2 : 4));
@@ -788,7 +789,7 @@ int launch_attention(RaggedArgs a, const AppendArgs* append, void* stream) {
     a.weight = kWideWeight;
     // (a tile holds no more rows than the batch)
     a.slot_rows = (int64_t)a.T * a.G <= a.few ? a.qs : a.ql;
-    per_cu = 2;
+    per_cu = 1;  // (a workgroup takes a CU: 2 units 157 us where one takes 139, 32 drafts on Q8)
   }
   a.target = (per_cu * cus + a.nkv - 1) / a.nkv;
   // Bounds: a sequence of R rows r has at most R / ql wide tiles and one more, or narrow

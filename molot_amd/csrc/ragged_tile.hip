@@ -177,7 +177,11 @@ struct Tile {
   static constexpr int kMerge = NWN / 2 * 16 * D * 4;
   static constexpr int kData = max2(max2(4 * IT * TB, NWN * TB), kMerge);
   static constexpr int kUnits = max2(NWN * 2, 4 * IT) * KT * 4;  // narrow: [wave][K, V][32]
-  static constexpr int LDS = kData + max2(kUnits, NW / 2 * 64 * 8);
+  static constexpr int kQ = kData + max2(kUnits, NW / 2 * 64 * 8);
+  // Narrow tiles of d = 256: q's pieces lie in LDS, the same for every wave (in registers, 64
+  // of them, beside the rows in flight and o they spill: 195 registers of fp32 kernels).
+  static constexpr bool QLDS = D > 128;
+  static constexpr int LDS = kQ + (QLDS ? D / 32 * 2 * 64 * 16 : 0);
   static_assert(LDS <= 160 * 1024, "fits a CU");
 
   using raw_t = Raw<T>;
@@ -471,22 +475,35 @@ __device__ __forceinline__ f32x4 mfma16_f16(f16x8_t a, f16x8_t b, f32x4 c) {
 
 // 16 rows of a wave (v_mfma_f32_16x16x32_f16): half the registers.  A lane holds the keys
 // 16*b + 4*(lane / 16) + i of row lane % 16, e = 4*b + i.
-template <int D, typename T, bool SC>
+template <int D, typename T, bool SC, bool QLDS>
 struct Rows16 : RowsBase<D, T, SC> {
   using B = RowsBase<D, T, SC>;
   using C = typename B::C;
   using B::fac, B::mark;
   static constexpr int NR = 16, NV = D / 16;
   static constexpr int QS = D / 32, NP = C::NP, RB = C::RB, PB = C::PB;
-  f16x8_t qh[QS], ql[QS];
+  f16x8_t qh[QLDS ? 1 : QS], ql[QLDS ? 1 : QS];
+  const f16x8_t* qs;  // QLDS: [step][piece][lane], at this lane
   f32x4 o[NV], s[2];
   uint32_t yh[4], yl[4];
 
   __device__ static __forceinline__ float gmax(float v) { return max_xor32(max_xor16(v)); }
   __device__ static __forceinline__ float gsum(float v) { return sum_xor32(sum_xor16(v)); }
   __device__ __forceinline__ void init(const RaggedArgs& a, const RaggedUnit& u, const RaggedSeq& sq, int h,
-                                       int r, int lane) {
-    B::template init<QS, 32>(a, u, sq, h, r, lane >> 4, gmax, qh, ql);
+                                       int r, int lane, char* lds = nullptr) {
+    if constexpr (QLDS) {  // (every wave writes the same)
+      f16x8_t hi[QS], lo[QS];
+      B::template init<QS, 32>(a, u, sq, h, r, lane >> 4, gmax, hi, lo);
+      f16x8_t* const to = reinterpret_cast<f16x8_t*>(lds) + lane;
+#pragma unroll
+      for (int q = 0; q < QS; ++q) {
+        to[128 * q] = hi[q];
+        to[128 * q + 64] = lo[q];
+      }
+      qs = to;
+    } else {
+      B::template init<QS, 32>(a, u, sq, h, r, lane >> 4, gmax, qh, ql);
+    }
 #pragma unroll
     for (int v = 0; v < NV; ++v) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -501,8 +518,11 @@ struct Rows16 : RowsBase<D, T, SC> {
     f32x4 low[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) s[b] = low[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    f16x8_t k[2][2][NP];
+    f16x8_t k[2][2][NP], x[2][2];
     auto read_k = [&](int q) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        x[q & 1][p] = QLDS ? qs[128 * q + 64 * p] : (p ? ql : qh)[QLDS ? 0 : q];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -515,12 +535,12 @@ struct Rows16 : RowsBase<D, T, SC> {
       if (q + 1 < QS) read_k(q + 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) s[b] = mfma16_f16(k[q & 1][b][0], qh[q], s[b]);
+      for (int b = 0; b < 2; ++b) s[b] = mfma16_f16(k[q & 1][b][0], x[q & 1][0], s[b]);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) low[b] = mfma16_f16(k[q & 1][b][0], ql[q], low[b]);
+      for (int b = 0; b < 2; ++b) low[b] = mfma16_f16(k[q & 1][b][0], x[q & 1][1], low[b]);
       if constexpr (NP == 2) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) low[b] = mfma16_f16(k[q & 1][b][1], qh[q], low[b]);
+        for (int b = 0; b < 2; ++b) low[b] = mfma16_f16(k[q & 1][b][1], x[q & 1][0], low[b]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -687,7 +707,7 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
   const typename C::Pages pg = C::pages(a, h);
 
   if (u.wide) {
-    using X = typename std::conditional<C::WR == 32, Rows32<D, T, SC>, Rows16<D, T, SC>>::type;
+    using X = typename std::conditional<C::WR == 32, Rows32<D, T, SC>, Rows16<D, T, SC, false>>::type;
     const bool rows = u.r0 + X::NR * w < sq.rows * a.G;  // else this wave only stages
     constexpr int KI = C::IT * KT;                       // keys an interval
     const int nint = (ntile + C::IT - 1) / C::IT;
@@ -782,17 +802,19 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
     return;
   }
 
-  Rows16<D, T, SC> x;
+  Rows16<D, T, SC, C::QLDS> x;
   const int r = u.r0 + (lane & 15);
   if (w >= C::NWN) {
-    x.init(a, u, sq, h, r, lane);
+    x.init(a, u, sq, h, r, lane, lds + C::kQ);
   } else {
     char* const buf = lds + w * C::TB;
     float* const ub = units + w * 2 * KT;
     // K and V each have their registers where those are few enough
     constexpr bool BOTH = C::CN * (int)sizeof(typename C::raw_t) <= 128;
     constexpr bool Q8 = std::is_same<T, q8_t>::value;
-    typename C::raw_t raw[BOTH ? 2 : 1][C::CN];
+    // (an fp32 tile of d = 256 takes 128: its halves one after the other)
+    constexpr int HALVES = C::CN * (int)sizeof(typename C::raw_t) > 256 ? 2 : 1, CH = C::CN / HALVES;
+    typename C::raw_t raw[BOTH ? 2 : 1][CH];
     float scale[2];          // (Q8: of key lane % 32)
     constexpr int RPI = 64 / LPR;  // rows of a load
     const int r_in = lane / LPR, j = lane % LPR, key = lane & 31;
@@ -803,20 +825,25 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
     auto ids = [&](int t) { return block_of(u.lo + t * KT + key); };
     auto slot_of = [&](int t) { return min(u.lo + t * KT + key, last); };
     auto place = [&](int t, int id) { return (unsigned)(C::row_at(pg, valid(id), slot_of(t)) >> 3); };
-    auto fetch = [&](int kv, int t, int id, unsigned off) {
+    auto fetch = [&](int kv, int t, int id, unsigned off, int half = 0) {
 #pragma unroll
-      for (int i = 0; i < C::CN; ++i)
-        C::load((kv ? vp : kp) + ((uint64_t)(unsigned)__shfl((int)off, r_in + RPI * i) << 3), true,
-                raw[BOTH ? kv : 0][i]);
+      for (int i = 0; i < CH; ++i)
+        C::load((kv ? vp : kp) + ((uint64_t)(unsigned)__shfl((int)off, r_in + RPI * (half * CH + i)) << 3),
+                true, raw[BOTH ? kv : 0][i]);
       if constexpr (Q8) scale[kv] = C::scale_at(pg, kv ? a.v : a.k, valid(id), slot_of(t));
     };
-    auto stage = [&](int kv) {
-      unsigned top[C::CN];
-      C::template pieces<C::CN, RPI>(raw[BOTH ? kv : 0], kv, r_in, j, buf, top);
+    auto stage = [&](int kv, unsigned off) {
       float* const to = ub + kv * KT;
-      if (j == 0) {
 #pragma unroll
-        for (int i = 0; i < C::CN; ++i) to[r_in + RPI * i] = __uint_as_float(top[i]);
+      for (int half = 0; half < HALVES; ++half) {
+        unsigned top[CH];
+        const int r = r_in + RPI * CH * half;
+        if (half) fetch(kv, 0, 0, off, half);
+        C::template pieces<CH, RPI>(raw[BOTH ? kv : 0], kv, r, j, buf, top);
+        if (j == 0) {
+#pragma unroll
+          for (int i = 0; i < CH; ++i) to[r + RPI * i] = __uint_as_float(top[i]);
+        }
       }
       asm volatile("" ::: "memory");  // the wave's own LDS: in order
       const unsigned mine = __float_as_uint(to[key]);
@@ -835,10 +862,11 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
       if (BOTH) fetch(1, w, id, off);
       idn = ids(w + C::NWN);
     }
-    x.init(a, u, sq, h, r, lane);  // (the first rows on their way)
+    x.init(a, u, sq, h, r, lane, lds + C::kQ);  // (the first rows on their way)
     for (int t = w; t < ntile; t += C::NWN) {
       const bool more = t + C::NWN < ntile;
-      stage(0);
+      stage(0, off);
+      const unsigned off1 = off;
       if (!BOTH) fetch(1, t, id, off);
       if (more) {
         id = idn;
@@ -848,7 +876,7 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
       }
       x.scores(buf, lane);
       asm volatile("" ::: "memory");
-      stage(1);
+      stage(1, off1);
       if (more) fetch(BOTH ? 1 : 0, t + C::NWN, id, off);
       x.softmax(ub, ub + KT, u.lo + t * KT, lane);
       x.pv(buf, lane);

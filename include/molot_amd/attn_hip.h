@@ -471,7 +471,8 @@ int molot_hip_kv_evict_paged(void* K, void* V, float* acc, int32_t* slot_pos,
  * their own a plan commits nothing until the caller takes them for the next one's
  * seq_lens and free_count.  free_blocks NULL (then done too): the table holds the new
  * rows' blocks already, and only the maps are made.
- * B, max_rows and max_blocks up to 2^20 (MOLOT_ENOTSUP past it). */
+ * B, max_rows and max_blocks up to 2^20 (MOLOT_ENOTSUP past it); B and T of the other
+ * entries too. */
 int molot_hip_ragged_plan(const int32_t* counts, const int32_t* done, const int32_t* pos,
                           const int32_t* seq_lens, int32_t* kv_lens, int32_t* block_table,
                           int32_t* free_blocks, const int32_t* free_count, int32_t* free_left,

@@ -798,7 +798,7 @@ int launch_attention(RaggedArgs a, const AppendArgs* append, void* stream) {
   const int64_t R = (int64_t)a.T * a.G;
   const int64_t seqs = std::min(a.T, a.B);
   const int64_t tiles = R / a.ql + seqs * std::max(1, (a.few + a.qs - 1) / a.qs);
-  if (R > 0x3FFFFFFF || (tiles + a.target) * a.nkv > 0x7FFFFFFF) return MOLOT_ENOTSUP;
+  if (R > 0x3FFFFFFF || (tiles + a.target) * a.nkv * threads > 0xFFFFFFFF) return MOLOT_ENOTSUP;
   a.max_units = (int)(tiles + a.target);
   a.max_parts = a.cap > a.min_keys ? 2 * a.target : 0;  // (else no tile is split)
   const Layout l(a, D);
@@ -841,6 +841,7 @@ int attention_args(RaggedArgs& a, const float* Q, const void* K, const void* V, 
       (!Q || !K || !V || !O || !block_table || !kv_lens || !row_start || Q == O))
     return MOLOT_EINVAL;
   if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(O)) return MOLOT_EINVAL;
+  if (T > kPlanMost || B > kPlanMost) return MOLOT_ENOTSUP;
   if (!(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f))) return MOLOT_EINVAL;
   a.q = Q;
   a.k = reinterpret_cast<const char*>(K);
@@ -876,6 +877,7 @@ int append_args(AppendArgs& a, float* q, const float* k_new, const float* v_new,
   if (!(eps >= 0.f && eps < INFINITY) || T < 0) return MOLOT_EINVAL;
   if (T > 0 && (!q || !row_pos || !row_slot || !k_new != !v_new || (k_new && (!K || !V))))
     return MOLOT_EINVAL;
+  if (T > kPlanMost) return MOLOT_ENOTSUP;
   a.q = q;
   a.k_new = k_new;
   a.v_new = v_new;

@@ -96,6 +96,12 @@ def test_sizes_the_kernels_are_not_built_for(bad):
 
 def test_more_rows_than_the_grid():
     assert attend(T=1 << 30, nq=64, nkv=4) == _lib.ENOTSUP
+    most = 1 << 20  # rows, and sequences
+    for fn in (attend, step):
+        assert fn(T=most + 1) == _lib.ENOTSUP and fn(B=most + 1) == _lib.ENOTSUP
+        # tiles * KV heads * threads past 2^32
+        assert fn(T=most, B=most, nq=64, nkv=64) == _lib.ENOTSUP
+    assert append(T=most + 1) == _lib.ENOTSUP
 
 
 def test_nothing_to_do():

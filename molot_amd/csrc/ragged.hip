@@ -291,11 +291,12 @@ __device__ __forceinline__ int wide_tiles(const RaggedArgs& a, int R) {
   return R / a.ql + (R % a.ql > a.few ? 1 : 0);
 }
 __device__ __forceinline__ int slim_tiles(const RaggedArgs& a, int R) {
-  return R % a.ql > a.few ? 0 : (R % a.ql + a.qs - 1) / a.qs;
+  const int rows = ragged_slim(a, R);
+  return R % a.ql > a.few ? 0 : (R % a.ql + rows - 1) / rows;
 }
 // A tile's keys: [lo, hi), kt of 32.
 struct UnitTile {
-  int seq, r0, lo, hi, wide, kt;
+  int seq, r0, lo, hi, wide, rows, kt;
   RaggedSeq s;
 };
 template <typename BEFORE>
@@ -303,12 +304,12 @@ __device__ __forceinline__ UnitTile unit_tile(const RaggedArgs& a, int t, int nw
   const int kind = t >= nwide, i = kind ? t - nwide : t;
   const int b = plan_find(a.B, i, [&](int s) { return before(s, kind); });
   const RaggedSeq s = ragged_seq(a, b);
-  const int R = s.rows * a.G, rows = kind ? a.qs : a.ql;
+  const int R = s.rows * a.G, rows = kind ? ragged_slim(a, R) : a.ql;
   const int r0 = (kind ? R / a.ql * a.ql : 0) + (i - before(b, kind)) * rows;
   const int r1 = min(r0 + rows, R) - 1;
   const int lo = ragged_lo(a, s.slot0 + r0 / a.G);
   const int hi = max(lo, ragged_hi(a, s.slot0 + r1 / a.G));
-  return {b, r0, lo, hi, !kind, (hi - lo + 31) >> 5, s};
+  return {b, r0, lo, hi, !kind, rows, (hi - lo + 31) >> 5, s};
 }
 
 // NT threads of one workgroup.
@@ -402,7 +403,7 @@ __device__ __forceinline__ void make_units(const RaggedArgs& a) {
     for (int i = 0; i < n; ++i) {
       if (at + i >= a.max_units || (n > 1 && pt + i >= a.max_parts)) break;  // (never: the bounds hold)
       const int lo = u.lo + size * i * 32, hi = i + 1 < n ? lo + size * 32 : u.hi;
-      a.units[at + i] = RaggedUnit{u.seq, u.r0, lo, hi, n > 1 ? pt + i : -1, i, n, u.wide, u.s, 0};
+      a.units[at + i] = RaggedUnit{u.seq, u.r0, lo, hi, n > 1 ? pt + i : -1, i, n, u.wide, u.s, u.rows};
       if (n > 1) a.part_unit[pt + i] = at + i;
     }
   }
@@ -624,7 +625,7 @@ __global__ __launch_bounds__(kMergeThreads) void ragged_merge_kernel(RaggedArgs 
   const RaggedUnit t = a.units[a.part_unit[p]];
   const RaggedSeq& s = t.s;
   const int n = t.nsplit, p0 = p - t.split;
-  const int rows = min(t.wide ? a.ql : a.qs, s.rows * a.G - t.r0);
+  const int rows = min(t.rows, s.rows * a.G - t.r0);
   const bool shared = n > kMergeFew;  // uniform
   const int first = t.split * gridDim.y + blockIdx.y, groups = n * gridDim.y;
   for (int i = shared ? first : first * kMergeWaves + w; i < rows;
@@ -784,11 +785,11 @@ int launch_attention(RaggedArgs a, const AppendArgs* append, void* stream) {
     threads = t.threads;
     a.qs = t.narrow;
     a.ql = t.wide;
-    a.few = 2 * a.qs;
+    a.few = 2 * kSlimRows;
     a.min_keys = 512;
     a.weight = kWideWeight;
     // (a tile holds no more rows than the batch)
-    a.slot_rows = (int64_t)a.T * a.G <= a.few ? a.qs : a.ql;
+    a.slot_rows = (int64_t)a.T * a.G <= kSlimRows ? kSlimRows : (int64_t)a.T * a.G <= a.few ? a.qs : a.ql;
     per_cu = 1;  // (a workgroup takes a CU: 2 units 157 us where one takes 139, 32 drafts on Q8)
   }
   a.target = (per_cu * cus + a.nkv - 1) / a.nkv;

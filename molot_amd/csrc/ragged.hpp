@@ -30,9 +30,9 @@ struct RaggedUnit {
   int lo, hi;    // keys [lo, hi)
   int part;      // of a split tile: the unit's place in the partials (-1: whole)
   int split, nsplit;
-  int wide;      // a tile of RaggedArgs::ql rows, else of qs
+  int wide;      // a wide tile
   RaggedSeq s;
-  int pad;
+  int rows;      // of the tile
 };
 static_assert(sizeof(RaggedUnit) == 48, "16-byte loads");
 
@@ -56,7 +56,7 @@ struct RaggedArgs {
   float* part_o;    // [part][nkv][slot_rows][D] unnormalised o
   float* part_ml;   // [part][nkv][slot_rows][2] (max in base 2, sum)
   int slot_rows;    // rows of a partial's slot
-  // Tiles: of ql rows r, and of qs for the last `few` of a sequence.
+  // Tiles: of ql rows r, and for the last `few` of a sequence narrow ones (ragged_slim).
   // Units: up to `target` of them (a KV head) beyond one a tile, of at least min_keys keys;
   // a key costs a wide tile `weight` times a narrow one's.
   int qs, ql, few, target, min_keys, weight;
@@ -80,6 +80,12 @@ __device__ __forceinline__ RaggedSeq ragged_seq(const RaggedArgs& a, int b) {
   const int s1 = max(s0, min(a.row_start[b + 1], a.T));
   const int n = max(0, min(a.kv_lens[b], a.max_blocks << a.page_shift));
   return {s0, s1 - s0, n - (s1 - s0)};
+}
+// Rows of the narrow tiles that a sequence of R rows r ends in: 16, or where more are left
+// the most that one takes (two tiles would read and convert every key twice).
+constexpr int kSlimRows = 16;
+__device__ __forceinline__ int ragged_slim(const RaggedArgs& a, int R) {
+  return R % a.ql > kSlimRows ? a.qs : kSlimRows;
 }
 // The keys [lo, hi) of the query row at `slot` (< 0: none).
 __device__ __forceinline__ int ragged_lo(const RaggedArgs& a, int slot) {

@@ -12,13 +12,19 @@
 // own tiles on their way from the pages to LDS.
 //
 // Wide tiles (prompts): 256 rows, 32 a wave (at d = 256, where those would take 256
-// registers for q and o, 16).  The workgroup stages an interval of one or two tiles of 32
-// keys together, double buffered.  Waves w and w + 4 share a SIMD: the first half of the waves stages the next interval after its products,
-// the second before them, so that one's conversions meet the other's products; the
-// interval after next is in flight meanwhile.
-// Narrow tiles (one row, drafts): 16 rows, every wave a key group by itself with
-// its own LDS, so no wave waits for another: a tile's K, then its V, take the same place,
-// and the next tile's are in flight.
+// registers for q and o, 128 rows, 16 a wave).  The workgroup stages an interval of one or two
+// tiles of 32 keys together, double buffered.  Waves w and w + 4 share a SIMD: the first half
+// of the waves stages the next interval after its products, the second before them, so that
+// one's conversions meet the other's products; the interval after next is in flight meanwhile.
+// What bounds them: the chain of an interval (staging, products, barrier).  2048 fresh rows at
+// 32q/8kv/d128 bf16, fp32 and Q8: 162, 198 and 156 us with units and merge (bf16 210 TFLOP/s of
+// the layer's 34 GFLOP, 36 % of the matrix cores' rate over two products a term); 512 after 16384:
+// 375, 475 and 330 us (bf16 372 TFLOP/s, 64 %).
+// Narrow tiles (one row, drafts): 16 rows or 32, every wave a key group by itself with its own
+// LDS, so no wave waits for another: a tile's K, then its V, take the same place, and the next
+// tile's are in flight.  What bounds them: the stream where there is enough of it (64 sequences
+// of one row after 100 to 3880, bf16, fp32 and Q8: 113, 196 and 76 us, the bytes at 4.6, 5.3 and
+// 3.6 TB/s), else a wave's chain a tile.
 // The key groups' (m, l, o) are merged through LDS at the end.
 #include "ragged.hpp"
 
@@ -30,6 +36,8 @@ namespace {
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+// q's pieces in LDS (a member that points there: else its reads would be flat ones)
+typedef const __attribute__((address_space(3))) f16x8_t* lds_q_t;
 
 // Maximum over aligned groups of N lanes (8, 16 or 32), as group_max.
 template <int CTRL>
@@ -174,14 +182,18 @@ struct Tile {
   static constexpr int CW = IT * KT * LPR / NT;   // chunks of 8 elements a thread, wide
   static constexpr int CN = KT * LPR / 64;        // and a lane, narrow
   static constexpr int max2(int x, int y) { return x > y ? x : y; }
-  static constexpr int kMerge = NWN / 2 * 16 * D * 4;
+  // Narrow tiles: rows at most (32 drafts of 20 rows and 500 to 9000 keys, 16 and 32 rows a
+  // tile: Q8 144 and 128 us, bf16 183 and 164, but fp32, whose reads bound it, 289 and 298).
+  static constexpr int SR = D <= 128 && sizeof(T) < 4 ? 32 : 16;
+  static constexpr int kMerge = NWN / 2 * SR * D * 4;
   static constexpr int kData = max2(max2(4 * IT * TB, NWN * TB), kMerge);
   static constexpr int kUnits = max2(NWN * 2, 4 * IT) * KT * 4;  // narrow: [wave][K, V][32]
   static constexpr int kQ = kData + max2(kUnits, NW / 2 * 64 * 8);
-  // Narrow tiles of d = 256: q's pieces lie in LDS, the same for every wave (in registers, 64
-  // of them, beside the rows in flight and o they spill: 195 registers of fp32 kernels).
+  // Narrow tiles of more than 16 rows or d > 128: q's pieces lie in LDS, the same for every
+  // wave (in registers, 64 of them, beside the rows in flight and o they spill: 195 registers
+  // of the fp32 kernels at d = 256).
   static constexpr bool QLDS = D > 128;
-  static constexpr int LDS = kQ + (QLDS ? D / 32 * 2 * 64 * 16 : 0);
+  static constexpr int LDS = kQ + SR * D * 4;
   static_assert(LDS <= 160 * 1024, "fits a CU");
 
   using raw_t = Raw<T>;
@@ -289,7 +301,9 @@ struct RowsBase {
 #pragma unroll
       for (int e = 0; e < 8; ++e) qm = fmaxf(qm, fabsf(x[e]));
     }
-    asm volatile("" : "+v"(qr));
+    int again = 0;  // (the pointer itself, kept from the compiler so, would make flat loads)
+    asm volatile("" : "+v"(again));
+    qr += again;
     const int shift = f16_row_shift(gmax(qm));
     qunit = f16_row_unit(shift);
 #pragma unroll
@@ -306,6 +320,22 @@ struct RowsBase {
     fac = 1.f;
     mark = 0.f;
     room = wide_room(u.hi - u.lo);
+  }
+  // The same into LDS, for every wave of the workgroup (each writes the same): [step][piece]
+  // [lane], at this lane.
+  template <int N, int STEP, typename GMAX>
+  __device__ __forceinline__ lds_q_t init_lds(const RaggedArgs& a, const RaggedUnit& u,
+                                             const RaggedSeq& sq, int h, int r, int lane, int part,
+                                             GMAX&& gmax, char* lds) {
+    f16x8_t hi[N], lo[N];
+    init<N, STEP>(a, u, sq, h, r, part, gmax, hi, lo);
+    f16x8_t* const to = reinterpret_cast<f16x8_t*>(lds) + lane;
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      to[128 * q] = hi[q];
+      to[128 * q + 64] = lo[q];
+    }
+    return (lds_q_t)to;
   }
   // The tile's probabilities of this lane's N keys, slot(e) their slots.
   template <int N, typename SLOT, typename GMAX>
@@ -327,22 +357,24 @@ struct RowsBase {
 };
 
 // 32 rows of a wave over its tiles (v_mfma_f32_32x32x16_f16).
-template <int D, typename T, bool SC>
+template <int D, typename T, bool SC, bool QLDS>
 struct Rows32 : RowsBase<D, T, SC> {
   using B = RowsBase<D, T, SC>;
   using C = typename B::C;
   using B::fac, B::mark;
   static constexpr int NR = 32, NV = D / 8;  // rows; vectors of 4 outputs a lane
   static constexpr int QS = D / 16, DB = D / 32, NP = C::NP, RB = C::RB, PB = C::PB;
-  f16x8_t qh[QS], ql[QS];
+  f16x8_t qh[QLDS ? 1 : QS], ql[QLDS ? 1 : QS];
+  lds_q_t qs;  // QLDS: [step][piece][lane], at this lane
   f32x16 o[DB], s;
   uint32_t yh[8], yl[8];
 
   __device__ static __forceinline__ float gmax(float v) { return max_xor32(v); }
   __device__ static __forceinline__ float gsum(float v) { return sum_xor32(v); }
   __device__ __forceinline__ void init(const RaggedArgs& a, const RaggedUnit& u, const RaggedSeq& sq, int h,
-                                       int r, int lane) {
-    B::template init<QS, 16>(a, u, sq, h, r, lane >> 5, gmax, qh, ql);
+                                       int r, int lane, char* lds = nullptr) {
+    if constexpr (QLDS) qs = B::template init_lds<QS, 16>(a, u, sq, h, r, lane, lane >> 5, gmax, lds);
+    else B::template init<QS, 16>(a, u, sq, h, r, lane >> 5, gmax, qh, ql);
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
@@ -370,28 +402,33 @@ struct Rows32 : RowsBase<D, T, SC> {
     const int kx = 16 * (hh ^ wk_f<D>(c32));
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
-    f16x8_t k[2][2][NP];
+    f16x8_t k[2][2][NP], x[2][2][2];
     auto read_k = [&](int k0) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          x[(k0 >> 1) & 1][j][p] = QLDS ? qs[128 * (k0 + j) + 64 * p] : (p ? ql : qh)[QLDS ? 0 : k0 + j];
 #pragma unroll
         for (int p = 0; p < NP; ++p)
           k[(k0 >> 1) & 1][j][p] =
               *reinterpret_cast<const f16x8_t*>(kr + p * PB + (kx ^ (32 * (k0 + j))));
+      }
     };
     read_k(0);
 #pragma unroll
     for (int k0 = 0; k0 < QS; k0 += 2) {
       if (k0 + 2 < QS) read_k(k0 + 2);
       __builtin_amdgcn_sched_barrier(0);
-      auto& c = k[(k0 >> 1) & 1];
+      const auto& c = k[(k0 >> 1) & 1];
+      const auto& y = x[(k0 >> 1) & 1];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if constexpr (NP == 2) s = mfma32_f16(c[j][1], qh[k0 + j], s);
-        s = mfma32_f16(c[j][0], ql[k0 + j], s);
+        if constexpr (NP == 2) s = mfma32_f16(c[j][1], y[j][0], s);
+        s = mfma32_f16(c[j][0], y[j][1], s);
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) s = mfma32_f16(c[j][0], qh[k0 + j], s);
+      for (int j = 0; j < 2; ++j) s = mfma32_f16(c[j][0], y[j][0], s);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -483,7 +520,7 @@ struct Rows16 : RowsBase<D, T, SC> {
   static constexpr int NR = 16, NV = D / 16;
   static constexpr int QS = D / 32, NP = C::NP, RB = C::RB, PB = C::PB;
   f16x8_t qh[QLDS ? 1 : QS], ql[QLDS ? 1 : QS];
-  const f16x8_t* qs;  // QLDS: [step][piece][lane], at this lane
+  lds_q_t qs;  // QLDS: [step][piece][lane], at this lane
   f32x4 o[NV], s[2];
   uint32_t yh[4], yl[4];
 
@@ -491,19 +528,8 @@ struct Rows16 : RowsBase<D, T, SC> {
   __device__ static __forceinline__ float gsum(float v) { return sum_xor32(sum_xor16(v)); }
   __device__ __forceinline__ void init(const RaggedArgs& a, const RaggedUnit& u, const RaggedSeq& sq, int h,
                                        int r, int lane, char* lds = nullptr) {
-    if constexpr (QLDS) {  // (every wave writes the same)
-      f16x8_t hi[QS], lo[QS];
-      B::template init<QS, 32>(a, u, sq, h, r, lane >> 4, gmax, hi, lo);
-      f16x8_t* const to = reinterpret_cast<f16x8_t*>(lds) + lane;
-#pragma unroll
-      for (int q = 0; q < QS; ++q) {
-        to[128 * q] = hi[q];
-        to[128 * q + 64] = lo[q];
-      }
-      qs = to;
-    } else {
-      B::template init<QS, 32>(a, u, sq, h, r, lane >> 4, gmax, qh, ql);
-    }
+    if constexpr (QLDS) qs = B::template init_lds<QS, 32>(a, u, sq, h, r, lane, lane >> 4, gmax, lds);
+    else B::template init<QS, 32>(a, u, sq, h, r, lane >> 4, gmax, qh, ql);
 #pragma unroll
     for (int v = 0; v < NV; ++v) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -707,7 +733,8 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
   const typename C::Pages pg = C::pages(a, h);
 
   if (u.wide) {
-    using X = typename std::conditional<C::WR == 32, Rows32<D, T, SC>, Rows16<D, T, SC, false>>::type;
+    using X = typename std::conditional<C::WR == 32, Rows32<D, T, SC, false>,
+                                        Rows16<D, T, SC, false>>::type;
     const bool rows = u.r0 + X::NR * w < sq.rows * a.G;  // else this wave only stages
     constexpr int KI = C::IT * KT;                       // keys an interval
     const int nint = (ntile + C::IT - 1) / C::IT;
@@ -802,97 +829,108 @@ __global__ __launch_bounds__((Tile<D, T, SC>::NT)) void ragged_tile_kernel(Ragge
     return;
   }
 
-  Rows16<D, T, SC, C::QLDS> x;
-  const int r = u.r0 + (lane & 15);
-  if (w >= C::NWN) {
-    x.init(a, u, sq, h, r, lane, lds + C::kQ);
-  } else {
-    char* const buf = lds + w * C::TB;
-    float* const ub = units + w * 2 * KT;
-    // K and V each have their registers where those are few enough
-    constexpr bool BOTH = C::CN * (int)sizeof(typename C::raw_t) <= 128;
-    constexpr bool Q8 = std::is_same<T, q8_t>::value;
-    // (an fp32 tile of d = 256 takes 128: its halves one after the other)
-    constexpr int HALVES = C::CN * (int)sizeof(typename C::raw_t) > 256 ? 2 : 1, CH = C::CN / HALVES;
-    typename C::raw_t raw[BOTH ? 2 : 1][CH];
-    float scale[2];          // (Q8: of key lane % 32)
-    constexpr int RPI = 64 / LPR;  // rows of a load
-    const int r_in = lane / LPR, j = lane % LPR, key = lane & 31;
-    const unsigned at = 8 * j < a.d ? 8 * j * (unsigned)sizeof(T) : 0;
-    const char *kp = a.k + at, *vp = a.v + at;
-    // A lane forms the place of one key, in units of 8 bytes, and the key's lanes take it
-    // from there.
-    auto ids = [&](int t) { return block_of(u.lo + t * KT + key); };
-    auto slot_of = [&](int t) { return min(u.lo + t * KT + key, last); };
-    auto place = [&](int t, int id) { return (unsigned)(C::row_at(pg, valid(id), slot_of(t)) >> 3); };
-    auto fetch = [&](int kv, int t, int id, unsigned off, int half = 0) {
+  auto narrow = [&](auto& x) {
+    using X = typename std::remove_reference<decltype(x)>::type;
+    const int r = u.r0 + (lane & (X::NR - 1));
+    if (w >= C::NWN) {
+      x.init(a, u, sq, h, r, lane, lds + C::kQ);
+    } else {
+      char* const buf = lds + w * C::TB;
+      float* const ub = units + w * 2 * KT;
+      // K and V each have their registers where those are few enough
+      constexpr bool BOTH = C::CN * (int)sizeof(typename C::raw_t) <= 128;
+      constexpr bool Q8 = std::is_same<T, q8_t>::value;
+      // (an fp32 tile of d = 256 takes 128: its halves one after the other)
+      constexpr int HALVES = C::CN * (int)sizeof(typename C::raw_t) > 256 ? 2 : 1, CH = C::CN / HALVES;
+      typename C::raw_t raw[BOTH ? 2 : 1][CH];
+      float scale[2];          // (Q8: of key lane % 32)
+      constexpr int RPI = 64 / LPR;  // rows of a load
+      const int r_in = lane / LPR, j = lane % LPR, key = lane & 31;
+      const unsigned at = 8 * j < a.d ? 8 * j * (unsigned)sizeof(T) : 0;
+      const char *kp = a.k + at, *vp = a.v + at;
+      // A lane forms the place of one key, in units of 8 bytes, and the key's lanes take it
+      // from there.
+      auto ids = [&](int t) { return block_of(u.lo + t * KT + key); };
+      auto slot_of = [&](int t) { return min(u.lo + t * KT + key, last); };
+      auto place = [&](int t, int id) { return (unsigned)(C::row_at(pg, valid(id), slot_of(t)) >> 3); };
+      auto fetch = [&](int kv, int t, int id, unsigned off, int half = 0) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i)
-        C::load((kv ? vp : kp) + ((uint64_t)(unsigned)__shfl((int)off, r_in + RPI * (half * CH + i)) << 3),
-                true, raw[BOTH ? kv : 0][i]);
-      if constexpr (Q8) scale[kv] = C::scale_at(pg, kv ? a.v : a.k, valid(id), slot_of(t));
-    };
-    auto stage = [&](int kv, unsigned off) {
-      float* const to = ub + kv * KT;
+        for (int i = 0; i < CH; ++i)
+          C::load((kv ? vp : kp) + ((uint64_t)(unsigned)__shfl((int)off, r_in + RPI * (half * CH + i)) << 3),
+                  true, raw[BOTH ? kv : 0][i]);
+        if constexpr (Q8) scale[kv] = C::scale_at(pg, kv ? a.v : a.k, valid(id), slot_of(t));
+      };
+      auto stage = [&](int kv, unsigned off) {
+        float* const to = ub + kv * KT;
 #pragma unroll
-      for (int half = 0; half < HALVES; ++half) {
-        unsigned top[CH];
-        const int r = r_in + RPI * CH * half;
-        if (half) fetch(kv, 0, 0, off, half);
-        C::template pieces<CH, RPI>(raw[BOTH ? kv : 0], kv, r, j, buf, top);
-        if (j == 0) {
+        for (int half = 0; half < HALVES; ++half) {
+          unsigned top[CH];
+          const int r = r_in + RPI * CH * half;
+          if (half) fetch(kv, 0, 0, off, half);
+          C::template pieces<CH, RPI>(raw[BOTH ? kv : 0], kv, r, j, buf, top);
+          if (j == 0) {
 #pragma unroll
-          for (int i = 0; i < CH; ++i) to[r + RPI * i] = __uint_as_float(top[i]);
+            for (int i = 0; i < CH; ++i) to[r + RPI * i] = __uint_as_float(top[i]);
+          }
         }
+        asm volatile("" ::: "memory");  // the wave's own LDS: in order
+        const unsigned mine = __float_as_uint(to[key]);
+        float unit;
+        if constexpr (Q8) unit = q8_unit(scale[kv], mine, kv);
+        else unit = unit_of(T{}, mine, kv);
+        to[key] = unit;  // (both lanes of a key the same)
+        asm volatile("" ::: "memory");
+      };
+      int id = 0, idn = 0;
+      unsigned off = 0;
+      if (w < ntile) {
+        id = ids(w);
+        off = place(w, id);
+        fetch(0, w, id, off);
+        if (BOTH) fetch(1, w, id, off);
+        idn = ids(w + C::NWN);
       }
-      asm volatile("" ::: "memory");  // the wave's own LDS: in order
-      const unsigned mine = __float_as_uint(to[key]);
-      float unit;
-      if constexpr (Q8) unit = q8_unit(scale[kv], mine, kv);
-      else unit = unit_of(T{}, mine, kv);
-      to[key] = unit;  // (both lanes of a key the same)
-      asm volatile("" ::: "memory");
-    };
-    int id = 0, idn = 0;
-    unsigned off = 0;
-    if (w < ntile) {
-      id = ids(w);
-      off = place(w, id);
-      fetch(0, w, id, off);
-      if (BOTH) fetch(1, w, id, off);
-      idn = ids(w + C::NWN);
+      x.init(a, u, sq, h, r, lane, lds + C::kQ);  // (the first rows on their way)
+      for (int t = w; t < ntile; t += C::NWN) {
+        const bool more = t + C::NWN < ntile;
+        stage(0, off);
+        const unsigned off1 = off;
+        if (!BOTH) fetch(1, t, id, off);
+        if (more) {
+          id = idn;
+          off = place(t + C::NWN, id);
+          idn = ids(t + 2 * C::NWN);
+          if (BOTH) fetch(0, t + C::NWN, id, off);
+        }
+        x.scores(buf, lane);
+        asm volatile("" ::: "memory");
+        stage(1, off1);
+        if (more) fetch(BOTH ? 1 : 0, t + C::NWN, id, off);
+        x.softmax(ub, ub + KT, u.lo + t * KT, lane);
+        x.pv(buf, lane);
+        asm volatile("" ::: "memory");
+      }
     }
-    x.init(a, u, sq, h, r, lane, lds + C::kQ);  // (the first rows on their way)
-    for (int t = w; t < ntile; t += C::NWN) {
-      const bool more = t + C::NWN < ntile;
-      stage(0, off);
-      const unsigned off1 = off;
-      if (!BOTH) fetch(1, t, id, off);
-      if (more) {
-        id = idn;
-        off = place(t + C::NWN, id);
-        idn = ids(t + 2 * C::NWN);
-        if (BOTH) fetch(0, t + C::NWN, id, off);
-      }
-      x.scores(buf, lane);
-      asm volatile("" ::: "memory");
-      stage(1, off1);
-      if (more) fetch(BOTH ? 1 : 0, t + C::NWN, id, off);
-      x.softmax(ub, ub + KT, u.lo + t * KT, lane);
-      x.pv(buf, lane);
-      asm volatile("" ::: "memory");
+    finish<1, C::NWN>(a, u, sq, h, x, 0, w, lds);
+  };
+  if constexpr (C::SR == 32) {
+    if (u.rows == 32) {
+      Rows32<D, T, SC, true> x;
+      narrow(x);
+      return;
     }
   }
-  finish<1, C::NWN>(a, u, sq, h, x, 0, w, lds);
+  Rows16<D, T, SC, C::QLDS> x;
+  narrow(x);
 }
 
 template <int D, bool SC>
 RaggedTile tile_of(int kv_dtype) {
-  using C = Tile<D, float, SC>;  // (the rows are every type's)
+  using C = Tile<D, float, SC>;  // (the wide rows are every type's)
   return {kv_dtype == MOLOT_KV_F32    ? ragged_tile_kernel<D, float, SC>
           : kv_dtype == MOLOT_KV_BF16 ? ragged_tile_kernel<D, bf16_t, SC>
                                       : ragged_tile_kernel<D, q8_t, SC>,
-          C::NT, C::QL, 16};
+          C::NT, C::QL, kv_dtype == MOLOT_KV_F32 ? C::SR : Tile<D, bf16_t, SC>::SR};
 }
 
 }  // namespace

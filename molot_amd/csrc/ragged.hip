@@ -27,7 +27,9 @@ using namespace molot_host;
 // takes ceil((len_b + count_b) / page) - ceil(len_b / page) blocks.  The free list is
 // a stack: finished sequences push their blocks (b, then the block's index, ascending),
 // then the new blocks are popped in the same order, so a block's place in the stack is
-// a prefix sum and every row finds its block by itself.  Nothing is committed before
+// a prefix sum and every row finds its block by itself.  What bounds it: one workgroup's chain
+// of loads, scans and the rows' search (5.5 us of 64 sequences; 18 of 4099, and 6 for their 64k
+// rows in a launch of their own).  Nothing is committed before
 // the whole batch is known to fit: a plan that fails writes its status, lengths as they
 // were, and rows of no sequence.
 struct PlanArgs {
@@ -282,7 +284,9 @@ __global__ __launch_bounds__(256) void ragged_rows_kernel(PlanArgs a) {
 // sequence, the keys each attends, and from their costs (a wide tile's key counts `weight`
 // narrow ones) the share of a workgroup that the chip holds at once.  Tiles that cost more are
 // split; so at most `target` units, one such workgroup each, come on top of one a tile.  The
-// list goes by cost, the largest first: the workgroups that start last are short.
+// list goes by cost, the largest first: the workgroups that start last are short.  One
+// workgroup's chain of loads and scans, 6 to 7 us of 7 to 64 sequences; in a step it runs beside
+// the append.
 constexpr int kUnitBuckets = 64;
 
 // Tiles of a sequence of R rows r: wide ones as long as more than `few` rows are left, then
@@ -415,7 +419,9 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_units_kernel(RaggedArgs a
 }
 
 // ---------------------------------------------------------------------------
-// Norms, RoPE and append of the packed rows: row r's heads normed and rotated at
+// Norms, RoPE and append of the packed rows (what bounds it: the stream, 103 MB of 2279 rows of
+// 32q/8kv/d128 bf16 in 24 us, 4.3 TB/s; 40 rows, 3.6 us: a wave's chain of loads, angles and
+// sums): row r's heads normed and rotated at
 // row_pos[r], k and v stored at row_slot[r] (< 0: the row is left as it is).  A
 // wave takes some heads of a row, lane l the pairs l, l + 64, ...; angles, sums and
 // roundings are those of rope_append_tok_kernel.
@@ -599,19 +605,21 @@ __global__ __launch_bounds__(kAppendThreads) void ragged_append_kernel(AppendArg
 
 // ---------------------------------------------------------------------------
 // Attention of any head dim and cache type: a unit's rows a wave each (ragged_own_row).
-// What bounds it: the latency of a key's rows and of the wave's sum, two keys at a time;
-// the units' splits fill the chip.
+// What bounds it: the latency of a key's rows and of the wave's sum, four keys at a time;
+// the units' splits (64 keys on, eight workgroups a CU) fill the chip.  16 sequences of one row
+// after 2000, 8q/2kv/d512: bf16 76 us (0.86 TB/s), Q8 94; 200 fresh fp32 rows 53.
 constexpr int kValuWaves = 4;
-template <int EPL>
+template <int EPL, typename T>
 __global__ __launch_bounds__(64 * kValuWaves) void ragged_valu_kernel(RaggedArgs a) {
   const int u = blockIdx.x / a.nkv, h = blockIdx.x - u * a.nkv;
   if (u >= a.head->nunits) return;
   const RaggedUnit t = a.units[u];
-  ragged_own_row<EPL>(a, t, h, t.r0 + (int)(threadIdx.x >> 6));
+  ragged_own_row<EPL, T>(a, t, h, t.r0 + (int)(threadIdx.x >> 6));
 }
 
 // ---------------------------------------------------------------------------
 // The merge of a split tile's n units: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+// Latency (unit, statistics, rows): 5 us of narrow tiles, 10 to 14 where wide ones are split.
 // The workgroups of the tile's parts share its rows: up to kMergeFew units a wave takes a
 // row by itself, past them a workgroup's waves share a row's units.
 constexpr int kMergeThreads = 256, kMergeWaves = kMergeThreads / 64, kMergeFew = 16;
@@ -759,23 +767,30 @@ struct Layout {
 // decoding sequences (bf16) 137 us at 3, 130 at 6, 127 at 8 and 10.
 constexpr int kWideWeight = 8;
 
+template <typename T>
+RaggedFn valu_of(int D) {
+  return D == 64    ? ragged_valu_kernel<1, T>
+         : D == 128 ? ragged_valu_kernel<2, T>
+         : D == 256 ? ragged_valu_kernel<4, T> : ragged_valu_kernel<8, T>;
+}
+
 // append, T rows: a step's, before the attention.
 int launch_attention(RaggedArgs a, const AppendArgs* append, void* stream) {
   LaunchLock lock(g_launch_mu);
   const int cus = num_cus();
   const int D = a.d <= 64 ? 64 : a.d <= 128 ? 128 : a.d <= 256 ? 256 : 512;
-  RaggedFn attend = a.d <= 64 ? ragged_valu_kernel<1>
-                    : a.d <= 128 ? ragged_valu_kernel<2>
-                    : a.d <= 256 ? ragged_valu_kernel<4> : ragged_valu_kernel<8>;
+  RaggedFn attend = a.kv_dtype == MOLOT_KV_F32    ? valu_of<float>(D)
+                    : a.kv_dtype == MOLOT_KV_BF16 ? valu_of<bf16_t>(D)
+                                                  : valu_of<q8_t>(D);
   RaggedFn merge = D == 64 ? ragged_merge_kernel<1>
                    : D == 128 ? ragged_merge_kernel<2>
                    : D == 256 ? ragged_merge_kernel<4> : ragged_merge_kernel<8>;
   int threads = 64 * kValuWaves;
   a.qs = a.ql = a.slot_rows = kValuWaves;
   a.few = 0;  // every tile a wide one
-  a.min_keys = 256;
+  a.min_keys = 64;
   a.weight = 1;
-  int per_cu = 4;
+  int per_cu = 8;
   // (the matrix-core kernel's offsets are of 31 bits within a block, and of 35 in a pool)
   const int64_t block = ((int64_t)a.nkv << a.page_shift) *
                         (a.kv_dtype == MOLOT_KV_Q8 ? a.d + 4 : a.d * (a.kv_dtype == MOLOT_KV_BF16 ? 2 : 4));

@@ -110,11 +110,6 @@ __device__ __forceinline__ int64_t ragged_row_of(const RaggedArgs& a, int blk, i
   scale = b0 + rows * a.d + 4 * ((int64_t)h * page + sl);
   return b0 + ((int64_t)h * page + sl) * a.d;
 }
-__device__ __forceinline__ int64_t ragged_row(const RaggedArgs& a, int blk, int h, int t,
-                                              int64_t& scale) {
-  return a.kv_dtype == MOLOT_KV_Q8 ? ragged_row_of<q8_t>(a, blk, h, t, scale)
-                                   : ragged_row_of<float>(a, blk, h, t, scale);
-}
 
 // The scores past the product of query row r (head h*G + g) at its slot.
 __device__ __forceinline__ RowScore ragged_score(const RaggedArgs& a, int head, int slot) {
@@ -122,24 +117,28 @@ __device__ __forceinline__ RowScore ragged_score(const RaggedArgs& a, int head, 
 }
 
 // Query row r of a unit by one wave, over the row's own keys alone: lanes over the head
-// dim (elements lane + 64*i), two keys in flight.  To O, or to the unit's partials.
+// dim (elements lane + 64*i), NK keys in flight.  To O, or to the unit's partials.
 // The rows of ragged_valu_kernel, and of the matrix-core kernel those over cached rows
 // that its pieces cannot hold (infinities, NaN): a row that they do not belong to is
 // not reached by them.
-template <int EPL>
+template <int EPL, typename T>
 __device__ __forceinline__ void ragged_own_row(const RaggedArgs& a, const RaggedUnit& u, int h, int r) {
-  constexpr int D = 64 * EPL;
+  constexpr int D = 64 * EPL, NK = 4;
+  constexpr bool Q8 = std::is_same<T, q8_t>::value;
   const int lane = threadIdx.x & 63;
   const RaggedSeq& s = u.s;
   if (r >= s.rows * a.G) return;
   const int m = r / a.G, g = r - m * a.G, slot = s.slot0 + m, head = h * a.G + g;
   const int lo = max(ragged_lo(a, slot), u.lo), hi = min(ragged_hi(a, slot), u.hi);
-  const bool q8 = a.kv_dtype == MOLOT_KV_Q8;
+  // (lanes past d read the row's last element, so that no load waits for a branch)
   auto elem = [&](const char* base, int64_t off, int e) {
-    if (q8) return (float)reinterpret_cast<const int8_t*>(base)[off + e];
-    if (a.kv_dtype == MOLOT_KV_BF16)
-      return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(base)[off + e] << 16);
-    return reinterpret_cast<const float*>(base)[off + e];
+    const int64_t i = off + min(e, a.d - 1);
+    float x;
+    if constexpr (Q8) x = (float)reinterpret_cast<const int8_t*>(base)[i];
+    else if constexpr (std::is_same<T, bf16_t>::value)
+      x = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(base)[i] << 16);
+    else x = reinterpret_cast<const float*>(base)[i];
+    return e < a.d ? x : 0.f;
   };
   const RowScore score = ragged_score(a, head, slot);
   const int64_t at = ((int64_t)(s.start + m) * a.nq + head) * a.d;
@@ -151,28 +150,38 @@ __device__ __forceinline__ void ragged_own_row(const RaggedArgs& a, const Ragged
   }
   const float qsc = a.scale * kLog2e;
   float mx = -INFINITY, l = 0.f;
-  for (int t0 = lo; t0 < hi; t0 += 2) {
-    float x[2], v[2][EPL];
+  for (int t0 = lo; t0 < hi; t0 += NK) {
+    float x[NK], k[NK][EPL], v[NK][EPL], ks[NK], vs[NK];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NK; ++j) {
       const int t = min(t0 + j, hi - 1);
       int64_t sc = 0;
-      const int64_t off = ragged_row(a, ragged_block(a, u.seq, t), h, t, sc);
-      const float ks = q8 ? *reinterpret_cast<const float*>(a.k + sc) : 1.f;
-      const float vs = q8 ? *reinterpret_cast<const float*>(a.v + sc) : 1.f;
-      float dot = 0.f;
+      const int64_t off = ragged_row_of<T>(a, ragged_block(a, u.seq, t), h, t, sc);
+      ks[j] = Q8 ? *reinterpret_cast<const float*>(a.k + sc) : 1.f;
+      vs[j] = Q8 ? *reinterpret_cast<const float*>(a.v + sc) : 1.f;
 #pragma unroll
       for (int i = 0; i < EPL; ++i) {
-        const int e = lane + 64 * i;
-        if (e < a.d) dot = fmaf(q[i], elem(a.k, off, e), dot);
-        v[j][i] = e < a.d ? elem(a.v, off, e) * vs : 0.f;
+        k[j][i] = elem(a.k, off, lane + 64 * i);
+        v[j][i] = elem(a.v, off, lane + 64 * i);
       }
-      x[j] = wave_reduce<false>(dot) * (ks * qsc);
     }
-    const float raw[2] = {x[0], x[1]};
-    score.apply<2>(x, [&](int j) { return t0 + j; }, [&](int j) { return raw[j]; });
-    if (t0 + 1 >= hi) x[1] = -INFINITY;
-    const float mn = fmaxf(mx, fmaxf(x[0], x[1]));
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) dot = fmaf(q[i], k[j][i], dot);
+      x[j] = wave_reduce<false>(dot) * (ks[j] * qsc);
+    }
+    float raw[NK];
+#pragma unroll
+    for (int j = 0; j < NK; ++j) raw[j] = x[j];
+    score.apply<NK>(x, [&](int j) { return t0 + j; }, [&](int j) { return raw[j]; });
+    float mn = mx;
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      if (t0 + j >= hi) x[j] = -INFINITY;
+      mn = fmaxf(mn, x[j]);
+    }
     if (mn > mx) {
       const float f = exp2_hw(mx - mn);
       l *= f;
@@ -181,12 +190,12 @@ __device__ __forceinline__ void ragged_own_row(const RaggedArgs& a, const Ragged
       mx = mn;
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NK; ++j) {
       if (t0 + j >= hi) break;
       const float p = x[j] == -INFINITY ? 0.f : exp2_hw(x[j] - mx);
       l += p;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) o[i] = fmaf(p, v[j][i], o[i]);
+      for (int i = 0; i < EPL; ++i) o[i] = fmaf(p, Q8 ? v[j][i] * vs[j] : v[j][i], o[i]);
     }
   }
   if (u.part >= 0) {

@@ -196,6 +196,7 @@ struct Tile {
   static constexpr int LDS = kQ + SR * D * 4;
   static_assert(LDS <= 160 * 1024, "fits a CU");
 
+  using elem_t = T;
   using raw_t = Raw<T>;
 
   // Where rows lie, in bytes: block blk at blk * block, row sl of KV head h of it at
@@ -652,7 +653,7 @@ __device__ __forceinline__ void finish(const RaggedArgs& a, const RaggedUnit& u,
   const int r = u.r0 + X::NR * rg + (lane & (X::NR - 1));
   // a row that the pieces cannot hold: the unit's rows again, each over its own keys
   if (__syncthreads_or(x.mark != 0.f)) {
-    for (int i = w; i < RG * X::NR; i += C::NW) ragged_own_row<D / 64>(a, u, h, u.r0 + i);
+    for (int i = w; i < RG * X::NR; i += C::NW) ragged_own_row<D / 64, typename C::elem_t>(a, u, h, u.r0 + i);
     return;
   }
   // the key groups' merge, halves at a time: o in units of 2^m

@@ -524,3 +524,90 @@ def test_two_graphs_of_one_stream(gpu):
                 want, tol = b.attend(q, 0.1)
                 close(O, want, tol)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("nq,nkv,d", [(8, 2, 128), (4, 4, 64), (10, 2, 96), (8, 4, 256)])
+def test_rows_about_a_narrow_tile(gpu, kv, nq, nkv, d):
+    """Sequences whose rows just fill a narrow tile of 16 or 32, or pass it: alone (partials of
+    that many rows), long enough to be split, and beside others and wide tiles."""
+    G = nq // nkv
+    for R in (15, 16, 17, 31, 32, 33):
+        n = -(-R // G)
+        run(kv, nq, nkv, d, [n], [5000])
+        run(kv, nq, nkv, d, [n], [3], softcap=30.0, alibi=True)
+        run(kv, nq, nkv, d, [n, 0, 1, n + 256 // G, n], [37, 9, 2000, 60, 1100], pad=3, window=700)
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("d", (64, 128, 256))
+def test_drafts_before_a_row_that_is_not_finite(gpu, d, value):
+    """A draft's row that is not finite: the rows before it, in the same narrow tile, stay exact,
+    and so do the other sequences."""
+    for G, count in ((4, 5), (1, 20), (3, 5)):
+        g = gen(4)
+        b = rr.Batch(g, "bf16", 2, d, [count, 1, count], [2100, 300, 40])
+        q = randn(g, b.T, 2 * G, d)
+        t = 2100 + count - 2
+        for which in ("K", "V"):
+            pool = getattr(b, which).view(b.blocks, 2, 16, d)
+            at = (int(b.table[0, t // 16]), slice(None), t % 16, 3)
+            was = pool[at].clone()
+            pool[at] = value
+            O = attend(b, q, 2 * G, 0.1)
+            pool[at] = was
+            want, tol = b.attend(q, 0.1)
+            keep = torch.ones(b.rows, dtype=torch.bool, device="cuda")
+            keep[count - 2:count] = False
+            close(O[keep], want[keep], tol)
+            if which == "V":
+                assert not torch.isfinite(O[~keep]).all()
+
+
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("d", (34, 320, 512))
+def test_split_rows_on_the_vector_alu(gpu, kv, d):
+    """Head dims off the matrix cores: long rows split in many units, all masks, slots past the end."""
+    d = d if kv != "q8" else (d + 3) // 4 * 4
+    run(kv, 8, 2, d, [1, 6, 0, 2], [6000, 700, 3, 1], pad=1)
+    run(kv, 8, 2, d, [1, 6, 0, 2], [6000, 700, 3, 1], window=65, softcap=20.0, alibi=True)
+    if kv != "q8":
+        run(kv, 8, 2, d, [1, 5], [66, 0], fill=math.nan)
+
+
+def test_one_graph_serves_smaller_ticks(gpu):
+    """Captured at its bounds, replayed over lengths that change between the replays: one row,
+    drafts and prompt parts by turns, each as the eager call has it."""
+    nq, nkv, d = 8, 2, 128
+    g = gen(9)
+    b = rr.Batch(g, "bf16", nkv, d, [300, 5, 1], [900, 1500, 40])
+    q = randn(g, b.T, nq, d)
+    O = torch.zeros_like(q)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        attend(b, q, nq, 0.1, O=O)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        attend(b, q, nq, 0.1, O=O)
+    starts, lens = b.row_start.clone(), b.kv_lens.clone()
+    for counts in ([300, 5, 1], [1, 1, 1], [5, 5, 0], [0, 0, 0], [40, 1, 8], [300, 5, 1]):
+        now = [0]
+        for c in counts:
+            now.append(now[-1] + c)
+        b.row_start.copy_(torch.tensor(now, dtype=torch.int32))
+        b.kv_lens.copy_(lens - torch.tensor([300 - counts[0], 5 - counts[1], 1 - counts[2]],
+                                            dtype=torch.int32, device="cuda").clamp(min=0))
+        O.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = O.clone()
+        want = attend(b, q, nq, 0.1, O=torch.full_like(q, 7.0))
+        torch.cuda.synchronize()
+        assert (got[now[-1]:] == 7.0).all()
+        # (the same kernels over the same lengths: at most another order of a tile's units)
+        assert float((got - want).abs().max()) <= 1e-6 * max(1.0, float(want.abs().max()))
+    b.row_start.copy_(starts)
+    b.kv_lens.copy_(lens)

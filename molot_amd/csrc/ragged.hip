@@ -800,8 +800,11 @@ int launch_attention(RaggedArgs a, const AppendArgs* append, void* stream) {
     threads = t.threads;
     a.qs = t.narrow;
     a.ql = t.wide;
-    a.few = 2 * kSlimRows;
-    a.min_keys = 512;
+    // Two narrow tiles at most.  16 sequences of 64 rows r after 2000, in narrow tiles and in a
+    // wide one: bf16 67 and 74 us, Q8 59 and 70 (two tiles of 32); fp32 123 and 98, d = 256 bf16
+    // (40 rows r) 102 and 54 (three or four of 16).
+    a.few = 2 * t.narrow;
+    a.min_keys = 512;  // (512 to 1024 the same; 256 leaves a wave one tile)
     a.weight = kWideWeight;
     // (a tile holds no more rows than the batch)
     a.slot_rows = (int64_t)a.T * a.G <= kSlimRows ? kSlimRows : (int64_t)a.T * a.G <= a.few ? a.qs : a.ql;

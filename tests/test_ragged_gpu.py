@@ -529,10 +529,10 @@ def test_two_graphs_of_one_stream(gpu):
 @pytest.mark.parametrize("kv", KVS)
 @pytest.mark.parametrize("nq,nkv,d", [(8, 2, 128), (4, 4, 64), (10, 2, 96), (8, 4, 256)])
 def test_rows_about_a_narrow_tile(gpu, kv, nq, nkv, d):
-    """Sequences whose rows just fill a narrow tile of 16 or 32, or pass it: alone (partials of
+    """Sequences whose rows just fill a narrow tile of 16 or 32, or two, or pass it: alone (partials of
     that many rows), long enough to be split, and beside others and wide tiles."""
     G = nq // nkv
-    for R in (15, 16, 17, 31, 32, 33):
+    for R in (15, 16, 17, 31, 32, 33, 63, 64, 65):
         n = -(-R // G)
         run(kv, nq, nkv, d, [n], [5000])
         run(kv, nq, nkv, d, [n], [3], softcap=30.0, alibi=True)

@@ -30,6 +30,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <stdexcept>
+#include <utility>
 #include <vector>
 
 #include "molot_amd/attn.hpp"
@@ -103,20 +104,23 @@ class PagedKVCache {
   // ---- decode: one new token for each sequence of a batch ----
   // Reserves a slot per sequence and uploads the batch's block table
   // [B][max_blocks] and lengths (counting the new token) on stream s.
-  // Throws "fwd: KV cache full" (forward.h:570) before any state of the
-  // step is set when the pool cannot hold the batch's new tokens.
+  // Throws "fwd: KV cache full" (forward.h:570) when the pool cannot hold the
+  // batch's new tokens.  A step that does not begin, for this reason or another,
+  // keeps no blocks: the pool and every sequence are as they were.
   void begin_decode(const std::vector<int>& ids, hipStream_t s = nullptr) {
     if (mode_ != Mode::None) throw std::runtime_error("PagedKVCache: a step is in progress");
     std::vector<int32_t> lens(ids.size());
     int maxb = 1;
+    Reserved blocks(*this);
     for (size_t i = 0; i < ids.size(); ++i) {
-      reserve(ids[i], 1);
+      blocks.take(ids[i], 1);
       lens[i] = seq(ids[i]).len + 1;
       maxb = std::max(maxb, (int)seq(ids[i]).blocks.size());
     }
     upload(ids, maxb, lens, s);
     batch_ = ids;
     mode_ = Mode::Decode;
+    blocks.keep();
   }
   // forward.h:554-591 for one layer over the batch: q [B][nq][hd] (normed
   // and rotated in place), k/v [B][nkv][hd] (normed, rotated, appended),
@@ -174,12 +178,14 @@ class PagedKVCache {
   void begin_prefill(int id, int M, hipStream_t s = nullptr) {
     if (mode_ != Mode::None) throw std::runtime_error("PagedKVCache: a step is in progress");
     if (M <= 0) throw std::runtime_error("PagedKVCache: empty prompt");
-    reserve(id, M);
+    Reserved blocks(*this);
+    blocks.take(id, M);
     batch_ = {id};
     const Seq& q = seq(id);
     upload(batch_, (int)q.blocks.size(), {q.len + M}, s);
     prefill_m_ = M;
     mode_ = Mode::Prefill;
+    blocks.keep();
   }
   // forward.h:367-399 for one layer: q [M][nq][hd] (normed, rotated in
   // place), k/v [M][nkv][hd], o [M][nq][hd]; positions pos0 .. pos0+M-1.
@@ -236,8 +242,8 @@ class PagedKVCache {
   // Their rows are packed in the order of ids: q [T][nq][hd], k/v [T][nkv][hd],
   // o [T][nq][hd], T = rows().  Reserves their slots and makes the batch's index arrays
   // on stream s (molot_hip_ragged_plan, over the tables of this class's allocator).
-  // Throws "fwd: KV cache full" before any state of the step is set, and for a cache
-  // held to a budget, whose books go by prefill() and decode_scored().
+  // Throws "fwd: KV cache full" as begin_decode does, with no sequence's blocks kept,
+  // and for a cache held to a budget, whose books go by prefill() and decode_scored().
   void begin_batch(const std::vector<int>& ids, const std::vector<int>& counts,
                    hipStream_t s = nullptr) {
     if (mode_ != Mode::None) throw std::runtime_error("PagedKVCache: a step is in progress");
@@ -256,8 +262,9 @@ class PagedKVCache {
       more[B + i] = seq(ids[i]).len;
     }
     if (rows == 0 || rows > (1 << 20)) throw std::runtime_error("PagedKVCache: a batch of no rows, or too many");
+    Reserved blocks(*this);
     for (size_t i = 0; i < B; ++i) {
-      reserve(ids[i], counts[i]);
+      blocks.take(ids[i], counts[i]);
       after[i] = seq(ids[i]).len + counts[i];
       maxb = std::max(maxb, (int)seq(ids[i]).blocks.size());
     }
@@ -279,6 +286,7 @@ class PagedKVCache {
     batch_ = ids;
     counts_ = counts;
     mode_ = Mode::Batch;
+    blocks.keep();
   }
   int rows() const { return T_; }
   // One layer over the batch: forward.h:554-591 for every row, q, k, v and o device
@@ -419,17 +427,40 @@ class PagedKVCache {
     if (cut_ && window > 0 && pos >= window)
       throw std::runtime_error("PagedKVCache: a window over a sequence that rows were evicted from");
   }
-  // Blocks for `tokens` more tokens of sequence id, from the shared pool.
-  void reserve(int id, int tokens) {
-    Seq& s = seq(id);
-    const int need = (s.len + tokens + page_ - 1) / page_;
-    if (need - (int)s.blocks.size() > (int)free_.size())
-      throw std::runtime_error("fwd: KV cache full");
-    while ((int)s.blocks.size() < need) {
-      s.blocks.push_back(free_.back());
-      free_.pop_back();
+  // The blocks that a step takes from the shared pool.  Those of a step that does not
+  // begin (no keep()) go back the way they came.
+  class Reserved {
+   public:
+    explicit Reserved(PagedKVCache& kv) : kv_(kv) {}
+    ~Reserved() {
+      for (; !from_.empty(); from_.pop_back()) {
+        std::vector<int>& blocks = kv_.seqs_[from_.back().first].blocks;
+        while (blocks.size() > from_.back().second) {
+          kv_.free_.push_back(blocks.back());  // (no more than it has held)
+          blocks.pop_back();
+        }
+      }
     }
-  }
+    Reserved(const Reserved&) = delete;
+    Reserved& operator=(const Reserved&) = delete;
+    // Blocks for `tokens` more tokens of sequence id.
+    void take(int id, int tokens) {
+      Seq& s = kv_.seq(id);
+      const int need = (s.len + tokens + kv_.page_ - 1) / kv_.page_;
+      if (need - (int)s.blocks.size() > (int)kv_.free_.size())
+        throw std::runtime_error("fwd: KV cache full");
+      from_.emplace_back(id, s.blocks.size());
+      while ((int)s.blocks.size() < need) {
+        s.blocks.push_back(kv_.free_.back());
+        kv_.free_.pop_back();
+      }
+    }
+    void keep() { from_.clear(); }
+
+   private:
+    PagedKVCache& kv_;
+    std::vector<std::pair<int, size_t>> from_;  // sequence, and the blocks it had
+  };
   // The batch's block table [B][maxb] and lengths to the device, through a
   // pinned staging buffer whose previous copy has finished (event).
   // (more: further words, after the positions)

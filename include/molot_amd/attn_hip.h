@@ -444,7 +444,8 @@ int molot_hip_kv_evict_paged(void* K, void* V, float* acc, int32_t* slot_pos,
  * sequence b, and kv_lens[b] counts them.  All index arrays are device int32; what
  * they hold is known to the device alone, so that a serving loop needs no copy to the
  * host and can be captured in a graph.  T is a bound of the rows (the arrays' length):
- * rows from row_start[B] on are left as they are.  num_blocks: blocks of the pool;
+ * rows from row_start[B] on are left as they are, and where row_start does not ascend
+ * attention leaves all of them.  num_blocks: blocks of the pool;
  * ids outside it are never followed (such a row is not stored, and attention over it
  * unspecified).
  *

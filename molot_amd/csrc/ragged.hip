@@ -319,17 +319,19 @@ __device__ __forceinline__ UnitTile unit_tile(const RaggedArgs& a, int t, int nw
 // NT threads of one workgroup.
 template <int NT>
 __device__ __forceinline__ void make_units(const RaggedArgs& a) {
-  __shared__ int sh[NT / 64], s_bucket[kUnitBuckets];
+  __shared__ int sh[NT / 64], s_bucket[kUnitBuckets], s_none;
   __shared__ unsigned long long s_cost;
   __shared__ int s_tiles[2 * (kPlanSeqs + 1)];
   const int tid = threadIdx.x;
   const bool in_lds = a.B <= kPlanSeqs;
-  if (tid == 0) s_cost = 0;
+  if (tid == 0) s_cost = s_none = 0;
   if (tid < kUnitBuckets) s_bucket[tid] = 0;
   int nwide = 0, nslim = 0;
+  bool none = false;
   for (int b0 = 0; b0 < a.B; b0 += NT) {
     const int b = b0 + tid;
     const int R = b < a.B ? ragged_seq(a, b).rows * a.G : 0;
+    none |= b < a.B && a.row_start[b + 1] < a.row_start[b];
     int t0, t1;
     const int w = nwide + block_scan<NT>(wide_tiles(a, R), sh, t0);
     const int s = nslim + block_scan<NT>(slim_tiles(a, R), sh, t1);
@@ -341,8 +343,14 @@ __device__ __forceinline__ void make_units(const RaggedArgs& a) {
       at[1] = s;
     }
   }
+  if (none) s_none = 1;  // (past the scans' barriers)
   __threadfence_block();
   __syncthreads();
+  // Starts that ascend are those of at most T rows, which the lists' bounds stand on.
+  if (s_none) {
+    if (tid == 0) a.head->nunits = a.head->nparts = 0;
+    return;
+  }
   const int ntiles = nwide + nslim;
   auto before = [&](int b, int kind) { return in_lds ? s_tiles[2 * b + kind] : a.tiles[2 * b + kind]; };
   // (a batch of at most NT tiles keeps them; a larger one finds each again)

@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, i
     int x = 0, y = 0, z = 0;  // (each at most N * kPlanMost: a wave's sum stays below 2^31)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (s[i].st) st = s[i].st;
+      st = min(st, s[i].st);
       x += s[i].count;
       y += s[i].take;
       z += s[i].give;

@@ -460,7 +460,8 @@ int molot_hip_kv_evict_paged(void* K, void* V, float* acc, int32_t* slot_pos,
  *                   row, or where the table's entry is no block of the pool);
  *   status          [1] 0, or why the batch was not planned: MOLOT_EINVAL (a negative
  *                   count or length, more rows than max_blocks * page, a free list
- *                   that is none), MOLOT_E2BIG (more rows than max_rows), MOLOT_ENOSPC
+ *                   that is none, a given-back or new block that is none of the
+ *                   pool's), MOLOT_E2BIG (more rows than max_rows), MOLOT_ENOSPC
  *                   (not enough blocks).  Then kv_lens = seq_lens, free_left =
  *                   free_count, the table is as it was, and the batch has no rows.
  * free_blocks [num_blocks] is the free list, a stack of free_count[0] ids: new blocks

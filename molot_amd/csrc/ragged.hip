@@ -154,6 +154,10 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, i
   const int tid = threadIdx.x;
   const bool pool = a.free_blocks != nullptr;
   const int count0 = pool ? *a.free_count : 0;
+  auto none = [&](int id) { return (unsigned)id >= (unsigned)a.num_blocks; };
+  // the list's top, on its way beside the sequences
+  const bool listed = pool && tid < count0 && count0 <= a.num_blocks;
+  const int id0 = listed ? a.free_blocks[count0 - 1 - tid] : 0;
   if (tid < 3) s_sum[tid] = 0;
   if (tid == 0) s_st = 0;
   // totals, and whether the batch fits
@@ -194,10 +198,13 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, i
   const int top = count0 + (int)(st ? 0 : give);
   // finished sequences' blocks above the stack's top (unused places if the plan fails)
   // (a sequence's blocks by a wave: their number is uneven, and a lane each would wait for
-  // the longest)
-  if (st == 0 && give > 0) {
+  // the longest), and whether they and the new blocks are blocks of the pool
+  if (st == 0 && (give > 0 || take > 0)) {
+    const int old = take > give ? (int)(take - give) : 0;  // new blocks off the list as it was
+    bool bad = tid < old && none(id0);
+    for (int i = tid + kPlanThreads; i < old; i += kPlanThreads) bad |= none(a.free_blocks[count0 - 1 - i]);
     int base = count0;
-    for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
+    for (int b0 = 0; give > 0 && b0 < a.B; b0 += kPlanThreads) {
       const PlanSeq s = plan_seq(a, b0 + tid);
       int all;
       const int at = base + block_scan<kPlanThreads>(s.give, sh, all);
@@ -208,14 +215,13 @@ __global__ __launch_bounds__(kPlanThreads) void ragged_plan_kernel(PlanArgs a, i
         const int32_t* from = a.block_table + (int64_t)(b0 + (tid & ~63) + l) * a.max_blocks;
         for (int j = tid & 63; j < n; j += 64) {
           const int id = from[j];
-          if ((unsigned)id >= (unsigned)a.num_blocks) atomicMin(&s_st, MOLOT_EINVAL);
+          bad |= none(id);
           a.free_blocks[to + j] = id;
         }
       }
     }
     __threadfence_block();
-    __syncthreads();
-    st = s_st;  // (a block that is none)
+    if (__syncthreads_or(bad)) st = MOLOT_EINVAL;
   }
   // the batch as it will be
   int row0 = 0, taken0 = 0;

@@ -48,3 +48,50 @@ def test_the_status_of_several_errors(gpu, B, apart, first):
     assert want["status"] == rr.E2BIG
     same = plan(counts, lens, table, page, num, max_rows, list(range(num))) == want
     assert same
+
+
+@pytest.mark.parametrize("B,each,max_rows", [(4, 20, 300), (300, 9, 2700), (5000, 1, 5000), (3, 2000, 6000)])
+def test_new_blocks_that_are_none(gpu, B, each, max_rows):
+    """Ids out of the pool among those that the new blocks come off: nothing is planned.  Below
+    them, and beneath what finished sequences give back, the list is not asked."""
+    page, width = 16, 130
+    need = B * -(-each // page)
+    num = need + 2 * page + 9
+    ids = list(range(num))[::-1]
+    counts, lens, table = [each] * B, [0] * B, [[-1] * width] * B
+    fits = rr.plan(counts, lens, table, page, num, max_rows, ids)
+    same = plan(counts, lens, table, page, num, max_rows, ids) == fits
+    assert fits["status"] == 0 and same
+    for at in {num - 1, num - 1 - need // 2, num - need}:  # the first, one between, the last taken
+        for value in (num, -1, 2 ** 31 - 1, -2 ** 31):
+            free = list(ids)
+            free[at] = value
+            got = plan(counts, lens, table, page, num, max_rows, free)
+            same = got == dict(status=rr.EINVAL, kv_lens=lens, table=table, free=free, row_start=[0] * (B + 1),
+                               row_seq=[-1] * max_rows, row_pos=[0] * max_rows, row_slot=[-1] * max_rows)
+            assert same, (at, value, got["status"])
+    free = list(ids)
+    free[num - need - 1] = num  # not taken
+    got = plan(counts, lens, table, page, num, max_rows, free)
+    same = got == dict(fits, free=free[:num - need])
+    assert same
+    # a finished sequence's blocks come off first: the list's own top is one further down
+    have = min(3, need)
+    lens, done = [have * page] + lens[1:], [1] + [0] * (B - 1)
+    table = [ids[num - have:] + [-1] * (width - have)] + table[1:]
+    free = ids[:num - have]
+    fits = rr.plan(counts, lens, table, page, num, max_rows, free, done)
+    same = plan(counts, lens, table, page, num, max_rows, free, done=done) == fits
+    assert fits["status"] == 0 and same
+    for at, st in ((len(free) - (need - have), rr.EINVAL), (len(free) - (need - have) - 1, 0)):
+        if at == len(free):  # nothing of the list is taken
+            continue
+        bad = list(free)
+        bad[at] = num
+        got = plan(counts, lens, table, page, num, max_rows, bad, done=done)
+        if st:
+            same = got["kv_lens"] == lens and got["table"] == table and got["free"] == bad
+            assert got["status"] == st and same and set(got["row_slot"]) == {-1}
+        else:
+            same = got == dict(fits, free=bad[:len(fits["free"])])
+            assert same

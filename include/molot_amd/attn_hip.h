@@ -497,8 +497,8 @@ int molot_hip_rope_append_ragged(float* q, const float* k_new, const float* v_ne
  * b is at slot s = kv_lens[b] - count + i, count its rows, and attends slots [t0, s],
  * t0 = max(0, s - window + 1) for window > 0 (else 0).  softcap and slopes as the scored
  * entries take them (0 and NULL: plain scores), i the slot.  Q and O [T][nq][d], O not Q.
- * max_len: a bound of every kv_lens[b] (the longest, or a table's capacity); slots past
- * it are left out. */
+ * max_len: a bound of every kv_lens[b] (the longest, or a table's capacity), up to
+ * 2^31 - 1025 (MOLOT_ENOTSUP past it); slots past it are left out. */
 int molot_hip_attn_ragged(const float* Q, const void* K, const void* V, float* O,
                           const int32_t* block_table, const int32_t* kv_lens,
                           const int32_t* row_start, int T, int B, int max_blocks, int num_blocks,

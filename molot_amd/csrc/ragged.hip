@@ -716,6 +716,11 @@ __global__ __launch_bounds__(kMergeThreads) void ragged_merge_kernel(RaggedArgs 
 
 // ---------------------------------------------------------------------------
 // Host.
+
+// Keys of a sequence: the kernels count them in an int, up to 511 past the last (the next
+// tile's blocks of the last wave, and what a tile or a split is rounded up to).
+constexpr int kMostKeys = 0x7FFFFFFF - 1024;
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 int shift_of(int page) {
@@ -874,7 +879,7 @@ int attention_args(RaggedArgs& a, const float* Q, const void* K, const void* V, 
       (!Q || !K || !V || !O || !block_table || !kv_lens || !row_start || Q == O))
     return MOLOT_EINVAL;
   if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(O)) return MOLOT_EINVAL;
-  if (T > kPlanMost || B > kPlanMost) return MOLOT_ENOTSUP;
+  if (T > kPlanMost || B > kPlanMost || max_len > kMostKeys) return MOLOT_ENOTSUP;
   if (!(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f))) return MOLOT_EINVAL;
   a.q = Q;
   a.k = reinterpret_cast<const char*>(K);

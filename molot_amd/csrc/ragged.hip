@@ -137,8 +137,17 @@ __device__ __forceinline__ int plan_find(int B, int r, START&& start) {
   return lo;
 }
 
+// Rounds of sequences at once, the fewest that even passes of at most kPlanBatch rounds take
+// (plan_rounds): 1500, 4096, 4099, 5121, 8192 and 65536 sequences of one row take 10.1, 14.4,
+// 15.0, 17.9, 20.3 and 105 us so, one round at a time 10.0, 15.3, 16.3, 18.3, 21.7 and 113;
+// 6 or 8 rounds at once no less (5121 17.8, 8192 21.0, 65536 107).
+constexpr int kPlanBatch = 5;
+int plan_rounds(int B) {
+  const int rounds = std::max(1, (B + kPlanThreads - 1) / kPlanThreads);
+  const int passes = (rounds + kPlanBatch - 1) / kPlanBatch;
+  return (rounds + passes - 1) / passes;
+}
 // Sequences b0 + tid, b0 + kPlanThreads + tid, ...: their loads in flight together.
-constexpr int kPlanBatch = 5;  // (of a batch of more than kPlanThreads)
 template <int N>
 __device__ __forceinline__ void plan_batch(const PlanArgs& a, int b0, PlanSeq (&s)[N]) {
 #pragma unroll
@@ -968,8 +977,12 @@ int molot_hip_ragged_plan(const int32_t* counts, const int32_t* done, const int3
     if (st) return st;
     a.taken = reinterpret_cast<int32_t*>(ws);
   }
-  hipLaunchKernelGGL(B <= kPlanThreads ? ragged_plan_kernel<1> : ragged_plan_kernel<kPlanBatch>, dim3(1),
-                     dim3(kPlanThreads), 0, (hipStream_t)stream, a, rows ? 1 : 0);
+  const int n = plan_rounds(B);
+  auto plan = n == 1   ? ragged_plan_kernel<1>
+              : n == 2 ? ragged_plan_kernel<2>
+              : n == 3 ? ragged_plan_kernel<3>
+              : n == 4 ? ragged_plan_kernel<4> : ragged_plan_kernel<kPlanBatch>;
+  hipLaunchKernelGGL(plan, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, a, rows ? 1 : 0);
   if (!rows && max_rows > 0)
     hipLaunchKernelGGL(ragged_rows_kernel, dim3((max_rows + 255) / 256), dim3(256), 0,
                        (hipStream_t)stream, a);

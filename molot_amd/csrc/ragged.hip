@@ -464,7 +464,12 @@ struct AppendArgs {
   int64_t slots;  // of the pool
   float eps;
 };
-constexpr int kAppendThreads = 256, kAppendWaves = kAppendThreads / 64, kAppendHeads = 10;
+constexpr int kAppendThreads = 256, kAppendWaves = kAppendThreads / 64;
+// Heads a wave at most, past the rows that fill the chip: each shares the wave's angles, and
+// fewer waves are in flight.  At most 2, 4, 6, 10 and 16 (us, normed rows): 4000 of 32q/8kv/d128
+// bf16 41, 37, 36, 35, 38, 8192 of them fp32 92, 87, 90, 94, 97; 8192 of 8q/8kv/d64 bf16 35, 31,
+// 33, 34, 39; of 8q/4kv/d256 47, 41, 42, 44, 47; 4000 of 64q/8kv/d128 69, 62, 56, 57, 54.
+constexpr int kAppendHeads = 6;
 
 // UNITS: a step's; one more workgroup forms the attention's units meanwhile.
 template <int KMAX, bool UNITS>

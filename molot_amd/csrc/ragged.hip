@@ -28,10 +28,10 @@ using namespace molot_host;
 // a stack: finished sequences push their blocks (b, then the block's index, ascending),
 // then the new blocks are popped in the same order, so a block's place in the stack is
 // a prefix sum and every row finds its block by itself.  What bounds it: one workgroup's chain
-// of loads, scans and the rows' search (5.5 us of 64 sequences; 18 of 4099, and 6 for their 64k
-// rows in a launch of their own).  Nothing is committed before
-// the whole batch is known to fit: a plan that fails writes its status, lengths as they
-// were, and rows of no sequence.
+// of loads, scans and the rows' search (6 us of 64 sequences; 19 of 4099, and 5.5 for their 64k
+// rows in a launch of their own).  Nothing is committed before the whole batch is known to
+// fit, in blocks of the pool: a plan that fails writes its status, lengths as they were, and
+// rows of no sequence.
 struct PlanArgs {
   const int32_t* counts;
   const int32_t* done;
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256) void ragged_rows_kernel(PlanArgs a) {
 // narrow ones) the share of a workgroup that the chip holds at once.  Tiles that cost more are
 // split; so at most `target` units, one such workgroup each, come on top of one a tile.  The
 // list goes by cost, the largest first: the workgroups that start last are short.  One
-// workgroup's chain of loads and scans, 6 to 7 us of 7 to 64 sequences; in a step it runs beside
+// workgroup's chain of loads and scans, 6 to 9 us of 3 to 64 sequences; in a step it runs beside
 // the append.
 constexpr int kUnitBuckets = 64;
 
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(kAppendThreads) void ragged_append_kernel(AppendArg
 // Attention of any head dim and cache type: a unit's rows a wave each (ragged_own_row).
 // What bounds it: the latency of a key's rows and of the wave's sum, four keys at a time;
 // the units' splits (64 keys on, eight workgroups a CU) fill the chip.  16 sequences of one row
-// after 2000, 8q/2kv/d512: bf16 76 us (0.86 TB/s), Q8 94; 200 fresh fp32 rows 53.
+// after 2000, 8q/2kv/d512: bf16 75 us (1.75 TB/s), Q8 90; 200 fresh fp32 rows 52.
 constexpr int kValuWaves = 4;
 template <int EPL, typename T>
 __global__ __launch_bounds__(64 * kValuWaves) void ragged_valu_kernel(RaggedArgs a) {
@@ -647,7 +647,7 @@ __global__ __launch_bounds__(64 * kValuWaves) void ragged_valu_kernel(RaggedArgs
 
 // ---------------------------------------------------------------------------
 // The merge of a split tile's n units: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
-// Latency (unit, statistics, rows): 5 us of narrow tiles, 10 to 14 where wide ones are split.
+// Latency (unit, statistics, rows): 4 to 6 us of narrow tiles, 10 to 14 where wide ones are split.
 // The workgroups of the tile's parts share its rows: up to kMergeFew units a wave takes a
 // row by itself, past them a workgroup's waves share a row's units.
 constexpr int kMergeThreads = 256, kMergeWaves = kMergeThreads / 64, kMergeFew = 16;

@@ -17,13 +17,14 @@
 // of the waves stages the next interval after its products, the second before them, so that
 // one's conversions meet the other's products; the interval after next is in flight meanwhile.
 // What bounds them: the chain of an interval (staging, products, barrier).  2048 fresh rows at
-// 32q/8kv/d128 bf16, fp32 and Q8: 162, 198 and 156 us with units and merge (bf16 210 TFLOP/s of
-// the layer's 34 GFLOP, 36 % of the matrix cores' rate over two products a term); 512 after 16384:
-// 375, 475 and 330 us (bf16 372 TFLOP/s, 64 %).
+// 32q/8kv/d128 bf16, fp32 and Q8, on several cards: 147 to 162, 184 to 198 and 143 to 156 us with
+// units and merge (bf16 212 to 234 TFLOP/s of the layer's 34 GFLOP, 37 to 40 % of the matrix cores'
+// rate over two products a term); 512 after 16384: 327 to 377, 468 to 480 and 313 to 337 us (bf16 370
+// to 427 TFLOP/s, 64 to 74 %).
 // Narrow tiles (one row, drafts): 16 rows or 32, every wave a key group by itself with its own
 // LDS, so no wave waits for another: a tile's K, then its V, take the same place, and the next
 // tile's are in flight.  What bounds them: the stream where there is enough of it (64 sequences
-// of one row after 100 to 3880, bf16, fp32 and Q8: 113, 196 and 76 us, the bytes at 4.6, 5.3 and
+// of one row after 100 to 3880, bf16, fp32 and Q8: 113, 195 and 74 us, the bytes at 4.6, 5.3 and
 // 3.6 TB/s), else a wave's chain a tile.
 // The key groups' (m, l, o) are merged through LDS at the end.
 #include "ragged.hpp"
